@@ -97,6 +97,15 @@ def copy_policy(kernel_max_bytes: int, split_min_bytes: int, n_copy_streams: int
 
 _vp = ctypes.c_void_p
 _sz = ctypes.c_size_t
+class Kv8Cache(ctypes.Structure):
+    """Mirror of ``ftx_kv8_cache``: one layer of a paged 8-bit KV cache and the sequences of a call."""
+
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("pages", ctypes.c_int64),
+                ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("starts", ctypes.c_void_p),
+                ("news", ctypes.c_void_p), ("width", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("page_tokens", ctypes.c_int), ("d", ctypes.c_int), ("format", ctypes.c_int)]
+
+
 _int = ctypes.c_int
 _uint = ctypes.c_uint
 
@@ -169,6 +178,13 @@ _SIGNATURES: dict[str, list] = {
                  _int, _int, ctypes.c_float, _vp],
     "ftx_rope_cache": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int64, ctypes.c_int64, _int, _int, _int,
                        ctypes.c_int64, _vp, _vp],
+    "ftx_kv8_append": [ctypes.POINTER(Kv8Cache), _vp, _vp, _vp, _vp, _vp, ctypes.c_int64, _vp, ctypes.c_int64,
+                       ctypes.c_int64, _int, _vp, _vp],
+    "ftx_kv8_attention_workspace": [ctypes.c_int64, ctypes.c_int64, _int, _int, _int, ctypes.c_int64,
+                                    ctypes.POINTER(_sz)],
+    "ftx_kv8_attention": [ctypes.POINTER(Kv8Cache), _vp, _vp, ctypes.c_int64, ctypes.c_int64, _int, _vp,
+                          ctypes.c_float, ctypes.c_int64, _vp, _sz, _vp],
+    "ftx_kv8_copy_pages": [_vp, _vp, ctypes.c_int64, ctypes.c_int64, _int, _int, _int, _vp, _vp, ctypes.c_int64, _vp],
     "ftx_silu_mul": [_vp, _vp, _vp, ctypes.c_int64, _vp],
     "ftx_fp8_linear_fused": [_vp, ctypes.c_int, _vp, _vp, _vp, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, _vp,
                              _vp, _sz, _vp],
@@ -177,6 +193,10 @@ _SIGNATURES: dict[str, list] = {
 FP8_EPILOGUE_NONE = 0
 FP8_EPILOGUE_SWIGLU = 1
 FP8_EPILOGUE_RESIDUAL = 2
+
+KV8_BLOCK = 32
+KV8_E4M3 = 0
+KV8_INT8 = 1
 
 NORM_NONE = 0
 NORM_RMS = 1

@@ -176,6 +176,60 @@ hipError_t launch_rope_cache(const RopeLaunch &p, hipStream_t stream);
 constexpr int64_t kSiluMulMax = (int64_t(1) << 35) - 4096;  // a thread for 8 values, within kMaxThreads
 hipError_t launch_silu_mul(const uint16_t *g, const uint16_t *u, uint16_t *y, int64_t n, hipStream_t stream);
 
+// One layer of a KV cache in pages of 8-bit codes (ftx_kvcache.hip), and the sequences of a call.
+constexpr int kKvBlock = FTX_KV8_BLOCK;  // tokens that share a scale
+constexpr int kKvRows = 16;              // rows of a tile: one side of the matrix instruction
+struct KvPages {
+  const uint8_t *codes;   // [pages][2][kv_heads][page_blocks][32 d]
+  const float *scales;    // [pages][2][kv_heads][page_blocks]
+  int64_t pages;
+  const int32_t *table;   // [batch][width] page numbers; rows table_stride apart
+  int64_t table_stride;
+  const int32_t *starts;  // [batch] tokens cached before the call's
+  const int32_t *news;    // [batch] tokens of the call, or null: all t of them
+  int width, kv_heads, page_blocks, page_shift, d;  // page_blocks = 1 << page_shift
+  bool fp8;
+};
+struct Kv8Attention {
+  KvPages kv;
+  const uint16_t *q;
+  uint16_t *o;
+  float *part;            // per-chunk values, maxima and sums (part_bytes), when splits > 1
+  int64_t q_stride[3], o_stride[3];  // batch, token, head, in elements
+  int batch, t, heads;
+  float scale_log2;
+  // planned
+  int rep, rows, row_tiles, splits, chunk;  // chunk: blocks of a split
+  int64_t tile_items;
+  size_t part_bytes;
+};
+void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, int cus);
+hipError_t launch_kv8_attention(const Kv8Attention &p, hipStream_t stream);
+struct Kv8Append {
+  KvPages kv;
+  uint8_t *codes;         // kv.codes and kv.scales, to write to
+  float *scales;
+  const uint16_t *q, *k, *v;
+  uint16_t *q_out;        // [batch][t][heads][d]
+  const float *cos, *sin; // [positions][d]
+  int64_t positions;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  int batch, t, heads;
+  int seq_blocks;         // blocks that t tokens touch at most
+  int64_t block_items;    // batch * seq_blocks * kv_heads * 2 workgroups
+};
+hipError_t launch_kv8_append(const Kv8Append &p, hipStream_t stream);
+constexpr int kKvCopyPairs = 256;  // of one launch: they travel as its argument
+struct Kv8Copy {
+  uint8_t *codes;
+  float *scales;
+  int64_t layers, pages, page_bytes, page_scales, pieces;
+  int n;
+  struct { int32_t src, dst; } pair[kKvCopyPairs];
+};
+int64_t kv8_copy_pieces(int64_t page_bytes);
+hipError_t launch_kv8_copy(const Kv8Copy &p, hipStream_t stream);
+
 // Staged copies from pageable host memory and the parallel host memcpy
 // (ftx_staged.hip).
 int staged_copy_h2d(void *dst, const void *src, size_t nbytes, hipStream_t stream);

@@ -1,0 +1,610 @@
+// A KV cache in pages of 8-bit codes, written for gfx950: writing positions into it, attention over it, copying
+// its pages.
+//
+// One layer of the cache is codes[page][side][kv head][block of the page][32 d bytes] (side 0: keys, 1: values) and
+// scales[page][side][kv head][block]; a block is 32 tokens of one head and a code c stands for c * scale. A
+// sequence's tokens lie in the pages that its row of the table names, in order; a page number outside the pool is
+// a hole, whose tokens no query sees and no write reaches.
+//
+// A block's bytes are in the order in which the matrix cores take them: the keys as [d / 16][32 tokens][16], the
+// values as [d][32 tokens]. A lane's 16 bytes of keys (one token, 16 of the sum over d) and 8 bytes of values (one
+// of d, 8 of the sum over tokens) are then operands as they lie, and a wave's load covers whole lines; values kept
+// token by token would have to be transposed through LDS by every reader.
+#include <algorithm>
+#include <cfloat>
+
+#include "ftx_internal.h"
+
+namespace ftx {
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kWave = 64;
+constexpr float kSlack = 8.0f;
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
+}
+__device__ __forceinline__ float bf16_value(uint32_t bits) { return __uint_as_float(bits << 16); }
+
+// What a call adds to a sequence or asks of it: `count` tokens after the `start` cached ones. Tokens past the
+// table's last page, and every token of a sequence whose start is negative, take no part.
+struct Span {
+  int start, count;
+};
+__device__ __forceinline__ Span span_of(const KvPages &c, int64_t b, int t) {
+  const int start = c.starts[b];
+  int count = c.news ? min(c.news[b], t) : t;
+  const int capacity = c.width * c.page_blocks * kKvBlock;
+  if (start < 0 || start >= capacity) return {0, 0};
+  return {start, max(0, min(count, capacity - start))};
+}
+
+// The page that holds a block of sequence b, or -1.
+__device__ __forceinline__ int page_of(const KvPages &c, int64_t b, int block) {
+  const int page = c.table[b * c.table_stride + (block >> c.page_shift)];
+  return static_cast<unsigned>(page) < static_cast<unsigned>(c.pages) ? page : -1;
+}
+
+// The number of a block of (page, side, head) in the layer: times 32 d its codes' offset, itself its scale's.
+__device__ __forceinline__ int64_t block_index(const KvPages &c, int page, int side, int head, int block) {
+  return ((static_cast<int64_t>(page) * 2 + side) * c.kv_heads + head) * c.page_blocks +
+         (block & (c.page_blocks - 1));
+}
+
+// ---- attention -------------------------------------------------------------------------------------------------
+//
+//   o[b, i, h, :] = sum_p w_p v_p / sum_p w_p,  w_p = exp(scale q[b, i, h, :] . k_p - max),  p <= start_b + i
+//
+// over the cached tokens p of the head that the group of `rep` query heads shares; a row that sees no token is 0.
+// Scores, the running maximum and the running sum are fp32. A code is exact in bf16 and enters the products as it
+// is: a block's key scale multiplies its scores, its value scale the probabilities, which are then rounded to bf16
+// (2^-9 of each at most, as in the attention over a bf16 cache).
+
+// Eight codes as bf16.
+template <bool FP8>
+__device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi) {
+  u32x4 w;
+  if constexpr (FP8) {
+    w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
+    w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
+    w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
+    w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int v = static_cast<int>(i < 2 ? lo : hi);
+      w[i] = pack_bf16(static_cast<float>(static_cast<int8_t>(v >> (16 * (i & 1)))),
+                       static_cast<float>(static_cast<int8_t>(v >> (16 * (i & 1) + 8))));
+    }
+  }
+  return __builtin_bit_cast(bf16x8, w);
+}
+
+// The first n of eight codes, the others 0.
+__device__ __forceinline__ u32x2 keep_codes(u32x2 v, int n) {
+  const uint64_t mask = n >= 8 ? ~0ull : n <= 0 ? 0ull : (1ull << (8 * n)) - 1;
+  return (u32x2){v[0] & static_cast<uint32_t>(mask), v[1] & static_cast<uint32_t>(mask >> 32)};
+}
+
+// The maximum (or sum) over the four lanes that hold one row.
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float row_sum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// The blocks that the 16 rows of a tile see.
+__device__ __forceinline__ int tile_blocks(const Kv8Attention &a, Span s, int tile) {
+  const int row0 = tile * kKvRows;
+  if (row0 / a.rep >= s.count) return 0;
+  const int last = min(min(row0 + kKvRows, a.rows) - 1, s.count * a.rep - 1) / a.rep;
+  return (s.start + last) / kKvBlock + 1;
+}
+
+// 16 rows (the query heads of a group and the tokens, row = token * rep + head of the group) over one chunk of the
+// keys; the four waves take its blocks in turn and join their sums through LDS. Nothing is staged: each wave loads
+// the next block's codes into registers while it works on this one.
+template <int D, bool FP8>
+__global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8Attention a) {
+  constexpr int kWaves = 4;
+  constexpr int kKLoads = D / 64;   // 16 bytes a lane, of each 16 keys of a block
+  constexpr int kDTiles = D / 16;
+  constexpr int kPitch = D + 4;
+  __shared__ __align__(16) float part[kWaves][kKvRows][kPitch];
+  __shared__ float part_m[kWaves][kKvRows], part_l[kWaves][kKvRows];
+
+  int64_t item = blockIdx.x;
+  const int split = static_cast<int>(item % a.splits);
+  item /= a.splits;
+  const int64_t tile_item = item;
+  const int tile = static_cast<int>(item % a.row_tiles);
+  item /= a.row_tiles;
+  const int kvh = static_cast<int>(item % a.kv.kv_heads);
+  const int64_t b = item / a.kv.kv_heads;
+  const Span span = span_of(a.kv, b, a.t);
+  const int blocks = tile_blocks(a, span, tile);
+  const int first = split * a.chunk;
+  if (a.splits > 1 && first >= blocks) return;
+  const int end = split == a.splits - 1 ? blocks : min(blocks, first + a.chunk);
+
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int r = lane & 15, g = lane >> 4;
+  const int row = min(tile * kKvRows + r, a.rows - 1);
+  const int token = row / a.rep;
+  const int head = kvh * a.rep + (row - token * a.rep);
+  const int seen = token < span.count ? span.start + token + 1 : 0;  // keys this lane's row sees
+  const int all = (tile * kKvRows) / a.rep < span.count ? span.start + (tile * kKvRows) / a.rep + 1 : 0;
+  const bool every_row = (min(tile * kKvRows + kKvRows, a.rows) - 1) / a.rep < span.count;
+  const int whole = every_row ? all : 0;  // every row of the tile sees keys below this
+  const int length = span.start + span.count;
+
+  bf16x8 qf[D / 32];
+  {
+    const uint16_t *qp = a.q + b * a.q_stride[0] + token * a.q_stride[1] + head * a.q_stride[2] + 16 * g;
+#pragma unroll
+    for (int i = 0; i < kKLoads; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        qf[2 * i + h] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(qp + 64 * i + 8 * h));
+  }
+
+  f32x4 o[kDTiles];
+#pragma unroll
+  for (int d = 0; d < kDTiles; ++d) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  float m = -FLT_MAX, l = 0.f;
+
+  struct Block {
+    u32x4 k[2][kKLoads];
+    u32x2 v[kDTiles];
+    float k_scale, v_scale;
+    bool hole;
+  };
+  const auto load = [&](Block &x, int block) {
+    const int page = page_of(a.kv, b, block);
+    x.hole = page < 0;
+    const int64_t ki = block_index(a.kv, max(page, 0), 0, kvh, block);
+    const int64_t vi = block_index(a.kv, max(page, 0), 1, kvh, block);
+    x.k_scale = a.kv.scales[ki];
+    x.v_scale = a.kv.scales[vi];
+    const uint8_t *kp = a.kv.codes + ki * (kKvBlock * D) + g * (16 * kKvBlock) + (8 * (r >> 2) + (r & 3)) * 16;
+    const uint8_t *vp = a.kv.codes + vi * (kKvBlock * D) + r * kKvBlock + 8 * g;
+#pragma unroll
+    for (int i = 0; i < kKLoads; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        x.k[s][i] = *reinterpret_cast<const u32x4 *>(kp + i * (64 * kKvBlock) + 64 * s);
+#pragma unroll
+    for (int d = 0; d < kDTiles; ++d) x.v[d] = *reinterpret_cast<const u32x2 *>(vp + d * (16 * kKvBlock));
+  };
+  // Key 8 g' + 4 s + c of a block is row 4 g' + c of score tile s, so lane group g holds the scores of keys 8 g ..
+  // 8 g + 7, the ones whose values it loads.
+  const auto work = [&](Block &x, int block) {
+    if (x.hole) return;
+    f32x4 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kKLoads; ++i) {
+        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen<FP8>(x.k[t][i][0], x.k[t][i][1]), qf[2 * i], s[t], 0, 0, 0);
+        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen<FP8>(x.k[t][i][2], x.k[t][i][3]), qf[2 * i + 1], s[t], 0, 0, 0);
+      }
+    }
+    const int key0 = block * kKvBlock;
+    float scale = a.scale_log2 * x.k_scale;
+    if (key0 + kKvBlock > whole) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[t][c] = key0 + 8 * g + 4 * t + c < seen ? s[t][c] * scale : -INFINITY;
+      scale = 1.0f;
+      if (key0 + kKvBlock > length) {
+#pragma unroll
+        for (int d = 0; d < kDTiles; ++d) x.v[d] = keep_codes(x.v[d], length - key0 - 8 * g);
+      }
+    }
+    float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    mx = row_max(mx) * scale;
+    if (__any(mx > m + kSlack)) {
+      const float m_new = fmaxf(m, mx);
+      const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < kDTiles; ++d)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[d][c] *= alpha;
+    }
+    u32x4 p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[e >> 1][2 * (e & 1)], scale, -m));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[e >> 1][2 * (e & 1) + 1], scale, -m));
+      l += p0 + p1;
+      p[e] = pack_bf16(p0 * x.v_scale, p1 * x.v_scale);
+    }
+#pragma unroll
+    for (int d = 0; d < kDTiles; ++d)
+      o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen<FP8>(x.v[d][0], x.v[d][1]), __builtin_bit_cast(bf16x8, p),
+                                                     o[d], 0, 0, 0);
+  };
+
+  if (first + wave < end) {
+    const int last = end - 1;  // loads ahead of the loop's end take the chunk's last block again
+    Block x, y;
+    int j = first + wave;
+    load(x, j);
+    for (;;) {
+      load(y, min(j + kWaves, last));
+      work(x, j);
+      j += kWaves;
+      if (j >= end) break;
+      load(x, min(j + kWaves, last));
+      work(y, j);
+      j += kWaves;
+      if (j >= end) break;
+    }
+  }
+
+  l = row_sum(l);
+#pragma unroll
+  for (int d = 0; d < kDTiles; ++d) *reinterpret_cast<f32x4 *>(&part[wave][r][16 * d + 4 * g]) = o[d];
+  if (g == 0) {
+    part_m[wave][r] = m;
+    part_l[wave][r] = l;
+  }
+  __syncthreads();
+  constexpr int kPer = D / 16;  // values of one row that a thread joins
+  const int out_r = threadIdx.x / 16, out_d = (threadIdx.x % 16) * kPer;
+  float top = -FLT_MAX;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, part_m[w][out_r]);
+  float sum = 0.f, acc[kPer];
+#pragma unroll
+  for (int c = 0; c < kPer; ++c) acc[c] = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float weight = __builtin_amdgcn_exp2f(part_m[w][out_r] - top);
+    sum = fmaf(weight, part_l[w][out_r], sum);
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) acc[c] = fmaf(weight, part[w][out_r][out_d + c], acc[c]);
+  }
+  if (a.splits > 1) {
+    const int64_t slots = a.tile_items * kKvRows;
+    const int64_t slot = split * slots + tile_item * kKvRows + out_r;
+    float *po = a.part + slot * D + out_d;
+#pragma unroll
+    for (int c = 0; c < kPer; c += 4) *reinterpret_cast<f32x4 *>(po + c) = (f32x4){acc[c], acc[c + 1], acc[c + 2], acc[c + 3]};
+    if (out_d == 0) {
+      float *pm = a.part + a.splits * slots * D;
+      pm[slot] = top;
+      pm[a.splits * slots + slot] = sum;
+    }
+    return;
+  }
+  const int out_row = tile * kKvRows + out_r;
+  if (out_row >= a.rows) return;
+  const int out_token = out_row / a.rep;
+  const int out_head = kvh * a.rep + (out_row - out_token * a.rep);
+  const float inv = sum != 0.f ? 1.0f / sum : 0.f;  // no key, no weight: the row is 0
+  uint16_t *op = a.o + b * a.o_stride[0] + out_token * a.o_stride[1] + out_head * a.o_stride[2] + out_d;
+#pragma unroll
+  for (int c = 0; c < kPer; c += 4)
+    *reinterpret_cast<u32x2 *>(op + c) =
+        (u32x2){pack_bf16(acc[c] * inv, acc[c + 1] * inv), pack_bf16(acc[c + 2] * inv, acc[c + 3] * inv)};
+}
+
+// o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the chunks that hold keys the tile sees, M the largest
+// m_i; D / 4 lanes a row.
+template <int D>
+__global__ __launch_bounds__(256) void kv8_join_kernel(Kv8Attention a) {
+  constexpr int kLanes = D / 4;
+  const int64_t slots = a.tile_items * kKvRows;
+  const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
+  const int c = threadIdx.x % kLanes;
+  if (at >= slots) return;
+  const int64_t tile_item = at / kKvRows;
+  const int tile = static_cast<int>(tile_item % a.row_tiles);
+  const int row = tile * kKvRows + static_cast<int>(at % kKvRows);
+  if (row >= a.rows) return;
+  const int64_t bkv = tile_item / a.row_tiles;
+  const int64_t b = bkv / a.kv.kv_heads;
+  const int used = min(a.splits, (tile_blocks(a, span_of(a.kv, b, a.t), tile) + a.chunk - 1) / a.chunk);
+  const float *pm = a.part + a.splits * slots * D;
+  const float *pl = pm + a.splits * slots;
+  constexpr int kBatch = 8;  // chunks whose loads are in flight together
+  float mx = -FLT_MAX, l = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int i0 = 0; i0 < used; i0 += kBatch) {
+    float m[kBatch], part_l[kBatch];
+    f32x4 part[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int64_t s = min(i0 + i, used - 1) * slots + at;
+      m[i] = pm[s];
+      part_l[i] = pl[s];
+      part[i] = *reinterpret_cast<const f32x4 *>(a.part + s * D + 4 * c);
+    }
+    float m_new = mx;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) m_new = fmaxf(m_new, m[i]);
+    const float alpha = __builtin_amdgcn_exp2f(mx - m_new);
+    l *= alpha;
+    acc *= alpha;
+    mx = m_new;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (i0 + i >= used) break;
+      const float w = __builtin_amdgcn_exp2f(m[i] - m_new);
+      l += w * part_l[i];
+      acc += w * part[i];
+    }
+  }
+  const float inv = l != 0.f ? 1.0f / l : 0.f;
+  const int token = row / a.rep;
+  const int head = static_cast<int>(bkv % a.kv.kv_heads) * a.rep + (row - token * a.rep);
+  uint16_t *op = a.o + b * a.o_stride[0] + token * a.o_stride[1] + head * a.o_stride[2] + 4 * c;
+  *reinterpret_cast<u32x2 *>(op) =
+      (u32x2){pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
+}
+
+template <int D, bool FP8>
+hipError_t launch_rows(const Kv8Attention &p, hipStream_t stream) {
+  hipLaunchKernelGGL((kv8_rows_kernel<D, FP8>), dim3(static_cast<unsigned>(p.tile_items * p.splits)), dim3(256), 0,
+                     stream, p);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess || p.splits == 1) return err;
+  const int64_t lanes = p.tile_items * kKvRows * (D / 4);
+  hipLaunchKernelGGL((kv8_join_kernel<D>), dim3(static_cast<unsigned>((lanes + 255) / 256)), dim3(256), kLdsToken,
+                     stream, p);
+  return hipGetLastError();
+}
+
+// ---- writing new positions ---------------------------------------------------------------------------------------
+//
+// The new tokens' y (keys rotated by the tables, halves against each other, values as they are) go into their
+// blocks under s = max(the block's scale if it holds older tokens, max |y| / top), top = 448 or 127, as the nearest
+// codes to y / s; where s grew, the older codes are rounded again to the nearest of c * (old s / s). Tokens of the
+// block past the new ones become 0. The maximum is over finite values (an infinity becomes the largest code, a NaN
+// the e4m3 NaN or the integer 0), and a scale below 2^-100 counts as 0, with codes of 0.
+//
+// The sums are the ones elementary operations make, each product and sum rounded to fp32 on its own (no fused
+// multiply-add), so the codes do not depend on how a compiler contracts them.
+constexpr float kTiny = 0x1p-100f;
+
+template <bool FP8>
+__device__ __forceinline__ uint32_t code4(const float *y) {
+  if constexpr (FP8) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = y[i] > 448.f ? 448.f : y[i] < -448.f ? -448.f : y[i];  // a NaN stays
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true));
+  } else {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float v = y[i] == y[i] ? fminf(fmaxf(rintf(y[i]), -127.f), 127.f) : 0.f;
+      w |= (static_cast<uint32_t>(static_cast<int>(v)) & 255u) << (8 * i);
+    }
+    return w;
+  }
+}
+
+template <bool FP8>
+__device__ __forceinline__ float code_value(uint32_t byte) {
+  if constexpr (FP8) return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(byte), 0);
+  return static_cast<float>(static_cast<int8_t>(byte));
+}
+
+// Eight rotated values of a head: x cos + rot(x) sin, rot(x) = (-upper half, lower half).
+template <int D>
+__device__ __forceinline__ void rotate8(const uint16_t *x, int d0, const float *cos, const float *sin, float *y) {
+#pragma clang fp contract(off)
+  const int other = d0 < D / 2 ? d0 + D / 2 : d0 - D / 2;
+  const u32x4 a = *reinterpret_cast<const u32x4 *>(x + d0), b = *reinterpret_cast<const u32x4 *>(x + other);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float va = bf16_value(a[i / 2] >> (16 * (i & 1)));
+    const float vb = bf16_value(b[i / 2] >> (16 * (i & 1)));
+    const float turned = d0 < D / 2 ? -vb : vb;
+    const float p = va * cos[d0 + i], q = turned * sin[d0 + i];
+    y[i] = p + q;
+  }
+}
+
+// Workgroups below `a.block_items` write one block of one head and side each; the others rotate the queries.
+template <int D, bool FP8>
+__global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
+#pragma clang fp contract(off)
+  constexpr int kChunks = D / 16;
+  constexpr float kTop = FP8 ? 448.f : 127.f;
+  const int64_t item = blockIdx.x;
+  if (item >= a.block_items) {  // the queries: eight values a thread
+    const int64_t at = ((item - a.block_items) * 256 + threadIdx.x) * 8;
+    const int64_t row = at / D;  // [batch, t, heads]
+    if (row >= static_cast<int64_t>(a.batch) * a.t * a.heads) return;
+    const int d0 = static_cast<int>(at % D);
+    const int64_t head = row % a.heads, bt = row / a.heads;
+    const int64_t b = bt / a.t;
+    const int i = static_cast<int>(bt % a.t);
+    const Span span = span_of(a.kv, b, a.t);
+    float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const int64_t pos = static_cast<int64_t>(span.start) + i;
+    if (i < span.count && pos < a.positions)
+      rotate8<D>(a.q + b * a.q_stride[0] + i * a.q_stride[1] + head * a.q_stride[2], d0, a.cos + pos * D, a.sin + pos * D, y);
+    *reinterpret_cast<u32x4 *>(a.q_out + row * D + d0) =
+        (u32x4){pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7])};
+    return;
+  }
+  __shared__ __align__(16) uint8_t tile[kKvBlock * D];
+  __shared__ float wave_max[4];
+  int64_t rest = item;
+  const int side = static_cast<int>(rest & 1);
+  rest >>= 1;
+  const int head = static_cast<int>(rest % a.kv.kv_heads);
+  rest /= a.kv.kv_heads;
+  const int nth = static_cast<int>(rest % a.seq_blocks);
+  const int64_t b = rest / a.seq_blocks;
+  Span span = span_of(a.kv, b, a.t);
+  span.count = static_cast<int>(min<int64_t>(span.count, max<int64_t>(0, a.positions - span.start)));
+  const int block = span.start / kKvBlock + nth;
+  const int lo = max(span.start, block * kKvBlock);  // the new tokens of this block: lo .. hi - 1
+  const int hi = min(span.start + span.count, (block + 1) * kKvBlock);
+  if (lo >= hi) return;
+  const int page = page_of(a.kv, b, block);
+  if (page < 0) return;
+  const int64_t index = block_index(a.kv, page, side, head, block);
+  uint8_t *codes = a.codes + index * (kKvBlock * D);
+  const int before = lo - block * kKvBlock;  // older tokens of the block
+
+  // thread: token of the block and 16 values of its head, all tokens' first
+  const int token = threadIdx.x % kKvBlock, chunk = threadIdx.x / kKvBlock;
+  const bool here = chunk < kChunks;
+  const int pos = block * kKvBlock + token;
+  const bool fresh = here && pos >= lo && pos < hi;
+  const bool older = here && pos < lo;
+  float y[16];
+  float largest = 0.f;
+  if (fresh) {
+    const int64_t i = pos - span.start;
+    if (side == 0) {
+      const uint16_t *x = a.k + b * a.k_stride[0] + i * a.k_stride[1] + head * a.k_stride[2];
+      const float *cos = a.cos + static_cast<int64_t>(pos) * D, *sin = a.sin + static_cast<int64_t>(pos) * D;
+      rotate8<D>(x, 16 * chunk, cos, sin, y);
+      rotate8<D>(x, 16 * chunk + 8, cos, sin, y + 8);
+    } else {
+      const uint16_t *x = a.v + b * a.v_stride[0] + i * a.v_stride[1] + head * a.v_stride[2] + 16 * chunk;
+      const u32x4 w0 = *reinterpret_cast<const u32x4 *>(x), w1 = *reinterpret_cast<const u32x4 *>(x + 8);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) y[j] = bf16_value((j < 8 ? w0[j / 2] : w1[j / 2 - 4]) >> (16 * (j & 1)));
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float v = fabsf(y[j]);
+      if (v <= FLT_MAX) largest = fmaxf(largest, v);
+    }
+  }
+#pragma unroll
+  for (int i = 1; i < kWave; i *= 2) largest = fmaxf(largest, __shfl_xor(largest, i));
+  if ((threadIdx.x & (kWave - 1)) == 0) wave_max[threadIdx.x / kWave] = largest;
+  if (before > 0 && threadIdx.x * 16 < kKvBlock * D)
+    *reinterpret_cast<u32x4 *>(tile + threadIdx.x * 16) = *reinterpret_cast<const u32x4 *>(codes + threadIdx.x * 16);
+  __syncthreads();
+  largest = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
+  const float made = largest * (1.0f / kTop);
+  const float old_scale = before > 0 ? a.scales[index] : 0.f;
+  const float scale = fmaxf(old_scale, made < kTiny ? 0.f : made);
+  const float inverse = scale > 0.f ? 1.0f / scale : 0.f;
+  const float ratio = scale > old_scale ? old_scale * inverse : 1.0f;
+  if (older) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      y[j] = code_value<FP8>(side == 0 ? tile[chunk * (16 * kKvBlock) + token * 16 + j]
+                                       : tile[(16 * chunk + j) * kKvBlock + token]) * ratio;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) y[j] = fresh ? y[j] * inverse : 0.f;
+  }
+  u32x4 w;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = code4<FP8>(y + 4 * j);
+  if (side == 0) {
+    if (here) *reinterpret_cast<u32x4 *>(codes + chunk * (16 * kKvBlock) + token * 16) = w;
+  } else {
+    __syncthreads();  // the older codes have been read
+    if (here) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        tile[(16 * chunk + j) * kKvBlock + token] = static_cast<uint8_t>(w[j / 4] >> (8 * (j & 3)));
+    }
+    __syncthreads();
+    if (threadIdx.x * 16 < kKvBlock * D)
+      *reinterpret_cast<u32x4 *>(codes + threadIdx.x * 16) = *reinterpret_cast<const u32x4 *>(tile + threadIdx.x * 16);
+  }
+  __syncthreads();  // every thread has read the old scale
+  if (threadIdx.x == 0) a.scales[index] = scale;
+}
+
+// ---- copying pages -------------------------------------------------------------------------------------------------
+
+constexpr int kCopyBytes = 32 * 1024;  // of one workgroup: eight 16-byte loads in flight a lane
+
+// The argument is read where it lies: as a value, its table of pairs would be copied into registers to be indexed.
+__global__ __launch_bounds__(256) void kv8_copy_kernel(Kv8Copy) {
+  const auto &a = *(const __attribute__((address_space(4))) Kv8Copy *)__builtin_amdgcn_kernarg_segment_ptr();
+  int64_t item = blockIdx.x;
+  const int piece = static_cast<int>(item % a.pieces);
+  item /= a.pieces;
+  const int pair = static_cast<int>(item % a.n);
+  const int64_t layer = item / a.n;
+  const int64_t from = layer * a.pages + a.pair[pair].src, to = layer * a.pages + a.pair[pair].dst;
+  const int64_t at = static_cast<int64_t>(piece) * kCopyBytes + threadIdx.x * 16;
+  const uint8_t *src = a.codes + from * a.page_bytes + at;
+  uint8_t *dst = a.codes + to * a.page_bytes + at;
+  u32x4 v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (at + i * 4096 < a.page_bytes) v[i] = *reinterpret_cast<const u32x4 *>(src + i * 4096);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (at + i * 4096 < a.page_bytes) *reinterpret_cast<u32x4 *>(dst + i * 4096) = v[i];
+  if (piece == 0)
+    for (int i = threadIdx.x; i < a.page_scales; i += 256) a.scales[to * a.page_scales + i] = a.scales[from * a.page_scales + i];
+}
+
+}  // namespace
+
+void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, int cus) {
+  p->rep = p->heads / p->kv.kv_heads;
+  p->rows = p->t * p->rep;
+  p->row_tiles = (p->rows + kKvRows - 1) / kKvRows;
+  p->tile_items = static_cast<int64_t>(p->batch) * p->kv.kv_heads * p->row_tiles;
+  const int64_t blocks = std::max<int64_t>(1, (max_tokens + kKvBlock - 1) / kKvBlock);
+  // Chunks of the keys until four workgroups per CU have work, each of at least two blocks a wave.
+  const int64_t want = std::max<int64_t>(1, (4 * cus + p->tile_items - 1) / p->tile_items);
+  const int64_t chunk = std::max<int64_t>(8, (blocks + want - 1) / want);
+  p->splits = static_cast<int>((blocks + chunk - 1) / chunk);
+  p->chunk = static_cast<int>(chunk);  // the last one goes on to the end of the sequence, whatever max_tokens says
+  p->part_bytes = p->splits > 1 ? static_cast<size_t>(p->splits) * p->tile_items * kKvRows * (p->kv.d + 2) * sizeof(float) : 0;
+}
+
+hipError_t launch_kv8_attention(const Kv8Attention &p, hipStream_t stream) {
+  if (p.kv.d == 128) return p.kv.fp8 ? launch_rows<128, true>(p, stream) : launch_rows<128, false>(p, stream);
+  return p.kv.fp8 ? launch_rows<64, true>(p, stream) : launch_rows<64, false>(p, stream);
+}
+
+hipError_t launch_kv8_append(const Kv8Append &p, hipStream_t stream) {
+  const int64_t values = static_cast<int64_t>(p.batch) * p.t * p.heads * p.kv.d;
+  const dim3 grid(static_cast<unsigned>(p.block_items + (values + 2047) / 2048)), block(256);
+  if (p.kv.d == 128) {
+    if (p.kv.fp8) hipLaunchKernelGGL((kv8_append_kernel<128, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((kv8_append_kernel<128, false>), grid, block, 0, stream, p);
+  } else {
+    if (p.kv.fp8) hipLaunchKernelGGL((kv8_append_kernel<64, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((kv8_append_kernel<64, false>), grid, block, 0, stream, p);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_kv8_copy(const Kv8Copy &p, hipStream_t stream) {
+  hipLaunchKernelGGL(kv8_copy_kernel, dim3(static_cast<unsigned>(p.layers * p.n * p.pieces)), dim3(256), kLdsToken,
+                     stream, p);
+  return hipGetLastError();
+}
+
+int64_t kv8_copy_pieces(int64_t page_bytes) { return (page_bytes + kCopyBytes - 1) / kCopyBytes; }
+
+}  // namespace ftx

@@ -8,6 +8,7 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <unordered_set>
 #include <vector>
 
 #include "ftx_internal.h"
@@ -1412,6 +1413,222 @@ int ftx_silu_mul(const void *g, const void *u, void *y, int64_t n, void *stream)
   if (rc != FTX_OK) return rc;
   FTX_HIP(ftx::launch_silu_mul(static_cast<const uint16_t *>(g), static_cast<const uint16_t *>(u),
                                static_cast<uint16_t *>(y), n, static_cast<hipStream_t>(stream)));
+  return FTX_OK;
+}
+
+namespace {
+
+constexpr int64_t kKvMaxPages = (int64_t(1) << 31) - 1;
+
+int check_kv8_shape(int64_t pages, int kv_heads, int page_tokens, int d) {
+  if (d != 64 && d != 128) return ftx::fail(FTX_ERR_UNSUPPORTED, "the 8-bit cache holds head dimensions 64 and 128");
+  if (page_tokens < ftx::kKvBlock || page_tokens > 4096 || (page_tokens & (page_tokens - 1)) != 0)
+    return ftx::fail(FTX_ERR_INVALID, "a page holds 32 times a power of two tokens, at most 4096");
+  if (pages < 1 || pages > kKvMaxPages || kv_heads < 1 || kv_heads > 65536)
+    return ftx::fail(FTX_ERR_INVALID, "cache dimensions");
+  return FTX_OK;
+}
+
+// Checks a cache and the call's sequences; fills what the kernels read of them.
+int kv8_pages(const ftx_kv8_cache *c, int64_t batch, int64_t t, int heads, ftx::KvPages *p) {
+  if (!c) return ftx::fail(FTX_ERR_INVALID, "cache is null");
+  int rc = check_kv8_shape(c->pages, c->kv_heads, c->page_tokens, c->d);
+  if (rc != FTX_OK) return rc;
+  if (c->format != FTX_KV8_E4M3 && c->format != FTX_KV8_INT8)
+    return ftx::fail(FTX_ERR_INVALID, "unknown cache format");
+  if (batch < 0 || t < 0) return ftx::fail(FTX_ERR_INVALID, "negative dimension");
+  if (heads < 1 || heads > 65536 || heads % c->kv_heads != 0)
+    return ftx::fail(FTX_ERR_INVALID, "heads must be a multiple of the cache's kv_heads");
+  if (batch > (int64_t(1) << 24) || t > (int64_t(1) << 24) ||
+      batch * heads > (int64_t(1) << 30) / std::max<int64_t>(t, 1))
+    return ftx::fail(FTX_ERR_INVALID, "cache call dimensions too large");
+  if (c->width < 0 || static_cast<int64_t>(c->width) * c->page_tokens > (int64_t(1) << 30) || c->table_stride < c->width)
+    return ftx::fail(FTX_ERR_INVALID, "the page table's width or stride");
+  p->width = c->width;
+  p->kv_heads = c->kv_heads;
+  p->page_blocks = c->page_tokens / ftx::kKvBlock;
+  p->page_shift = 0;
+  while ((1 << p->page_shift) < p->page_blocks) ++p->page_shift;
+  p->d = c->d;
+  p->fp8 = c->format == FTX_KV8_E4M3;
+  p->pages = c->pages;
+  if (batch == 0 || t == 0) return FTX_OK;
+  const int64_t blocks = c->pages * 2 * c->kv_heads * p->page_blocks;
+  rc = check_operand(c->codes, blocks, ftx::kKvBlock * c->d, "cache codes");
+  if (rc == FTX_OK) rc = check_operand(c->scales, blocks, 4, "cache scales");
+  const struct { const int32_t *p; int64_t n; const char *what; } ints[3] = {
+      {c->table, (batch - 1) * c->table_stride + c->width, "page table"},
+      {c->starts, batch, "starts"},
+      {c->news, batch, "news"}};
+  for (int i = 0; i < 3 && rc == FTX_OK; ++i) {
+    if (i == 2 && !ints[i].p) continue;
+    if (i == 0 && c->width == 0) continue;
+    if (!ints[i].p || reinterpret_cast<uintptr_t>(ints[i].p) % 4 != 0)
+      return ftx::fail(FTX_ERR_INVALID, std::string(ints[i].what) + " is null or not 4-byte aligned");
+    rc = ftx::check_device_range(ints[i].p, static_cast<size_t>(ints[i].n * 4), ints[i].what);
+  }
+  if (rc != FTX_OK) return rc;
+  p->codes = static_cast<const uint8_t *>(c->codes);
+  p->scales = c->scales;
+  p->table = c->table;
+  p->table_stride = c->table_stride;
+  p->starts = c->starts;
+  p->news = c->news;
+  return FTX_OK;
+}
+
+int check_view(const void *ptr, const int64_t *stride, int64_t n0, int64_t n1, int64_t n2, int64_t d, const char *what,
+               int64_t *out) {
+  const int64_t extent = view_extent(stride, n0, n1, n2, d);
+  if (extent < 0)
+    return ftx::fail(FTX_ERR_INVALID, std::string(what) + ": strides must be multiples of 8 and not negative");
+  for (int i = 0; i < 3; ++i) out[i] = stride[i];
+  return check_operand(ptr, extent, 2, what);
+}
+
+int plan_kv8(int64_t max_tokens, ftx::Kv8Attention *p) {
+  int cus = 256;
+  ftx::DeviceState *st = nullptr;
+  if (ftx::device_state(&st) == FTX_OK) cus = st->cu_count;
+  ftx::plan_kv8_attention(p, std::min<int64_t>(max_tokens, int64_t(1) << 30), cus);
+  if (p->tile_items > ftx::kMaxThreads / (256 * static_cast<int64_t>(p->splits)))
+    return ftx::fail(FTX_ERR_UNSUPPORTED, "cache attention: more workgroups than one launch holds");
+  return FTX_OK;
+}
+
+}  // namespace
+
+int ftx_kv8_append(const ftx_kv8_cache *cache, const void *q, const void *k, const void *v, const float *cos,
+                   const float *sin, int64_t positions, void *q_out, int64_t batch, int64_t t, int heads,
+                   const int64_t *strides, void *stream) {
+  FTX_REQUIRE_LIVE();
+  ftx::Kv8Append p{};
+  int rc = kv8_pages(cache, batch, t, heads, &p.kv);
+  if (rc != FTX_OK) return rc;
+  if (positions < 0 || positions > (int64_t(1) << 40)) return ftx::fail(FTX_ERR_INVALID, "rotary positions");
+  if (batch == 0 || t == 0) return FTX_OK;
+  if (!strides) return ftx::fail(FTX_ERR_INVALID, "strides is null");
+  const int d = cache->d, kv = cache->kv_heads;
+  rc = check_view(q, strides, batch, t, heads, d, "append q", p.q_stride);
+  if (rc == FTX_OK) rc = check_view(k, strides + 3, batch, t, kv, d, "append k", p.k_stride);
+  if (rc == FTX_OK) rc = check_view(v, strides + 6, batch, t, kv, d, "append v", p.v_stride);
+  if (rc == FTX_OK) rc = check_operand(q_out, batch * t * heads * d, 2, "append q output");
+  if (rc == FTX_OK && positions > 0) rc = check_operand(cos, positions * d, 4, "rotary cos");
+  if (rc == FTX_OK && positions > 0) rc = check_operand(sin, positions * d, 4, "rotary sin");
+  if (rc != FTX_OK) return rc;
+  p.codes = static_cast<uint8_t *>(cache->codes);
+  p.scales = cache->scales;
+  p.q = static_cast<const uint16_t *>(q);
+  p.k = static_cast<const uint16_t *>(k);
+  p.v = static_cast<const uint16_t *>(v);
+  p.q_out = static_cast<uint16_t *>(q_out);
+  p.cos = cos;
+  p.sin = sin;
+  p.positions = positions;
+  p.batch = static_cast<int>(batch);
+  p.t = static_cast<int>(t);
+  p.heads = heads;
+  p.seq_blocks = static_cast<int>((t + 2 * ftx::kKvBlock - 2) / ftx::kKvBlock);
+  p.block_items = batch * p.seq_blocks * kv * 2;
+  if (p.block_items + batch * t * heads * d / 2048 + 1 > ftx::kMaxThreads / 256)
+    return ftx::fail(FTX_ERR_UNSUPPORTED, "cache append: more workgroups than one launch holds");
+  FTX_HIP(ftx::launch_kv8_append(p, static_cast<hipStream_t>(stream)));
+  return FTX_OK;
+}
+
+int ftx_kv8_attention_workspace(int64_t batch, int64_t t, int heads, int kv_heads, int d, int64_t max_tokens,
+                                size_t *bytes) {
+  if (!bytes) return ftx::fail(FTX_ERR_INVALID, "bytes is null");
+  int rc = check_kv8_shape(1, kv_heads, ftx::kKvBlock, d);
+  if (rc != FTX_OK) return rc;
+  if (batch < 0 || t < 0 || max_tokens < 0) return ftx::fail(FTX_ERR_INVALID, "negative dimension");
+  if (heads < 1 || heads > 65536 || heads % kv_heads != 0)
+    return ftx::fail(FTX_ERR_INVALID, "heads must be a multiple of the cache's kv_heads");
+  if (batch > (int64_t(1) << 24) || t > (int64_t(1) << 24) ||
+      batch * heads > (int64_t(1) << 30) / std::max<int64_t>(t, 1))
+    return ftx::fail(FTX_ERR_INVALID, "cache call dimensions too large");
+  *bytes = 0;
+  if (batch == 0 || t == 0) return FTX_OK;
+  ftx::Kv8Attention p{};
+  p.kv.kv_heads = kv_heads;
+  p.kv.d = d;
+  p.batch = static_cast<int>(batch);
+  p.t = static_cast<int>(t);
+  p.heads = heads;
+  rc = plan_kv8(max_tokens, &p);
+  if (rc == FTX_OK) *bytes = p.part_bytes;
+  return rc;
+}
+
+int ftx_kv8_attention(const ftx_kv8_cache *cache, const void *q, void *o, int64_t batch, int64_t t, int heads,
+                      const int64_t *strides, float scale, int64_t max_tokens, void *workspace, size_t workspace_bytes,
+                      void *stream) {
+  FTX_REQUIRE_LIVE();
+  ftx::Kv8Attention p{};
+  int rc = kv8_pages(cache, batch, t, heads, &p.kv);
+  if (rc != FTX_OK) return rc;
+  if (max_tokens < 0) return ftx::fail(FTX_ERR_INVALID, "negative dimension");
+  if (!(scale > 0.f) || std::isinf(scale)) return ftx::fail(FTX_ERR_INVALID, "attention needs a positive scale");
+  if (batch == 0 || t == 0) return FTX_OK;
+  if (!strides) return ftx::fail(FTX_ERR_INVALID, "strides is null");
+  rc = check_view(q, strides, batch, t, heads, cache->d, "attention q", p.q_stride);
+  if (rc == FTX_OK) rc = check_view(o, strides + 3, batch, t, heads, cache->d, "attention o", p.o_stride);
+  if (rc != FTX_OK) return rc;
+  p.q = static_cast<const uint16_t *>(q);
+  p.o = static_cast<uint16_t *>(o);
+  p.batch = static_cast<int>(batch);
+  p.t = static_cast<int>(t);
+  p.heads = heads;
+  p.scale_log2 = scale * 1.44269504088896340736f;
+  rc = plan_kv8(max_tokens, &p);
+  if (rc != FTX_OK) return rc;
+  if (p.part_bytes > 0) {
+    if (workspace_bytes < p.part_bytes)
+      return ftx::fail(FTX_ERR_INVALID, "cache attention needs a workspace of " + std::to_string(p.part_bytes) +
+                                            " bytes (ftx_kv8_attention_workspace)");
+    rc = check_operand(workspace, static_cast<int64_t>(p.part_bytes), 1, "attention workspace");
+    if (rc != FTX_OK) return rc;
+    p.part = static_cast<float *>(workspace);
+  }
+  FTX_HIP(ftx::launch_kv8_attention(p, static_cast<hipStream_t>(stream)));
+  return FTX_OK;
+}
+
+int ftx_kv8_copy_pages(void *codes, float *scales, int64_t layers, int64_t pages, int kv_heads, int page_tokens, int d,
+                       const int32_t *src, const int32_t *dst, int64_t n, void *stream) {
+  FTX_REQUIRE_LIVE();
+  int rc = check_kv8_shape(pages, kv_heads, page_tokens, d);
+  if (rc != FTX_OK) return rc;
+  if (layers < 0 || n < 0 || layers > 65536) return ftx::fail(FTX_ERR_INVALID, "page copy dimensions");
+  if (layers == 0 || n == 0) return FTX_OK;
+  if (!src || !dst) return ftx::fail(FTX_ERR_INVALID, "null pointer");
+  std::unordered_set<int32_t> targets;
+  for (int64_t i = 0; i < n; ++i) {
+    if (src[i] < 0 || src[i] >= pages || dst[i] < 0 || dst[i] >= pages)
+      return ftx::fail(FTX_ERR_INVALID, "page copy: a page number outside the pool");
+    if (!targets.insert(dst[i]).second) return ftx::fail(FTX_ERR_INVALID, "page copy: a page is written twice");
+  }
+  for (int64_t i = 0; i < n; ++i)
+    if (targets.count(src[i])) return ftx::fail(FTX_ERR_INVALID, "page copy: a page is read and written");
+  ftx::Kv8Copy p;
+  p.page_scales = static_cast<int64_t>(2) * kv_heads * (page_tokens / ftx::kKvBlock);
+  p.page_bytes = p.page_scales * ftx::kKvBlock * d;
+  p.pieces = ftx::kv8_copy_pieces(p.page_bytes);
+  rc = check_operand(codes, layers * pages, p.page_bytes, "cache codes");
+  if (rc == FTX_OK) rc = check_operand(scales, layers * pages, p.page_scales * 4, "cache scales");
+  if (rc != FTX_OK) return rc;
+  // pairs of one launch: as many as travel as an argument, and as one launch has workgroups for
+  const int64_t most = std::min<int64_t>(ftx::kKvCopyPairs, ftx::kMaxThreads / 256 / (layers * p.pieces));
+  if (most < 1) return ftx::fail(FTX_ERR_UNSUPPORTED, "page copy: more workgroups than one launch holds");
+  p.codes = static_cast<uint8_t *>(codes);
+  p.scales = scales;
+  p.layers = layers;
+  p.pages = pages;
+  for (int64_t i0 = 0; i0 < n; i0 += most) {
+    p.n = static_cast<int>(std::min(most, n - i0));
+    for (int i = 0; i < p.n; ++i) p.pair[i] = {src[i0 + i], dst[i0 + i]};
+    FTX_HIP(ftx::launch_kv8_copy(p, static_cast<hipStream_t>(stream)));
+  }
   return FTX_OK;
 }
 

@@ -405,6 +405,68 @@ int ftx_rope_cache(const void *q, const void *k, const void *v, const void *cos,
 /* y = bf16(bf16(silu(g)) * u) over n values (a multiple of 8). */
 int ftx_silu_mul(const void *g, const void *u, void *y, int64_t n, void *stream);
 
+/* ---- a KV cache in pages of 8-bit codes --------------------------------------
+ * No reference counterpart. One layer is codes, bytes [pages][2][kv_heads]
+ * [page_tokens / 32][32 d] (keys, then values), and scales, fp32 [pages][2]
+ * [kv_heads][page_tokens / 32]: a block of 32 tokens of a head shares a scale,
+ * and a code c stands for c * scale. format: FTX_KV8_E4M3 or FTX_KV8_INT8
+ * (-127 .. 127). A block's keys are stored as [d / 16][32][16], its values as
+ * [d][32]. page_tokens: 32 times a power of two, at most 4096; d: 64 or 128.
+ *
+ * A sequence's token p lies in page table[b][p / page_tokens] (int32, rows
+ * table_stride apart, width of them used); a number outside [0, pages) is a
+ * hole, whose tokens are not seen and not written. The call's t tokens follow
+ * the starts[b] cached ones (int32); news (int32, or NULL for t each) says how
+ * many of the t there are. A sequence with a negative start takes no part, and
+ * neither do tokens past the table's width. Table, starts and news are device
+ * memory, read when the kernels run.
+ *
+ * ftx_kv8_append: q [batch, t, heads, d] is rotated by the fp32 tables cos and
+ * sin [positions, d] (halves against each other; fp32 arithmetic) into q_out
+ * (contiguous; rows that take no part are 0), the rotated k and v
+ * [batch, t, kv_heads, d] become codes of their blocks, with the scale
+ *   s = max(the block's scale if it holds tokens before starts[b], max |y| / top)
+ * over the new tokens' finite y, top = 448 or 127; a code is the nearest to
+ * y / s, ties to even. Where s grew, the block's older codes are rounded again;
+ * tokens of the block past the new ones become 0. A scale below 2^-100 is 0,
+ * with codes of 0; an infinity becomes the largest code, a NaN the e4m3 NaN or
+ * the integer 0. Tokens past the tables are not written. strides: batch, token
+ * and head of q, k and v, multiples of 8. No two sequences of a call may name
+ * one page for tokens that it writes.
+ *
+ * ftx_kv8_attention: o[b, i, h] = sum_p softmax_p(scale * q[b, i, h] . k_p) v_p
+ * over the cached tokens p <= starts[b] + i of kv head h / (heads / kv_heads);
+ * the call's tokens have been appended. Rows that take no part or see no token
+ * are 0. strides: batch, token and head of q and o. max_tokens: the longest
+ * sequence, new tokens included, as far as the caller knows; it shapes the
+ * launch, not the result. workspace: ftx_kv8_attention_workspace bytes.
+ *
+ * ftx_kv8_copy_pages: in each of `layers` layers that lie back to back, pages
+ * src[i] are copied to dst[i] (host arrays). No dst occurs twice or as a src. */
+#define FTX_KV8_BLOCK 32
+#define FTX_KV8_E4M3 0
+#define FTX_KV8_INT8 1
+typedef struct ftx_kv8_cache {
+  void *codes;
+  float *scales;
+  int64_t pages;
+  const int32_t *table;
+  int64_t table_stride;
+  const int32_t *starts;
+  const int32_t *news;
+  int width, kv_heads, page_tokens, d, format;
+} ftx_kv8_cache;
+int ftx_kv8_append(const ftx_kv8_cache *cache, const void *q, const void *k, const void *v, const float *cos,
+                   const float *sin, int64_t positions, void *q_out, int64_t batch, int64_t t, int heads,
+                   const int64_t *strides, void *stream);
+int ftx_kv8_attention_workspace(int64_t batch, int64_t t, int heads, int kv_heads, int d, int64_t max_tokens,
+                                size_t *bytes);
+int ftx_kv8_attention(const ftx_kv8_cache *cache, const void *q, void *o, int64_t batch, int64_t t, int heads,
+                      const int64_t *strides, float scale, int64_t max_tokens, void *workspace, size_t workspace_bytes,
+                      void *stream);
+int ftx_kv8_copy_pages(void *codes, float *scales, int64_t layers, int64_t pages, int kv_heads, int page_tokens, int d,
+                       const int32_t *src, const int32_t *dst, int64_t n, void *stream);
+
 /* ---- checksums (size-independent parity checks on device data) ----------- */
 /* Order-sensitive 64-bit checksum of nbytes at dev (FNV-1a over 8-byte lanes,
  * folded per 4 KiB block); result written to *out after stream sync. */
