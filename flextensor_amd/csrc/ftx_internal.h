@@ -178,7 +178,7 @@ hipError_t launch_silu_mul(const uint16_t *g, const uint16_t *u, uint16_t *y, in
 
 // One layer of a KV cache in pages of 8-bit codes (ftx_kvcache.hip), and the sequences of a call.
 constexpr int kKvBlock = FTX_KV8_BLOCK;  // tokens that share a scale
-constexpr int kKvRows = 16;              // rows of a tile: one side of the matrix instruction
+constexpr int kKvRows = 16;              // rows of a decode tile: one side of the matrix instruction
 struct KvPages {
   const uint8_t *codes;   // [pages][2][kv_heads][page_blocks][32 d]
   const float *scales;    // [pages][2][kv_heads][page_blocks]
@@ -199,11 +199,13 @@ struct Kv8Attention {
   int batch, t, heads;
   float scale_log2;
   // planned
-  int rep, rows, row_tiles, splits, chunk;  // chunk: blocks of a split
-  int64_t tile_items;
+  int rep, rows, tile_rows, row_tiles, splits, chunk, xcds;  // chunk: blocks of a split
+  int waves;              // of a workgroup, 32 rows each; 0: the decode kernel
+  int64_t tile_items;     // batch * kv heads * row tiles
+  uint32_t items;         // times the splits
   size_t part_bytes;
 };
-void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, int cus);
+void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, int cus, int xcds);
 hipError_t launch_kv8_attention(const Kv8Attention &p, hipStream_t stream);
 struct Kv8Append {
   KvPages kv;
@@ -223,11 +225,11 @@ constexpr int kKvCopyPairs = 256;  // of one launch: they travel as its argument
 struct Kv8Copy {
   uint8_t *codes;
   float *scales;
-  int64_t layers, pages, page_bytes, page_scales, pieces;
-  int n;
+  int64_t layers, pages;
+  uint32_t page_bytes, page_scales, pieces, n;  // pieces: workgroups of a page
   struct { int32_t src, dst; } pair[kKvCopyPairs];
 };
-int64_t kv8_copy_pieces(int64_t page_bytes);
+uint32_t kv8_copy_pieces(uint32_t page_bytes);
 hipError_t launch_kv8_copy(const Kv8Copy &p, hipStream_t stream);
 
 // Staged copies from pageable host memory and the parallel host memcpy

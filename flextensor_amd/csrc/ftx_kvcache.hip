@@ -24,6 +24,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWave = 64;
 constexpr float kSlack = 8.0f;
@@ -103,11 +104,21 @@ __device__ __forceinline__ float row_sum(float v) {
   return v + __shfl_xor(v, 32);
 }
 
-// The blocks that the 16 rows of a tile see.
+// The same over a value and its partner's in the other half of the wave.
+__device__ __forceinline__ float half_max(float v) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// The blocks that the rows of a tile see.
 __device__ __forceinline__ int tile_blocks(const Kv8Attention &a, Span s, int tile) {
-  const int row0 = tile * kKvRows;
+  const int row0 = tile * a.tile_rows;
   if (row0 / a.rep >= s.count) return 0;
-  const int last = min(min(row0 + kKvRows, a.rows) - 1, s.count * a.rep - 1) / a.rep;
+  const int last = min(min(row0 + a.tile_rows, a.rows) - 1, s.count * a.rep - 1) / a.rep;
   return (s.start + last) / kKvBlock + 1;
 }
 
@@ -115,7 +126,7 @@ __device__ __forceinline__ int tile_blocks(const Kv8Attention &a, Span s, int ti
 // keys; the four waves take its blocks in turn and join their sums through LDS. Nothing is staged: each wave loads
 // the next block's codes into registers while it works on this one.
 template <int D, bool FP8>
-__global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8Attention a) {
+__global__ __launch_bounds__(256, 3) void kv8_rows_kernel(Kv8Attention a) {
   constexpr int kWaves = 4;
   constexpr int kKLoads = D / 64;   // 16 bytes a lane, of each 16 keys of a block
   constexpr int kDTiles = D / 16;
@@ -123,14 +134,14 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8Attention a) {
   __shared__ __align__(16) float part[kWaves][kKvRows][kPitch];
   __shared__ float part_m[kWaves][kKvRows], part_l[kWaves][kKvRows];
 
-  int64_t item = blockIdx.x;
-  const int split = static_cast<int>(item % a.splits);
-  item /= a.splits;
+  uint32_t item = blockIdx.x;  // 32-bit divisions: a launch has fewer than 2^24 workgroups
+  const int split = static_cast<int>(item % static_cast<uint32_t>(a.splits));
+  item /= static_cast<uint32_t>(a.splits);
   const int64_t tile_item = item;
-  const int tile = static_cast<int>(item % a.row_tiles);
-  item /= a.row_tiles;
-  const int kvh = static_cast<int>(item % a.kv.kv_heads);
-  const int64_t b = item / a.kv.kv_heads;
+  const int tile = static_cast<int>(item % static_cast<uint32_t>(a.row_tiles));
+  item /= static_cast<uint32_t>(a.row_tiles);
+  const int kvh = static_cast<int>(item % static_cast<uint32_t>(a.kv.kv_heads));
+  const int64_t b = item / static_cast<uint32_t>(a.kv.kv_heads);
   const Span span = span_of(a.kv, b, a.t);
   const int blocks = tile_blocks(a, span, tile);
   const int first = split * a.chunk;
@@ -227,14 +238,20 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8Attention a) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[d][c] *= alpha;
     }
+    // p times the value scale in one operation: 2^(s - m + log2(scale)); the sum of the p takes it out again. A
+    // scale of 0 stands beside codes of 0, whose weight does not matter.
+    const float factor = x.v_scale > 0.f ? x.v_scale : 1.0f;
+    const float offset = __builtin_amdgcn_logf(factor) - m;
+    float sum = 0.f;
     u32x4 p;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[e >> 1][2 * (e & 1)], scale, -m));
-      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[e >> 1][2 * (e & 1) + 1], scale, -m));
-      l += p0 + p1;
-      p[e] = pack_bf16(p0 * x.v_scale, p1 * x.v_scale);
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[e >> 1][2 * (e & 1)], scale, offset));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[e >> 1][2 * (e & 1) + 1], scale, offset));
+      sum += p0 + p1;
+      p[e] = pack_bf16(p0, p1);
     }
+    l = fmaf(sum, __builtin_amdgcn_rcpf(factor), l);
 #pragma unroll
     for (int d = 0; d < kDTiles; ++d)
       o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen<FP8>(x.v[d][0], x.v[d][1]), __builtin_bit_cast(bf16x8, p),
@@ -306,21 +323,265 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8Attention a) {
         (u32x2){pack_bf16(acc[c] * inv, acc[c + 1] * inv), pack_bf16(acc[c + 2] * inv, acc[c + 3] * inv)};
 }
 
+// Prompts: 32 rows a wave, NW waves that share tiles of 64 keys. The workgroup loads a tile's codes into registers,
+// widens each once and writes it to LDS in the order in which a lane reads its operands, 16 bytes at 16 * lane: no
+// bank is met twice and the inner loop is that of the attention over a bf16 cache. Two tiles are in LDS and the
+// codes of a third in registers, so one barrier a tile is enough: a tile is written while the one before it is in
+// use, into the buffer whose last readers have passed the barrier.
+//
+// S^T = K Q^T gives a lane 16 of a block's 32 scores of one row, keys 8 a + 4 g + c (g the half of the wave); V's
+// operands are written in that order.
+template <int D, bool FP8, int NW, bool SPLIT>
+__global__ __launch_bounds__(NW * kWave, 2) void kv8_tile_kernel(Kv8Attention a) {
+  constexpr int kThreads = NW * kWave;
+  constexpr int kKeys = 64, kSub = 2;
+  constexpr int kBlockBytes = kKvBlock * D;          // codes of a block's side
+  constexpr int kBlockUnits = kBlockBytes / 16;      // 16-byte loads
+  constexpr int kSideUnits = kSub * kBlockUnits;
+  constexpr int kUnits = 2 * kSideUnits / kThreads;  // of one thread
+  constexpr int kSide = kKeys * D * 2;               // LDS bytes of a tile's side
+  constexpr int kQSteps = D / 16, kDTiles = D / 32;
+  static_assert(2 * kSideUnits % kThreads == 0 && kBlockUnits % kWave == 0, "a wave's units are of one block and side");
+  __shared__ __align__(1024) uint8_t lds[2][2 * kSide];
+
+  const uint32_t per_xcd = (a.items + a.xcds - 1) / a.xcds;
+  uint32_t item = (blockIdx.x % a.xcds) * per_xcd + blockIdx.x / a.xcds;
+  if (item >= a.items) return;
+  const int split = SPLIT ? static_cast<int>(item % static_cast<uint32_t>(a.splits)) : 0;
+  if (SPLIT) item /= static_cast<uint32_t>(a.splits);
+  const uint32_t bkv = item / static_cast<uint32_t>(a.row_tiles);
+  const int tile = a.row_tiles - 1 - static_cast<int>(item - bkv * a.row_tiles);  // the longest first
+  const int64_t tile_item = static_cast<int64_t>(bkv) * a.row_tiles + tile;
+  const int64_t b = bkv / static_cast<uint32_t>(a.kv.kv_heads);
+  const int kvh = static_cast<int>(bkv % static_cast<uint32_t>(a.kv.kv_heads));
+  const Span span = span_of(a.kv, b, a.t);
+  const int blocks = tile_blocks(a, span, tile);
+  const int first = SPLIT ? split * a.chunk : 0;
+  if (SPLIT && first >= blocks) return;
+  const int end = !SPLIT || split == a.splits - 1 ? blocks : min(blocks, first + a.chunk);
+  const int n_tiles = (end - first + kSub - 1) / kSub;
+
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int r = lane & 31, g = lane >> 5;
+  const int row0 = tile * (32 * NW) + wave * 32;
+  const int row = min(row0 + r, a.rows - 1);
+  const int token = row / a.rep;
+  const int head = kvh * a.rep + (row - token * a.rep);
+  const int length = span.start + span.count;
+  const int seen = row0 + r < a.rows && token < span.count ? span.start + token + 1 : 0;  // keys this lane's row sees
+  const int last_row = min(row0 + 32, a.rows) - 1;
+  const int wave_end = row0 < a.rows && row0 / a.rep < span.count ? min(span.start + last_row / a.rep + 1, length) : 0;
+  // every row of the wave sees keys below this
+  const int whole = row0 + 32 <= a.rows && last_row / a.rep < span.count ? span.start + row0 / a.rep + 1 : 0;
+
+  struct Unit {  // 16 bytes of codes on their way to LDS
+    u32x4 w;
+    int keep;    // values: the tokens of them that the sequence has
+  };
+  Unit units[kUnits];
+  struct Scales {
+    float key[kSub], value[kSub];
+    bool hole[kSub];
+  };
+  const auto load = [&](int t) {  // clamped to the chunk's last block, whose scores and values are masked twice over
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const int u0 = i * kThreads + wave * kWave;  // the wave's first unit
+      const int side = u0 / kSideUnits, sub = u0 % kSideUnits / kBlockUnits;
+      const int block = first + t * kSub + sub;
+      const int page = page_of(a.kv, b, min(block, end - 1));
+      const int64_t index = block_index(a.kv, max(page, 0), side, kvh, min(block, end - 1));
+      units[i].w = *reinterpret_cast<const u32x4 *>(a.kv.codes + index * kBlockBytes + (u0 % kBlockUnits + lane) * 16);
+      units[i].keep = page < 0 || block >= end ? 0 : length - block * kKvBlock;
+    }
+  };
+  const auto store = [&](int t) {
+    uint8_t *base = lds[t & 1];
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const int u0 = i * kThreads + wave * kWave;
+      const int side = u0 / kSideUnits, sub = u0 % kSideUnits / kBlockUnits;
+      const int unit = u0 % kBlockUnits + lane;
+      uint8_t *to = base + side * kSide + sub * (kSide / kSub);
+      u32x4 w = units[i].w;
+      if (side == 0) {  // unit: [d / 16][token], one step of the sum over d, both halves of the wave
+        to += unit / 32 * 1024 + unit % 32 * 16;
+        *reinterpret_cast<bf16x8 *>(to) = widen<FP8>(w[0], w[1]);
+        *reinterpret_cast<bf16x8 *>(to + 512) = widen<FP8>(w[2], w[3]);
+      } else {  // unit: [d][half of the tokens], one step of the sum over tokens
+        if (units[i].keep < kKvBlock) {
+          const int n = units[i].keep - unit % 2 * 16;
+          const u32x2 lo = keep_codes((u32x2){w[0], w[1]}, n), hi = keep_codes((u32x2){w[2], w[3]}, n - 8);
+          w = (u32x4){lo[0], lo[1], hi[0], hi[1]};
+        }
+        const int d = unit / 2;
+        to += (d / 32 * 2 + unit % 2) * 1024 + d % 32 * 16;
+        *reinterpret_cast<bf16x8 *>(to) = widen<FP8>(w[0], w[2]);
+        *reinterpret_cast<bf16x8 *>(to + 512) = widen<FP8>(w[1], w[3]);
+      }
+    }
+  };
+  const auto scales_of = [&](int t) {
+    Scales x;
+#pragma unroll
+    for (int j = 0; j < kSub; ++j) {
+      const int block = min(first + t * kSub + j, end - 1);
+      const int page = page_of(a.kv, b, block);
+      x.hole[j] = page < 0;
+      x.key[j] = a.kv.scales[block_index(a.kv, max(page, 0), 0, kvh, block)];
+      x.value[j] = a.kv.scales[block_index(a.kv, max(page, 0), 1, kvh, block)];
+    }
+    return x;
+  };
+
+  // Queries: lane (r, g) holds elements 16 ks + 8 g .. + 7 of its row for every step ks.
+  bf16x8 qf[kQSteps];
+  {
+    const uint16_t *qp = a.q + b * a.q_stride[0] + token * a.q_stride[1] + head * a.q_stride[2] + 8 * g;
+#pragma unroll
+    for (int ks = 0; ks < kQSteps; ++ks)
+      qf[ks] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(qp + 16 * ks));
+  }
+  f32x16 o[kDTiles];
+#pragma unroll
+  for (int d = 0; d < kDTiles; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+  float m = -FLT_MAX, l = 0.f;
+
+  Scales next = {};
+  if (n_tiles > 0) {
+    load(0);
+    next = scales_of(0);
+    store(0);
+    if (n_tiles > 1) load(1);
+  }
+  for (int t = 0; t < n_tiles; ++t) {
+    __syncthreads();
+    const Scales x = next;
+    if (t + 1 < n_tiles) {
+      next = scales_of(t + 1);
+      store(t + 1);
+      if (t + 2 < n_tiles) load(t + 2);
+    }
+    const int key0 = (first + t * kSub) * kKvBlock;
+    if (key0 >= wave_end) continue;
+    const uint8_t *kt = lds[t & 1] + lane * 16;
+    const uint8_t *vt = kt + kSide;
+    f32x16 s[kSub];
+#pragma unroll
+    for (int j = 0; j < kSub; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[j][e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < kQSteps; ++ks)
+#pragma unroll
+      for (int j = 0; j < kSub; ++j)
+        s[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            *reinterpret_cast<const bf16x8 *>(kt + j * (kSide / kSub) + ks * 1024), qf[ks], s[j], 0, 0, 0);
+    float scale[kSub];
+#pragma unroll
+    for (int j = 0; j < kSub; ++j) {
+      scale[j] = a.scale_log2 * x.key[j];
+      const int block = first + t * kSub + j;
+      if (x.hole[j] || block >= end || (block + 1) * kKvBlock > whole) {
+        const int limit = x.hole[j] || block >= end ? 0 : seen - block * kKvBlock;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[j][e] = 8 * (e >> 2) + 4 * g + (e & 3) < limit ? s[j][e] * scale[j] : -INFINITY;
+        scale[j] = 1.0f;
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kSub; ++j) {
+      float part = s[j][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) part = fmaxf(part, s[j][e]);
+      mx = fmaxf(mx, part * scale[j]);
+    }
+    mx = half_max(mx);
+    if (__any(mx > m + kSlack)) {
+      const float m_new = fmaxf(m, mx);
+      const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < kDTiles; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+    }
+    bf16x8 p[2 * kSub];  // times the value scale, as above
+#pragma unroll
+    for (int j = 0; j < kSub; ++j) {
+      const float factor = x.value[j] > 0.f && !x.hole[j] && first + t * kSub + j < end ? x.value[j] : 1.0f;
+      const float offset = __builtin_amdgcn_logf(factor) - m;
+      float sum = 0.f;
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[j][e], scale[j], offset));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[j][e + 1], scale[j], offset));
+        sum += p0 + p1;
+        w[e / 2] = pack_bf16(p0, p1);
+      }
+      l = fmaf(sum, __builtin_amdgcn_rcpf(factor), l);
+      p[2 * j] = __builtin_bit_cast(bf16x8, (u32x4){w[0], w[1], w[2], w[3]});
+      p[2 * j + 1] = __builtin_bit_cast(bf16x8, (u32x4){w[4], w[5], w[6], w[7]});
+    }
+#pragma unroll
+    for (int f = 0; f < 2 * kSub; ++f)
+#pragma unroll
+      for (int d = 0; d < kDTiles; ++d)
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            *reinterpret_cast<const bf16x8 *>(vt + (f / 2) * (kSide / kSub) + (d * 2 + f % 2) * 1024), p[f], o[d], 0, 0, 0);
+  }
+
+  if (row0 + r >= a.rows) return;
+  l = half_sum(l);
+  if (SPLIT) {
+    const int64_t slots = a.tile_items * a.tile_rows;
+    const int64_t slot = split * slots + tile_item * a.tile_rows + wave * 32 + r;
+    float *po = a.part + slot * D;
+#pragma unroll
+    for (int d = 0; d < kDTiles; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4 *>(po + d * 32 + q * 8 + 4 * g) =
+            (f32x4){o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
+    if (g == 0) {
+      float *pm = a.part + a.splits * slots * D;
+      pm[slot] = m;
+      pm[a.splits * slots + slot] = l;
+    }
+    return;
+  }
+  const float inv = l != 0.f ? 1.0f / l : 0.f;  // no key, no weight: the row is 0
+  uint16_t *op = a.o + b * a.o_stride[0] + token * a.o_stride[1] + head * a.o_stride[2] + 4 * g;
+#pragma unroll
+  for (int d = 0; d < kDTiles; ++d)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<u32x2 *>(op + d * 32 + q * 8) =
+          (u32x2){pack_bf16(o[d][4 * q] * inv, o[d][4 * q + 1] * inv),
+                  pack_bf16(o[d][4 * q + 2] * inv, o[d][4 * q + 3] * inv)};
+}
+
 // o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the chunks that hold keys the tile sees, M the largest
 // m_i; D / 4 lanes a row.
 template <int D>
 __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8Attention a) {
   constexpr int kLanes = D / 4;
-  const int64_t slots = a.tile_items * kKvRows;
+  const int64_t slots = a.tile_items * a.tile_rows;
   const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
   const int c = threadIdx.x % kLanes;
   if (at >= slots) return;
-  const int64_t tile_item = at / kKvRows;
-  const int tile = static_cast<int>(tile_item % a.row_tiles);
-  const int row = tile * kKvRows + static_cast<int>(at % kKvRows);
+  const uint32_t tile_item = static_cast<uint32_t>(at) / static_cast<uint32_t>(a.tile_rows);
+  const int tile = static_cast<int>(tile_item % static_cast<uint32_t>(a.row_tiles));
+  const int row = tile * a.tile_rows + static_cast<int>(static_cast<uint32_t>(at) % static_cast<uint32_t>(a.tile_rows));
   if (row >= a.rows) return;
-  const int64_t bkv = tile_item / a.row_tiles;
-  const int64_t b = bkv / a.kv.kv_heads;
+  const uint32_t bkv = tile_item / static_cast<uint32_t>(a.row_tiles);
+  const int64_t b = bkv / static_cast<uint32_t>(a.kv.kv_heads);
   const int used = min(a.splits, (tile_blocks(a, span_of(a.kv, b, a.t), tile) + a.chunk - 1) / a.chunk);
   const float *pm = a.part + a.splits * slots * D;
   const float *pl = pm + a.splits * slots;
@@ -354,19 +615,30 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8Attention a) {
   }
   const float inv = l != 0.f ? 1.0f / l : 0.f;
   const int token = row / a.rep;
-  const int head = static_cast<int>(bkv % a.kv.kv_heads) * a.rep + (row - token * a.rep);
+  const int head = static_cast<int>(bkv % static_cast<uint32_t>(a.kv.kv_heads)) * a.rep + (row - token * a.rep);
   uint16_t *op = a.o + b * a.o_stride[0] + token * a.o_stride[1] + head * a.o_stride[2] + 4 * c;
   *reinterpret_cast<u32x2 *>(op) =
       (u32x2){pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
 }
 
+template <int D, bool FP8, int NW>
+void start_tiles(const Kv8Attention &p, hipStream_t stream) {
+  const dim3 grid((p.items + p.xcds - 1) / p.xcds * p.xcds), block(NW * kWave);
+  if (p.splits > 1) hipLaunchKernelGGL((kv8_tile_kernel<D, FP8, NW, true>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((kv8_tile_kernel<D, FP8, NW, false>), grid, block, 0, stream, p);
+}
+
 template <int D, bool FP8>
-hipError_t launch_rows(const Kv8Attention &p, hipStream_t stream) {
-  hipLaunchKernelGGL((kv8_rows_kernel<D, FP8>), dim3(static_cast<unsigned>(p.tile_items * p.splits)), dim3(256), 0,
-                     stream, p);
+hipError_t launch_attend(const Kv8Attention &p, hipStream_t stream) {
+  switch (p.waves) {
+    case 0: hipLaunchKernelGGL((kv8_rows_kernel<D, FP8>), dim3(p.items), dim3(256), 0, stream, p); break;
+    case 2: start_tiles<D, FP8, 2>(p, stream); break;
+    case 4: start_tiles<D, FP8, 4>(p, stream); break;
+    default: start_tiles<D, FP8, 8>(p, stream); break;
+  }
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || p.splits == 1) return err;
-  const int64_t lanes = p.tile_items * kKvRows * (D / 4);
+  const int64_t lanes = p.tile_items * p.tile_rows * (D / 4);
   hipLaunchKernelGGL((kv8_join_kernel<D>), dim3(static_cast<unsigned>((lanes + 255) / 256)), dim3(256), kLdsToken,
                      stream, p);
   return hipGetLastError();
@@ -434,12 +706,13 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
   const int64_t item = blockIdx.x;
   if (item >= a.block_items) {  // the queries: eight values a thread
     const int64_t at = ((item - a.block_items) * 256 + threadIdx.x) * 8;
-    const int64_t row = at / D;  // [batch, t, heads]
+    const int64_t row = at / D;  // [batch, t, heads], at most 2^30
     if (row >= static_cast<int64_t>(a.batch) * a.t * a.heads) return;
     const int d0 = static_cast<int>(at % D);
-    const int64_t head = row % a.heads, bt = row / a.heads;
-    const int64_t b = bt / a.t;
-    const int i = static_cast<int>(bt % a.t);
+    const uint32_t bt = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.heads);
+    const int64_t head = static_cast<uint32_t>(row) % static_cast<uint32_t>(a.heads);
+    const int64_t b = bt / static_cast<uint32_t>(a.t);
+    const int i = static_cast<int>(bt % static_cast<uint32_t>(a.t));
     const Span span = span_of(a.kv, b, a.t);
     float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     const int64_t pos = static_cast<int64_t>(span.start) + i;
@@ -451,13 +724,13 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
   }
   __shared__ __align__(16) uint8_t tile[kKvBlock * D];
   __shared__ float wave_max[4];
-  int64_t rest = item;
+  uint32_t rest = blockIdx.x;
   const int side = static_cast<int>(rest & 1);
   rest >>= 1;
-  const int head = static_cast<int>(rest % a.kv.kv_heads);
-  rest /= a.kv.kv_heads;
-  const int nth = static_cast<int>(rest % a.seq_blocks);
-  const int64_t b = rest / a.seq_blocks;
+  const int head = static_cast<int>(rest % static_cast<uint32_t>(a.kv.kv_heads));
+  rest /= static_cast<uint32_t>(a.kv.kv_heads);
+  const int nth = static_cast<int>(rest % static_cast<uint32_t>(a.seq_blocks));
+  const int64_t b = rest / static_cast<uint32_t>(a.seq_blocks);
   Span span = span_of(a.kv, b, a.t);
   span.count = static_cast<int>(min<int64_t>(span.count, max<int64_t>(0, a.positions - span.start)));
   const int block = span.start / kKvBlock + nth;
@@ -545,45 +818,61 @@ constexpr int kCopyBytes = 32 * 1024;  // of one workgroup: eight 16-byte loads 
 // The argument is read where it lies: as a value, its table of pairs would be copied into registers to be indexed.
 __global__ __launch_bounds__(256) void kv8_copy_kernel(Kv8Copy) {
   const auto &a = *(const __attribute__((address_space(4))) Kv8Copy *)__builtin_amdgcn_kernarg_segment_ptr();
-  int64_t item = blockIdx.x;
-  const int piece = static_cast<int>(item % a.pieces);
+  uint32_t item = blockIdx.x;
+  const uint32_t piece = item % a.pieces;
   item /= a.pieces;
-  const int pair = static_cast<int>(item % a.n);
+  const uint32_t pair = item % a.n;
   const int64_t layer = item / a.n;
   const int64_t from = layer * a.pages + a.pair[pair].src, to = layer * a.pages + a.pair[pair].dst;
-  const int64_t at = static_cast<int64_t>(piece) * kCopyBytes + threadIdx.x * 16;
-  const uint8_t *src = a.codes + from * a.page_bytes + at;
-  uint8_t *dst = a.codes + to * a.page_bytes + at;
-  u32x4 v[8];
+  const uint32_t bytes = a.page_bytes, at = piece * kCopyBytes;
+  const u32x4 *src = reinterpret_cast<const u32x4 *>(a.codes + from * bytes + at) + threadIdx.x;
+  u32x4 *dst = reinterpret_cast<u32x4 *>(a.codes + to * bytes + at) + threadIdx.x;
+  if (at + kCopyBytes <= bytes) {
+    u32x4 v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (at + i * 4096 < a.page_bytes) v[i] = *reinterpret_cast<const u32x4 *>(src + i * 4096);
+    for (int i = 0; i < 8; ++i) v[i] = src[i * 256];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (at + i * 4096 < a.page_bytes) *reinterpret_cast<u32x4 *>(dst + i * 4096) = v[i];
-  if (piece == 0)
-    for (int i = threadIdx.x; i < a.page_scales; i += 256) a.scales[to * a.page_scales + i] = a.scales[from * a.page_scales + i];
+    for (int i = 0; i < 8; ++i) dst[i * 256] = v[i];
+  } else {  // a page is whole workgroup loads of 4096 bytes: two sides of 32 tokens of 64 bytes at least
+#pragma unroll 1
+    for (uint32_t i = 0; i < (bytes - at) / 4096; ++i) dst[i * 256] = src[i * 256];
+  }
+  if (piece == 0) {
+    const int n = a.page_scales;
+    const float *from_scales = a.scales + from * n;
+    float *to_scales = a.scales + to * n;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n; i += 256) to_scales[i] = from_scales[i];
+  }
 }
 
 }  // namespace
 
-void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, int cus) {
+void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, int cus, int xcds) {
+  p->xcds = std::max(1, xcds);
   p->rep = p->heads / p->kv.kv_heads;
   p->rows = p->t * p->rep;
-  p->row_tiles = (p->rows + kKvRows - 1) / kKvRows;
-  p->tile_items = static_cast<int64_t>(p->batch) * p->kv.kv_heads * p->row_tiles;
+  const int64_t heads = static_cast<int64_t>(p->batch) * p->kv.kv_heads;
   const int64_t blocks = std::max<int64_t>(1, (max_tokens + kKvBlock - 1) / kKvBlock);
-  // Chunks of the keys until four workgroups per CU have work, each of at least two blocks a wave.
-  const int64_t want = std::max<int64_t>(1, (4 * cus + p->tile_items - 1) / p->tile_items);
+  // Up to 16 rows (decode) the codes go from memory straight into the products; more rows share them through LDS.
+  p->waves = p->rows <= kKvRows ? 0 : p->rows <= 64 ? 2 : p->rows <= 128 ? 4 : 8;
+  p->tile_rows = p->waves == 0 ? kKvRows : 32 * p->waves;
+  p->row_tiles = (p->rows + p->tile_rows - 1) / p->tile_rows;
+  p->tile_items = heads * p->row_tiles;
+  // Chunks of the keys until every CU has its workgroups, each of at least two blocks a wave.
+  const int64_t per_cu = p->waves == 0 ? 4 : p->waves == 2 ? 4 : p->waves == 4 ? 2 : 1;
+  const int64_t want = std::max<int64_t>(1, per_cu * cus / p->tile_items);
   const int64_t chunk = std::max<int64_t>(8, (blocks + want - 1) / want);
   p->splits = static_cast<int>((blocks + chunk - 1) / chunk);
   p->chunk = static_cast<int>(chunk);  // the last one goes on to the end of the sequence, whatever max_tokens says
-  p->part_bytes = p->splits > 1 ? static_cast<size_t>(p->splits) * p->tile_items * kKvRows * (p->kv.d + 2) * sizeof(float) : 0;
+  const int64_t items = p->tile_items * p->splits;
+  p->items = static_cast<uint32_t>(std::min<int64_t>(items, UINT32_MAX));  // too many for a launch: the caller refuses
+  p->part_bytes = p->splits > 1 ? static_cast<size_t>(items) * p->tile_rows * (p->kv.d + 2) * sizeof(float) : 0;
 }
 
 hipError_t launch_kv8_attention(const Kv8Attention &p, hipStream_t stream) {
-  if (p.kv.d == 128) return p.kv.fp8 ? launch_rows<128, true>(p, stream) : launch_rows<128, false>(p, stream);
-  return p.kv.fp8 ? launch_rows<64, true>(p, stream) : launch_rows<64, false>(p, stream);
+  if (p.kv.d == 128) return p.kv.fp8 ? launch_attend<128, true>(p, stream) : launch_attend<128, false>(p, stream);
+  return p.kv.fp8 ? launch_attend<64, true>(p, stream) : launch_attend<64, false>(p, stream);
 }
 
 hipError_t launch_kv8_append(const Kv8Append &p, hipStream_t stream) {
@@ -600,11 +889,11 @@ hipError_t launch_kv8_append(const Kv8Append &p, hipStream_t stream) {
 }
 
 hipError_t launch_kv8_copy(const Kv8Copy &p, hipStream_t stream) {
-  hipLaunchKernelGGL(kv8_copy_kernel, dim3(static_cast<unsigned>(p.layers * p.n * p.pieces)), dim3(256), kLdsToken,
+  hipLaunchKernelGGL(kv8_copy_kernel, dim3(static_cast<unsigned>(p.layers) * p.n * p.pieces), dim3(256), kLdsToken,
                      stream, p);
   return hipGetLastError();
 }
 
-int64_t kv8_copy_pieces(int64_t page_bytes) { return (page_bytes + kCopyBytes - 1) / kCopyBytes; }
+uint32_t kv8_copy_pieces(uint32_t page_bytes) { return (page_bytes + kCopyBytes - 1) / kCopyBytes; }
 
 }  // namespace ftx

@@ -1487,11 +1487,15 @@ int check_view(const void *ptr, const int64_t *stride, int64_t n0, int64_t n1, i
 }
 
 int plan_kv8(int64_t max_tokens, ftx::Kv8Attention *p) {
-  int cus = 256;
+  int cus = 256, xcds = 8;
   ftx::DeviceState *st = nullptr;
-  if (ftx::device_state(&st) == FTX_OK) cus = st->cu_count;
-  ftx::plan_kv8_attention(p, std::min<int64_t>(max_tokens, int64_t(1) << 30), cus);
-  if (p->tile_items > ftx::kMaxThreads / (256 * static_cast<int64_t>(p->splits)))
+  if (ftx::device_state(&st) == FTX_OK) {
+    cus = st->cu_count;
+    xcds = st->xcd_count;
+  }
+  ftx::plan_kv8_attention(p, std::min<int64_t>(max_tokens, int64_t(1) << 30), cus, xcds);
+  const int64_t join_rows = p->splits > 1 ? p->tile_items * p->tile_rows : 0;
+  if (static_cast<int64_t>(p->items) + p->xcds > ftx::kMaxThreads / 512 || join_rows > ftx::kMaxThreads / 32 - 256)
     return ftx::fail(FTX_ERR_UNSUPPORTED, "cache attention: more workgroups than one launch holds");
   return FTX_OK;
 }
@@ -1611,11 +1615,14 @@ int ftx_kv8_copy_pages(void *codes, float *scales, int64_t layers, int64_t pages
   for (int64_t i = 0; i < n; ++i)
     if (targets.count(src[i])) return ftx::fail(FTX_ERR_INVALID, "page copy: a page is read and written");
   ftx::Kv8Copy p;
-  p.page_scales = static_cast<int64_t>(2) * kv_heads * (page_tokens / ftx::kKvBlock);
-  p.page_bytes = p.page_scales * ftx::kKvBlock * d;
+  const int64_t page_scales = static_cast<int64_t>(2) * kv_heads * (page_tokens / ftx::kKvBlock);
+  const int64_t page_bytes = page_scales * ftx::kKvBlock * d;
+  if (page_bytes > int64_t(1) << 30) return ftx::fail(FTX_ERR_UNSUPPORTED, "page copy: a page of over 2^30 bytes");
+  p.page_scales = static_cast<uint32_t>(page_scales);
+  p.page_bytes = static_cast<uint32_t>(page_bytes);
   p.pieces = ftx::kv8_copy_pieces(p.page_bytes);
-  rc = check_operand(codes, layers * pages, p.page_bytes, "cache codes");
-  if (rc == FTX_OK) rc = check_operand(scales, layers * pages, p.page_scales * 4, "cache scales");
+  rc = check_operand(codes, layers * pages, page_bytes, "cache codes");
+  if (rc == FTX_OK) rc = check_operand(scales, layers * pages, page_scales * 4, "cache scales");
   if (rc != FTX_OK) return rc;
   // pairs of one launch: as many as travel as an argument, and as one launch has workgroups for
   const int64_t most = std::min<int64_t>(ftx::kKvCopyPairs, ftx::kMaxThreads / 256 / (layers * p.pieces));
@@ -1625,8 +1632,8 @@ int ftx_kv8_copy_pages(void *codes, float *scales, int64_t layers, int64_t pages
   p.layers = layers;
   p.pages = pages;
   for (int64_t i0 = 0; i0 < n; i0 += most) {
-    p.n = static_cast<int>(std::min(most, n - i0));
-    for (int i = 0; i < p.n; ++i) p.pair[i] = {src[i0 + i], dst[i0 + i]};
+    p.n = static_cast<uint32_t>(std::min(most, n - i0));
+    for (uint32_t i = 0; i < p.n; ++i) p.pair[i] = {src[i0 + i], dst[i0 + i]};
     FTX_HIP(ftx::launch_kv8_copy(p, static_cast<hipStream_t>(stream)));
   }
   return FTX_OK;
