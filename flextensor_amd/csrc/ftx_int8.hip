@@ -1,0 +1,410 @@
+// Matrix product of 8-bit integers with a scale for each token and each channel, written for gfx950.
+//
+//   y[m, n] = bf16(s_x[m] s_w[n] sum_k c[m, k] w[n, k]),   c = round(x / s_x),  s_x = max_k |x| / 127
+//
+// x is bf16 [M, K], w int8 [N, K] (-127 .. 127, K contiguous), s_w fp32 [N]. The sums are exact 32-bit integers
+// (K is at most 131072, so 127^2 K fits), whatever their order; the scales are applied in fp32 and the result is
+// rounded once.
+//
+// int8_quantize_kernel writes c into rows of a multiple of 256 bytes whose ends are 0. The products' loads then
+// need no care at the end of K: what they read of w past it, the start of the next row, meets zeros. Loads past the
+// last row come back as 0 from the buffer descriptor.
+#include <algorithm>
+#include <cfloat>
+
+#include "ftx_internal.h"
+
+namespace ftx {
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+
+constexpr int kWave = 64;
+constexpr float kTiny = 0x1p-100f;  // a scale below this counts as 0
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
+}
+__device__ __forceinline__ float bf16_value(uint32_t bits) { return __uint_as_float(bits << 16); }
+
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  static_assert(N < 64, "vmcnt holds six bits");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | ((N >> 4) << 14));
+}
+
+__device__ __forceinline__ void ring_barrier() {
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave's LDS reads are done
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// (min of 64-bit integers would go through doubles)
+__device__ __forceinline__ int64_t least(int64_t a, int64_t b) { return a < b ? a : b; }
+
+// A quotient or remainder of a workgroup's number, computed on the vector unit, as the scalar that it is.
+__device__ __forceinline__ int uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(static_cast<int>(v)); }
+
+// 16 bytes per lane from base + offset + step into lds + 16 * lane; zeros where that is not below `bytes`.
+__device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t bytes, uint32_t offset, uint32_t step,
+                                            uint8_t *lds) {
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, bytes, 0x00027000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *)lds, 16, offset, step, 0, 0);
+}
+
+// ---- codes and scales of the rows --------------------------------------------------------------------------------
+//
+// The largest magnitude's bits order as integers, and a NaN's are above all: a row that holds an infinity or a NaN
+// gets the scale NaN, and codes of 0. Each row is read twice, the second time from the caches.
+
+__device__ __forceinline__ uint32_t largest8(u32x4 v, uint32_t top) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = max(top, max(v[i] & 0x7fffu, v[i] >> 16 & 0x7fffu));
+  return top;
+}
+
+// The scale of a row whose largest magnitude has these bf16 bits, and what its values are multiplied by.
+__device__ __forceinline__ float row_scale(uint32_t top, float *inverse) {
+#pragma clang fp contract(off)
+  const float made = bf16_value(top) * (1.0f / 127.0f);
+  const float scale = made < kTiny ? 0.f : made;
+  *inverse = top >= 0x7f80u || scale == 0.f ? 0.f : 1.0f / scale;
+  return top >= 0x7f80u ? __uint_as_float(0x7fc00000u) : scale;
+}
+
+__device__ __forceinline__ uint32_t code2(uint32_t pair, float inverse) {
+#pragma clang fp contract(off)
+  const float lo = rintf(bf16_value(pair) * inverse), hi = rintf(__uint_as_float(pair & 0xffff0000u) * inverse);
+  const int a = static_cast<int>(fminf(fmaxf(lo, -127.f), 127.f)), b = static_cast<int>(fminf(fmaxf(hi, -127.f), 127.f));
+  return (static_cast<uint32_t>(a) & 255u) | (static_cast<uint32_t>(b) & 255u) << 8;
+}
+
+__device__ __forceinline__ u32x2 code8(u32x4 v, float inverse) {
+  return inverse == 0.f ? (u32x2){0u, 0u}  // an infinity times 0 is none
+                        : (u32x2){code2(v[0], inverse) | code2(v[1], inverse) << 16,
+                                  code2(v[2], inverse) | code2(v[3], inverse) << 16};
+}
+
+__global__ __launch_bounds__(256) void int8_quantize_kernel(const uint16_t *__restrict__ x, int64_t x_stride,
+                                                            uint8_t *__restrict__ codes, int64_t code_stride,
+                                                            float *__restrict__ scales, int k) {
+  __shared__ uint32_t wave_top[4];
+  const int64_t row = blockIdx.x;
+  const u32x4 *xr = reinterpret_cast<const u32x4 *>(x + row * x_stride);
+  const int n = k / 8;
+  uint32_t top = 0;
+  for (int i = threadIdx.x; i < n; i += 256) top = largest8(xr[i], top);
+#pragma unroll
+  for (int i = 1; i < kWave; i *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), i)));
+  if (threadIdx.x % kWave == 0) wave_top[threadIdx.x / kWave] = top;
+  __syncthreads();
+  top = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
+  float inverse;
+  const float scale = row_scale(top, &inverse);
+  u32x2 *to = reinterpret_cast<u32x2 *>(codes + row * code_stride);
+  for (int i = threadIdx.x; i < code_stride / 8; i += 256) to[i] = i < n ? code8(xr[i], inverse) : (u32x2){0u, 0u};
+  if (threadIdx.x == 0) scales[row] = scale;
+}
+
+// ---- up to 16 rows -------------------------------------------------------------------------------------------------
+//
+// A workgroup owns 16 channels over the whole of K; its eight waves take windows of 256 bytes of every row in turn,
+// straight into registers as the operands of v_mfma_i32_16x16x64_i8 (lane (r, g): 16 bytes of row r), three windows
+// in flight, and their sums meet in LDS. Bound by the bytes of w.
+
+constexpr int kWindow = 256;
+
+__global__ __launch_bounds__(512, 4) void int8_rows_kernel(Int8Linear p) {
+  __shared__ i32x4 part[8][kWave];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int r = lane & 15, g = lane >> 4;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
+  const int rows = static_cast<int>(least(16, p.n - n0));
+  const auto w = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p.w + n0 * p.k), 0, rows * p.k, 0x00027000);
+  const auto c = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p.codes), 0, p.m * p.code_stride, 0x00027000);
+  const uint32_t w_at = r * p.k + 16 * g, c_at = r * p.code_stride + 16 * g;
+  struct Window {
+    u32x4 w[4], c[4];
+  };
+  const auto load = [&](Window &x, int window) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x.w[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(w, w_at, window * kWindow + 64 * i, 0));
+      x.c[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(c, c_at, window * kWindow + 64 * i, 0));
+    }
+  };
+  i32x4 acc = {0, 0, 0, 0};
+  const auto work = [&](const Window &x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, x.w[i]), __builtin_bit_cast(i32x4, x.c[i]), acc, 0, 0, 0);
+  };
+  const int windows = p.code_stride / kWindow, last = windows - 1;
+  if (wave < windows) {
+    Window x, y, z;
+    int i = wave;
+    load(x, i);
+    load(y, min(i + 8, last));
+    for (;;) {  // loads past the end take the last window again
+      load(z, min(i + 16, last));
+      work(x);
+      if ((i += 8) >= windows) break;
+      load(x, min(i + 16, last));
+      work(y);
+      if ((i += 8) >= windows) break;
+      load(y, min(i + 16, last));
+      work(z);
+      if ((i += 8) >= windows) break;
+    }
+  }
+  part[wave][lane] = acc;
+  __syncthreads();
+  // thread: token t, channel c; lane t + 16 g of each wave holds channels 4 g .. 4 g + 3
+  const int t = threadIdx.x / 16, ch = threadIdx.x % 16;
+  if (t >= p.m || ch >= rows) return;
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum += part[i][t + 16 * (ch / 4)][ch % 4];
+  const float y = static_cast<float>(sum) * p.x_scale[t] * p.w_scale[n0 + ch];
+  p.y[t * p.n + n0 + ch] = static_cast<uint16_t>(pack_bf16(y, 0.f));
+}
+
+// ---- tiles -----------------------------------------------------------------------------------------------------------
+//
+// TM tokens x TN channels a workgroup, K in steps of 128. A step's rows go straight from memory into one of two
+// stages of LDS; row R's 16-byte chunk c lies at slot c ^ (R / 2 % 8), which spreads the 16 rows that a phase of
+// ds_read_b128 touches over all banks. The next step's loads are in flight during a step's products.
+// v_mfma_i32_32x32x32_i8 takes the channels as rows and the tokens as columns, so a lane ends with four neighbouring
+// channels of a token at a time; they reach y through LDS, in whole lines.
+
+template <int TM, int TN, int WM, int WN, bool SPLIT>
+__global__ __launch_bounds__(WM * WN * kWave, 2) void int8_tile_kernel(Int8Linear p) {
+  constexpr int kWaves = WM * WN;
+  constexpr int kStep = 128;
+  constexpr int kStage = (TM + TN) * kStep;
+  constexpr int kLoads = kStage / 1024 / kWaves;   // of one wave
+  constexpr int kMT = TM / WM / 32, kNT = TN / WN / 32;
+  constexpr int kTokenLoads = TM / 8 / kWaves;     // the first of them
+  static_assert(kStage / 1024 % kWaves == 0 && TM / 8 % kWaves == 0, "every wave issues the same loads");
+  __shared__ __align__(1024) uint8_t lds[2 * kStage];
+  const uint32_t per_xcd = (p.items + p.xcds - 1) / p.xcds;
+  uint32_t item = (blockIdx.x % p.xcds) * per_xcd + blockIdx.x / p.xcds;
+  if (blockIdx.x / p.xcds >= per_xcd || item >= p.items) return;
+  const int split = SPLIT ? uniform(item % static_cast<uint32_t>(p.splits)) : 0;
+  if (SPLIT) item /= static_cast<uint32_t>(p.splits);
+  const uint32_t run = item / (p.band * p.n_tiles), at = item - run * p.band * p.n_tiles;
+  const uint32_t rows = min(static_cast<uint32_t>(p.band), p.m_tiles - run * p.band);
+  const int64_t m0 = static_cast<int64_t>(uniform(run * p.band + at % rows)) * TM;
+  const int64_t n0 = static_cast<int64_t>(uniform(at / rows)) * TN;
+
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int r = lane & 31, g = lane >> 5;
+  const int wm = wave / WN, wn = wave % WN;
+  // Load i of a wave brings rows 8 (i kWaves + wave) .. + 7 of 128 bytes, the tokens' first, then the channels'.
+  const uint8_t *tokens = p.codes + m0 * p.code_stride, *channels = p.w + n0 * p.k;
+  const uint32_t token_bytes = static_cast<uint32_t>(least((p.m - m0) * p.code_stride, 0x7fffffff));
+  const uint32_t channel_bytes = static_cast<uint32_t>(least((p.n - n0) * p.k, 0x7fffffff));
+  uint32_t offset[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int R = (i * kWaves + wave) * 8 + lane / 8 - (i < kTokenLoads ? 0 : TM);
+    offset[i] = R * (i < kTokenLoads ? p.code_stride : p.k) + ((lane % 8) ^ (R / 2 % 8)) * 16;
+  }
+  const auto issue = [&](int step) {
+    uint8_t *base = lds + (step & 1) * kStage + wave * 1024;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      load_to_lds(i < kTokenLoads ? tokens : channels, i < kTokenLoads ? token_bytes : channel_bytes, offset[i],
+                  step * kStep, base + i * kWaves * 1024);
+  };
+  uint32_t a_at[kNT], b_at[kMT];
+#pragma unroll
+  for (int i = 0; i < kNT; ++i) a_at[i] = TM * kStep + (wn * kNT * 32 + i * 32 + r) * kStep;
+#pragma unroll
+  for (int j = 0; j < kMT; ++j) b_at[j] = (wm * kMT * 32 + j * 32 + r) * kStep;
+  const uint32_t swizzle = r / 2 % 8;
+
+  i32x16 acc[kNT][kMT];
+#pragma unroll
+  for (int i = 0; i < kNT; ++i)
+#pragma unroll
+    for (int j = 0; j < kMT; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+
+  const int all = (p.k + kStep - 1) / kStep;
+  const int first = SPLIT ? split * p.split_steps : 0;
+  const int end = SPLIT ? min(all, first + p.split_steps) : all;
+  issue(first);
+  for (int step = first; step < end; ++step) {
+    wait_vmcnt<0>();
+    ring_barrier();
+    if (step + 1 < end) issue(step + 1);
+    const uint8_t *stage = lds + (step & 1) * kStage;
+    // the operands of the next 32 of K are read during this one's products
+    i32x4 a[2][kNT], b[2][kMT];
+    const auto read = [&](int ks) {
+      const uint32_t chunk = ((2 * ks + g) ^ swizzle) * 16;
+#pragma unroll
+      for (int i = 0; i < kNT; ++i) a[ks & 1][i] = *reinterpret_cast<const i32x4 *>(stage + a_at[i] + chunk);
+#pragma unroll
+      for (int j = 0; j < kMT; ++j) b[ks & 1][j] = *reinterpret_cast<const i32x4 *>(stage + b_at[j] + chunk);
+    };
+    read(0);
+#pragma unroll
+    for (int ks = 0; ks < kStep / 32; ++ks) {
+      if (ks + 1 < kStep / 32) read(ks + 1);
+#pragma unroll
+      for (int j = 0; j < kMT; ++j)
+#pragma unroll
+        for (int i = 0; i < kNT; ++i)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[ks & 1][i], b[ks & 1][j], acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  if (SPLIT) {  // integer sums [split][m][n]
+#pragma unroll
+    for (int j = 0; j < kMT; ++j) {
+      const int64_t t = m0 + wm * kMT * 32 + j * 32 + r;
+      if (t >= p.m) continue;
+#pragma unroll
+      for (int i = 0; i < kNT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int64_t ch = n0 + wn * kNT * 32 + i * 32 + 8 * q + 4 * g;
+          int *to = p.part + (split * p.m + t) * p.part_stride + ch;
+          if (ch < p.part_stride)
+            *reinterpret_cast<i32x4 *>(to) = (i32x4){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        }
+    }
+    return;
+  }
+  // 32 tokens x the wave's channels at a time through this wave's part of LDS, 16 bytes between rows against conflicts
+  constexpr int kPitch = kNT * 64 + 16;
+  static_assert(32 * kPitch * kWaves <= 2 * kStage, "the epilogue fits the stages");
+  __syncthreads();  // the last step has been read
+  uint8_t *mine = lds + wave * 32 * kPitch;
+#pragma unroll
+  for (int j = 0; j < kMT; ++j) {
+    const int64_t t0 = m0 + wm * kMT * 32 + j * 32;
+    const int64_t c0 = n0 + wn * kNT * 32;
+    const float x_scale = t0 + r < p.m ? p.x_scale[t0 + r] : 0.f;
+#pragma unroll
+    for (int i = 0; i < kNT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int64_t ch = c0 + i * 32 + 8 * q + 4 * g + e;
+          y[e] = static_cast<float>(acc[i][j][4 * q + e]) * x_scale * (ch < p.n ? p.w_scale[ch] : 0.f);
+        }
+        *reinterpret_cast<u32x2 *>(mine + r * kPitch + (i * 32 + 8 * q + 4 * g) * 2) =
+            (u32x2){pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
+      }
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    constexpr int kLanes = kNT * 4;  // 16 bytes each, of one token
+#pragma unroll
+    for (int i = 0; i < 32 * kLanes / kWave; ++i) {
+      const int row = i * (kWave / kLanes) + lane / kLanes, col = lane % kLanes;
+      const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + row * kPitch + col * 16);
+      if (t0 + row >= p.m) continue;
+      uint16_t *to = p.y + (t0 + row) * p.n + c0 + col * 8;
+      if (c0 + col * 8 + 8 <= p.n && p.n % 8 == 0) {
+        *reinterpret_cast<u32x4 *>(to) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c0 + col * 8 + e < p.n) to[e] = static_cast<uint16_t>(v[e / 2] >> (16 * (e & 1)));
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+  }
+}
+
+// y = bf16(s_x s_w sum over the splits), four channels a thread.
+__global__ __launch_bounds__(256) void int8_join_kernel(Int8Linear p) {
+  const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  const int64_t size = p.m * p.part_stride;
+  if (at >= size) return;
+  const int64_t t = at / p.part_stride, ch = at % p.part_stride;
+  i32x4 sum = {0, 0, 0, 0};
+  for (int i = 0; i < p.splits; ++i) sum += *reinterpret_cast<const i32x4 *>(p.part + i * size + at);
+  const float x_scale = p.x_scale[t];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (ch + e < p.n)
+      p.y[t * p.n + ch + e] = static_cast<uint16_t>(pack_bf16(static_cast<float>(sum[e]) * x_scale * p.w_scale[ch + e], 0.f));
+}
+
+template <int TM, int TN, int WM, int WN>
+void start_tiles(const Int8Linear &p, hipStream_t stream) {
+  const dim3 grid((p.items + p.xcds - 1) / p.xcds * p.xcds), block(WM * WN * kWave);
+  if (p.splits > 1) hipLaunchKernelGGL((int8_tile_kernel<TM, TN, WM, WN, true>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((int8_tile_kernel<TM, TN, WM, WN, false>), grid, block, 0, stream, p);
+}
+
+}  // namespace
+
+hipError_t launch_int8_quantize(const uint16_t *x, int64_t x_stride, uint8_t *codes, int64_t code_stride, float *scales,
+                                int64_t m, int k, hipStream_t stream) {
+  hipLaunchKernelGGL(int8_quantize_kernel, dim3(static_cast<unsigned>(m)), dim3(256), kLdsToken, stream, x, x_stride,
+                     codes, code_stride, scales, k);
+  return hipGetLastError();
+}
+
+void plan_int8_linear(Int8Linear *p, int cus, int xcds) {
+  p->xcds = std::max(1, xcds);
+  p->splits = 1;
+  p->split_steps = 0;
+  p->part_stride = (p->n + 3) / 4 * 4;
+  p->band = 8;
+  if (p->m <= 16) {
+    p->tile_m = 16;
+    p->items = static_cast<uint32_t>((p->n + 15) / 16);
+    p->part_bytes = 0;
+    return;
+  }
+  const auto tiles = [&](int64_t tm, int64_t tn) { return ((p->m + tm - 1) / tm) * ((p->n + tn - 1) / tn); };
+  p->tile_m = p->m > 128 && tiles(256, 256) >= cus ? 256 : p->m > 64 ? 128 : 64;
+  p->tile_n = p->tile_m == 256 ? 256 : 128;
+  p->m_tiles = static_cast<uint32_t>((p->m + p->tile_m - 1) / p->tile_m);
+  p->n_tiles = static_cast<uint32_t>((p->n + p->tile_n - 1) / p->tile_n);
+  const int64_t count = static_cast<int64_t>(p->m_tiles) * p->n_tiles;
+  const int steps = (p->k + 127) / 128;
+  const int64_t want = std::min<int64_t>(p->tile_m == 256 ? 1 : std::max<int64_t>(1, 2 * cus / count), (steps + 7) / 8);
+  p->split_steps = static_cast<int>((steps + want - 1) / want);
+  p->splits = (steps + p->split_steps - 1) / p->split_steps;
+  p->items = static_cast<uint32_t>(std::min<int64_t>(count * p->splits, UINT32_MAX));
+  p->part_bytes = p->splits > 1 ? static_cast<size_t>(p->splits) * p->m * p->part_stride * 4 : 0;
+}
+
+hipError_t launch_int8_linear(const Int8Linear &p, hipStream_t stream) {
+  switch (p.tile_m) {
+    case 16: hipLaunchKernelGGL(int8_rows_kernel, dim3(p.items), dim3(512), 0, stream, p); break;
+    case 64: start_tiles<64, 128, 1, 4>(p, stream); break;
+    case 128: start_tiles<128, 128, 2, 2>(p, stream); break;
+    default: start_tiles<256, 256, 2, 4>(p, stream); break;
+  }
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess || p.splits == 1) return err;
+  const int64_t threads = p.m * p.part_stride / 4;
+  hipLaunchKernelGGL(int8_join_kernel, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), kLdsToken, stream,
+                     p);
+  return hipGetLastError();
+}
+
+}  // namespace ftx

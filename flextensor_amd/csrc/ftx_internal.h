@@ -232,6 +232,28 @@ struct Kv8Copy {
 uint32_t kv8_copy_pieces(uint32_t page_bytes);
 hipError_t launch_kv8_copy(const Kv8Copy &p, hipStream_t stream);
 
+// The matrix product of 8-bit integers (ftx_int8.hip).
+constexpr int64_t kInt8MaxK = 131072;  // 127^2 K fits 32-bit sums
+constexpr int64_t int8_code_stride(int64_t k) { return (k + 255) / 256 * 256; }  // bytes of a row of codes
+struct Int8Linear {
+  const uint8_t *codes;   // [m][code_stride], 0 from k on
+  const float *x_scale;   // [m]
+  const uint8_t *w;       // [n][k]
+  const float *w_scale;   // [n]
+  uint16_t *y;            // bf16 [m][n]
+  int *part;              // [splits][m][part_stride] sums, when splits > 1
+  int64_t m, n, part_stride;
+  int k, code_stride;
+  // planned
+  int tile_m, tile_n, splits, split_steps, band, xcds;  // tile_m 16: the kernel of up to 16 rows
+  uint32_t m_tiles, n_tiles, items;
+  size_t part_bytes;
+};
+void plan_int8_linear(Int8Linear *p, int cus, int xcds);
+hipError_t launch_int8_linear(const Int8Linear &p, hipStream_t stream);
+hipError_t launch_int8_quantize(const uint16_t *x, int64_t x_stride, uint8_t *codes, int64_t code_stride, float *scales,
+                                int64_t m, int k, hipStream_t stream);
+
 // Staged copies from pageable host memory and the parallel host memcpy
 // (ftx_staged.hip).
 int staged_copy_h2d(void *dst, const void *src, size_t nbytes, hipStream_t stream);

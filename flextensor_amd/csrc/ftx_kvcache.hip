@@ -47,6 +47,12 @@ __device__ __forceinline__ Span span_of(const KvPages &c, int64_t b, int t) {
   return {start, max(0, min(count, capacity - start))};
 }
 
+// (min of 64-bit integers would go through doubles)
+__device__ __forceinline__ int64_t least(int64_t a, int64_t b) { return a < b ? a : b; }
+
+// A quotient or remainder of a workgroup's number, computed on the vector unit, as the scalar that it is.
+__device__ __forceinline__ int uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(static_cast<int>(v)); }
+
 // The page that holds a block of sequence b, or -1.
 __device__ __forceinline__ int page_of(const KvPages &c, int64_t b, int block) {
   const int page = c.table[b * c.table_stride + (block >> c.page_shift)];
@@ -135,13 +141,13 @@ __global__ __launch_bounds__(256, 3) void kv8_rows_kernel(Kv8Attention a) {
   __shared__ float part_m[kWaves][kKvRows], part_l[kWaves][kKvRows];
 
   uint32_t item = blockIdx.x;  // 32-bit divisions: a launch has fewer than 2^24 workgroups
-  const int split = static_cast<int>(item % static_cast<uint32_t>(a.splits));
-  item /= static_cast<uint32_t>(a.splits);
+  const int split = uniform(item % static_cast<uint32_t>(a.splits));
+  item = uniform(item / static_cast<uint32_t>(a.splits));
   const int64_t tile_item = item;
-  const int tile = static_cast<int>(item % static_cast<uint32_t>(a.row_tiles));
+  const int tile = uniform(item % static_cast<uint32_t>(a.row_tiles));
   item /= static_cast<uint32_t>(a.row_tiles);
-  const int kvh = static_cast<int>(item % static_cast<uint32_t>(a.kv.kv_heads));
-  const int64_t b = item / static_cast<uint32_t>(a.kv.kv_heads);
+  const int kvh = uniform(item % static_cast<uint32_t>(a.kv.kv_heads));
+  const int64_t b = uniform(item / static_cast<uint32_t>(a.kv.kv_heads));
   const Span span = span_of(a.kv, b, a.t);
   const int blocks = tile_blocks(a, span, tile);
   const int first = split * a.chunk;
@@ -332,7 +338,7 @@ __global__ __launch_bounds__(256, 3) void kv8_rows_kernel(Kv8Attention a) {
 // S^T = K Q^T gives a lane 16 of a block's 32 scores of one row, keys 8 a + 4 g + c (g the half of the wave); V's
 // operands are written in that order.
 template <int D, bool FP8, int NW, bool SPLIT>
-__global__ __launch_bounds__(NW * kWave, 2) void kv8_tile_kernel(Kv8Attention a) {
+__global__ __launch_bounds__(NW * kWave, D == 128 && NW == 2 ? 1 : 2) void kv8_tile_kernel(Kv8Attention a) {
   constexpr int kThreads = NW * kWave;
   constexpr int kKeys = 64, kSub = 2;
   constexpr int kBlockBytes = kKvBlock * D;          // codes of a block's side
@@ -347,13 +353,13 @@ __global__ __launch_bounds__(NW * kWave, 2) void kv8_tile_kernel(Kv8Attention a)
   const uint32_t per_xcd = (a.items + a.xcds - 1) / a.xcds;
   uint32_t item = (blockIdx.x % a.xcds) * per_xcd + blockIdx.x / a.xcds;
   if (item >= a.items) return;
-  const int split = SPLIT ? static_cast<int>(item % static_cast<uint32_t>(a.splits)) : 0;
+  const int split = SPLIT ? uniform(item % static_cast<uint32_t>(a.splits)) : 0;
   if (SPLIT) item /= static_cast<uint32_t>(a.splits);
-  const uint32_t bkv = item / static_cast<uint32_t>(a.row_tiles);
-  const int tile = a.row_tiles - 1 - static_cast<int>(item - bkv * a.row_tiles);  // the longest first
+  const uint32_t bkv = uniform(item / static_cast<uint32_t>(a.row_tiles));
+  const int tile = uniform(a.row_tiles - 1 - (item - bkv * a.row_tiles));  // the longest first
   const int64_t tile_item = static_cast<int64_t>(bkv) * a.row_tiles + tile;
-  const int64_t b = bkv / static_cast<uint32_t>(a.kv.kv_heads);
-  const int kvh = static_cast<int>(bkv % static_cast<uint32_t>(a.kv.kv_heads));
+  const int64_t b = uniform(bkv / static_cast<uint32_t>(a.kv.kv_heads));
+  const int kvh = uniform(bkv % static_cast<uint32_t>(a.kv.kv_heads));
   const Span span = span_of(a.kv, b, a.t);
   const int blocks = tile_blocks(a, span, tile);
   const int first = SPLIT ? split * a.chunk : 0;
@@ -727,12 +733,12 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
   uint32_t rest = blockIdx.x;
   const int side = static_cast<int>(rest & 1);
   rest >>= 1;
-  const int head = static_cast<int>(rest % static_cast<uint32_t>(a.kv.kv_heads));
+  const int head = uniform(rest % static_cast<uint32_t>(a.kv.kv_heads));
   rest /= static_cast<uint32_t>(a.kv.kv_heads);
-  const int nth = static_cast<int>(rest % static_cast<uint32_t>(a.seq_blocks));
-  const int64_t b = rest / static_cast<uint32_t>(a.seq_blocks);
+  const int nth = uniform(rest % static_cast<uint32_t>(a.seq_blocks));
+  const int64_t b = uniform(rest / static_cast<uint32_t>(a.seq_blocks));
   Span span = span_of(a.kv, b, a.t);
-  span.count = static_cast<int>(min<int64_t>(span.count, max<int64_t>(0, a.positions - span.start)));
+  span.count = static_cast<int>(least(span.count, a.positions > span.start ? a.positions - span.start : 0));
   const int block = span.start / kKvBlock + nth;
   const int lo = max(span.start, block * kKvBlock);  // the new tokens of this block: lo .. hi - 1
   const int hi = min(span.start + span.count, (block + 1) * kKvBlock);
@@ -819,10 +825,10 @@ constexpr int kCopyBytes = 32 * 1024;  // of one workgroup: eight 16-byte loads 
 __global__ __launch_bounds__(256) void kv8_copy_kernel(Kv8Copy) {
   const auto &a = *(const __attribute__((address_space(4))) Kv8Copy *)__builtin_amdgcn_kernarg_segment_ptr();
   uint32_t item = blockIdx.x;
-  const uint32_t piece = item % a.pieces;
+  const uint32_t piece = uniform(item % a.pieces);
   item /= a.pieces;
-  const uint32_t pair = item % a.n;
-  const int64_t layer = item / a.n;
+  const uint32_t pair = uniform(item % a.n);
+  const int64_t layer = uniform(item / a.n);
   const int64_t from = layer * a.pages + a.pair[pair].src, to = layer * a.pages + a.pair[pair].dst;
   const uint32_t bytes = a.page_bytes, at = piece * kCopyBytes;
   const u32x4 *src = reinterpret_cast<const u32x4 *>(a.codes + from * bytes + at) + threadIdx.x;

@@ -1639,6 +1639,96 @@ int ftx_kv8_copy_pages(void *codes, float *scales, int64_t layers, int64_t pages
   return FTX_OK;
 }
 
+namespace {
+
+int check_int8(int64_t m, int64_t n, int64_t k) {
+  if (m < 0 || n < 0 || k < 0) return ftx::fail(FTX_ERR_INVALID, "negative dimension");
+  if (k % 16 != 0) return ftx::fail(FTX_ERR_UNSUPPORTED, "the int8 linear needs k to be a multiple of 16");
+  if (k > ftx::kInt8MaxK)
+    return ftx::fail(FTX_ERR_UNSUPPORTED, "the int8 linear's 32-bit sums hold up to " + std::to_string(ftx::kInt8MaxK) +
+                                              " values of k");
+  if (m > (int64_t(1) << 24) - 1 || n > (int64_t(1) << 24))
+    return ftx::fail(FTX_ERR_INVALID, "linear dimensions too large");
+  return FTX_OK;
+}
+
+int plan_int8(int64_t m, int64_t n, int64_t k, ftx::Int8Linear *p) {
+  int rc = check_int8(m, n, k);
+  if (rc != FTX_OK) return rc;
+  p->m = m;
+  p->n = n;
+  p->k = static_cast<int>(k);
+  p->code_stride = static_cast<int>(ftx::int8_code_stride(k));
+  if (m == 0 || n == 0) return FTX_OK;
+  int cus = 256, xcds = 8;
+  ftx::DeviceState *st = nullptr;
+  if (ftx::device_state(&st) == FTX_OK) {
+    cus = st->cu_count;
+    xcds = st->xcd_count;
+  }
+  ftx::plan_int8_linear(p, cus, xcds);
+  if (static_cast<int64_t>(p->items) + p->xcds > ftx::kMaxThreads / 512 ||
+      (p->splits > 1 && m * p->part_stride > (int64_t(1) << 33)))
+    return ftx::fail(FTX_ERR_UNSUPPORTED, "int8 linear: more workgroups than one launch holds");
+  return FTX_OK;
+}
+
+}  // namespace
+
+int ftx_int8_quantize(const void *x, int64_t x_stride, void *codes, float *scales, int64_t m, int64_t k, void *stream) {
+  FTX_REQUIRE_LIVE();
+  int rc = check_int8(m, 0, k);
+  if (rc != FTX_OK) return rc;
+  if (x_stride < k || x_stride % 8 != 0 || x_stride > int64_t(1) << 38)
+    return ftx::fail(FTX_ERR_INVALID, "int8 quantize: rows of x must not overlap and start at multiples of 8 elements");
+  if (m == 0) return FTX_OK;
+  if (k > 0) rc = check_operand(x, (m - 1) * x_stride + k, 2, "int8 input");
+  if (rc == FTX_OK && k > 0) rc = check_operand(codes, m * ftx::int8_code_stride(k), 1, "int8 codes");
+  if (rc == FTX_OK) rc = check_operand(scales, m, 4, "int8 row scales");
+  if (rc != FTX_OK) return rc;
+  FTX_HIP(ftx::launch_int8_quantize(static_cast<const uint16_t *>(x), x_stride, static_cast<uint8_t *>(codes),
+                                    ftx::int8_code_stride(k), scales, m, static_cast<int>(k),
+                                    static_cast<hipStream_t>(stream)));
+  return FTX_OK;
+}
+
+int ftx_int8_matmul_workspace(int64_t m, int64_t n, int64_t k, size_t *bytes) {
+  if (!bytes) return ftx::fail(FTX_ERR_INVALID, "bytes is null");
+  ftx::Int8Linear p{};
+  int rc = plan_int8(m, n, k, &p);
+  if (rc == FTX_OK) *bytes = p.part_bytes;
+  return rc;
+}
+
+int ftx_int8_matmul(const void *codes, const float *x_scale, const void *w, const float *w_scale, void *y, int64_t m,
+                    int64_t n, int64_t k, void *workspace, size_t workspace_bytes, void *stream) {
+  FTX_REQUIRE_LIVE();
+  ftx::Int8Linear p{};
+  int rc = plan_int8(m, n, k, &p);
+  if (rc != FTX_OK) return rc;
+  if (m == 0 || n == 0) return FTX_OK;
+  if (k > 0) rc = check_operand(codes, m * p.code_stride, 1, "int8 codes");
+  if (rc == FTX_OK && k > 0) rc = check_operand(w, n * k, 1, "int8 weight");
+  if (rc == FTX_OK) rc = check_operand(x_scale, m, 4, "int8 row scales");
+  if (rc == FTX_OK) rc = check_operand(w_scale, n, 4, "int8 channel scales");
+  if (rc == FTX_OK) rc = check_operand(y, m * n, 2, "int8 output");
+  if (rc == FTX_OK && p.part_bytes > 0) {
+    if (workspace_bytes < p.part_bytes)
+      return ftx::fail(FTX_ERR_INVALID, "the int8 linear needs a workspace of " + std::to_string(p.part_bytes) +
+                                            " bytes (ftx_int8_matmul_workspace)");
+    rc = check_operand(workspace, static_cast<int64_t>(p.part_bytes), 1, "int8 workspace");
+  }
+  if (rc != FTX_OK) return rc;
+  p.codes = static_cast<const uint8_t *>(codes);
+  p.x_scale = x_scale;
+  p.w = static_cast<const uint8_t *>(w);
+  p.w_scale = w_scale;
+  p.y = static_cast<uint16_t *>(y);
+  p.part = static_cast<int *>(workspace);
+  FTX_HIP(ftx::launch_int8_linear(p, static_cast<hipStream_t>(stream)));
+  return FTX_OK;
+}
+
 int ftx_scatter_plan_create(const ftx_desc *descs, int n_desc, size_t tile_bytes, ftx_scatter_plan **plan) {
   FTX_REQUIRE_LIVE();
   if (!plan) return ftx::fail(FTX_ERR_INVALID, "plan is null");

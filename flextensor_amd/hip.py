@@ -773,6 +773,93 @@ def fp8_linear_residual(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tens
     return _fp8_fused(x, [weight], [scale], nat.FP8_EPILOGUE_RESIDUAL, residual, "fp8_linear_residual")
 
 
+INT8_LINEAR_MAX_K = 131072  # the 32-bit sums hold 127^2 times this
+_INT8_WORKSPACE: dict[tuple, int] = {}
+
+
+def int8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(codes, scales)`` of bf16 rows [m, k]: ``codes = round(x / s)`` with a row's ``s = max |x| / 127``
+    (``ftx_int8_quantize``).
+
+    The codes' rows are ``k`` rounded up to a multiple of 256 long and end in zeros, the layout that
+    :func:`int8_matmul` reads. A row that holds an infinity or a NaN has the scale NaN. ``k`` is a multiple of 16;
+    rows may be strided.
+    """
+    if x.dim() != 2:
+        raise ValueError(f"int8_quantize takes rows [m, k], got {tuple(x.shape)}")
+    _check_operands("int8_quantize", x=x)
+    m, k = x.shape
+    if k % 16 or k > INT8_LINEAR_MAX_K:
+        raise ValueError(f"int8_quantize needs k a multiple of 16, up to {INT8_LINEAR_MAX_K}, not {k}")
+    stride = x.stride(0) if m > 1 else k
+    if x.stride(1) != 1 or stride < k or stride % 8 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        stride = k
+    codes = torch.empty((m, (k + 255) // 256 * 256), dtype=torch.int8, device=x.device)
+    scales = torch.empty(m, dtype=torch.float32, device=x.device)
+    nat.call("ftx_int8_quantize", x.data_ptr(), stride, codes.data_ptr(), scales.data_ptr(), m, k, _stream())
+    return codes, scales
+
+
+def _check_int8_weight(what: str, weight: torch.Tensor, scale: torch.Tensor, k: int, device: torch.device) -> int:
+    if weight.dtype != torch.int8 or scale.dtype != torch.float32:
+        raise TypeError(f"{what} needs an int8 weight and an fp32 scale, got {weight.dtype} and {scale.dtype}")
+    if weight.dim() != 2 or weight.shape[1] != k or scale.shape != weight.shape[:1]:
+        raise ValueError(f"{what} shape mismatch: weight {tuple(weight.shape)}, scale {tuple(scale.shape)}, k {k}")
+    if weight.device != device or scale.device != device:
+        raise ValueError(f"{what} needs weight and scale on {device}")
+    if not _packed(weight, scale):
+        raise ValueError(f"{what} needs a contiguous, 16-byte aligned weight and scale")
+    return weight.shape[0]
+
+
+def int8_matmul(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """``bf16((codes @ weight.T) * scales[:, None] * scale)`` of what :func:`int8_quantize` returns
+    (``ftx_int8_matmul``): several weights [n, k] that share an input quantise it once. ``weight``: int8, -127 ..
+    127; ``scale``: fp32 [n]. The sums are exact integers; each output is rounded once."""
+    if weight.dim() != 2:
+        raise ValueError(f"int8_matmul takes a weight [n, k], got {tuple(weight.shape)}")
+    k = weight.shape[1]
+    if codes.dtype != torch.int8 or scales.dtype != torch.float32:
+        raise TypeError(f"int8_matmul takes int8 codes and fp32 scales, got {codes.dtype} and {scales.dtype}")
+    if k % 16 or k > INT8_LINEAR_MAX_K or codes.dim() != 2 or codes.shape[1] != (k + 255) // 256 * 256 or \
+            scales.shape != codes.shape[:1]:
+        raise ValueError(f"int8_matmul takes the codes and scales of int8_quantize for k = {k}, got "
+                         f"{tuple(codes.shape)} and {tuple(scales.shape)}")
+    if not codes.is_cuda or codes.get_device() != torch._C._cuda_getDevice() or scales.device != codes.device:
+        raise ValueError(f"int8_matmul runs on the current GPU, its input is on {codes.device} and {scales.device}")
+    if not _packed(codes, scales):
+        raise ValueError("int8_matmul needs contiguous, 16-byte aligned codes and scales")
+    n = _check_int8_weight("int8_matmul", weight, scale, k, codes.device)
+    return _int8_matmul(codes, scales, weight, scale, codes.shape[0], n, k)
+
+
+def _int8_matmul(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, m: int, n: int,
+                 k: int) -> torch.Tensor:
+    y = torch.empty((m, n), dtype=torch.bfloat16, device=codes.device)
+    ws_bytes = _INT8_WORKSPACE.get((m, n, k))
+    if ws_bytes is None:
+        got = ctypes.c_size_t(0)
+        nat.call("ftx_int8_matmul_workspace", m, n, k, ctypes.byref(got))
+        if len(_INT8_WORKSPACE) >= 4096:
+            _INT8_WORKSPACE.clear()
+        ws_bytes = _INT8_WORKSPACE[m, n, k] = int(got.value)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=codes.device) if ws_bytes else None
+    nat.call("ftx_int8_matmul", codes.data_ptr(), scales.data_ptr(), weight.data_ptr(), scale.data_ptr(), y.data_ptr(),
+             m, n, k, ws.data_ptr() if ws is not None else None, ws_bytes, _stream())
+    return y
+
+
+def int8_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """``x @ (weight * scale[:, None]).T`` with ``x`` rounded to 8 bits, a scale for each row: :func:`int8_quantize`,
+    then :func:`int8_matmul`. ``x``: bf16 [m, k], ``weight``: int8 [n, k], ``scale``: fp32 [n]; no backward."""
+    if x.dim() != 2:
+        raise ValueError(f"int8_linear takes x [m, k], got {tuple(x.shape)}")
+    n = _check_int8_weight("int8_linear", weight, scale, x.shape[1], x.device)
+    codes, scales = int8_quantize(x)
+    return _int8_matmul(codes, scales, weight, scale, x.shape[0], n, x.shape[1])
+
+
 BF16_LINEAR_MAX_ROWS = 16
 
 

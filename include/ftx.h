@@ -405,6 +405,23 @@ int ftx_rope_cache(const void *q, const void *k, const void *v, const void *cos,
 /* y = bf16(bf16(silu(g)) * u) over n values (a multiple of 8). */
 int ftx_silu_mul(const void *g, const void *u, void *y, int64_t n, void *stream);
 
+/* ---- matrix product of 8-bit integers ---------------------------------------
+ * No reference counterpart. ftx_int8_quantize: each row of bf16 x [m, k] (rows
+ * x_stride elements apart, a multiple of 8; k a multiple of 16, at most 131072)
+ * becomes codes round(x / s), ties to even, with s = max |x| * fl(1/127) in
+ * scales; s below 2^-100 is 0, with codes of 0, and a row that holds an infinity
+ * or a NaN has codes of 0 and the scale NaN. codes: [m] rows of k bytes rounded
+ * up to a multiple of 256 (FTX_INT8_CODE_STRIDE), the rest 0.
+ * ftx_int8_matmul: y[m, n] = bf16((sum_k codes[m, k] w[n, k]) x_scale[m]
+ * w_scale[n]) of such rows and int8 w [n, k] (-127 .. 127, contiguous); the sums
+ * are exact. workspace: ftx_int8_matmul_workspace bytes (0 unless K is split).
+ * Pointers are 16-byte aligned. */
+#define FTX_INT8_CODE_STRIDE(k) (((int64_t)(k) + 255) / 256 * 256)
+int ftx_int8_quantize(const void *x, int64_t x_stride, void *codes, float *scales, int64_t m, int64_t k, void *stream);
+int ftx_int8_matmul_workspace(int64_t m, int64_t n, int64_t k, size_t *bytes);
+int ftx_int8_matmul(const void *codes, const float *x_scale, const void *w, const float *w_scale, void *y, int64_t m,
+                    int64_t n, int64_t k, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- a KV cache in pages of 8-bit codes --------------------------------------
  * No reference counterpart. One layer is codes, bytes [pages][2][kv_heads]
  * [page_tokens / 32][32 d] (keys, then values), and scales, fp32 [pages][2]
