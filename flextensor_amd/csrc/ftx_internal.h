@@ -178,7 +178,6 @@ hipError_t launch_silu_mul(const uint16_t *g, const uint16_t *u, uint16_t *y, in
 
 // One layer of a KV cache in pages of 8-bit codes (ftx_kvcache.hip), and the sequences of a call.
 constexpr int kKvBlock = FTX_KV8_BLOCK;  // tokens that share a scale
-constexpr int kKvRows = 16;              // rows of a decode tile: one side of the matrix instruction
 struct KvPages {
   const uint8_t *codes;   // [pages][2][kv_heads][page_blocks][32 d]
   const float *scales;    // [pages][2][kv_heads][page_blocks]

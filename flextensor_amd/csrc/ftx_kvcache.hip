@@ -65,6 +65,24 @@ __device__ __forceinline__ int64_t block_index(const KvPages &c, int page, int s
          (block & (c.page_blocks - 1));
 }
 
+// Pages and scales of 64 blocks, a lane each: a kernel reads them at once, and its loop over the blocks takes them
+// from the lanes without waiting for memory. Lane i holds block first + i * step; blocks past `last` are it again.
+struct BlockList {
+  int page;
+  float key_scale, value_scale;
+};
+__device__ __forceinline__ BlockList block_list(const KvPages &c, int64_t b, int head, int first, int step, int last) {
+  const int block = min(first + static_cast<int>(threadIdx.x % 64) * step, last);
+  BlockList x;
+  x.page = page_of(c, b, block);
+  x.key_scale = c.scales[block_index(c, max(x.page, 0), 0, head, block)];
+  x.value_scale = c.scales[block_index(c, max(x.page, 0), 1, head, block)];
+  return x;
+}
+__device__ __forceinline__ float lane_float(float v, int lane) {
+  return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(v)), lane)));
+}
+
 // ---- attention -------------------------------------------------------------------------------------------------
 //
 //   o[b, i, h, :] = sum_p w_p v_p / sum_p w_p,  w_p = exp(scale q[b, i, h, :] . k_p - max),  p <= start_b + i
@@ -100,17 +118,8 @@ __device__ __forceinline__ u32x2 keep_codes(u32x2 v, int n) {
   return (u32x2){v[0] & static_cast<uint32_t>(mask), v[1] & static_cast<uint32_t>(mask >> 32)};
 }
 
-// The maximum (or sum) over the four lanes that hold one row.
-__device__ __forceinline__ float row_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
-}
-__device__ __forceinline__ float row_sum(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
-}
-
-// The same over a value and its partner's in the other half of the wave.
+// The maximum (or sum) of a value and its partner's in the other half of the wave, and over the four lanes that hold
+// one row of 16.
 __device__ __forceinline__ float half_max(float v) {
   const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
@@ -118,6 +127,14 @@ __device__ __forceinline__ float half_max(float v) {
 __device__ __forceinline__ float half_sum(float v) {
   const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+__device__ __forceinline__ float row_max(float v) {
+  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return half_max(fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1])));
+}
+__device__ __forceinline__ float row_sum(float v) {
+  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return half_sum(__uint_as_float(s[0]) + __uint_as_float(s[1]));
 }
 
 // The blocks that the rows of a tile see.
@@ -128,17 +145,17 @@ __device__ __forceinline__ int tile_blocks(const Kv8Attention &a, Span s, int ti
   return (s.start + last) / kKvBlock + 1;
 }
 
-// 16 rows (the query heads of a group and the tokens, row = token * rep + head of the group) over one chunk of the
-// keys; the four waves take its blocks in turn and join their sums through LDS. Nothing is staged: each wave loads
-// the next block's codes into registers while it works on this one.
-template <int D, bool FP8>
-__global__ __launch_bounds__(256, 3) void kv8_rows_kernel(Kv8Attention a) {
-  constexpr int kWaves = 4;
+// Few rows: RT tiles of 16 (row = token * rep + head of the group) over one chunk of the keys; the eight waves take its
+// blocks in turn and join their sums through LDS. Nothing is staged: each wave loads the next block's codes into
+// registers while it works on this one, and widens a code once for all its rows.
+template <int D, bool FP8, int RT>
+__global__ __launch_bounds__(512, 2) void kv8_rows_kernel(Kv8Attention a) {
+  constexpr int kWaves = 8;
   constexpr int kKLoads = D / 64;   // 16 bytes a lane, of each 16 keys of a block
   constexpr int kDTiles = D / 16;
   constexpr int kPitch = D + 4;
-  __shared__ __align__(16) float part[kWaves][kKvRows][kPitch];
-  __shared__ float part_m[kWaves][kKvRows], part_l[kWaves][kKvRows];
+  __shared__ __align__(16) float part[kWaves][16][kPitch];
+  __shared__ float part_m[kWaves][16], part_l[kWaves][16];
 
   uint32_t item = blockIdx.x;  // 32-bit divisions: a launch has fewer than 2^24 workgroups
   const int split = uniform(item % static_cast<uint32_t>(a.splits));
@@ -157,29 +174,37 @@ __global__ __launch_bounds__(256, 3) void kv8_rows_kernel(Kv8Attention a) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 15, g = lane >> 4;
-  const int row = min(tile * kKvRows + r, a.rows - 1);
-  const int token = row / a.rep;
-  const int head = kvh * a.rep + (row - token * a.rep);
-  const int seen = token < span.count ? span.start + token + 1 : 0;  // keys this lane's row sees
-  const int all = (tile * kKvRows) / a.rep < span.count ? span.start + (tile * kKvRows) / a.rep + 1 : 0;
-  const bool every_row = (min(tile * kKvRows + kKvRows, a.rows) - 1) / a.rep < span.count;
-  const int whole = every_row ? all : 0;  // every row of the tile sees keys below this
+  const int row0 = tile * (16 * RT);
   const int length = span.start + span.count;
-
-  bf16x8 qf[D / 32];
-  {
+  const int last_token = (min(row0 + 16 * RT, a.rows) - 1) / a.rep;
+  const int whole = last_token < span.count ? span.start + row0 / a.rep + 1 : 0;  // every row sees keys below this
+  int seen[RT];  // keys this lane's rows see
+  bf16x8 qf[RT][D / 32];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int row = min(row0 + 16 * t + r, a.rows - 1);
+    const int token = row / a.rep;
+    const int head = kvh * a.rep + (row - token * a.rep);
+    seen[t] = token < span.count ? span.start + token + 1 : 0;
     const uint16_t *qp = a.q + b * a.q_stride[0] + token * a.q_stride[1] + head * a.q_stride[2] + 16 * g;
 #pragma unroll
     for (int i = 0; i < kKLoads; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        qf[2 * i + h] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(qp + 64 * i + 8 * h));
+        qf[t][2 * i + h] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(qp + 64 * i + 8 * h));
   }
 
-  f32x4 o[kDTiles];
+  f32x4 o[RT][kDTiles];
+  float m[RT], l[RT];
 #pragma unroll
-  for (int d = 0; d < kDTiles; ++d) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  float m = -FLT_MAX, l = 0.f;
+  for (int t = 0; t < RT; ++t) {
+    // The reference maximum, in units of log2, starts at the lowest finite value: while no key of the row counts,
+    // -inf less it is -inf, a weight of zero.
+    m[t] = -FLT_MAX;
+    l[t] = 0.f;
+#pragma unroll
+    for (int d = 0; d < kDTiles; ++d) o[t][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  }
 
   struct Block {
     u32x4 k[2][kKLoads];
@@ -187,146 +212,161 @@ __global__ __launch_bounds__(256, 3) void kv8_rows_kernel(Kv8Attention a) {
     float k_scale, v_scale;
     bool hole;
   };
-  const auto load = [&](Block &x, int block) {
-    const int page = page_of(a.kv, b, block);
+  BlockList list;
+  const uint32_t k_lane = g * (16 * kKvBlock) + (8 * (r >> 2) + (r & 3)) * 16, v_lane = r * kKvBlock + 8 * g;
+  const auto load = [&](Block &x, int nth) {  // the wave's nth block; past the chunk's end its last one again
+    const int at = nth % kWave;
+    if (at == 0) list = block_list(a.kv, b, kvh, first + wave + nth * kWaves, kWaves, end - 1);
+    const int page = __builtin_amdgcn_readlane(list.page, at);
+    const int block = min(first + wave + nth * kWaves, end - 1);
     x.hole = page < 0;
-    const int64_t ki = block_index(a.kv, max(page, 0), 0, kvh, block);
-    const int64_t vi = block_index(a.kv, max(page, 0), 1, kvh, block);
-    x.k_scale = a.kv.scales[ki];
-    x.v_scale = a.kv.scales[vi];
-    const uint8_t *kp = a.kv.codes + ki * (kKvBlock * D) + g * (16 * kKvBlock) + (8 * (r >> 2) + (r & 3)) * 16;
-    const uint8_t *vp = a.kv.codes + vi * (kKvBlock * D) + r * kKvBlock + 8 * g;
+    x.k_scale = lane_float(list.key_scale, at);
+    x.v_scale = lane_float(list.value_scale, at);
+    const uint8_t *kp = a.kv.codes + block_index(a.kv, max(page, 0), 0, kvh, block) * (kKvBlock * D);
+    const uint8_t *vp = a.kv.codes + block_index(a.kv, max(page, 0), 1, kvh, block) * (kKvBlock * D);
 #pragma unroll
     for (int i = 0; i < kKLoads; ++i)
 #pragma unroll
       for (int s = 0; s < 2; ++s)
-        x.k[s][i] = *reinterpret_cast<const u32x4 *>(kp + i * (64 * kKvBlock) + 64 * s);
+        x.k[s][i] = *reinterpret_cast<const u32x4 *>(kp + k_lane + (i * (64 * kKvBlock) + 64 * s));
 #pragma unroll
-    for (int d = 0; d < kDTiles; ++d) x.v[d] = *reinterpret_cast<const u32x2 *>(vp + d * (16 * kKvBlock));
+    for (int d = 0; d < kDTiles; ++d) x.v[d] = *reinterpret_cast<const u32x2 *>(vp + v_lane + d * (16 * kKvBlock));
   };
-  // Key 8 g' + 4 s + c of a block is row 4 g' + c of score tile s, so lane group g holds the scores of keys 8 g ..
+  // Key 8 g' + 4 h + c of a block is row 4 g' + c of score tile h, so lane group g holds the scores of keys 8 g ..
   // 8 g + 7, the ones whose values it loads.
-  const auto work = [&](Block &x, int block) {
-    if (x.hole) return;
-    f32x4 s[2];
+  const auto work = [&](Block &x, int block) {  // a hole's loads are used like any others: nothing waits for them
+    f32x4 s[RT][2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      s[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) s[t][h] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < kKLoads; ++i) {
-        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen<FP8>(x.k[t][i][0], x.k[t][i][1]), qf[2 * i], s[t], 0, 0, 0);
-        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen<FP8>(x.k[t][i][2], x.k[t][i][3]), qf[2 * i + 1], s[t], 0, 0, 0);
+        const bf16x8 lo = widen<FP8>(x.k[h][i][0], x.k[h][i][1]), hi = widen<FP8>(x.k[h][i][2], x.k[h][i][3]);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, qf[t][2 * i], s[t][h], 0, 0, 0);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, qf[t][2 * i + 1], s[t][h], 0, 0, 0);
       }
     }
     const int key0 = block * kKvBlock;
     float scale = a.scale_log2 * x.k_scale;
-    if (key0 + kKvBlock > whole) {
+    if (x.hole || key0 + kKvBlock > whole) {
+      const int kept = x.hole ? 0 : length - key0;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < RT; ++t) {
+        const int limit = x.hole ? 0 : seen[t] - key0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s[t][c] = key0 + 8 * g + 4 * t + c < seen ? s[t][c] * scale : -INFINITY;
-      scale = 1.0f;
-      if (key0 + kKvBlock > length) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int d = 0; d < kDTiles; ++d) x.v[d] = keep_codes(x.v[d], length - key0 - 8 * g);
+          for (int c = 0; c < 4; ++c) s[t][h][c] = 8 * g + 4 * h + c < limit ? s[t][h][c] * scale : -INFINITY;
       }
-    }
-    float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    mx = row_max(mx) * scale;
-    if (__any(mx > m + kSlack)) {
-      const float m_new = fmaxf(m, mx);
-      const float alpha = __builtin_amdgcn_exp2f(m - m_new);
-      m = m_new;
-      l *= alpha;
+      scale = 1.0f;
+      if (kept < kKvBlock) {
 #pragma unroll
-      for (int d = 0; d < kDTiles; ++d)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[d][c] *= alpha;
+        for (int d = 0; d < kDTiles; ++d) x.v[d] = keep_codes(x.v[d], kept - 8 * g);
+      }
     }
     // p times the value scale in one operation: 2^(s - m + log2(scale)); the sum of the p takes it out again. A
     // scale of 0 stands beside codes of 0, whose weight does not matter.
-    const float factor = x.v_scale > 0.f ? x.v_scale : 1.0f;
-    const float offset = __builtin_amdgcn_logf(factor) - m;
-    float sum = 0.f;
-    u32x4 p;
+    const float factor = x.v_scale == 0.f || x.hole ? 1.0f : x.v_scale;
+    const float log_factor = __builtin_amdgcn_logf(factor), inverse = __builtin_amdgcn_rcpf(factor);
+    u32x4 p[RT];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[e >> 1][2 * (e & 1)], scale, offset));
-      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[e >> 1][2 * (e & 1) + 1], scale, offset));
-      sum += p0 + p1;
-      p[e] = pack_bf16(p0, p1);
+    for (int t = 0; t < RT; ++t) {
+      float mx = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
+                       fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
+      mx = row_max(mx) * scale;
+      // The maximum is only raised when a score exceeds it by more than 2^kSlack: the probabilities keep their
+      // relative precision, and the accumulators are rescaled a few times per row instead of once per block.
+      if (__any(mx > m[t] + kSlack)) {
+        const float m_new = fmaxf(m[t], mx);
+        const float alpha = __builtin_amdgcn_exp2f(m[t] - m_new);
+        m[t] = m_new;
+        l[t] *= alpha;
+#pragma unroll
+        for (int d = 0; d < kDTiles; ++d)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[t][d][c] *= alpha;
+      }
+      const float offset = log_factor - m[t];
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][e >> 1][2 * (e & 1)], scale, offset));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[t][e >> 1][2 * (e & 1) + 1], scale, offset));
+        sum += p0 + p1;
+        p[t][e] = pack_bf16(p0, p1);
+      }
+      l[t] = fmaf(sum, inverse, l[t]);
     }
-    l = fmaf(sum, __builtin_amdgcn_rcpf(factor), l);
 #pragma unroll
-    for (int d = 0; d < kDTiles; ++d)
-      o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen<FP8>(x.v[d][0], x.v[d][1]), __builtin_bit_cast(bf16x8, p),
-                                                     o[d], 0, 0, 0);
+    for (int d = 0; d < kDTiles; ++d) {
+      const bf16x8 v = widen<FP8>(x.v[d][0], x.v[d][1]);
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, p[t]), o[t][d], 0, 0, 0);
+    }
   };
 
-  if (first + wave < end) {
-    const int last = end - 1;  // loads ahead of the loop's end take the chunk's last block again
+  const int n = (end - first - wave + kWaves - 1) / kWaves;  // the wave's blocks
+  if (n > 0) {
     Block x, y;
-    int j = first + wave;
-    load(x, j);
-    for (;;) {
-      load(y, min(j + kWaves, last));
-      work(x, j);
-      j += kWaves;
-      if (j >= end) break;
-      load(x, min(j + kWaves, last));
-      work(y, j);
-      j += kWaves;
-      if (j >= end) break;
+    load(x, 0);
+    for (int i = 0;;) {
+      load(y, i + 1);
+      work(x, first + wave + i * kWaves);
+      if (++i >= n) break;
+      load(x, i + 1);
+      work(y, first + wave + i * kWaves);
+      if (++i >= n) break;
     }
   }
 
-  l = row_sum(l);
 #pragma unroll
-  for (int d = 0; d < kDTiles; ++d) *reinterpret_cast<f32x4 *>(&part[wave][r][16 * d + 4 * g]) = o[d];
-  if (g == 0) {
-    part_m[wave][r] = m;
-    part_l[wave][r] = l;
-  }
-  __syncthreads();
-  constexpr int kPer = D / 16;  // values of one row that a thread joins
-  const int out_r = threadIdx.x / 16, out_d = (threadIdx.x % 16) * kPer;
-  float top = -FLT_MAX;
+  for (int t = 0; t < RT; ++t) {
+    if (t > 0) __syncthreads();  // the rows before have been joined
+    l[t] = row_sum(l[t]);
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, part_m[w][out_r]);
-  float sum = 0.f, acc[kPer];
-#pragma unroll
-  for (int c = 0; c < kPer; ++c) acc[c] = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const float weight = __builtin_amdgcn_exp2f(part_m[w][out_r] - top);
-    sum = fmaf(weight, part_l[w][out_r], sum);
-#pragma unroll
-    for (int c = 0; c < kPer; ++c) acc[c] = fmaf(weight, part[w][out_r][out_d + c], acc[c]);
-  }
-  if (a.splits > 1) {
-    const int64_t slots = a.tile_items * kKvRows;
-    const int64_t slot = split * slots + tile_item * kKvRows + out_r;
-    float *po = a.part + slot * D + out_d;
-#pragma unroll
-    for (int c = 0; c < kPer; c += 4) *reinterpret_cast<f32x4 *>(po + c) = (f32x4){acc[c], acc[c + 1], acc[c + 2], acc[c + 3]};
-    if (out_d == 0) {
-      float *pm = a.part + a.splits * slots * D;
-      pm[slot] = top;
-      pm[a.splits * slots + slot] = sum;
+    for (int d = 0; d < kDTiles; ++d) *reinterpret_cast<f32x4 *>(&part[wave][r][16 * d + 4 * g]) = o[t][d];
+    if (g == 0) {
+      part_m[wave][r] = m[t];
+      part_l[wave][r] = l[t];
     }
-    return;
-  }
-  const int out_row = tile * kKvRows + out_r;
-  if (out_row >= a.rows) return;
-  const int out_token = out_row / a.rep;
-  const int out_head = kvh * a.rep + (out_row - out_token * a.rep);
-  const float inv = sum != 0.f ? 1.0f / sum : 0.f;  // no key, no weight: the row is 0
-  uint16_t *op = a.o + b * a.o_stride[0] + out_token * a.o_stride[1] + out_head * a.o_stride[2] + out_d;
+    __syncthreads();
+    // a thread joins four values of one row
+    const int in_tile = threadIdx.x / (D / 4), out_d = threadIdx.x % (D / 4) * 4;
+    const int out_row = row0 + 16 * t + in_tile;
+    if (in_tile >= 16 || out_row >= a.rows) continue;
+    float top = -FLT_MAX;
 #pragma unroll
-  for (int c = 0; c < kPer; c += 4)
-    *reinterpret_cast<u32x2 *>(op + c) =
-        (u32x2){pack_bf16(acc[c] * inv, acc[c + 1] * inv), pack_bf16(acc[c + 2] * inv, acc[c + 3] * inv)};
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, part_m[w][in_tile]);
+    float sum = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float weight = __builtin_amdgcn_exp2f(part_m[w][in_tile] - top);
+      sum = fmaf(weight, part_l[w][in_tile], sum);
+      acc += weight * *reinterpret_cast<const f32x4 *>(&part[w][in_tile][out_d]);
+    }
+    if (a.splits > 1) {
+      const int64_t slots = a.tile_items * a.tile_rows;
+      const int64_t slot = split * slots + tile_item * a.tile_rows + 16 * t + in_tile;
+      *reinterpret_cast<f32x4 *>(a.part + slot * D + out_d) = acc;
+      if (out_d == 0) {
+        float *pm = a.part + a.splits * slots * D;
+        pm[slot] = top;
+        pm[a.splits * slots + slot] = sum;
+      }
+      continue;
+    }
+    const int out_token = out_row / a.rep;
+    const int out_head = kvh * a.rep + (out_row - out_token * a.rep);
+    const float inv = sum != 0.f ? 1.0f / sum : 0.f;  // no key, no weight: the row is 0
+    uint16_t *op = a.o + b * a.o_stride[0] + out_token * a.o_stride[1] + out_head * a.o_stride[2] + out_d;
+    *reinterpret_cast<u32x2 *>(op) =
+        (u32x2){pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
+  }
 }
 
 // Prompts: 32 rows a wave, NW waves that share tiles of 64 keys. The workgroup loads a tile's codes into registers,
@@ -338,7 +378,7 @@ __global__ __launch_bounds__(256, 3) void kv8_rows_kernel(Kv8Attention a) {
 // S^T = K Q^T gives a lane 16 of a block's 32 scores of one row, keys 8 a + 4 g + c (g the half of the wave); V's
 // operands are written in that order.
 template <int D, bool FP8, int NW, bool SPLIT>
-__global__ __launch_bounds__(NW * kWave, D == 128 && NW == 2 ? 1 : 2) void kv8_tile_kernel(Kv8Attention a) {
+__global__ __launch_bounds__(NW * kWave, 2) void kv8_tile_kernel(Kv8Attention a) {
   constexpr int kThreads = NW * kWave;
   constexpr int kKeys = 64, kSub = 2;
   constexpr int kBlockBytes = kKvBlock * D;          // codes of a block's side
@@ -388,19 +428,33 @@ __global__ __launch_bounds__(NW * kWave, D == 128 && NW == 2 ? 1 : 2) void kv8_t
   Unit units[kUnits];
   struct Scales {
     float key[kSub], value[kSub];
-    bool hole[kSub];
+    bool hole[kSub];  // or past the chunk's end
   };
-  const auto load = [&](int t) {  // clamped to the chunk's last block, whose scores and values are masked twice over
+  BlockList list;
+  const auto load = [&](int t) {  // past the chunk's last block it again, masked
+    const int at = t * kSub % kWave;
+    if (at == 0) list = block_list(a.kv, b, kvh, first + t * kSub, 1, end - 1);
+    Scales x;
+    int page[kSub];
+#pragma unroll
+    for (int j = 0; j < kSub; ++j) {
+      page[j] = __builtin_amdgcn_readlane(list.page, at + j);
+      x.key[j] = lane_float(list.key_scale, at + j);
+      x.value[j] = lane_float(list.value_scale, at + j);
+      x.hole[j] = page[j] < 0 || first + t * kSub + j >= end;
+    }
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
       const int u0 = i * kThreads + wave * kWave;  // the wave's first unit
       const int side = u0 / kSideUnits, sub = u0 % kSideUnits / kBlockUnits;
       const int block = first + t * kSub + sub;
-      const int page = page_of(a.kv, b, min(block, end - 1));
-      const int64_t index = block_index(a.kv, max(page, 0), side, kvh, min(block, end - 1));
-      units[i].w = *reinterpret_cast<const u32x4 *>(a.kv.codes + index * kBlockBytes + (u0 % kBlockUnits + lane) * 16);
-      units[i].keep = page < 0 || block >= end ? 0 : length - block * kKvBlock;
+      const int own = sub == 0 ? page[0] : page[1];
+      const uint8_t *from =
+          a.kv.codes + block_index(a.kv, max(own, 0), side, kvh, min(block, end - 1)) * kBlockBytes;
+      units[i].w = *reinterpret_cast<const u32x4 *>(from + (u0 % kBlockUnits + lane) * 16);
+      units[i].keep = own < 0 || block >= end ? 0 : length - block * kKvBlock;
     }
+    return x;
   };
   const auto store = [&](int t) {
     uint8_t *base = lds[t & 1];
@@ -428,19 +482,6 @@ __global__ __launch_bounds__(NW * kWave, D == 128 && NW == 2 ? 1 : 2) void kv8_t
       }
     }
   };
-  const auto scales_of = [&](int t) {
-    Scales x;
-#pragma unroll
-    for (int j = 0; j < kSub; ++j) {
-      const int block = min(first + t * kSub + j, end - 1);
-      const int page = page_of(a.kv, b, block);
-      x.hole[j] = page < 0;
-      x.key[j] = a.kv.scales[block_index(a.kv, max(page, 0), 0, kvh, block)];
-      x.value[j] = a.kv.scales[block_index(a.kv, max(page, 0), 1, kvh, block)];
-    }
-    return x;
-  };
-
   // Queries: lane (r, g) holds elements 16 ks + 8 g .. + 7 of its row for every step ks.
   bf16x8 qf[kQSteps];
   {
@@ -456,20 +497,19 @@ __global__ __launch_bounds__(NW * kWave, D == 128 && NW == 2 ? 1 : 2) void kv8_t
     for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
   float m = -FLT_MAX, l = 0.f;
 
-  Scales next = {};
+  Scales x = {}, next = {}, later = {};
   if (n_tiles > 0) {
-    load(0);
-    next = scales_of(0);
+    next = load(0);
     store(0);
-    if (n_tiles > 1) load(1);
+    if (n_tiles > 1) later = load(1);
   }
   for (int t = 0; t < n_tiles; ++t) {
     __syncthreads();
-    const Scales x = next;
+    x = next;
+    next = later;
     if (t + 1 < n_tiles) {
-      next = scales_of(t + 1);
       store(t + 1);
-      if (t + 2 < n_tiles) load(t + 2);
+      if (t + 2 < n_tiles) later = load(t + 2);
     }
     const int key0 = (first + t * kSub) * kKvBlock;
     if (key0 >= wave_end) continue;
@@ -491,8 +531,8 @@ __global__ __launch_bounds__(NW * kWave, D == 128 && NW == 2 ? 1 : 2) void kv8_t
     for (int j = 0; j < kSub; ++j) {
       scale[j] = a.scale_log2 * x.key[j];
       const int block = first + t * kSub + j;
-      if (x.hole[j] || block >= end || (block + 1) * kKvBlock > whole) {
-        const int limit = x.hole[j] || block >= end ? 0 : seen - block * kKvBlock;
+      if (x.hole[j] || (block + 1) * kKvBlock > whole) {
+        const int limit = x.hole[j] ? 0 : seen - block * kKvBlock;
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[j][e] = 8 * (e >> 2) + 4 * g + (e & 3) < limit ? s[j][e] * scale[j] : -INFINITY;
         scale[j] = 1.0f;
@@ -520,7 +560,7 @@ __global__ __launch_bounds__(NW * kWave, D == 128 && NW == 2 ? 1 : 2) void kv8_t
     bf16x8 p[2 * kSub];  // times the value scale, as above
 #pragma unroll
     for (int j = 0; j < kSub; ++j) {
-      const float factor = x.value[j] > 0.f && !x.hole[j] && first + t * kSub + j < end ? x.value[j] : 1.0f;
+      const float factor = x.value[j] == 0.f || x.hole[j] ? 1.0f : x.value[j];
       const float offset = __builtin_amdgcn_logf(factor) - m;
       float sum = 0.f;
       uint32_t w[8];
@@ -574,35 +614,35 @@ __global__ __launch_bounds__(NW * kWave, D == 128 && NW == 2 ? 1 : 2) void kv8_t
 }
 
 // o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the chunks that hold keys the tile sees, M the largest
-// m_i; D / 4 lanes a row.
+// m_i. A workgroup a row: groups of D / 4 lanes take the chunks in turn, so that few rows over many chunks wait for
+// a few loads and not for one after the other, and meet in LDS.
 template <int D>
 __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8Attention a) {
-  constexpr int kLanes = D / 4;
-  const int64_t slots = a.tile_items * a.tile_rows;
-  const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
-  const int c = threadIdx.x % kLanes;
-  if (at >= slots) return;
-  const uint32_t tile_item = static_cast<uint32_t>(at) / static_cast<uint32_t>(a.tile_rows);
-  const int tile = static_cast<int>(tile_item % static_cast<uint32_t>(a.row_tiles));
-  const int row = tile * a.tile_rows + static_cast<int>(static_cast<uint32_t>(at) % static_cast<uint32_t>(a.tile_rows));
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes, kBatch = 4;
+  __shared__ f32x4 part_o[kGroups][kLanes];
+  __shared__ float part_m[kGroups], part_l[kGroups];
+  const int64_t slots = a.tile_items * a.tile_rows, at = blockIdx.x;
+  const uint32_t tile_item = uniform(blockIdx.x / static_cast<uint32_t>(a.tile_rows));
+  const int tile = uniform(tile_item % static_cast<uint32_t>(a.row_tiles));
+  const int row = tile * a.tile_rows + uniform(blockIdx.x % static_cast<uint32_t>(a.tile_rows));
   if (row >= a.rows) return;
-  const uint32_t bkv = tile_item / static_cast<uint32_t>(a.row_tiles);
-  const int64_t b = bkv / static_cast<uint32_t>(a.kv.kv_heads);
+  const uint32_t bkv = uniform(tile_item / static_cast<uint32_t>(a.row_tiles));
+  const int64_t b = uniform(bkv / static_cast<uint32_t>(a.kv.kv_heads));
   const int used = min(a.splits, (tile_blocks(a, span_of(a.kv, b, a.t), tile) + a.chunk - 1) / a.chunk);
   const float *pm = a.part + a.splits * slots * D;
   const float *pl = pm + a.splits * slots;
-  constexpr int kBatch = 8;  // chunks whose loads are in flight together
+  const int c = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   float mx = -FLT_MAX, l = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int i0 = 0; i0 < used; i0 += kBatch) {
-    float m[kBatch], part_l[kBatch];
-    f32x4 part[kBatch];
+  for (int i0 = group; i0 < used; i0 += kGroups * kBatch) {
+    float m[kBatch], part[kBatch];
+    f32x4 o[kBatch];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int64_t s = min(i0 + i, used - 1) * slots + at;
+    for (int i = 0; i < kBatch; ++i) {  // past the last chunk it again, with a weight of zero below
+      const int64_t s = min(i0 + i * kGroups, used - 1) * slots + at;
       m[i] = pm[s];
-      part_l[i] = pl[s];
-      part[i] = *reinterpret_cast<const f32x4 *>(a.part + s * D + 4 * c);
+      part[i] = pl[s];
+      o[i] = *reinterpret_cast<const f32x4 *>(a.part + s * D + 4 * c);
     }
     float m_new = mx;
 #pragma unroll
@@ -613,15 +653,32 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8Attention a) {
     mx = m_new;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      if (i0 + i >= used) break;
+      if (i0 + i * kGroups >= used) break;
       const float w = __builtin_amdgcn_exp2f(m[i] - m_new);
-      l += w * part_l[i];
-      acc += w * part[i];
+      l += w * part[i];
+      acc += w * o[i];
     }
+  }
+  part_o[group][c] = acc;
+  if (c == 0) {
+    part_m[group] = mx;
+    part_l[group] = l;
+  }
+  __syncthreads();
+  if (group > 0) return;
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) mx = fmaxf(mx, part_m[i]);
+  l = 0.f;
+  acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    const float w = __builtin_amdgcn_exp2f(part_m[i] - mx);
+    l += w * part_l[i];
+    acc += w * part_o[i][c];
   }
   const float inv = l != 0.f ? 1.0f / l : 0.f;
   const int token = row / a.rep;
-  const int head = static_cast<int>(bkv % static_cast<uint32_t>(a.kv.kv_heads)) * a.rep + (row - token * a.rep);
+  const int head = uniform(bkv % static_cast<uint32_t>(a.kv.kv_heads)) * a.rep + (row - token * a.rep);
   uint16_t *op = a.o + b * a.o_stride[0] + token * a.o_stride[1] + head * a.o_stride[2] + 4 * c;
   *reinterpret_cast<u32x2 *>(op) =
       (u32x2){pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
@@ -637,15 +694,16 @@ void start_tiles(const Kv8Attention &p, hipStream_t stream) {
 template <int D, bool FP8>
 hipError_t launch_attend(const Kv8Attention &p, hipStream_t stream) {
   switch (p.waves) {
-    case 0: hipLaunchKernelGGL((kv8_rows_kernel<D, FP8>), dim3(p.items), dim3(256), 0, stream, p); break;
-    case 2: start_tiles<D, FP8, 2>(p, stream); break;
+    case 0:
+      if (p.rows <= 16) hipLaunchKernelGGL((kv8_rows_kernel<D, FP8, 1>), dim3(p.items), dim3(512), 0, stream, p);
+      else hipLaunchKernelGGL((kv8_rows_kernel<D, FP8, 2>), dim3(p.items), dim3(512), 0, stream, p);
+      break;
     case 4: start_tiles<D, FP8, 4>(p, stream); break;
     default: start_tiles<D, FP8, 8>(p, stream); break;
   }
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || p.splits == 1) return err;
-  const int64_t lanes = p.tile_items * p.tile_rows * (D / 4);
-  hipLaunchKernelGGL((kv8_join_kernel<D>), dim3(static_cast<unsigned>((lanes + 255) / 256)), dim3(256), kLdsToken,
+  hipLaunchKernelGGL((kv8_join_kernel<D>), dim3(static_cast<unsigned>(p.tile_items * p.tile_rows)), dim3(256), 0,
                      stream, p);
   return hipGetLastError();
 }
@@ -861,16 +919,24 @@ void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, int cus, int xcds) 
   const int64_t heads = static_cast<int64_t>(p->batch) * p->kv.kv_heads;
   const int64_t blocks = std::max<int64_t>(1, (max_tokens + kKvBlock - 1) / kKvBlock);
   // Up to 16 rows (decode) the codes go from memory straight into the products; more rows share them through LDS.
-  p->waves = p->rows <= kKvRows ? 0 : p->rows <= 64 ? 2 : p->rows <= 128 ? 4 : 8;
-  p->tile_rows = p->waves == 0 ? kKvRows : 32 * p->waves;
+  p->waves = p->rows <= 64 ? 0 : 8;
+  p->tile_rows = p->waves > 0 ? 32 * p->waves : p->rows <= 16 ? p->rows : 32;
   p->row_tiles = (p->rows + p->tile_rows - 1) / p->tile_rows;
   p->tile_items = heads * p->row_tiles;
-  // Chunks of the keys until every CU has its workgroups, each of at least two blocks a wave.
-  const int64_t per_cu = p->waves == 0 ? 4 : p->waves == 2 ? 4 : p->waves == 4 ? 2 : 1;
-  const int64_t want = std::max<int64_t>(1, per_cu * cus / p->tile_items);
-  const int64_t chunk = std::max<int64_t>(8, (blocks + want - 1) / want);
-  p->splits = static_cast<int>((blocks + chunk - 1) / chunk);
-  p->chunk = static_cast<int>(chunk);  // the last one goes on to the end of the sequence, whatever max_tokens says
+  // How often the keys are split. A round of workgroups, one a CU, takes its blocks and a start of about 16 more; the
+  // join takes about 30 (decode: 0.1 us a block; 16 blocks of 8 heads 6.8 us, split in two 9.0). Splits fill whole
+  // rounds: 8 heads over 1001 blocks 18.0 us in 32 splits, 21.9 in 63, 36 in 4; 256 heads over 129 blocks 48.5 us
+  // unsplit and 56 in two.
+  const auto cost = [&](int64_t splits) {
+    return (p->tile_items * splits + cus - 1) / cus * ((blocks + splits - 1) / splits + 16) + (splits > 1 ? 30 : 0);
+  };
+  int64_t splits = 1;
+  for (int64_t rounds = 1; rounds <= 8; ++rounds) {
+    const int64_t s = std::min(rounds * cus / p->tile_items, blocks / 8);
+    if (s > 1 && cost(s) < cost(splits)) splits = s;
+  }
+  p->chunk = static_cast<int>((blocks + splits - 1) / splits);  // the last one goes on to the end of the sequence,
+  p->splits = static_cast<int>((blocks + p->chunk - 1) / p->chunk);  // whatever max_tokens says
   const int64_t items = p->tile_items * p->splits;
   p->items = static_cast<uint32_t>(std::min<int64_t>(items, UINT32_MAX));  // too many for a launch: the caller refuses
   p->part_bytes = p->splits > 1 ? static_cast<size_t>(items) * p->tile_rows * (p->kv.d + 2) * sizeof(float) : 0;

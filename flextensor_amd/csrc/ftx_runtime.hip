@@ -1495,7 +1495,7 @@ int plan_kv8(int64_t max_tokens, ftx::Kv8Attention *p) {
   }
   ftx::plan_kv8_attention(p, std::min<int64_t>(max_tokens, int64_t(1) << 30), cus, xcds);
   const int64_t join_rows = p->splits > 1 ? p->tile_items * p->tile_rows : 0;
-  if (static_cast<int64_t>(p->items) + p->xcds > ftx::kMaxThreads / 512 || join_rows > ftx::kMaxThreads / 32 - 256)
+  if (static_cast<int64_t>(p->items) + p->xcds > ftx::kMaxThreads / 512 || join_rows > ftx::kMaxThreads / 256)
     return ftx::fail(FTX_ERR_UNSUPPORTED, "cache attention: more workgroups than one launch holds");
   return FTX_OK;
 }
