@@ -198,8 +198,8 @@ struct Kv8Attention {
   int batch, t, heads;
   float scale_log2;
   // planned
-  int rep, rows, tile_rows, row_tiles, splits, chunk, xcds;  // chunk: blocks of a split
-  int waves;              // of a workgroup, 32 rows each; 0: the decode kernel
+  int rep, rows, row_tiles, splits, chunk, xcds;  // chunk: blocks of a split
+  int tile_rows;          // up to 16 or 32: the kernel of few rows; else the prompts'
   int64_t tile_items;     // batch * kv heads * row tiles
   uint32_t items;         // times the splits
   size_t part_bytes;

@@ -28,6 +28,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWave = 64;
 constexpr float kSlack = 8.0f;
+constexpr int kTileWaves = 8;  // of an attention workgroup
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
@@ -149,7 +150,7 @@ __device__ __forceinline__ int tile_blocks(const Kv8Attention &a, Span s, int ti
 // blocks in turn and join their sums through LDS. Nothing is staged: each wave loads the next block's codes into
 // registers while it works on this one, and widens a code once for all its rows.
 template <int D, bool FP8, int RT>
-__global__ __launch_bounds__(512, 2) void kv8_rows_kernel(Kv8Attention a) {
+__global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Attention a) {
   constexpr int kWaves = 8;
   constexpr int kKLoads = D / 64;   // 16 bytes a lane, of each 16 keys of a block
   constexpr int kDTiles = D / 16;
@@ -369,17 +370,16 @@ __global__ __launch_bounds__(512, 2) void kv8_rows_kernel(Kv8Attention a) {
   }
 }
 
-// Prompts: 32 rows a wave, NW waves that share tiles of 64 keys. The workgroup loads a tile's codes into registers,
-// widens each once and writes it to LDS in the order in which a lane reads its operands, 16 bytes at 16 * lane: no
-// bank is met twice and the inner loop is that of the attention over a bf16 cache. Two tiles are in LDS and the
-// codes of a third in registers, so one barrier a tile is enough: a tile is written while the one before it is in
-// use, into the buffer whose last readers have passed the barrier.
+// Prompts: eight waves of 32 rows share tiles of 64 keys. The workgroup loads a tile's codes into registers, widens
+// each once and writes it to LDS in the order in which a lane reads its operands, 16 bytes at 16 * lane: no bank is
+// met twice and the inner loop is that of the attention over a bf16 cache. A tile is written while the one before it
+// is in use and the codes of the one after it are on their way, with one barrier a tile.
 //
 // S^T = K Q^T gives a lane 16 of a block's 32 scores of one row, keys 8 a + 4 g + c (g the half of the wave); V's
 // operands are written in that order.
-template <int D, bool FP8, int NW, bool SPLIT>
-__global__ __launch_bounds__(NW * kWave, 2) void kv8_tile_kernel(Kv8Attention a) {
-  constexpr int kThreads = NW * kWave;
+template <int D, bool FP8, bool SPLIT>
+__global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Attention a) {
+  constexpr int kThreads = kTileWaves * kWave;
   constexpr int kKeys = 64, kSub = 2;
   constexpr int kBlockBytes = kKvBlock * D;          // codes of a block's side
   constexpr int kBlockUnits = kBlockBytes / 16;      // 16-byte loads
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void kv8_tile_kernel(Kv8Attention a)
   constexpr int kSide = kKeys * D * 2;               // LDS bytes of a tile's side
   constexpr int kQSteps = D / 16, kDTiles = D / 32;
   static_assert(2 * kSideUnits % kThreads == 0 && kBlockUnits % kWave == 0, "a wave's units are of one block and side");
-  __shared__ __align__(1024) uint8_t lds[2][2 * kSide];
+  __shared__ __align__(1024) uint8_t lds[4 * kSide];  // two tiles of keys, two of values
 
   const uint32_t per_xcd = (a.items + a.xcds - 1) / a.xcds;
   uint32_t item = (blockIdx.x % a.xcds) * per_xcd + blockIdx.x / a.xcds;
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void kv8_tile_kernel(Kv8Attention a)
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 31, g = lane >> 5;
-  const int row0 = tile * (32 * NW) + wave * 32;
+  const int row0 = tile * (32 * kTileWaves) + wave * 32;
   const int row = min(row0 + r, a.rows - 1);
   const int token = row / a.rep;
   const int head = kvh * a.rep + (row - token * a.rep);
@@ -421,6 +421,9 @@ __global__ __launch_bounds__(NW * kWave, 2) void kv8_tile_kernel(Kv8Attention a)
   // every row of the wave sees keys below this
   const int whole = row0 + 32 <= a.rows && last_row / a.rep < span.count ? span.start + row0 / a.rep + 1 : 0;
 
+  const auto side_of = [&](int i) {  // known when compiled where a unit of all waves is of one side
+    return kSideUnits >= kThreads ? i * kThreads / kSideUnits : (i * kThreads + wave * kWave) / kSideUnits;
+  };
   struct Unit {  // 16 bytes of codes on their way to LDS
     u32x4 w;
     int keep;    // values: the tokens of them that the sequence has
@@ -446,7 +449,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void kv8_tile_kernel(Kv8Attention a)
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
       const int u0 = i * kThreads + wave * kWave;  // the wave's first unit
-      const int side = u0 / kSideUnits, sub = u0 % kSideUnits / kBlockUnits;
+      const int side = side_of(i), sub = u0 % kSideUnits / kBlockUnits;
       const int block = first + t * kSub + sub;
       const int own = sub == 0 ? page[0] : page[1];
       const uint8_t *from =
@@ -456,32 +459,31 @@ __global__ __launch_bounds__(NW * kWave, 2) void kv8_tile_kernel(Kv8Attention a)
     }
     return x;
   };
+  // Where the 16 bytes go: keys are units of [d / 16][token], one step of the sum over d for both halves of the wave;
+  // values of [d][half of the tokens], one step of the sum over tokens, whose words the halves take in turn.
+  uint32_t store_at[kUnits];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    const int u0 = i * kThreads + wave * kWave, unit = u0 % kBlockUnits + lane, d = unit / 2;
+    store_at[i] = u0 % kSideUnits / kBlockUnits * (kSide / kSub) +
+                  (side_of(i) == 0 ? unit / 32 * 1024 + unit % 32 * 16 : (d / 32 * 2 + unit % 2) * 1024 + d % 32 * 16);
+  }
   const auto store = [&](int t) {
-    uint8_t *base = lds[t & 1];
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
-      const int u0 = i * kThreads + wave * kWave;
-      const int side = u0 / kSideUnits, sub = u0 % kSideUnits / kBlockUnits;
-      const int unit = u0 % kBlockUnits + lane;
-      uint8_t *to = base + side * kSide + sub * (kSide / kSub);
+      const int side = side_of(i);
       u32x4 w = units[i].w;
-      if (side == 0) {  // unit: [d / 16][token], one step of the sum over d, both halves of the wave
-        to += unit / 32 * 1024 + unit % 32 * 16;
-        *reinterpret_cast<bf16x8 *>(to) = widen<FP8>(w[0], w[1]);
-        *reinterpret_cast<bf16x8 *>(to + 512) = widen<FP8>(w[2], w[3]);
-      } else {  // unit: [d][half of the tokens], one step of the sum over tokens
-        if (units[i].keep < kKvBlock) {
-          const int n = units[i].keep - unit % 2 * 16;
-          const u32x2 lo = keep_codes((u32x2){w[0], w[1]}, n), hi = keep_codes((u32x2){w[2], w[3]}, n - 8);
-          w = (u32x4){lo[0], lo[1], hi[0], hi[1]};
-        }
-        const int d = unit / 2;
-        to += (d / 32 * 2 + unit % 2) * 1024 + d % 32 * 16;
-        *reinterpret_cast<bf16x8 *>(to) = widen<FP8>(w[0], w[2]);
-        *reinterpret_cast<bf16x8 *>(to + 512) = widen<FP8>(w[1], w[3]);
+      if (side != 0 && units[i].keep < kKvBlock) {
+        const int n = units[i].keep - lane % 2 * 16;
+        const u32x2 lo = keep_codes((u32x2){w[0], w[1]}, n), hi = keep_codes((u32x2){w[2], w[3]}, n - 8);
+        w = (u32x4){lo[0], lo[1], hi[0], hi[1]};
       }
+      uint8_t *to = lds + (side == 0 ? t & 1 : 2 + (t & 1)) * kSide + store_at[i];
+      *reinterpret_cast<bf16x8 *>(to) = widen<FP8>(w[0], side == 0 ? w[1] : w[2]);
+      *reinterpret_cast<bf16x8 *>(to + 512) = widen<FP8>(side == 0 ? w[2] : w[1], w[3]);
     }
   };
+
   // Queries: lane (r, g) holds elements 16 ks + 8 g .. + 7 of its row for every step ks.
   bf16x8 qf[kQSteps];
   {
@@ -490,6 +492,11 @@ __global__ __launch_bounds__(NW * kWave, 2) void kv8_tile_kernel(Kv8Attention a)
     for (int ks = 0; ks < kQSteps; ++ks)
       qf[ks] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(qp + 16 * ks));
   }
+  // The queries are in registers before the loop: where they may still be on their way as it is entered, every
+  // round waits for the codes that it has just asked for (2.0 us a tile).
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  asm volatile("" ::: "memory");
   f32x16 o[kDTiles];
 #pragma unroll
   for (int d = 0; d < kDTiles; ++d)
@@ -497,35 +504,37 @@ __global__ __launch_bounds__(NW * kWave, 2) void kv8_tile_kernel(Kv8Attention a)
     for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
   float m = -FLT_MAX, l = 0.f;
 
-  Scales x = {}, next = {}, later = {};
-  if (n_tiles > 0) {
-    next = load(0);
-    store(0);
-    if (n_tiles > 1) later = load(1);
-  }
-  for (int t = 0; t < n_tiles; ++t) {
-    __syncthreads();
-    x = next;
-    next = later;
-    if (t + 1 < n_tiles) {
-      store(t + 1);
-      if (t + 2 < n_tiles) later = load(t + 2);
-    }
-    const int key0 = (first + t * kSub) * kKvBlock;
-    if (key0 >= wave_end) continue;
-    const uint8_t *kt = lds[t & 1] + lane * 16;
-    const uint8_t *vt = kt + kSide;
-    f32x16 s[kSub];
+  // Operands are read a few products ahead of their use, the first ones before other work: LDS answers after some
+  // 130 cycles, four products of a wave.
+  constexpr int kAhead = 3;
+  bf16x8 kf[kAhead + 1][kSub], vf[2][kDTiles];
+  const auto read_keys = [&](int t, int ks) {
+    const uint8_t *from = lds + (t & 1) * kSide + lane * 16 + ks * 1024;
+#pragma unroll
+    for (int j = 0; j < kSub; ++j)
+      kf[ks % (kAhead + 1)][j] = *reinterpret_cast<const bf16x8 *>(from + j * (kSide / kSub));
+  };
+  const auto read_values = [&](int t, int f) {
+    const uint8_t *from = lds + (2 + (t & 1)) * kSide + lane * 16 + (f / 2) * (kSide / kSub) + f % 2 * 1024;
+#pragma unroll
+    for (int d = 0; d < kDTiles; ++d) vf[f & 1][d] = *reinterpret_cast<const bf16x8 *>(from + d * 2048);
+  };
+  f32x16 s[kSub];  // scores of the tile in hand
+  const auto scores = [&](int t) {
 #pragma unroll
     for (int j = 0; j < kSub; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[j][e] = 0.f;
 #pragma unroll
-    for (int ks = 0; ks < kQSteps; ++ks)
+    for (int ks = 0; ks < kQSteps; ++ks) {
+      if (ks + kAhead < kQSteps) read_keys(t, ks + kAhead);
 #pragma unroll
       for (int j = 0; j < kSub; ++j)
-        s[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            *reinterpret_cast<const bf16x8 *>(kt + j * (kSide / kSub) + ks * 1024), qf[ks], s[j], 0, 0, 0);
+        s[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks % (kAhead + 1)][j], qf[ks], s[j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  const auto weigh = [&](int t, const Scales &x) {  // softmax, then the values
     float scale[kSub];
 #pragma unroll
     for (int j = 0; j < kSub; ++j) {
@@ -576,11 +585,40 @@ __global__ __launch_bounds__(NW * kWave, 2) void kv8_tile_kernel(Kv8Attention a)
       p[2 * j + 1] = __builtin_bit_cast(bf16x8, (u32x4){w[4], w[5], w[6], w[7]});
     }
 #pragma unroll
-    for (int f = 0; f < 2 * kSub; ++f)
+    for (int f = 0; f < 2 * kSub; ++f) {
+      if (f + 1 < 2 * kSub) read_values(t, f + 1);
 #pragma unroll
       for (int d = 0; d < kDTiles; ++d)
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            *reinterpret_cast<const bf16x8 *>(vt + (f / 2) * (kSide / kSub) + (d * 2 + f % 2) * 1024), p[f], o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[f & 1][d], p[f], o[d], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  const auto sees = [&](int t) { return (first + t * kSub) * kKvBlock < wave_end; };  // any key of the tile
+
+  Scales x = {}, next = {}, later = {};
+  if (n_tiles > 0) {
+    next = load(0);
+    store(0);
+    if (n_tiles > 1) later = load(1);
+  }
+  for (int t = 0; t < n_tiles; ++t) {
+    __syncthreads();
+    x = next;
+    next = later;
+    if (sees(t)) {
+#pragma unroll
+      for (int ks = 0; ks < kAhead; ++ks) read_keys(t, ks);
+    }
+    if (t + 1 < n_tiles) {
+      store(t + 1);
+      if (t + 2 < n_tiles) later = load(t + 2);
+    }
+    if (sees(t)) {
+      scores(t);
+      read_values(t, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      weigh(t, x);
+    }
   }
 
   if (row0 + r >= a.rows) return;
@@ -684,23 +722,13 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8Attention a) {
       (u32x2){pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
 }
 
-template <int D, bool FP8, int NW>
-void start_tiles(const Kv8Attention &p, hipStream_t stream) {
-  const dim3 grid((p.items + p.xcds - 1) / p.xcds * p.xcds), block(NW * kWave);
-  if (p.splits > 1) hipLaunchKernelGGL((kv8_tile_kernel<D, FP8, NW, true>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((kv8_tile_kernel<D, FP8, NW, false>), grid, block, 0, stream, p);
-}
-
 template <int D, bool FP8>
 hipError_t launch_attend(const Kv8Attention &p, hipStream_t stream) {
-  switch (p.waves) {
-    case 0:
-      if (p.rows <= 16) hipLaunchKernelGGL((kv8_rows_kernel<D, FP8, 1>), dim3(p.items), dim3(512), 0, stream, p);
-      else hipLaunchKernelGGL((kv8_rows_kernel<D, FP8, 2>), dim3(p.items), dim3(512), 0, stream, p);
-      break;
-    case 4: start_tiles<D, FP8, 4>(p, stream); break;
-    default: start_tiles<D, FP8, 8>(p, stream); break;
-  }
+  const dim3 block(kTileWaves * kWave), grid(p.items), xcd_grid((p.items + p.xcds - 1) / p.xcds * p.xcds);
+  if (p.tile_rows <= 16) hipLaunchKernelGGL((kv8_rows_kernel<D, FP8, 1>), grid, block, 0, stream, p);
+  else if (p.tile_rows == 32) hipLaunchKernelGGL((kv8_rows_kernel<D, FP8, 2>), grid, block, 0, stream, p);
+  else if (p.splits > 1) hipLaunchKernelGGL((kv8_tile_kernel<D, FP8, true>), xcd_grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((kv8_tile_kernel<D, FP8, false>), xcd_grid, block, 0, stream, p);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || p.splits == 1) return err;
   hipLaunchKernelGGL((kv8_join_kernel<D>), dim3(static_cast<unsigned>(p.tile_items * p.tile_rows)), dim3(256), 0,
@@ -912,29 +940,44 @@ __global__ __launch_bounds__(256) void kv8_copy_kernel(Kv8Copy) {
 
 }  // namespace
 
+// Which kernel runs, and how often the keys are split, by what it costs in units of 0.1 us: a round of workgroups, one
+// a CU, takes a start and its blocks; the join a launch and the partial values' way through memory and back.
+//                                 a block  a start
+//   up to 16 rows                       1       16
+//   tiles of 32 rows                    2       30
+//   tiles of 256 rows                  10       40
+// Measured, us, on eight heads unless said: 1 token (8 rows) over 500 keys 6.8 unsplit, 9.0 in two; over 32000 18.0 in
+// 32 splits, 21.9 in 63, 36 in 4; 256 heads over 4096 keys 48.5 unsplit, 56 in two. 512 rows over 500 keys 10.9 in
+// tiles of 32 and 26.8 in tiles of 256, over 4000 31.4 and 38.0, over 30000 132 and 98; 128 heads of 512 rows over
+// 2000 keys 205 and 111, 32 heads 52.5 and 62. Up to 64 rows tiles of 32 were never slower (14.6 and 18.7 over 4000).
 void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, int cus, int xcds) {
   p->xcds = std::max(1, xcds);
   p->rep = p->heads / p->kv.kv_heads;
   p->rows = p->t * p->rep;
   const int64_t heads = static_cast<int64_t>(p->batch) * p->kv.kv_heads;
   const int64_t blocks = std::max<int64_t>(1, (max_tokens + kKvBlock - 1) / kKvBlock);
-  // Up to 16 rows (decode) the codes go from memory straight into the products; more rows share them through LDS.
-  p->waves = p->rows <= 64 ? 0 : 8;
-  p->tile_rows = p->waves > 0 ? 32 * p->waves : p->rows <= 16 ? p->rows : 32;
+  int64_t best = INT64_MAX, splits = 1;
+  const auto weigh = [&](int tile_rows, int64_t block_cost, int64_t start_cost) {
+    const int64_t items = heads * ((p->rows + tile_rows - 1) / tile_rows);
+    for (int64_t rounds = 0; rounds <= 8; ++rounds) {  // whole rounds of splits, or none
+      const int64_t s = rounds == 0 ? 1 : std::min(rounds * cus / items, blocks / 8);
+      if (s < 1 || (rounds > 0 && s == 1)) continue;
+      const int64_t cost = (items * s + cus - 1) / cus * ((blocks + s - 1) / s * block_cost + start_cost) +
+                           (s > 1 ? 30 + items * tile_rows * s / 385 : 0);
+      if (cost >= best) continue;
+      best = cost;
+      splits = s;
+      p->tile_rows = tile_rows;
+    }
+  };
+  if (p->rows <= 16) {
+    weigh(p->rows, 1, 16);
+  } else {
+    weigh(32, 2, 30);
+    if (p->rows > 64) weigh(32 * kTileWaves, 10, 40);
+  }
   p->row_tiles = (p->rows + p->tile_rows - 1) / p->tile_rows;
   p->tile_items = heads * p->row_tiles;
-  // How often the keys are split. A round of workgroups, one a CU, takes its blocks and a start of about 16 more; the
-  // join takes about 30 (decode: 0.1 us a block; 16 blocks of 8 heads 6.8 us, split in two 9.0). Splits fill whole
-  // rounds: 8 heads over 1001 blocks 18.0 us in 32 splits, 21.9 in 63, 36 in 4; 256 heads over 129 blocks 48.5 us
-  // unsplit and 56 in two.
-  const auto cost = [&](int64_t splits) {
-    return (p->tile_items * splits + cus - 1) / cus * ((blocks + splits - 1) / splits + 16) + (splits > 1 ? 30 : 0);
-  };
-  int64_t splits = 1;
-  for (int64_t rounds = 1; rounds <= 8; ++rounds) {
-    const int64_t s = std::min(rounds * cus / p->tile_items, blocks / 8);
-    if (s > 1 && cost(s) < cost(splits)) splits = s;
-  }
   p->chunk = static_cast<int>((blocks + splits - 1) / splits);  // the last one goes on to the end of the sequence,
   p->splits = static_cast<int>((blocks + p->chunk - 1) / p->chunk);  // whatever max_tokens says
   const int64_t items = p->tile_items * p->splits;

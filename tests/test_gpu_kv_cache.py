@@ -268,3 +268,40 @@ def test_copy_pages_copies_bytes(gpu, dtype, layers, pages, kv, page, d, n):
     want[:, dst], want_scales[:, dst] = want[:, src], want_scales[:, src]
     kvc.copy_pages(codes, scales, src, dst)
     assert torch.equal(codes.view(torch.uint8), want) and torch.equal(scales, want_scales)
+
+
+def _attend64_gpu(q, codes, scales, table, starts, new):
+    """The same on the GPU, head by head, for prompts."""
+    b, t, h, d = q.shape
+    kv, size = codes.shape[2], codes.shape[3] * BLOCK
+    out = torch.zeros(b, t, h, d, dtype=torch.float64, device=q.device)
+    for n in range(b):
+        count = new[n] if new is not None else t
+        length = starts[n] + count
+        keys, vals = (x[0, :length].double() for x in kvc.read(codes, scales, table[n: n + 1, : -(-length // size)]))
+        seen = torch.arange(length, device=q.device) <= starts[n] + torch.arange(count, device=q.device)[:, None]
+        for head in range(h):
+            j = head // (h // kv)
+            s = (q[n, :count, head].double() @ keys[:, j].t().contiguous() / math.sqrt(d)).masked_fill(~seen, -math.inf)
+            out[n, :count, head] = torch.softmax(s, -1) @ vals[:, j].contiguous()
+    return out
+
+
+@pytest.mark.parametrize("dtype", FORMATS)
+@pytest.mark.parametrize("b,t,h,kv,d,page,starts,new", [
+    (1, 300, 64, 64, 128, 64, [0], None), (2, 290, 64, 64, 64, 32, [33, 0], [290, 1]),  # tiles of 256 rows, unsplit
+    (1, 257, 128, 128, 128, 128, [511], None),
+    (1, 64, 64, 8, 128, 64, [30000], None), (2, 300, 24, 8, 64, 64, [9000, 20], [300, 299]),  # and split over the keys
+])
+def test_prompts_match_float64(gpu, dtype, b, t, h, kv, d, page, starts, new):
+    width = (max(starts) + t + page - 1) // page
+    codes, scales = _pool(gpu, b * width, kv, page, d, dtype)
+    g = _gen(gpu, b, t, h, d, page)
+    table = torch.randperm(b * width, device=gpu, generator=g).view(b, width).int()
+    q = torch.randn(b, t, h, d, device=gpu, generator=g).mul(2.0).bfloat16()
+    starts_t = torch.tensor(starts, dtype=torch.int32, device=gpu)
+    new_t = torch.tensor(new, dtype=torch.int32, device=gpu) if new is not None else None
+    want = _attend64_gpu(q, codes, scales, table, starts, new)
+    got = kvc.attention(q, codes, scales, table, starts_t, new_t).double()
+    assert (got - want).norm() <= TWO_ROUNDINGS * want.norm()
+    assert ((got - want).norm(dim=-1) <= 4 * TWO_ROUNDINGS * want.norm(dim=-1).clamp(min=1e-30)).all()
