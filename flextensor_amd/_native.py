@@ -181,6 +181,9 @@ _SIGNATURES: dict[str, list] = {
     "ftx_int8_quantize": [_vp, ctypes.c_int64, _vp, _vp, ctypes.c_int64, ctypes.c_int64, _vp],
     "ftx_int8_matmul_workspace": [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(_sz)],
     "ftx_int8_matmul": [_vp, _vp, _vp, _vp, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp, _sz, _vp],
+    "ftx_int8_linear_workspace": [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(_sz)],
+    "ftx_int8_linear": [_vp, ctypes.c_int64, _vp, _vp, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp, _sz,
+                        _vp],
     "ftx_kv8_append": [ctypes.POINTER(Kv8Cache), _vp, _vp, _vp, _vp, _vp, ctypes.c_int64, _vp, ctypes.c_int64,
                        ctypes.c_int64, _int, _vp, _vp],
     "ftx_kv8_attention_workspace": [ctypes.c_int64, ctypes.c_int64, _int, _int, _int, ctypes.c_int64,

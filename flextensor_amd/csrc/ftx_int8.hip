@@ -63,7 +63,8 @@ __device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t bytes,
 // ---- codes and scales of the rows --------------------------------------------------------------------------------
 //
 // The largest magnitude's bits order as integers, and a NaN's are above all: a row that holds an infinity or a NaN
-// gets the scale NaN, and codes of 0. Each row is read twice, the second time from the caches.
+// gets the scale NaN, and codes of 0. A row of up to 8192 values is held in the registers of 256 threads, of up to
+// 32768 of 1024 (one row of 28672: 7.6 us with 256 threads that read it twice); what is longer is read twice.
 
 __device__ __forceinline__ uint32_t largest8(u32x4 v, uint32_t top) {
 #pragma unroll
@@ -93,24 +94,39 @@ __device__ __forceinline__ u32x2 code8(u32x4 v, float inverse) {
                                   code2(v[2], inverse) | code2(v[3], inverse) << 16};
 }
 
-__global__ __launch_bounds__(256) void int8_quantize_kernel(const uint16_t *__restrict__ x, int64_t x_stride,
-                                                            uint8_t *__restrict__ codes, int64_t code_stride,
-                                                            float *__restrict__ scales, int k) {
-  __shared__ uint32_t wave_top[4];
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void int8_quantize_kernel(const uint16_t *__restrict__ x, int64_t x_stride,
+                                                                uint8_t *__restrict__ codes, int64_t code_stride,
+                                                                float *__restrict__ scales, int k) {
+  constexpr int kHeld = 4;  // vectors of 8 values that a thread keeps
+  __shared__ uint32_t wave_top[THREADS / kWave];
   const int64_t row = blockIdx.x;
   const u32x4 *xr = reinterpret_cast<const u32x4 *>(x + row * x_stride);
-  const int n = k / 8;
+  const int n = k / 8, first = threadIdx.x;
+  u32x4 held[kHeld];
   uint32_t top = 0;
-  for (int i = threadIdx.x; i < n; i += 256) top = largest8(xr[i], top);
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    held[i] = (u32x4){0u, 0u, 0u, 0u};
+    if (first + i * THREADS < n) held[i] = xr[first + i * THREADS];
+  }
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) top = largest8(held[i], top);
+  for (int i = first + kHeld * THREADS; i < n; i += THREADS) top = largest8(xr[i], top);
 #pragma unroll
   for (int i = 1; i < kWave; i *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), i)));
   if (threadIdx.x % kWave == 0) wave_top[threadIdx.x / kWave] = top;
   __syncthreads();
-  top = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
+#pragma unroll
+  for (int i = 0; i < THREADS / kWave; ++i) top = max(top, wave_top[i]);
   float inverse;
   const float scale = row_scale(top, &inverse);
   u32x2 *to = reinterpret_cast<u32x2 *>(codes + row * code_stride);
-  for (int i = threadIdx.x; i < code_stride / 8; i += 256) to[i] = i < n ? code8(xr[i], inverse) : (u32x2){0u, 0u};
+  const int end = static_cast<int>(code_stride / 8);  // past n the row ends in zeros
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (first + i * THREADS < end) to[first + i * THREADS] = code8(held[i], inverse);
+  for (int i = first + kHeld * THREADS; i < end; i += THREADS) to[i] = i < n ? code8(xr[i], inverse) : (u32x2){0u, 0u};
   if (threadIdx.x == 0) scales[row] = scale;
 }
 
@@ -245,32 +261,47 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void int8_tile_kernel(Int8Linea
   const int all = (p.k + kStep - 1) / kStep;
   const int first = SPLIT ? split * p.split_steps : 0;
   const int end = SPLIT ? min(all, first + p.split_steps) : all;
-  issue(first);
-  for (int step = first; step < end; ++step) {
-    wait_vmcnt<0>();
-    ring_barrier();
-    if (step + 1 < end) issue(step + 1);
+  i32x4 a[2][kNT], b[2][kMT];  // operands of 32 of K, the next ones read during this one's products
+  const auto read = [&](int step, int ks) {
     const uint8_t *stage = lds + (step & 1) * kStage;
-    // the operands of the next 32 of K are read during this one's products
-    i32x4 a[2][kNT], b[2][kMT];
-    const auto read = [&](int ks) {
-      const uint32_t chunk = ((2 * ks + g) ^ swizzle) * 16;
+    const uint32_t chunk = ((2 * ks + g) ^ swizzle) * 16;
 #pragma unroll
-      for (int i = 0; i < kNT; ++i) a[ks & 1][i] = *reinterpret_cast<const i32x4 *>(stage + a_at[i] + chunk);
+    for (int i = 0; i < kNT; ++i) a[ks & 1][i] = *reinterpret_cast<const i32x4 *>(stage + a_at[i] + chunk);
 #pragma unroll
-      for (int j = 0; j < kMT; ++j) b[ks & 1][j] = *reinterpret_cast<const i32x4 *>(stage + b_at[j] + chunk);
-    };
-    read(0);
+    for (int j = 0; j < kMT; ++j) b[ks & 1][j] = *reinterpret_cast<const i32x4 *>(stage + b_at[j] + chunk);
+  };
+  const auto multiply = [&](int ks) {
 #pragma unroll
-    for (int ks = 0; ks < kStep / 32; ++ks) {
-      if (ks + 1 < kStep / 32) read(ks + 1);
+    for (int j = 0; j < kMT; ++j)
 #pragma unroll
-      for (int j = 0; j < kMT; ++j)
+      for (int i = 0; i < kNT; ++i)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[ks & 1][i], b[ks & 1][j], acc[i][j], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  constexpr int kLast = kStep / 32 - 1;
+  issue(first);
+  if (first + 1 < end) {
+    issue(first + 1);
+    wait_vmcnt<kLoads>();
+  } else {
+    wait_vmcnt<0>();
+  }
+  ring_barrier();
+  read(first, 0);
+  for (int step = first; step < end; ++step) {
 #pragma unroll
-        for (int i = 0; i < kNT; ++i)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[ks & 1][i], b[ks & 1][j], acc[i][j], 0, 0, 0);
+    for (int ks = 0; ks < kLast; ++ks) {
+      read(step, ks + 1);
+      multiply(ks);
+    }
+    if (step + 1 < end) {  // the stage has been read by all: the barrier and the next one's first reads meet its last products
+      wait_vmcnt<0>();
+      ring_barrier();
+      if (step + 2 < end) issue(step + 2);
+      read(step + 1, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
+    multiply(kLast);
   }
 
   if (SPLIT) {  // integer sums [split][m][n]
@@ -361,34 +392,72 @@ void start_tiles(const Int8Linear &p, hipStream_t stream) {
 
 hipError_t launch_int8_quantize(const uint16_t *x, int64_t x_stride, uint8_t *codes, int64_t code_stride, float *scales,
                                 int64_t m, int k, hipStream_t stream) {
-  hipLaunchKernelGGL(int8_quantize_kernel, dim3(static_cast<unsigned>(m)), dim3(256), kLdsToken, stream, x, x_stride,
-                     codes, code_stride, scales, k);
+  const dim3 grid(static_cast<unsigned>(m));
+  if (k <= 8192)
+    hipLaunchKernelGGL(int8_quantize_kernel<256>, grid, dim3(256), kLdsToken, stream, x, x_stride, codes, code_stride,
+                       scales, k);
+  else
+    hipLaunchKernelGGL(int8_quantize_kernel<1024>, grid, dim3(1024), kLdsToken, stream, x, x_stride, codes,
+                       code_stride, scales, k);
   return hipGetLastError();
 }
 
+// Which kernel and how often K is split, by what it costs in 0.01 us: the larger of the products (a step of 128 of K
+// takes a workgroup `alone` at least, a CU `shared` for each of its workgroups) and of reading w (5.3 TB/s, 4.2 with
+// fewer than three workgroups for two CUs), a start, and the join of the splits. Tiles of 256 x 256 have a CU to themselves,
+// so theirs come in whole rounds.
+//                    alone  shared  start
+//   64 x 128            80      41     400
+//   128 x 128           95      64     700
+//   256 x 256     150, 190 in more rounds than one     1000
+// Measured, us: 28672 x 8192 of 40 rows 49.0 in tiles of 64 split in two, 58.2 unsplit; of 200 rows 118, 74.6 and 101
+// in tiles of 64, 128 and 256, of 512 rows 193, 150 and 114, of 1000 360, 292 and 239; 4096 x 4096 of 512 rows 21.3,
+// 25.0 and 49.2; 8192 x 28672 of 512 rows 131 in tiles of 256 split in four, 164 in tiles of 128 split in two. Up to
+// 16 rows the kernel without tiles is the faster one while w is small (11008 x 4096 of 13 rows 12.9, in tiles 15.1) or
+// the rows are few (28672 x 8192 of one row 44.3, of four 50.7 and 45.0 in tiles, of 13 63.4 and 45.8): each of its
+// workgroups reads all rows' codes.
 void plan_int8_linear(Int8Linear *p, int cus, int xcds) {
   p->xcds = std::max(1, xcds);
-  p->splits = 1;
-  p->split_steps = 0;
   p->part_stride = (p->n + 3) / 4 * 4;
-  p->band = 8;
-  if (p->m <= 16) {
+  const int64_t steps = std::max(1, (p->k + 127) / 128);
+  const int64_t reading = p->n * p->k / 53000;
+  int64_t best = INT64_MAX, splits = 1;
+  const auto weigh = [&](int tm, int tn, int64_t alone, int64_t shared, int64_t start) {
+    const int64_t tiles = ((p->m + tm - 1) / tm) * ((p->n + tn - 1) / tn);
+    for (int64_t s = 1; s <= 16 && (s == 1 || steps / s >= 2); s *= 2) {
+      const int64_t items = tiles * s, length = (steps + s - 1) / s;
+      const int64_t rounds = (items + cus - 1) / cus;
+      const int64_t products = tm == 256 ? rounds * length * (rounds == 1 ? alone : shared)
+                                         : length * std::max(alone, shared * items / cus);
+      const int64_t cost = std::max(products, 2 * items < 3 * cus ? reading * 5 / 4 : reading) + start +
+                           (s > 1 ? 250 + p->m * p->n * s / 5000 : 0);
+      if (cost >= best) continue;
+      best = cost;
+      splits = s;
+      p->tile_m = tm;
+      p->tile_n = tn;
+    }
+  };
+  weigh(64, 128, 80, 41, 400);
+  if (p->m > 64) weigh(128, 128, 95, 64, 700);
+  if (p->m > 128) weigh(256, 256, 150, 190, 1000);
+  if (p->m <= 16 && reading * (1000 + 35 * p->m) / 1000 + 250 <= best) {
     p->tile_m = 16;
+    p->splits = 1;
     p->items = static_cast<uint32_t>((p->n + 15) / 16);
     p->part_bytes = 0;
     return;
   }
-  const auto tiles = [&](int64_t tm, int64_t tn) { return ((p->m + tm - 1) / tm) * ((p->n + tn - 1) / tn); };
-  p->tile_m = p->m > 128 && tiles(256, 256) >= cus ? 256 : p->m > 64 ? 128 : 64;
-  p->tile_n = p->tile_m == 256 ? 256 : 128;
   p->m_tiles = static_cast<uint32_t>((p->m + p->tile_m - 1) / p->tile_m);
   p->n_tiles = static_cast<uint32_t>((p->n + p->tile_n - 1) / p->tile_n);
-  const int64_t count = static_cast<int64_t>(p->m_tiles) * p->n_tiles;
-  const int steps = (p->k + 127) / 128;
-  const int64_t want = std::min<int64_t>(p->tile_m == 256 ? 1 : std::max<int64_t>(1, 2 * cus / count), (steps + 7) / 8);
-  p->split_steps = static_cast<int>((steps + want - 1) / want);
-  p->splits = (steps + p->split_steps - 1) / p->split_steps;
-  p->items = static_cast<uint32_t>(std::min<int64_t>(count * p->splits, UINT32_MAX));
+  // An XCD walks a run of up to 12 tiles of tokens before its next tile of channels, equal runs: their codes and the
+  // channels' are in its L2 for the others.
+  const uint32_t runs = (p->m_tiles + 11) / 12;
+  p->band = static_cast<int>((p->m_tiles + runs - 1) / runs);
+  p->split_steps = static_cast<int>((steps + splits - 1) / splits);
+  p->splits = static_cast<int>((steps + p->split_steps - 1) / p->split_steps);
+  const int64_t items = static_cast<int64_t>(p->m_tiles) * p->n_tiles * p->splits;
+  p->items = static_cast<uint32_t>(std::min<int64_t>(items, UINT32_MAX));  // too many for a launch: the caller refuses
   p->part_bytes = p->splits > 1 ? static_cast<size_t>(p->splits) * p->m * p->part_stride * 4 : 0;
 }
 

@@ -1700,6 +1700,26 @@ int ftx_int8_matmul_workspace(int64_t m, int64_t n, int64_t k, size_t *bytes) {
   return rc;
 }
 
+namespace {
+
+// The operands of a planned product but for its codes and their scales.
+int check_int8_product(ftx::Int8Linear *p, const void *w, const float *w_scale, void *y) {
+  int rc = FTX_OK;
+  if (p->k > 0) rc = check_operand(w, p->n * p->k, 1, "int8 weight");
+  if (rc == FTX_OK) rc = check_operand(w_scale, p->n, 4, "int8 channel scales");
+  if (rc == FTX_OK) rc = check_operand(y, p->m * p->n, 2, "int8 output");
+  p->w = static_cast<const uint8_t *>(w);
+  p->w_scale = w_scale;
+  p->y = static_cast<uint16_t *>(y);
+  return rc;
+}
+
+// The workspace of ftx_int8_linear: the codes, their scales and the split sums, in that order.
+size_t int8_scale_offset(const ftx::Int8Linear &p) { return static_cast<size_t>(p.m) * p.code_stride; }
+size_t int8_part_offset(const ftx::Int8Linear &p) { return int8_scale_offset(p) + (p.m * 4 + 255) / 256 * 256; }
+
+}  // namespace
+
 int ftx_int8_matmul(const void *codes, const float *x_scale, const void *w, const float *w_scale, void *y, int64_t m,
                     int64_t n, int64_t k, void *workspace, size_t workspace_bytes, void *stream) {
   FTX_REQUIRE_LIVE();
@@ -1708,23 +1728,55 @@ int ftx_int8_matmul(const void *codes, const float *x_scale, const void *w, cons
   if (rc != FTX_OK) return rc;
   if (m == 0 || n == 0) return FTX_OK;
   if (k > 0) rc = check_operand(codes, m * p.code_stride, 1, "int8 codes");
-  if (rc == FTX_OK && k > 0) rc = check_operand(w, n * k, 1, "int8 weight");
   if (rc == FTX_OK) rc = check_operand(x_scale, m, 4, "int8 row scales");
-  if (rc == FTX_OK) rc = check_operand(w_scale, n, 4, "int8 channel scales");
-  if (rc == FTX_OK) rc = check_operand(y, m * n, 2, "int8 output");
+  if (rc == FTX_OK) rc = check_int8_product(&p, w, w_scale, y);
   if (rc == FTX_OK && p.part_bytes > 0) {
     if (workspace_bytes < p.part_bytes)
-      return ftx::fail(FTX_ERR_INVALID, "the int8 linear needs a workspace of " + std::to_string(p.part_bytes) +
+      return ftx::fail(FTX_ERR_INVALID, "the int8 product needs a workspace of " + std::to_string(p.part_bytes) +
                                             " bytes (ftx_int8_matmul_workspace)");
     rc = check_operand(workspace, static_cast<int64_t>(p.part_bytes), 1, "int8 workspace");
   }
   if (rc != FTX_OK) return rc;
   p.codes = static_cast<const uint8_t *>(codes);
   p.x_scale = x_scale;
-  p.w = static_cast<const uint8_t *>(w);
-  p.w_scale = w_scale;
-  p.y = static_cast<uint16_t *>(y);
   p.part = static_cast<int *>(workspace);
+  FTX_HIP(ftx::launch_int8_linear(p, static_cast<hipStream_t>(stream)));
+  return FTX_OK;
+}
+
+int ftx_int8_linear_workspace(int64_t m, int64_t n, int64_t k, size_t *bytes) {
+  if (!bytes) return ftx::fail(FTX_ERR_INVALID, "bytes is null");
+  ftx::Int8Linear p{};
+  int rc = plan_int8(m, n, k, &p);
+  if (rc == FTX_OK) *bytes = m == 0 || n == 0 ? 0 : int8_part_offset(p) + p.part_bytes;
+  return rc;
+}
+
+int ftx_int8_linear(const void *x, int64_t x_stride, const void *w, const float *w_scale, void *y, int64_t m, int64_t n,
+                    int64_t k, void *workspace, size_t workspace_bytes, void *stream) {
+  FTX_REQUIRE_LIVE();
+  ftx::Int8Linear p{};
+  int rc = plan_int8(m, n, k, &p);
+  if (rc != FTX_OK) return rc;
+  if (x_stride < k || x_stride % 8 != 0 || x_stride > int64_t(1) << 38)
+    return ftx::fail(FTX_ERR_INVALID, "int8 linear: rows of x must not overlap and start at multiples of 8 elements");
+  if (m == 0 || n == 0) return FTX_OK;
+  if (k > 0) rc = check_operand(x, (m - 1) * x_stride + k, 2, "int8 input");
+  if (rc == FTX_OK) rc = check_int8_product(&p, w, w_scale, y);
+  if (rc != FTX_OK) return rc;
+  const size_t need = int8_part_offset(p) + p.part_bytes;
+  if (workspace_bytes < need)
+    return ftx::fail(FTX_ERR_INVALID, "the int8 linear needs a workspace of " + std::to_string(need) +
+                                          " bytes (ftx_int8_linear_workspace)");
+  rc = check_operand(workspace, static_cast<int64_t>(need), 1, "int8 workspace");
+  if (rc != FTX_OK) return rc;
+  uint8_t *ws = static_cast<uint8_t *>(workspace);
+  float *scales = reinterpret_cast<float *>(ws + int8_scale_offset(p));
+  FTX_HIP(ftx::launch_int8_quantize(static_cast<const uint16_t *>(x), x_stride, ws, p.code_stride, scales, m, p.k,
+                                    static_cast<hipStream_t>(stream)));
+  p.codes = ws;
+  p.x_scale = scales;
+  p.part = reinterpret_cast<int *>(ws + int8_part_offset(p));
   FTX_HIP(ftx::launch_int8_linear(p, static_cast<hipStream_t>(stream)));
   return FTX_OK;
 }

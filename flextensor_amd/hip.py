@@ -777,6 +777,22 @@ INT8_LINEAR_MAX_K = 131072  # the 32-bit sums hold 127^2 times this
 _INT8_WORKSPACE: dict[tuple, int] = {}
 
 
+def _int8_rows(what: str, x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """Checked rows [m, k] and their stride, a copy where they cannot be read 16 bytes at a time."""
+    if x.dim() != 2:
+        raise ValueError(f"{what} takes rows [m, k], got {tuple(x.shape)}")
+    _check_operands(what, x=x)
+    m, k = x.shape
+    if k % 16 or k > INT8_LINEAR_MAX_K:
+        raise ValueError(f"{what} needs k a multiple of 16, up to {INT8_LINEAR_MAX_K}, not {k}")
+    stride, inner = x.stride()
+    if m <= 1:
+        stride = k
+    if (inner != 1 and k > 1) or stride < k or stride % 8 or x.data_ptr() % 16:
+        x, stride = x.clone(memory_format=torch.contiguous_format), k
+    return x, stride
+
+
 def int8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``(codes, scales)`` of bf16 rows [m, k]: ``codes = round(x / s)`` with a row's ``s = max |x| / 127``
     (``ftx_int8_quantize``).
@@ -785,16 +801,8 @@ def int8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     :func:`int8_matmul` reads. A row that holds an infinity or a NaN has the scale NaN. ``k`` is a multiple of 16;
     rows may be strided.
     """
-    if x.dim() != 2:
-        raise ValueError(f"int8_quantize takes rows [m, k], got {tuple(x.shape)}")
-    _check_operands("int8_quantize", x=x)
+    x, stride = _int8_rows("int8_quantize", x)
     m, k = x.shape
-    if k % 16 or k > INT8_LINEAR_MAX_K:
-        raise ValueError(f"int8_quantize needs k a multiple of 16, up to {INT8_LINEAR_MAX_K}, not {k}")
-    stride = x.stride(0) if m > 1 else k
-    if x.stride(1) != 1 or stride < k or stride % 8 or x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
-        stride = k
     codes = torch.empty((m, (k + 255) // 256 * 256), dtype=torch.int8, device=x.device)
     scales = torch.empty(m, dtype=torch.float32, device=x.device)
     nat.call("ftx_int8_quantize", x.data_ptr(), stride, codes.data_ptr(), scales.data_ptr(), m, k, _stream())
@@ -831,33 +839,40 @@ def int8_matmul(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor,
     if not _packed(codes, scales):
         raise ValueError("int8_matmul needs contiguous, 16-byte aligned codes and scales")
     n = _check_int8_weight("int8_matmul", weight, scale, k, codes.device)
-    return _int8_matmul(codes, scales, weight, scale, codes.shape[0], n, k)
-
-
-def _int8_matmul(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, m: int, n: int,
-                 k: int) -> torch.Tensor:
+    m = codes.shape[0]
     y = torch.empty((m, n), dtype=torch.bfloat16, device=codes.device)
-    ws_bytes = _INT8_WORKSPACE.get((m, n, k))
-    if ws_bytes is None:
-        got = ctypes.c_size_t(0)
-        nat.call("ftx_int8_matmul_workspace", m, n, k, ctypes.byref(got))
-        if len(_INT8_WORKSPACE) >= 4096:
-            _INT8_WORKSPACE.clear()
-        ws_bytes = _INT8_WORKSPACE[m, n, k] = int(got.value)
+    ws_bytes = _int8_workspace("ftx_int8_matmul_workspace", m, n, k)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=codes.device) if ws_bytes else None
     nat.call("ftx_int8_matmul", codes.data_ptr(), scales.data_ptr(), weight.data_ptr(), scale.data_ptr(), y.data_ptr(),
              m, n, k, ws.data_ptr() if ws is not None else None, ws_bytes, _stream())
     return y
 
 
+def _int8_workspace(name: str, m: int, n: int, k: int) -> int:
+    key = (name, m, n, k)
+    got = _INT8_WORKSPACE.get(key)
+    if got is None:
+        b = ctypes.c_size_t(0)
+        nat.call(name, m, n, k, ctypes.byref(b))
+        if len(_INT8_WORKSPACE) >= 4096:
+            _INT8_WORKSPACE.clear()
+        got = _INT8_WORKSPACE[key] = int(b.value)
+    return got
+
+
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     """``x @ (weight * scale[:, None]).T`` with ``x`` rounded to 8 bits, a scale for each row: :func:`int8_quantize`,
-    then :func:`int8_matmul`. ``x``: bf16 [m, k], ``weight``: int8 [n, k], ``scale``: fp32 [n]; no backward."""
-    if x.dim() != 2:
-        raise ValueError(f"int8_linear takes x [m, k], got {tuple(x.shape)}")
-    n = _check_int8_weight("int8_linear", weight, scale, x.shape[1], x.device)
-    codes, scales = int8_quantize(x)
-    return _int8_matmul(codes, scales, weight, scale, x.shape[0], n, x.shape[1])
+    then :func:`int8_matmul`, in one call (``ftx_int8_linear``). ``x``: bf16 [m, k], k a multiple of 16; ``weight``:
+    int8 [n, k], -127 .. 127; ``scale``: fp32 [n]; no backward."""
+    x, stride = _int8_rows("int8_linear", x)
+    m, k = x.shape
+    n = _check_int8_weight("int8_linear", weight, scale, k, x.device)
+    y = torch.empty((m, n), dtype=torch.bfloat16, device=x.device)
+    ws_bytes = _int8_workspace("ftx_int8_linear_workspace", m, n, k)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+    nat.call("ftx_int8_linear", x.data_ptr(), stride, weight.data_ptr(), scale.data_ptr(), y.data_ptr(), m, n, k,
+             ws.data_ptr(), ws_bytes, _stream())
+    return y
 
 
 BF16_LINEAR_MAX_ROWS = 16

@@ -415,12 +415,16 @@ int ftx_silu_mul(const void *g, const void *u, void *y, int64_t n, void *stream)
  * ftx_int8_matmul: y[m, n] = bf16((sum_k codes[m, k] w[n, k]) x_scale[m]
  * w_scale[n]) of such rows and int8 w [n, k] (-127 .. 127, contiguous); the sums
  * are exact. workspace: ftx_int8_matmul_workspace bytes (0 unless K is split).
- * Pointers are 16-byte aligned. */
+ * ftx_int8_linear: the one, then the other, with the codes in its workspace
+ * (ftx_int8_linear_workspace bytes). Pointers are 16-byte aligned. */
 #define FTX_INT8_CODE_STRIDE(k) (((int64_t)(k) + 255) / 256 * 256)
 int ftx_int8_quantize(const void *x, int64_t x_stride, void *codes, float *scales, int64_t m, int64_t k, void *stream);
 int ftx_int8_matmul_workspace(int64_t m, int64_t n, int64_t k, size_t *bytes);
 int ftx_int8_matmul(const void *codes, const float *x_scale, const void *w, const float *w_scale, void *y, int64_t m,
                     int64_t n, int64_t k, void *workspace, size_t workspace_bytes, void *stream);
+int ftx_int8_linear_workspace(int64_t m, int64_t n, int64_t k, size_t *bytes);
+int ftx_int8_linear(const void *x, int64_t x_stride, const void *w, const float *w_scale, void *y, int64_t m, int64_t n,
+                    int64_t k, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---- a KV cache in pages of 8-bit codes --------------------------------------
  * No reference counterpart. One layer is codes, bytes [pages][2][kv_heads]
