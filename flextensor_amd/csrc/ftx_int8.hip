@@ -196,13 +196,15 @@ __global__ __launch_bounds__(512, 4) void int8_rows_kernel(Int8Linear p) {
 
 // ---- tiles -----------------------------------------------------------------------------------------------------------
 //
-// TM tokens x TN channels a workgroup, K in steps of 128. A step's rows go straight from memory into one of two
+// TM tokens x TN channels a workgroup, K in steps of 128. A step's rows go straight from memory into one of STAGES
 // stages of LDS; row R's 16-byte chunk c lies at slot c ^ (R / 2 % 8), which spreads the 16 rows that a phase of
-// ds_read_b128 touches over all banks. The next step's loads are in flight during a step's products.
+// ds_read_b128 touches over all banks. The other stages' loads are in flight during a step's products: one step's
+// where many rows keep the matrix cores busy, two where w's bytes are what takes time (28672 x 8192 of 32 rows in
+// tiles of 64 x 128: 60.7 us with two stages, 50.3 with three, 50.2 with four).
 // v_mfma_i32_32x32x32_i8 takes the channels as rows and the tokens as columns, so a lane ends with four neighbouring
 // channels of a token at a time; they reach y through LDS, in whole lines.
 
-template <int TM, int TN, int WM, int WN, bool SPLIT>
+template <int TM, int TN, int WM, int WN, int STAGES, bool SPLIT>
 __global__ __launch_bounds__(WM * WN * kWave, 2) void int8_tile_kernel(Int8Linear p) {
   constexpr int kWaves = WM * WN;
   constexpr int kStep = 128;
@@ -211,7 +213,7 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void int8_tile_kernel(Int8Linea
   constexpr int kMT = TM / WM / 32, kNT = TN / WN / 32;
   constexpr int kTokenLoads = TM / 8 / kWaves;     // the first of them
   static_assert(kStage / 1024 % kWaves == 0 && TM / 8 % kWaves == 0, "every wave issues the same loads");
-  __shared__ __align__(1024) uint8_t lds[2 * kStage];
+  __shared__ __align__(1024) uint8_t lds[STAGES * kStage];
   const uint32_t per_xcd = (p.items + p.xcds - 1) / p.xcds;
   uint32_t item = (blockIdx.x % p.xcds) * per_xcd + blockIdx.x / p.xcds;
   if (blockIdx.x / p.xcds >= per_xcd || item >= p.items) return;
@@ -237,7 +239,7 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void int8_tile_kernel(Int8Linea
     offset[i] = R * (i < kTokenLoads ? p.code_stride : p.k) + ((lane % 8) ^ (R / 2 % 8)) * 16;
   }
   const auto issue = [&](int step) {
-    uint8_t *base = lds + (step & 1) * kStage + wave * 1024;
+    uint8_t *base = lds + step % STAGES * kStage + wave * 1024;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
       load_to_lds(i < kTokenLoads ? tokens : channels, i < kTokenLoads ? token_bytes : channel_bytes, offset[i],
@@ -263,7 +265,7 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void int8_tile_kernel(Int8Linea
   const int end = SPLIT ? min(all, first + p.split_steps) : all;
   i32x4 a[2][kNT], b[2][kMT];  // operands of 32 of K, the next ones read during this one's products
   const auto read = [&](int step, int ks) {
-    const uint8_t *stage = lds + (step & 1) * kStage;
+    const uint8_t *stage = lds + step % STAGES * kStage;
     const uint32_t chunk = ((2 * ks + g) ^ swizzle) * 16;
 #pragma unroll
     for (int i = 0; i < kNT; ++i) a[ks & 1][i] = *reinterpret_cast<const i32x4 *>(stage + a_at[i] + chunk);
@@ -279,13 +281,12 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void int8_tile_kernel(Int8Linea
     __builtin_amdgcn_sched_barrier(0);
   };
   constexpr int kLast = kStep / 32 - 1;
-  issue(first);
-  if (first + 1 < end) {
-    issue(first + 1);
-    wait_vmcnt<kLoads>();
-  } else {
-    wait_vmcnt<0>();
-  }
+  // vmcnt counts this wave's loads: the ones of the steps after the one that is waited for may be on their way
+#pragma unroll
+  for (int i = 0; i < STAGES; ++i)
+    if (first + i < end) issue(first + i);
+  if (first + STAGES <= end) wait_vmcnt<(STAGES - 1) * kLoads>();
+  else wait_vmcnt<0>();
   ring_barrier();
   read(first, 0);
   for (int step = first; step < end; ++step) {
@@ -295,9 +296,10 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void int8_tile_kernel(Int8Linea
       multiply(ks);
     }
     if (step + 1 < end) {  // the stage has been read by all: the barrier and the next one's first reads meet its last products
-      wait_vmcnt<0>();
+      if (step + STAGES <= end) wait_vmcnt<(STAGES - 2) * kLoads>();
+      else wait_vmcnt<0>();
       ring_barrier();
-      if (step + 2 < end) issue(step + 2);
+      if (step + STAGES < end) issue(step + STAGES);
       read(step + 1, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -323,7 +325,7 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void int8_tile_kernel(Int8Linea
   }
   // 32 tokens x the wave's channels at a time through this wave's part of LDS, 16 bytes between rows against conflicts
   constexpr int kPitch = kNT * 64 + 16;
-  static_assert(32 * kPitch * kWaves <= 2 * kStage, "the epilogue fits the stages");
+  static_assert(32 * kPitch * kWaves <= STAGES * kStage, "the epilogue fits the stages");
   __syncthreads();  // the last step has been read
   uint8_t *mine = lds + wave * 32 * kPitch;
 #pragma unroll
@@ -381,11 +383,11 @@ __global__ __launch_bounds__(256) void int8_join_kernel(Int8Linear p) {
       p.y[t * p.n + ch + e] = static_cast<uint16_t>(pack_bf16(static_cast<float>(sum[e]) * x_scale * p.w_scale[ch + e], 0.f));
 }
 
-template <int TM, int TN, int WM, int WN>
+template <int TM, int TN, int WM, int WN, int STAGES>
 void start_tiles(const Int8Linear &p, hipStream_t stream) {
   const dim3 grid((p.items + p.xcds - 1) / p.xcds * p.xcds), block(WM * WN * kWave);
-  if (p.splits > 1) hipLaunchKernelGGL((int8_tile_kernel<TM, TN, WM, WN, true>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((int8_tile_kernel<TM, TN, WM, WN, false>), grid, block, 0, stream, p);
+  if (p.splits > 1) hipLaunchKernelGGL((int8_tile_kernel<TM, TN, WM, WN, STAGES, true>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((int8_tile_kernel<TM, TN, WM, WN, STAGES, false>), grid, block, 0, stream, p);
 }
 
 }  // namespace
@@ -403,19 +405,18 @@ hipError_t launch_int8_quantize(const uint16_t *x, int64_t x_stride, uint8_t *co
 }
 
 // Which kernel and how often K is split, by what it costs in 0.01 us: the larger of the products (a step of 128 of K
-// takes a workgroup `alone` at least, a CU `shared` for each of its workgroups) and of reading w (5.3 TB/s, 4.2 with
-// fewer than three workgroups for two CUs), a start, and the join of the splits. Tiles of 256 x 256 have a CU to themselves,
-// so theirs come in whole rounds.
+// takes a workgroup `alone` at least, a CU `shared` for each of its workgroups) and of reading w (5.3 TB/s), a start,
+// and the join of the splits. Tiles of 256 x 256 have a CU to themselves, so theirs come in whole rounds.
 //                    alone  shared  start
-//   64 x 128            80      41     400
+//   64 x 128            45      41     400
 //   128 x 128           95      64     700
 //   256 x 256     150, 190 in more rounds than one     1000
-// Measured, us: 28672 x 8192 of 40 rows 49.0 in tiles of 64 split in two, 58.2 unsplit; of 200 rows 118, 74.6 and 101
-// in tiles of 64, 128 and 256, of 512 rows 193, 150 and 114, of 1000 360, 292 and 239; 4096 x 4096 of 512 rows 21.3,
-// 25.0 and 49.2; 8192 x 28672 of 512 rows 131 in tiles of 256 split in four, 164 in tiles of 128 split in two. Up to
-// 16 rows the kernel without tiles is the faster one while w is small (11008 x 4096 of 13 rows 12.9, in tiles 15.1) or
-// the rows are few (28672 x 8192 of one row 44.3, of four 50.7 and 45.0 in tiles, of 13 63.4 and 45.8): each of its
-// workgroups reads all rows' codes.
+// Measured, us: 28672 x 8192 of 32 rows 50.3 in tiles of 64, 54.3 split in two; 8192 x 28672 106.7, in four 44.8; 4096
+// x 4096 17.7 and 11.2. 28672 x 8192 of 200 rows 118, 74.6 and 101 in tiles of 64, 128 and 256, of 512 rows 193, 150 and
+// 114, of 1000 360, 292 and 239; 8192 x 28672 of 512 rows 131 in tiles of 256 split in four, 164 in tiles of 128 split
+// in two. Up to 16 rows the kernel without tiles is the faster one while w is small (4096 x 4096 of 13 rows 6.7, in
+// tiles 10.4) or the rows are few (28672 x 8192 of one row 44.3, of 13 63.4 and 50.1): each of its workgroups reads all
+// rows' codes.
 void plan_int8_linear(Int8Linear *p, int cus, int xcds) {
   p->xcds = std::max(1, xcds);
   p->part_stride = (p->n + 3) / 4 * 4;
@@ -429,7 +430,7 @@ void plan_int8_linear(Int8Linear *p, int cus, int xcds) {
       const int64_t rounds = (items + cus - 1) / cus;
       const int64_t products = tm == 256 ? rounds * length * (rounds == 1 ? alone : shared)
                                          : length * std::max(alone, shared * items / cus);
-      const int64_t cost = std::max(products, 2 * items < 3 * cus ? reading * 5 / 4 : reading) + start +
+      const int64_t cost = std::max(products, reading) + start +
                            (s > 1 ? 250 + p->m * p->n * s / 5000 : 0);
       if (cost >= best) continue;
       best = cost;
@@ -438,7 +439,7 @@ void plan_int8_linear(Int8Linear *p, int cus, int xcds) {
       p->tile_n = tn;
     }
   };
-  weigh(64, 128, 80, 41, 400);
+  weigh(64, 128, 45, 41, 400);
   if (p->m > 64) weigh(128, 128, 95, 64, 700);
   if (p->m > 128) weigh(256, 256, 150, 190, 1000);
   if (p->m <= 16 && reading * (1000 + 35 * p->m) / 1000 + 250 <= best) {
@@ -464,9 +465,9 @@ void plan_int8_linear(Int8Linear *p, int cus, int xcds) {
 hipError_t launch_int8_linear(const Int8Linear &p, hipStream_t stream) {
   switch (p.tile_m) {
     case 16: hipLaunchKernelGGL(int8_rows_kernel, dim3(p.items), dim3(512), 0, stream, p); break;
-    case 64: start_tiles<64, 128, 1, 4>(p, stream); break;
-    case 128: start_tiles<128, 128, 2, 2>(p, stream); break;
-    default: start_tiles<256, 256, 2, 4>(p, stream); break;
+    case 64: start_tiles<64, 128, 1, 4, 3>(p, stream); break;
+    case 128: start_tiles<128, 128, 2, 2, 2>(p, stream); break;
+    default: start_tiles<256, 256, 2, 4, 2>(p, stream); break;
   }
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || p.splits == 1) return err;
