@@ -779,9 +779,12 @@ _INT8_WORKSPACE: dict[tuple, int] = {}
 
 def _int8_rows(what: str, x: torch.Tensor) -> tuple[torch.Tensor, int]:
     """Checked rows [m, k] and their stride, a copy where they cannot be read 16 bytes at a time."""
-    if x.dim() != 2:
-        raise ValueError(f"{what} takes rows [m, k], got {tuple(x.shape)}")
-    _check_operands(what, x=x)
+    if (type(x) not in _PLAIN_TYPES or x.dtype is not torch.bfloat16 or x.dim() != 2
+            or x.get_device() != torch._C._cuda_getDevice() or (x.requires_grad and torch.is_grad_enabled())
+            or torch.autograd.forward_ad._current_level >= 0):
+        if x.dim() != 2:
+            raise ValueError(f"{what} takes rows [m, k], got {tuple(x.shape)}")
+        _check_operands(what, x=x)
     m, k = x.shape
     if k % 16 or k > INT8_LINEAR_MAX_K:
         raise ValueError(f"{what} needs k a multiple of 16, up to {INT8_LINEAR_MAX_K}, not {k}")
@@ -809,16 +812,17 @@ def int8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return codes, scales
 
 
-def _check_int8_weight(what: str, weight: torch.Tensor, scale: torch.Tensor, k: int, device: torch.device) -> int:
-    if weight.dtype != torch.int8 or scale.dtype != torch.float32:
+def _check_int8_weight(what: str, weight: torch.Tensor, scale: torch.Tensor, k: int, device: int) -> int:
+    if weight.dtype is not torch.int8 or scale.dtype is not torch.float32:
         raise TypeError(f"{what} needs an int8 weight and an fp32 scale, got {weight.dtype} and {scale.dtype}")
-    if weight.dim() != 2 or weight.shape[1] != k or scale.shape != weight.shape[:1]:
-        raise ValueError(f"{what} shape mismatch: weight {tuple(weight.shape)}, scale {tuple(scale.shape)}, k {k}")
-    if weight.device != device or scale.device != device:
-        raise ValueError(f"{what} needs weight and scale on {device}")
+    shape = weight.shape
+    if len(shape) != 2 or shape[1] != k or scale.shape != shape[:1]:
+        raise ValueError(f"{what} shape mismatch: weight {tuple(shape)}, scale {tuple(scale.shape)}, k {k}")
+    if weight.get_device() != device or scale.get_device() != device:
+        raise ValueError(f"{what} needs weight and scale on cuda:{device}")
     if not _packed(weight, scale):
         raise ValueError(f"{what} needs a contiguous, 16-byte aligned weight and scale")
-    return weight.shape[0]
+    return shape[0]
 
 
 def int8_matmul(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
@@ -838,7 +842,7 @@ def int8_matmul(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor,
         raise ValueError(f"int8_matmul runs on the current GPU, its input is on {codes.device} and {scales.device}")
     if not _packed(codes, scales):
         raise ValueError("int8_matmul needs contiguous, 16-byte aligned codes and scales")
-    n = _check_int8_weight("int8_matmul", weight, scale, k, codes.device)
+    n = _check_int8_weight("int8_matmul", weight, scale, k, codes.get_device())
     m = codes.shape[0]
     y = torch.empty((m, n), dtype=torch.bfloat16, device=codes.device)
     ws_bytes = _int8_workspace("ftx_int8_matmul_workspace", m, n, k)
@@ -866,12 +870,14 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor) -> t
     int8 [n, k], -127 .. 127; ``scale``: fp32 [n]; no backward."""
     x, stride = _int8_rows("int8_linear", x)
     m, k = x.shape
-    n = _check_int8_weight("int8_linear", weight, scale, k, x.device)
-    y = torch.empty((m, n), dtype=torch.bfloat16, device=x.device)
+    device = x.get_device()
+    n = _check_int8_weight("int8_linear", weight, scale, k, device)
+    where = x.device
+    y = torch.empty((m, n), dtype=torch.bfloat16, device=where)
     ws_bytes = _int8_workspace("ftx_int8_linear_workspace", m, n, k)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=where)
     nat.call("ftx_int8_linear", x.data_ptr(), stride, weight.data_ptr(), scale.data_ptr(), y.data_ptr(), m, n, k,
-             ws.data_ptr(), ws_bytes, _stream())
+             ws.data_ptr(), ws_bytes, _stream(device))
     return y
 
 

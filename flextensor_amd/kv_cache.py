@@ -30,18 +30,23 @@ FORMATS = {torch.float8_e4m3fn: nat.KV8_E4M3, torch.int8: nat.KV8_INT8}
 MAX_PAGE_TOKENS = 4096
 
 
-def _ints(what: str, name: str, t: torch.Tensor, shape: tuple[int, ...], device: int) -> None:
+_PLAIN = hip._PLAIN_TYPES
+_Strides6 = ctypes.c_int64 * 6
+_Strides9 = ctypes.c_int64 * 9
+
+
+def _check_ints(what: str, name: str, t: torch.Tensor, dims: int, batch: int, device: int) -> None:
     if type(t) is not torch.Tensor or t.dtype != torch.int32:
         raise TypeError(f"{what} takes {name} as an int32 tensor")
-    if tuple(t.shape) != shape or t.get_device() != device:
-        raise ValueError(f"{what} needs {name} {shape} on cuda:{device}, got {tuple(t.shape)} on {t.device}")
-    if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{what} needs {name} contiguous in its last dimension")
+    if t.dim() != dims or t.shape[0] != batch or t.get_device() != device:
+        raise ValueError(f"{what} needs {name} of {batch} sequences on cuda:{device}, got {tuple(t.shape)} on {t.device}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1 or dims == 2 and batch > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{what} needs {name} in rows that do not overlap, not of strides {t.stride()}")
 
 
-def _pool(what: str, codes: torch.Tensor, scales: torch.Tensor, dims: int) -> None:
+def _check_pool(what: str, codes: torch.Tensor, scales: torch.Tensor, dims: int) -> None:
     for name, t in (("codes", codes), ("scales", scales)):
-        if type(t) not in hip._PLAIN_TYPES:
+        if type(t) not in _PLAIN:
             raise TypeError(f"{what} takes plain tensors, {name} is a {type(t).__name__}")
     if codes.dtype not in FORMATS or scales.dtype != torch.float32:
         raise TypeError(f"{what} takes float8_e4m3fn or int8 codes and fp32 scales, got {codes.dtype} and {scales.dtype}")
@@ -58,37 +63,62 @@ def _pool(what: str, codes: torch.Tensor, scales: torch.Tensor, dims: int) -> No
                          f"values each, not {tuple(codes.shape)}")
 
 
-def _cache(what: str, q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor,
-           starts: torch.Tensor, new: torch.Tensor | None) -> nat.Kv8Cache:
-    _pool(what, codes, scales, 5)
-    b, _, h, d = q.shape
-    pages, _, kv, blocks, block_bytes = codes.shape
-    if block_bytes != BLOCK * d or h % kv:
-        raise ValueError(f"{what}: queries {tuple(q.shape)} do not fit a cache of {kv} heads of {block_bytes // BLOCK}")
-    device = codes.get_device()
-    _ints(what, "table", table, (b, table.shape[-1] if table.dim() == 2 else -1), device)
-    _ints(what, "starts", starts, (b,), device)
-    if new is not None:
-        _ints(what, "new", new, (b,), device)
-    width = table.shape[1]
-    if table.stride(0) < width and b > 1:
-        raise ValueError(f"{what} needs a table whose rows do not overlap, not of strides {table.stride()}")
-    return nat.Kv8Cache(codes.data_ptr(), scales.data_ptr(), pages, table.data_ptr() or None,
-                        max(table.stride(0), width), starts.data_ptr(), new.data_ptr() if new is not None else None,
-                        width, kv, blocks * BLOCK, d, FORMATS[codes.dtype])
-
-
-def _heads(what: str, **tensors: torch.Tensor) -> list[tuple[int, int, int]]:
-    """The strides of [batch, token, head, d] tensors that the kernels can read, else an error."""
-    strides = []
+def _check_heads(what: str, **tensors: torch.Tensor) -> None:
     for name, t in tensors.items():
         if t.dim() != 4:
             raise ValueError(f"{what} takes [batch, token, head, d] tensors, {name} is {tuple(t.shape)}")
-        strides.append(hip._head_strides(t))
-        if strides[-1] is None:
+    hip._check_operands(what, **tensors)
+    for name, t in tensors.items():
+        if hip._head_strides(t) is None:
             raise ValueError(f"{what} reads {name} 16 bytes at a time: it must be contiguous along d and 16-byte "
                              f"aligned, with strides that are multiples of 8, not {t.stride()}")
+
+
+def _heads(what: str, device: int, *tensors: torch.Tensor) -> list[int]:
+    """The strides of [batch, token, head, d] operands that the kernels can read (a call's q, k and v), else an error."""
+    strides: list[int] = []
+    grad = torch.is_grad_enabled()
+    plain = torch.autograd.forward_ad._current_level < 0
+    for t in tensors:
+        if (type(t) not in _PLAIN or t.dtype is not torch.bfloat16 or t.dim() != 4 or t.get_device() != device
+                or not plain or (grad and t.requires_grad)):
+            _check_heads(what, **dict(zip("qkv", tensors)))
+        got = hip._head_strides(t)
+        if got is None:
+            _check_heads(what, **dict(zip("qkv", tensors)))
+        strides += got
     return strides
+
+
+def _cache(what: str, q: torch.Tensor, device: int, codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor,
+           starts: torch.Tensor, new: torch.Tensor | None) -> nat.Kv8Cache:
+    b, _, h, d = q.shape
+    shape, dtype, i32 = codes.shape, codes.dtype, torch.int32
+    ptr, scales_ptr = codes.data_ptr(), scales.data_ptr()
+    if (type(codes) not in _PLAIN or type(scales) not in _PLAIN or dtype not in FORMATS or len(shape) != 5
+            or scales.dtype is not torch.float32 or shape[:4] != scales.shape or shape[1] != 2
+            or codes.get_device() != device or scales.get_device() != device or (ptr | scales_ptr) % 16
+            or not codes.is_contiguous() or not scales.is_contiguous() or shape[4] not in (2048, 4096)
+            or shape[3] & (shape[3] - 1) or not 1 <= shape[3] <= MAX_PAGE_TOKENS // BLOCK):
+        _check_pool(what, codes, scales, 5)
+    pages, _, kv, blocks, block_bytes = shape
+    if block_bytes != BLOCK * d or h % kv:
+        raise ValueError(f"{what}: queries {tuple(q.shape)} do not fit a cache of {kv} heads of {block_bytes // BLOCK}")
+    if table.dtype is not i32 or starts.dtype is not i32 or table.dim() != 2 or starts.shape != (b,) or (
+            table.get_device() != device or starts.get_device() != device or not starts.is_contiguous()
+            or type(table) is not torch.Tensor or type(starts) is not torch.Tensor
+            or table.shape[0] != b or not table.is_contiguous()):
+        _check_ints(what, "table", table, 2, b, device)
+        _check_ints(what, "starts", starts, 1, b, device)
+    new_ptr = None
+    if new is not None:
+        if type(new) is not torch.Tensor or new.dtype is not i32 or new.shape != (b,) or new.get_device() != device or (
+                not new.is_contiguous()):
+            _check_ints(what, "new", new, 1, b, device)
+        new_ptr = new.data_ptr()
+    width = table.shape[1]
+    return nat.Kv8Cache(ptr, scales_ptr, pages, table.data_ptr() or None, max(table.stride(0), width),
+                        starts.data_ptr(), new_ptr, width, kv, blocks * BLOCK, d, FORMATS[dtype])
 
 
 def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -103,23 +133,24 @@ def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
     positions, and holes are left out; the queries of tokens left out are 0. Two sequences of a call must not write
     into one page.
     """
-    strides = _heads("append", q=q, k=k, v=v)
-    hip._check_operands("append", q=q, k=k, v=v)
-    cache = _cache("append", q, codes, scales, table, starts, new)
-    b, t, h, d = q.shape
+    device = torch._C._cuda_getDevice() if q.is_cuda else -2  # -1 is the host's
+    strides = _heads("append", device, q, k, v)
+    cache = _cache("append", q, device, codes, scales, table, starts, new)
+    b, t, h, d = shape = q.shape
     if k.shape != (b, t, cache.kv_heads, d) or v.shape != k.shape:
         raise ValueError(f"append operands differ: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} for "
                          f"{cache.kv_heads} cached heads")
+    cos_ptr, sin_ptr = cos.data_ptr(), sin.data_ptr()
     for name, x in (("cos", cos), ("sin", sin)):
-        if type(x) not in hip._PLAIN_TYPES or x.dtype != torch.float32:
+        if type(x) not in _PLAIN or x.dtype is not torch.float32:
             raise TypeError(f"append takes {name} as an fp32 tensor")
-        if x.dim() != 2 or x.shape != cos.shape or x.shape[1] != d or x.get_device() != q.get_device() or not hip._packed(x):
-            raise ValueError(f"append needs cos and sin [positions, {d}], contiguous and on {q.device}")
+        if x.dim() != 2 or x.shape != cos.shape or x.shape[1] != d or x.get_device() != device or not x.is_contiguous() or (
+                (cos_ptr | sin_ptr) % 16):
+            raise ValueError(f"append needs cos and sin [positions, {d}], contiguous, 16-byte aligned and on {q.device}")
     torch._C._increment_version((codes, scales))  # as an in-place operation, for what autograd saved
-    out = torch.empty((b, t, h, d), dtype=torch.bfloat16, device=q.device)
-    nat.call("ftx_kv8_append", ctypes.byref(cache), q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(),
-             sin.data_ptr(), cos.shape[0], out.data_ptr(), b, t, h,
-             (ctypes.c_int64 * 9)(*strides[0], *strides[1], *strides[2]), hip._stream())
+    out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
+    nat.call("ftx_kv8_append", ctypes.byref(cache), q.data_ptr(), k.data_ptr(), v.data_ptr(), cos_ptr, sin_ptr,
+             cos.shape[0], out.data_ptr(), b, t, h, _Strides9(*strides), hip._stream(device))
     return out
 
 
@@ -138,9 +169,9 @@ def attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, table:
     and changes no result beyond the order of the sums. ``scale``: 1 / sqrt(d) if None. A NaN that a sequence holds
     may reach earlier tokens of the same call.
     """
-    strides = _heads("attention", q=q)[0]
-    hip._check_operands("attention", q=q)
-    cache = _cache("attention", q, codes, scales, table, starts, new)
+    device = torch._C._cuda_getDevice() if q.is_cuda else -2  # -1 is the host's
+    strides = _heads("attention", device, q)
+    cache = _cache("attention", q, device, codes, scales, table, starts, new)
     b, t, h, d = q.shape
     longest = cache.width * cache.page_tokens
     if max_tokens is not None:
@@ -148,6 +179,7 @@ def attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, table:
             raise ValueError(f"max_tokens must not be negative, got {max_tokens}")
         longest = min(longest, max_tokens)
     out = torch.empty_like(q)
+    strides += hip._head_strides(out)
     shape = (b, t, h, cache.kv_heads, d, longest)
     ws_bytes = _WORKSPACE.get(shape)
     if ws_bytes is None:
@@ -158,8 +190,8 @@ def attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, table:
         ws_bytes = _WORKSPACE[shape] = int(got.value)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     nat.call("ftx_kv8_attention", ctypes.byref(cache), q.data_ptr(), out.data_ptr(), b, t, h,
-             (ctypes.c_int64 * 6)(*strides, *_heads("attention", out=out)[0]), d ** -0.5 if scale is None else scale,
-             longest, ws.data_ptr() if ws is not None else None, ws_bytes, hip._stream())
+             _Strides6(*strides), d ** -0.5 if scale is None else scale, longest,
+             ws.data_ptr() if ws is not None else None, ws_bytes, hip._stream(device))
     return out
 
 
@@ -167,7 +199,7 @@ def copy_pages(codes: torch.Tensor, scales: torch.Tensor, src: list[int], dst: l
     """Copies pages ``src[i]`` to ``dst[i]`` in every layer of a pool, [layers, pages, ...] codes and scales
     (``ftx_kv8_copy_pages``). No page is written twice or both read and written. The numbers travel with the launch:
     nothing is uploaded."""
-    _pool("copy_pages", codes, scales, 6)
+    _check_pool("copy_pages", codes, scales, 6)
     if len(src) != len(dst):
         raise ValueError(f"copy_pages takes as many sources as targets, got {len(src)} and {len(dst)}")
     layers, pages, _, kv, blocks, block_bytes = codes.shape
