@@ -216,9 +216,12 @@ struct Kv8Append {
   int64_t positions;
   int64_t q_stride[3], k_stride[3], v_stride[3];
   int batch, t, heads;
+  // planned
   int seq_blocks;         // blocks that t tokens touch at most
-  int64_t block_items;    // batch * seq_blocks * kv_heads * 2 workgroups
+  int heads_each;         // heads of a workgroup
+  int64_t block_items, query_items;  // workgroups that write blocks, and that rotate queries
 };
+void plan_kv8_append(Kv8Append *p, int cus);
 hipError_t launch_kv8_append(const Kv8Append &p, hipStream_t stream);
 constexpr int kKvCopyPairs = 256;  // of one launch: they travel as its argument
 struct Kv8Copy {

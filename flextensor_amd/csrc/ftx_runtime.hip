@@ -1532,9 +1532,11 @@ int ftx_kv8_append(const ftx_kv8_cache *cache, const void *q, const void *k, con
   p.batch = static_cast<int>(batch);
   p.t = static_cast<int>(t);
   p.heads = heads;
-  p.seq_blocks = static_cast<int>((t + 2 * ftx::kKvBlock - 2) / ftx::kKvBlock);
-  p.block_items = batch * p.seq_blocks * kv * 2;
-  if (p.block_items + batch * t * heads * d / 2048 + 1 > ftx::kMaxThreads / 256)
+  int cus = 256;
+  ftx::DeviceState *st = nullptr;
+  if (ftx::device_state(&st) == FTX_OK) cus = st->cu_count;
+  ftx::plan_kv8_append(&p, cus);
+  if (p.block_items + p.query_items > ftx::kMaxThreads / 256)
     return ftx::fail(FTX_ERR_UNSUPPORTED, "cache append: more workgroups than one launch holds");
   FTX_HIP(ftx::launch_kv8_append(p, static_cast<hipStream_t>(stream)));
   return FTX_OK;

@@ -780,7 +780,7 @@ _INT8_WORKSPACE: dict[tuple, int] = {}
 def _int8_rows(what: str, x: torch.Tensor) -> tuple[torch.Tensor, int]:
     """Checked rows [m, k] and their stride, a copy where they cannot be read 16 bytes at a time."""
     if (type(x) not in _PLAIN_TYPES or x.dtype is not torch.bfloat16 or x.dim() != 2
-            or x.get_device() != torch._C._cuda_getDevice() or (x.requires_grad and torch.is_grad_enabled())
+            or not x.is_cuda or x.get_device() != torch._C._cuda_getDevice() or (x.requires_grad and torch.is_grad_enabled())
             or torch.autograd.forward_ad._current_level >= 0):
         if x.dim() != 2:
             raise ValueError(f"{what} takes rows [m, k], got {tuple(x.shape)}")

@@ -26,10 +26,11 @@ import torch.nn.functional as F
 from torch import nn
 from torch.nn.modules import module as torch_module
 
-from . import hip
+from . import hip, kv_cache
 
 
 FP8_E4M3_MAX = 448.0
+INT8_MAX = 127.0
 
 
 def init_normal_(model: nn.Module, seed: int, std: float = 0.02, init_device: str = "cpu") -> nn.Module:
@@ -37,7 +38,8 @@ def init_normal_(model: nn.Module, seed: int, std: float = 0.02, init_device: st
 
     An ``Fp8Linear`` draws its weight the same way, then stores it as
     float8_e4m3fn with a per-output-channel scale ``absmax / 448`` (bf16); the
-    quantised weight is ``round_e4m3(w / scale)``.
+    quantised weight is ``round_e4m3(w / scale)``. An ``Int8Linear``'s is
+    ``round(w / scale)`` with ``absmax / 127`` (fp32).
     """
     gen = torch.Generator(device=init_device).manual_seed(seed)
     with torch.no_grad():
@@ -47,6 +49,13 @@ def init_normal_(model: nn.Module, seed: int, std: float = 0.02, init_device: st
                 w.normal_(0.0, std, generator=gen)
                 scale = (w.abs().amax(dim=1) / FP8_E4M3_MAX).clamp_min(1e-12).to(torch.bfloat16)
                 mod.weight.copy_((w / scale.float()[:, None]).to(torch.float8_e4m3fn))
+                mod.scale.copy_(scale)
+                continue
+            if isinstance(mod, Int8Linear):
+                w = torch.empty(mod.weight.shape, dtype=torch.float32, device=init_device)
+                w.normal_(0.0, std, generator=gen)
+                scale = (w.abs().amax(dim=1) / INT8_MAX).clamp_min(1e-12)
+                mod.weight.copy_((w / scale[:, None]).round().to(torch.int8))
                 mod.scale.copy_(scale)
                 continue
             for p in mod.parameters(recurse=False):
@@ -106,13 +115,14 @@ class LlamaShape:
     eps: float = 1e-5
     rope_theta: float = 10000.0
     fp8: bool = False  # projection weights in float8_e4m3fn with per-output-channel bf16 scales
+    int8: bool = False  # projection weights and their inputs in 8-bit integers, fp32 scales per channel and per token
 
     def layer_bytes(self, itemsize: int = 2) -> int:
         h, d = self.hidden, self.head_dim
         mats = h * self.n_heads * d + 2 * h * self.n_kv_heads * d + self.n_heads * d * h + 3 * h * self.inter
-        if self.fp8:
+        if self.fp8 or self.int8:
             outs = self.n_heads * d + 2 * self.n_kv_heads * d + h + 2 * self.inter + h
-            return mats + 2 * outs + 2 * 2 * h
+            return mats + (2 if self.fp8 else 4) * outs + 2 * 2 * h
         return itemsize * (mats + 2 * h)
 
 
@@ -159,6 +169,37 @@ class Fp8Linear(nn.Module):
         return F.linear(x, w) * self.scale
 
 
+class Int8Linear(nn.Module):
+    """y = x @ (W_int8 * scale[:, None])^T with x rounded to 8 bits, a scale for each row (token).
+
+    On the GPU (bf16 inputs, K a multiple of 16) the library's integer kernels run; the sums of code products are
+    exact there. Other calls compute the same codes and their products in float32.
+    """
+
+    def __init__(self, in_features: int, out_features: int) -> None:
+        super().__init__()
+        self.weight = nn.Parameter(torch.empty(out_features, in_features, dtype=torch.int8), requires_grad=False)
+        self.scale = nn.Parameter(torch.ones(out_features, dtype=torch.float32), requires_grad=False)
+
+    def kernel_eligible(self, x: torch.Tensor) -> bool:
+        """Whether the library kernels take this call: non-empty bf16 rows, K a multiple of 16, and a contiguous,
+        16-byte aligned weight and scale (``raw_block_transfer`` packs weights back to back without alignment)."""
+        k = x.shape[-1]
+        return (x.numel() > 0 and k % 16 == 0 and k <= hip.INT8_LINEAR_MAX_K and hip.kernel_call(x)
+                and x.numel() // k < 1 << 24 and hip._packed(self.weight, self.scale))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        k = x.shape[-1]
+        if self.kernel_eligible(x):
+            y = hip.int8_linear(x.reshape(x.numel() // k, k), self.weight, self.scale)
+            return y.view(*x.shape[:-1], y.shape[-1])
+        xf = x.float()
+        scale = xf.abs().amax(-1, keepdim=True) * torch.tensor(1 / INT8_MAX, dtype=torch.float32)
+        scale = torch.where(scale < 2.0 ** -100, 0.0, scale)
+        codes = (xf * torch.where(scale > 0, 1.0 / scale, 0.0)).round().clamp(-INT8_MAX, INT8_MAX)
+        return (F.linear(codes, self.weight.float()) * scale * self.scale).to(x.dtype)
+
+
 class Linear(nn.Linear):
     """``nn.Linear`` whose forward on a few bf16 GPU rows (a decode batch) is the library's one-launch kernel."""
 
@@ -189,6 +230,17 @@ def fp8_group(x: torch.Tensor, layers: list[nn.Module]) -> list[torch.Tensor] | 
         return None
     ys = hip.fp8_linear_group(x.reshape(x.numel() // k, k), [lin.weight for lin in layers],
                               [lin.scale for lin in layers])
+    return [y.view(*x.shape[:-1], y.shape[-1]) for y in ys]
+
+
+def int8_group(x: torch.Tensor, layers: list[nn.Module]) -> list[torch.Tensor] | None:
+    """The outputs of several ``Int8Linear`` layers on one input, which is rounded to 8 bits once, or None when any of
+    them would not take the kernel or would run more than its own forward when called."""
+    if not all(isinstance(lin, Int8Linear) and lin.kernel_eligible(x) and _plain_call(lin) for lin in layers):
+        return None
+    k = x.shape[-1]
+    codes, scales = hip.int8_quantize(x.reshape(x.numel() // k, k))
+    ys = [hip.int8_matmul(codes, scales, lin.weight, lin.scale) for lin in layers]
     return [y.view(*x.shape[:-1], y.shape[-1]) for y in ys]
 
 
@@ -231,6 +283,8 @@ def linear_group(x: torch.Tensor, layers: list[nn.Module]) -> list[torch.Tensor]
     """The outputs of several linear layers on one input in one launch, or None when no kernel takes the group."""
     if _bf16_fusable(x, layers):
         return hip.bf16_linear_unchecked(x, [lin.weight for lin in layers])
+    if type(layers[0]) is Int8Linear:
+        return int8_group(x, layers)
     return fp8_group(x, layers)
 
 
@@ -250,6 +304,8 @@ def linear_residual(x: torch.Tensor, lin: nn.Module, residual: torch.Tensor) -> 
 
 
 def _proj(s: LlamaShape, n_in: int, n_out: int, dtype: torch.dtype) -> nn.Module:
+    if s.int8:
+        return Int8Linear(n_in, n_out)
     return Fp8Linear(n_in, n_out) if s.fp8 else Linear(n_in, n_out, bias=False, dtype=dtype)
 
 
@@ -286,9 +342,11 @@ class Attention(nn.Module):
         self.wo = _proj(s, s.n_heads * s.head_dim, s.hidden, dtype)
 
     def forward(self, x: torch.Tensor, pos: int, cos: torch.Tensor, sin: torch.Tensor,
-                cache_k: torch.Tensor, cache_v: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+                cache_k: torch.Tensor | kv_cache.KVLayer, cache_v: torch.Tensor | None,
+                residual: torch.Tensor | None = None) -> torch.Tensor:
         """The attention block's output, plus ``residual`` when given (folded into the output projection's
-        launch for decode batches)."""
+        launch for decode batches). ``cache_k`` may be a layer of a paged 8-bit cache, which holds both keys and
+        values and knows the sequences' positions."""
         s = self.s
         b, t, _ = x.shape
         qkv = linear_group(x, [self.wq, self.wk, self.wv])
@@ -296,6 +354,9 @@ class Attention(nn.Module):
         q = q.view(b, t, s.n_heads, s.head_dim)
         k = k.view(b, t, s.n_kv_heads, s.head_dim)
         v = v.view(b, t, s.n_kv_heads, s.head_dim)
+        if isinstance(cache_k, kv_cache.KVLayer):
+            o = cache_k.attend(cache_k.append(q, k, v, cos, sin))
+            return self._output(o.view(b, t, s.n_heads * s.head_dim), residual)
         o = hip.rope_attention(q, k, v, cos, sin, pos, cache_k, cache_v)
         if o is not None:
             return self._output(o.view(b, t, s.n_heads * s.head_dim), residual)
@@ -341,7 +402,7 @@ class DecoderLayer(nn.Module):
         self.down = _proj(s, s.inter, s.hidden, dtype)
 
     def forward(self, x: torch.Tensor, pos: int, cos: torch.Tensor, sin: torch.Tensor,
-                cache_k: torch.Tensor, cache_v: torch.Tensor) -> torch.Tensor:
+                cache_k: torch.Tensor | kv_cache.KVLayer, cache_v: torch.Tensor | None) -> torch.Tensor:
         x = self.attn(self.attn_norm(x), pos, cos, sin, cache_k, cache_v, residual=x)
         h = self.mlp_norm(x)
         act = linear_swiglu(h, self.gate, self.up)
@@ -377,11 +438,24 @@ class LlamaModel(nn.Module):
         self.cache_k = [torch.zeros(shape, dtype=dt, device=device) for _ in range(s.n_layers)]
         self.cache_v = [torch.zeros(shape, dtype=dt, device=device) for _ in range(s.n_layers)]
 
-    def forward(self, tokens: torch.Tensor, pos: int = 0) -> torch.Tensor:
-        """Logits of the last position, float32."""
+    def init_paged_cache(self, pages: int, page_tokens: int = 64, dtype: torch.dtype = torch.float8_e4m3fn,
+                         device: torch.device | str = "cuda") -> kv_cache.PagedKVCache:
+        """A pool of ``pages`` for this model's layers; its steps go to :meth:`forward`."""
+        s = self.shape
+        return kv_cache.PagedKVCache(s.n_layers, s.n_kv_heads, s.head_dim, pages, page_tokens, dtype, device)
+
+    def forward(self, tokens: torch.Tensor, pos: int = 0, step: kv_cache.KVStep | None = None) -> torch.Tensor:
+        """Logits of the last position, float32. With a ``step`` of a paged cache the tokens are its sequences' next
+        ones (``pos`` does not matter), and the logits those of each sequence's last token in the step."""
         x = self.embed(tokens)
         for i, layer in enumerate(self.layers):
-            x = layer(x, pos, self.rope_cos, self.rope_sin, self.cache_k[i], self.cache_v[i])
+            if step is not None:
+                x = layer(x, pos, self.rope_cos, self.rope_sin, step.layer(i), None)
+            else:
+                x = layer(x, pos, self.rope_cos, self.rope_sin, self.cache_k[i], self.cache_v[i])
+        if step is not None and min(step.counts) < x.shape[1]:
+            last = (step.new.long() - 1).clamp_min(0).view(-1, 1, 1).expand(-1, 1, x.shape[2])
+            x = x.gather(1, last)
         return self.lm_head(self.norm(x[:, -1:])).float()
 
 
@@ -415,6 +489,35 @@ def generate(model: LlamaModel, prompt: torch.Tensor, steps: int) -> tuple[torch
         pos += 1
     out.append(tok)
     return torch.cat(out, dim=1), all_logits
+
+
+@torch.no_grad()
+def generate_paged(model: LlamaModel, cache: kv_cache.PagedKVCache, prompts: list[list[int]], steps: int,
+                   samples: int = 1) -> tuple[list[int], torch.Tensor, list[torch.Tensor]]:
+    """Greedy decoding of prompts of different lengths over a paged 8-bit cache.
+
+    The prompts are one ragged pass. Each is then forked into ``samples`` sequences that share its pages; sample j
+    starts from its j-th likeliest token. Returns the sequences (in the cache until closed), their tokens
+    ``[prompts * samples, steps]`` and the logits of every step.
+    """
+    longest = max(len(p) for p in prompts)
+    device = model.rope_cos.device
+    tokens = torch.tensor([p + [0] * (longest - len(p)) for p in prompts], device=device)
+    roots = [cache.open() for _ in prompts]
+    step = cache.begin(roots, [len(p) for p in prompts])
+    logits = model(tokens, step=step)
+    cache.commit(step)
+    sequences = [s for root in roots for s in [root, *(cache.fork(root) for _ in range(samples - 1))]]
+    tok = logits[:, -1].topk(samples, -1).indices.reshape(-1, 1)
+    out, all_logits = [tok], [logits]
+    for _ in range(steps - 1):
+        step = cache.begin(sequences, 1)
+        logits = model(tok, step=step)
+        cache.commit(step)
+        all_logits.append(logits)
+        tok = logits.argmax(-1)
+        out.append(tok)
+    return sequences, torch.cat(out, dim=1), all_logits
 
 
 def prompt_tokens(batch: int, length: int, vocab: int, seed: int = 0) -> torch.Tensor:

@@ -70,7 +70,9 @@ def test_quantize_of_extreme_rows(gpu):
 _SHAPES = [
     (1, 1, 16), (1, 257, 272), (2, 16, 256), (16, 100, 4096), (13, 1000, 2064), (9, 4096, 11008),   # up to 16 rows
     (17, 129, 272), (33, 300, 1040), (64, 128, 8192), (65, 1000, 640), (128, 257, 4112), (200, 4096, 1024),
-    (129, 511, 144), (300, 2048, 4096), (777, 8200, 528), (2111, 8190, 272), (257, 30000, 1040),
+    (129, 511, 144), (300, 2048, 4096), (777, 8200, 528), (2111, 8190, 272), (257, 30000, 1040),  # tiles of 64 tokens
+    (13, 28672, 8192), (200, 28670, 4096), (100, 28672, 8192),                  # of 64 and 128, K split or not
+    (300, 30001, 1040), (512, 8192, 28672),                                     # of 256
 ]
 
 
@@ -79,7 +81,8 @@ def test_linear_matches_exact_sums(gpu, m, n, k):
     x, w, scale = _inputs(gpu, m, n, k)
     codes, want_scales = _quantised(x)
     got = hip.int8_linear(x, w, scale).cpu().double()
-    want = codes.double() @ w.cpu().double().t() * want_scales[:, None].double() * scale.cpu().double()
+    want = codes.to(gpu).double() @ w.double().t() * want_scales[:, None].to(gpu).double() * scale.double()
+    want = want.cpu()
     assert ((got - want).abs() <= ONE_ROUNDING * want.abs()).all()
 
 
