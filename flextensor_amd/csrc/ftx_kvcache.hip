@@ -90,8 +90,8 @@ __device__ __forceinline__ float lane_float(float v, int lane) {
 //
 // over the cached tokens p of the head that the group of `rep` query heads shares; a row that sees no token is 0.
 // Scores, the running maximum and the running sum are fp32. A code is exact in bf16 and enters the products as it
-// is: a block's key scale multiplies its scores, its value scale the probabilities, which are then rounded to bf16
-// (2^-9 of each at most, as in the attention over a bf16 cache).
+// is: a block's key scale multiplies its scores, its value scale the probabilities. Prompts round those to bf16
+// (2^-9 of each at most, as in the attention over a bf16 cache), few rows do not.
 
 // Eight codes as bf16.
 template <bool FP8>
@@ -269,10 +269,11 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
       }
     }
     // p times the value scale in one operation: 2^(s - m + log2(scale)); the sum of the p takes it out again. A
-    // scale of 0 stands beside codes of 0, whose weight does not matter.
+    // scale of 0 stands beside codes of 0, whose weight does not matter. The products take it in two parts of eight
+    // bits: these kernels wait for memory, and have the time for a result that is only rounded at its end.
     const float factor = x.v_scale == 0.f || x.hole ? 1.0f : x.v_scale;
     const float log_factor = __builtin_amdgcn_logf(factor), inverse = __builtin_amdgcn_rcpf(factor);
-    u32x4 p[RT];
+    u32x4 p[RT], rest[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       float mx = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
@@ -298,6 +299,7 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
         const float p1 = __builtin_amdgcn_exp2f(fmaf(s[t][e >> 1][2 * (e & 1) + 1], scale, offset));
         sum += p0 + p1;
         p[t][e] = pack_bf16(p0, p1);
+        rest[t][e] = pack_bf16(p0 - bf16_value(p[t][e]), p1 - __uint_as_float(p[t][e] & 0xffff0000u));
       }
       l[t] = fmaf(sum, inverse, l[t]);
     }
@@ -305,8 +307,10 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
     for (int d = 0; d < kDTiles; ++d) {
       const bf16x8 v = widen<FP8>(x.v[d][0], x.v[d][1]);
 #pragma unroll
-      for (int t = 0; t < RT; ++t)
+      for (int t = 0; t < RT; ++t) {
         o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, p[t]), o[t][d], 0, 0, 0);
+        o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, rest[t]), o[t][d], 0, 0, 0);
+      }
     }
   };
 
