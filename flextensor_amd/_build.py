@@ -11,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -19,6 +20,9 @@ LIB_PATH = PKG_DIR / "libftx_hip.so"
 SOURCES = ("ftx_runtime.hip", "ftx_kernels.hip", "ftx_gemm.hip", "ftx_attention.hip", "ftx_layers.hip",
            "ftx_int8.hip", "ftx_kvcache.hip", "ftx_staged.hip", "ftx_expcode.hip")
 OFFLOAD_ARCH = "gfx950"
+# The same library's serving calls, taking torch tensors (a CPython extension, host code only).
+TORCH_SOURCE = CSRC / "ftx_torch.cpp"
+TORCH_LIB_PATH = PKG_DIR / "_ftx_torch.so"
 
 
 def _torch_lib_dir() -> str:
@@ -53,22 +57,58 @@ def hipcc_command(output: Path = LIB_PATH) -> list[str]:
     ]
 
 
+def torch_command(output: Path = TORCH_LIB_PATH) -> list[str]:
+    import torch
+
+    include = Path(torch.__file__).resolve().parent / "include"
+    torch_lib = _torch_lib_dir()
+    return [
+        shutil.which("g++") or "/usr/bin/g++",
+        "-O2",
+        "-std=c++17",
+        "-fPIC",
+        "-shared",
+        "-Wall",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        f"-isystem{include}",
+        f"-isystem{include / 'torch/csrc/api/include'}",
+        f"-isystem{sysconfig.get_paths()['include']}",
+        str(TORCH_SOURCE),
+        "-o",
+        str(output),
+        f"-L{PKG_DIR}",
+        f"-l:{LIB_PATH.name}",
+        f"-L{torch_lib}",
+        "-ltorch_python",
+        "-ltorch",
+        "-ltorch_cpu",
+        "-lc10",
+        "-Wl,-rpath,$ORIGIN",
+        f"-Wl,-rpath,{torch_lib}",
+    ]
+
+
 def build(verbose: bool = False) -> Path:
-    """Compile the library; always rebuilds. Returns the path of the ``.so``."""
-    tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = hipcc_command(tmp)
+    """Compile the library and its torch binding; always rebuilds. Returns the path of the library."""
+    _compile(hipcc_command, LIB_PATH, verbose)
+    _compile(torch_command, TORCH_LIB_PATH, verbose)
+    return LIB_PATH
+
+
+def _compile(command, path: Path, verbose: bool) -> None:
+    tmp = path.with_suffix(".so.tmp")
+    cmd = command(tmp)
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True, check=False)
     if proc.returncode != 0:
         sys.stderr.write(proc.stdout + proc.stderr)
-        raise RuntimeError(f"hipcc failed with exit code {proc.returncode}")
+        raise RuntimeError(f"{Path(cmd[0]).name} failed with exit code {proc.returncode}")
     noise = "is not a recognized feature for this target"
     warnings = [ln for ln in (proc.stdout + proc.stderr).splitlines() if ln.strip() and noise not in ln]
     if warnings and verbose:
         sys.stderr.write("\n".join(warnings) + "\n")
-    os.replace(tmp, LIB_PATH)
-    return LIB_PATH
+    os.replace(tmp, path)
 
 
 if __name__ == "__main__":

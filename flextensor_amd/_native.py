@@ -268,6 +268,31 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
         return lib
 
 
+_torch_calls = None
+
+
+def torch_calls():
+    """The library's calls that take torch tensors (``csrc/ftx_torch.cpp``): each returns its result, the status of a
+    failed C call, or None for arguments that it leaves to the Python function of the same name."""
+    global _torch_calls
+    if _torch_calls is None:
+        load()
+        try:
+            from . import _ftx_torch
+        except ImportError as e:
+            raise FtxLibraryMissing(f"the torch binding of {LIB_PATH.name} is missing or does not load ({e}); build it "
+                                    "with `python -m flextensor_amd._build`") from e
+        _torch_calls = _ftx_torch
+    return _torch_calls
+
+
+def result(got):
+    """What a call of :func:`torch_calls` returned; raises the FtxError of a status."""
+    if type(got) is int:
+        check(got)
+    return got
+
+
 def lib() -> ctypes.CDLL:
     return _lib if _lib is not None else load()
 

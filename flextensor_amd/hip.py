@@ -774,7 +774,6 @@ def fp8_linear_residual(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tens
 
 
 INT8_LINEAR_MAX_K = 131072  # the 32-bit sums hold 127^2 times this
-_INT8_WORKSPACE: dict[tuple, int] = {}
 
 
 def _int8_rows(what: str, x: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -829,6 +828,11 @@ def int8_matmul(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor,
     """``bf16((codes @ weight.T) * scales[:, None] * scale)`` of what :func:`int8_quantize` returns
     (``ftx_int8_matmul``): several weights [n, k] that share an input quantise it once. ``weight``: int8, -127 ..
     127; ``scale``: fp32 [n]. The sums are exact integers; each output is rounded once."""
+    if codes.is_cuda:
+        device = torch._C._cuda_getDevice()
+        got = nat.torch_calls().int8_matmul(codes, scales, weight, scale, device, _stream(device))
+        if got is not None:
+            return nat.result(got)
     if weight.dim() != 2:
         raise ValueError(f"int8_matmul takes a weight [n, k], got {tuple(weight.shape)}")
     k = weight.shape[1]
@@ -853,21 +857,20 @@ def int8_matmul(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor,
 
 
 def _int8_workspace(name: str, m: int, n: int, k: int) -> int:
-    key = (name, m, n, k)
-    got = _INT8_WORKSPACE.get(key)
-    if got is None:
-        b = ctypes.c_size_t(0)
-        nat.call(name, m, n, k, ctypes.byref(b))
-        if len(_INT8_WORKSPACE) >= 4096:
-            _INT8_WORKSPACE.clear()
-        got = _INT8_WORKSPACE[key] = int(b.value)
-    return got
+    b = ctypes.c_size_t(0)
+    nat.call(name, m, n, k, ctypes.byref(b))
+    return int(b.value)
 
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     """``x @ (weight * scale[:, None]).T`` with ``x`` rounded to 8 bits, a scale for each row: :func:`int8_quantize`,
     then :func:`int8_matmul`, in one call (``ftx_int8_linear``). ``x``: bf16 [m, k], k a multiple of 16; ``weight``:
     int8 [n, k], -127 .. 127; ``scale``: fp32 [n]; no backward."""
+    if x.is_cuda and torch.autograd.forward_ad._current_level < 0:
+        device = torch._C._cuda_getDevice()
+        got = nat.torch_calls().int8_linear(x, weight, scale, device, _stream(device))
+        if got is not None:
+            return nat.result(got)
     x, stride = _int8_rows("int8_linear", x)
     m, k = x.shape
     device = x.get_device()

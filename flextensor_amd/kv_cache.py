@@ -35,6 +35,10 @@ _Strides6 = ctypes.c_int64 * 6
 _Strides9 = ctypes.c_int64 * 9
 
 
+def _device(t: torch.Tensor) -> int:
+    return torch._C._cuda_getDevice() if t.is_cuda else -2  # -1 is the host's
+
+
 def _check_ints(what: str, name: str, t: torch.Tensor, dims: int, batch: int, device: int) -> None:
     if type(t) is not torch.Tensor or t.dtype != torch.int32:
         raise TypeError(f"{what} takes {name} as an int32 tensor")
@@ -133,7 +137,11 @@ def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
     positions, and holes are left out; the queries of tokens left out are 0. Two sequences of a call must not write
     into one page.
     """
-    device = torch._C._cuda_getDevice() if q.is_cuda else -2  # -1 is the host's
+    device = _device(q)
+    if device >= 0 and torch.autograd.forward_ad._current_level < 0:
+        got = nat.torch_calls().append(q, k, v, cos, sin, codes, scales, table, starts, new, device, hip._stream(device))
+        if got is not None:
+            return nat.result(got)
     strides = _heads("append", device, q, k, v)
     cache = _cache("append", q, device, codes, scales, table, starts, new)
     b, t, h, d = shape = q.shape
@@ -154,9 +162,6 @@ def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
     return out
 
 
-_WORKSPACE: dict[tuple, int] = {}
-
-
 def attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor, starts: torch.Tensor,
               new: torch.Tensor | None = None, max_tokens: int | None = None,
               scale: float | None = None) -> torch.Tensor:
@@ -169,7 +174,12 @@ def attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, table:
     and changes no result beyond the order of the sums. ``scale``: 1 / sqrt(d) if None. A NaN that a sequence holds
     may reach earlier tokens of the same call.
     """
-    device = torch._C._cuda_getDevice() if q.is_cuda else -2  # -1 is the host's
+    device = _device(q)
+    if device >= 0 and torch.autograd.forward_ad._current_level < 0:
+        got = nat.torch_calls().attention(q, codes, scales, table, starts, new, max_tokens, scale, device,
+                                          hip._stream(device))
+        if got is not None:
+            return nat.result(got)
     strides = _heads("attention", device, q)
     cache = _cache("attention", q, device, codes, scales, table, starts, new)
     b, t, h, d = q.shape
@@ -180,14 +190,9 @@ def attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, table:
         longest = min(longest, max_tokens)
     out = torch.empty_like(q)
     strides += hip._head_strides(out)
-    shape = (b, t, h, cache.kv_heads, d, longest)
-    ws_bytes = _WORKSPACE.get(shape)
-    if ws_bytes is None:
-        got = ctypes.c_size_t(0)
-        nat.call("ftx_kv8_attention_workspace", *shape, ctypes.byref(got))
-        if len(_WORKSPACE) >= 4096:
-            _WORKSPACE.clear()
-        ws_bytes = _WORKSPACE[shape] = int(got.value)
+    got = ctypes.c_size_t(0)
+    nat.call("ftx_kv8_attention_workspace", b, t, h, cache.kv_heads, d, longest, ctypes.byref(got))
+    ws_bytes = int(got.value)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     nat.call("ftx_kv8_attention", ctypes.byref(cache), q.data_ptr(), out.data_ptr(), b, t, h,
              _Strides6(*strides), d ** -0.5 if scale is None else scale, longest,
@@ -199,6 +204,12 @@ def copy_pages(codes: torch.Tensor, scales: torch.Tensor, src: list[int], dst: l
     """Copies pages ``src[i]`` to ``dst[i]`` in every layer of a pool, [layers, pages, ...] codes and scales
     (``ftx_kv8_copy_pages``). No page is written twice or both read and written. The numbers travel with the launch:
     nothing is uploaded."""
+    device = _device(codes)
+    if device >= 0 and torch.autograd.forward_ad._current_level < 0:
+        got = nat.torch_calls().copy_pages(codes, scales, src, dst, device, hip._stream(device))
+        if got is not None:
+            nat.result(got)
+            return
     _check_pool("copy_pages", codes, scales, 6)
     if len(src) != len(dst):
         raise ValueError(f"copy_pages takes as many sources as targets, got {len(src)} and {len(dst)}")

@@ -8,6 +8,7 @@ the attention over a bf16 cache, an output rounded once from products whose prob
 from __future__ import annotations
 
 import math
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -306,3 +307,42 @@ def test_prompts_match_float64(gpu, dtype, b, t, h, kv, d, page, starts, new):
     got = kvc.attention(q, codes, scales, table, starts_t, new_t).double()
     assert (got - want).norm() <= TWO_ROUNDINGS * want.norm()
     assert ((got - want).norm(dim=-1) <= 4 * TWO_ROUNDINGS * want.norm(dim=-1).clamp(min=1e-30)).all()
+
+
+@pytest.mark.parametrize("dtype", FORMATS)
+@pytest.mark.parametrize("t", [1, 40])
+def test_both_host_paths_are_the_same_operations(gpu, dtype, t, monkeypatch):
+    """The binding's calls and the Python functions behind them end in the same launches; both count as a write."""
+    b, h, kv, d, page = 3, 4, 2, 64, 32
+    results = []
+    for plain in (False, True):
+        if plain:
+            nothing = lambda *args: None
+            calls = SimpleNamespace(append=nothing, attention=nothing, copy_pages=nothing)
+            monkeypatch.setattr(kvc.nat, "torch_calls", lambda: calls)
+        codes, scales = _pool(gpu, 9, kv, page, d, dtype)
+        table = torch.tensor([[0, 1, 2], [3, 4, 5], [6, 7, 8]], dtype=torch.int32, device=gpu)
+        starts = torch.tensor([0, 31, -1], dtype=torch.int32, device=gpu)
+        x = torch.randn(b, t, h + 2 * kv, d, device=gpu, generator=_gen(gpu, t)).to(torch.bfloat16)
+        cos, sin = _tables(d, 96, gpu)
+        versions = codes._version, scales._version
+        q = kvc.append(x[:, :, :h], x[:, :, h:h + kv], x[:, :, h + kv:], cos, sin, codes, scales, table, starts)
+        assert codes._version > versions[0] and scales._version > versions[1]
+        y = kvc.attention(q, codes, scales, table, starts, max_tokens=80, scale=0.2)
+        pool, pool_scales = codes[None].clone(), scales[None].clone()
+        version = pool._version
+        kvc.copy_pages(pool, pool_scales, [0, 3], [7, 8])
+        assert pool._version > version
+        results.append([r.view(torch.uint8) for r in (q, codes, scales, y, pool, pool_scales)])
+    for one, other in zip(*results):
+        assert torch.equal(one, other)
+
+
+def test_forward_differentiation_is_refused(gpu):
+    codes, scales = _pool(gpu, 1, 1, 32, 64, torch.int8)
+    table = torch.zeros(1, 1, dtype=torch.int32, device=gpu)
+    q = torch.zeros(1, 1, 1, 64, device=gpu, dtype=torch.bfloat16)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(q, torch.ones_like(q))
+        with pytest.raises((TypeError, ValueError, RuntimeError, NotImplementedError)):
+            kvc.attention(dual, codes, scales, table, table[:, 0])

@@ -295,3 +295,27 @@ def test_int8_linear_on_the_host_is_the_definition():
     shape = W.LlamaShape(n_layers=1, hidden=64, n_heads=2, n_kv_heads=1, head_dim=32, inter=96, int8=True)
     layer = W.DecoderLayer(shape, torch.bfloat16)
     assert sum(p.numel() * p.element_size() for p in layer.parameters()) == shape.layer_bytes()
+
+
+def test_a_missing_torch_binding_fails_loudly(monkeypatch):
+    import sys
+
+    import flextensor_amd
+    from flextensor_amd import _native as nat
+
+    monkeypatch.setattr(nat, "_torch_calls", None)
+    monkeypatch.delattr(flextensor_amd, "_ftx_torch", raising=False)
+    monkeypatch.setitem(sys.modules, "flextensor_amd._ftx_torch", None)
+    with pytest.raises(nat.FtxLibraryMissing, match="torch binding"):
+        nat.torch_calls()
+
+
+def test_the_torch_binding_leaves_what_it_does_not_know_alone():
+    from flextensor_amd import _native as nat
+
+    calls = nat.torch_calls()
+    t = torch.zeros(2, 2, 2, 64, dtype=torch.bfloat16)
+    for name, n in (("append", 12), ("attention", 10), ("copy_pages", 6), ("int8_linear", 5), ("int8_matmul", 6)):
+        call = getattr(calls, name)
+        for args in ((), (None,) * n, (t,) * (n - 2) + (0, 0), ([],) * (n - 2) + (0, 0)):  # too few, no tensors, the host's
+            assert call(*args) is None
