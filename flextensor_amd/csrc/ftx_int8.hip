@@ -72,6 +72,17 @@ __device__ __forceinline__ uint32_t largest8(u32x4 v, uint32_t top) {
   return top;
 }
 
+// The largest of a wave's values, in every lane: pairs, quads, eights and sixteens of lanes, then the four sixteens.
+__device__ __forceinline__ uint32_t wave_largest(uint32_t v) {
+  const auto with = [&](auto other) { v = max(v, static_cast<uint32_t>(other)); };
+  with(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xb1, 15, 15, true));   // quad_perm 1 0 3 2
+  with(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4e, 15, 15, true));   // quad_perm 2 3 0 1
+  with(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x141, 15, 15, true));  // row_half_mirror
+  with(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x140, 15, 15, true));  // row_mirror
+  const auto lane = [&](int i) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), i)); };
+  return max(max(lane(0), lane(16)), max(lane(32), lane(48)));
+}
+
 // The scale of a row whose largest magnitude has these bf16 bits, and what its values are multiplied by.
 __device__ __forceinline__ float row_scale(uint32_t top, float *inverse) {
 #pragma clang fp contract(off)
@@ -94,11 +105,12 @@ __device__ __forceinline__ u32x2 code8(u32x4 v, float inverse) {
                                   code2(v[2], inverse) | code2(v[3], inverse) << 16};
 }
 
+constexpr int kHeld = 4;  // vectors of 8 values that a thread keeps
+
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void int8_quantize_kernel(const uint16_t *__restrict__ x, int64_t x_stride,
                                                                 uint8_t *__restrict__ codes, int64_t code_stride,
                                                                 float *__restrict__ scales, int k) {
-  constexpr int kHeld = 4;  // vectors of 8 values that a thread keeps
   __shared__ uint32_t wave_top[THREADS / kWave];
   const int64_t row = blockIdx.x;
   const u32x4 *xr = reinterpret_cast<const u32x4 *>(x + row * x_stride);
@@ -113,8 +125,7 @@ __global__ __launch_bounds__(THREADS) void int8_quantize_kernel(const uint16_t *
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) top = largest8(held[i], top);
   for (int i = first + kHeld * THREADS; i < n; i += THREADS) top = largest8(xr[i], top);
-#pragma unroll
-  for (int i = 1; i < kWave; i *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), i)));
+  top = wave_largest(top);
   if (threadIdx.x % kWave == 0) wave_top[threadIdx.x / kWave] = top;
   __syncthreads();
 #pragma unroll
@@ -132,66 +143,142 @@ __global__ __launch_bounds__(THREADS) void int8_quantize_kernel(const uint16_t *
 
 // ---- up to 16 rows -------------------------------------------------------------------------------------------------
 //
-// A workgroup owns 16 channels over the whole of K; its eight waves take windows of 256 bytes of every row in turn,
-// straight into registers as the operands of v_mfma_i32_16x16x64_i8 (lane (r, g): 16 bytes of row r), three windows
-// in flight, and their sums meet in LDS. Bound by the bytes of w.
+// The codes lie in LDS; a workgroup then walks groups of 16 channels over the whole of K. Its eight waves take windows
+// of 256 bytes of the channels in turn, straight into registers as the operands of v_mfma_i32_16x16x64_i8 (lane (r, g):
+// 16 bytes of channel r), three windows in flight across the ends of groups, and their sums meet in LDS. Bound by the
+// bytes of w.
+//
+// CODES bytes of LDS hold the rows, 16 bytes between them against conflicts. Where a row or a few make at most
+// kHeldRows vectors of 8 values a thread (FUSED), each workgroup rounds x itself and there is no other launch.
 
 constexpr int kWindow = 256;
+constexpr int kHeldRow = 512 * 8;  // values of a row that this kernel's threads hold one vector each of
+constexpr int kHeldRows = 8;       // that a thread may hold (4096 x 4096 of 8 rows: 9.1 us, with codes from a launch 9.4)
+constexpr int kFusedCodes = kHeldRows * (kHeldRow + 16), kSomeCodes = 60 << 10, kMostCodes = 143 << 10;
 
-__global__ __launch_bounds__(512, 4) void int8_rows_kernel(Int8Linear p) {
-  __shared__ i32x4 part[8][kWave];
+template <bool FUSED, int CODES>
+__global__ __launch_bounds__(512, CODES <= kSomeCodes ? 4 : 2) void int8_rows_kernel(Int8Linear p) {
+  __shared__ __align__(16) uint8_t codes[CODES];
+  __shared__ i32x4 part[2][8][kWave];
+  __shared__ float row_scales[16];
+  __shared__ uint32_t row_top[kHeldRows];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 15, g = lane >> 4;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
-  const int rows = static_cast<int>(least(16, p.n - n0));
-  const auto w = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p.w + n0 * p.k), 0, rows * p.k, 0x00027000);
-  const auto c = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p.codes), 0, p.m * p.code_stride, 0x00027000);
-  const uint32_t w_at = r * p.k + 16 * g, c_at = r * p.code_stride + 16 * g;
-  struct Window {
-    u32x4 w[4], c[4];
-  };
-  const auto load = [&](Window &x, int window) {
+  const int m = static_cast<int>(p.m), pitch = p.code_stride + 16;
+  const int windows = p.code_stride / kWindow, steps = (windows + 7) / 8;
+  // thread: token t, channel ch of a group; lane t + 16 g of each wave's sums holds channels 4 g .. 4 g + 3
+  const int t = threadIdx.x / 16, ch = threadIdx.x % 16;
+  const uint32_t per_row = (p.k + kHeldRow - 1) / kHeldRow;
+  const int items = m * per_row;
+  u32x4 held[kHeldRows];
+  if (FUSED) {  // ahead of the loads of w, which come in while the codes are made
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x.w[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(w, w_at, window * kWindow + 64 * i, 0));
-      x.c[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(c, c_at, window * kWindow + 64 * i, 0));
+    for (int j = 0; j < kHeldRows; ++j) {
+      const int row = uniform(j / per_row), col = uniform(j % per_row);
+      const auto x = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p.x + row * p.x_stride), 0,
+                                                       row < m ? p.k * 2 : 0, 0x00027000);
+      held[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                              x, col * kHeldRow * 2 + threadIdx.x * 16, 0, 0));
     }
+    if (threadIdx.x < kHeldRows) row_top[threadIdx.x] = 0;
+  }
+  const auto scale_of = [&](uint32_t group) {
+    const int64_t at = static_cast<int64_t>(group) * 16 + ch;
+    return at < p.n ? p.w_scale[at] : 0.f;
   };
-  i32x4 acc = {0, 0, 0, 0};
-  const auto work = [&](const Window &x) {
+  float w_scale = scale_of(blockIdx.x);
+
+  const uint32_t w_at = r * p.k + 16 * g;
+  uint32_t load_group = blockIdx.x;
+  int load_step = 0;
+  const auto load = [&](u32x4 (&w)[4]) {  // the next window; zeros past the row's end for this wave and past the last group
+    const int64_t n0 = static_cast<int64_t>(load_group) * 16;
+    const int rows = load_group < p.items ? static_cast<int>(least(16, p.n - n0)) : 0;
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p.w + (rows > 0 ? n0 * p.k : 0)), 0,
+                                                        rows * p.k, 0x00027000);
+    const int window = load_step * 8 + wave;
+    const uint32_t at = window < windows ? w_at + window * kWindow : 0x40000000u;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, x.w[i]), __builtin_bit_cast(i32x4, x.c[i]), acc, 0, 0, 0);
+      w[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at + 64 * i, 0, 0));
+    if (++load_step == steps) load_step = 0, load_group += p.groups;
   };
-  const int windows = p.code_stride / kWindow, last = windows - 1;
-  if (wave < windows) {
-    Window x, y, z;
-    int i = wave;
-    load(x, i);
-    load(y, min(i + 8, last));
-    for (;;) {  // loads past the end take the last window again
-      load(z, min(i + 16, last));
-      work(x);
-      if ((i += 8) >= windows) break;
-      load(x, min(i + 16, last));
-      work(y);
-      if ((i += 8) >= windows) break;
-      load(y, min(i + 16, last));
-      work(z);
-      if ((i += 8) >= windows) break;
-    }
-  }
-  part[wave][lane] = acc;
-  __syncthreads();
-  // thread: token t, channel c; lane t + 16 g of each wave holds channels 4 g .. 4 g + 3
-  const int t = threadIdx.x / 16, ch = threadIdx.x % 16;
-  if (t >= p.m || ch >= rows) return;
-  int sum = 0;
+  u32x4 x[4], y[4], z[4];
+  load(x);
+  load(y);
+
+  if (FUSED) {
+    ring_barrier();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sum += part[i][t + 16 * (ch / 4)][ch % 4];
-  const float y = static_cast<float>(sum) * p.x_scale[t] * p.w_scale[n0 + ch];
-  p.y[t * p.n + n0 + ch] = static_cast<uint16_t>(pack_bf16(y, 0.f));
+    for (int j = 0; j < kHeldRows; ++j) {
+      if (j >= items) break;
+      const uint32_t top = wave_largest(largest8(held[j], 0));
+      if (lane == 0) atomicMax(&row_top[uniform(j / per_row)], top);
+    }
+    ring_barrier();
+#pragma unroll
+    for (int j = 0; j < kHeldRows; ++j) {
+      if (j >= items) break;
+      const int row = uniform(j / per_row), at = uniform(j % per_row) * kHeldRow + threadIdx.x * 8;
+      float inverse;
+      const float scale = row_scale(row_top[row], &inverse);
+      if (at < p.code_stride) *reinterpret_cast<u32x2 *>(codes + row * pitch + at) = code8(held[j], inverse);
+      if (threadIdx.x == 0) row_scales[row] = scale;
+    }
+  } else {
+    constexpr int kBatch = 8;
+    const uint32_t of_row = p.code_stride / 16, all = m * of_row;
+    const u32x4 *from = reinterpret_cast<const u32x4 *>(p.codes);
+    for (uint32_t first = threadIdx.x; first < all; first += 512 * kBatch) {
+      u32x4 v[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) v[i] = from[min(first + i * 512, all - 1)];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const uint32_t at = min(first + i * 512, all - 1);  // the last one again: the same bytes
+        *reinterpret_cast<u32x4 *>(codes + at * 16 + at / of_row * 16) = v[i];
+      }
+    }
+    if (threadIdx.x < m) row_scales[threadIdx.x] = p.x_scale[threadIdx.x];
+  }
+  ring_barrier();
+
+  const uint32_t c_at = min(r, m - 1) * pitch + 16 * g;
+  i32x4 acc = {0, 0, 0, 0};
+  uint32_t group = blockIdx.x;
+  int step = 0, side = 0;
+  const auto work = [&](const u32x4 (&w)[4]) {  // returns whether it was the last one
+    const uint8_t *c = codes + c_at + min(step * 8 + wave, windows - 1) * kWindow;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w[i]),
+                                                  *reinterpret_cast<const i32x4 *>(c + 64 * i), acc, 0, 0, 0);
+    if (++step < steps) return false;
+    part[side][wave][lane] = acc;
+    ring_barrier();  // the other side's sums have been read by all
+    const int64_t at = static_cast<int64_t>(group) * 16 + ch;
+    if (t < m && at < p.n) {
+      int sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += part[side][i][t + 16 * (ch / 4)][ch % 4];
+      p.y[t * p.n + at] = static_cast<uint16_t>(pack_bf16(static_cast<float>(sum) * row_scales[t] * w_scale, 0.f));
+    }
+    acc = (i32x4){0, 0, 0, 0};
+    step = 0;
+    side ^= 1;
+    group += p.groups;
+    w_scale = scale_of(group);
+    return group >= p.items;
+  };
+  for (;;) {
+    load(z);
+    if (work(x)) break;
+    load(x);
+    if (work(y)) break;
+    load(y);
+    if (work(z)) break;
+  }
 }
 
 // ---- tiles -----------------------------------------------------------------------------------------------------------
@@ -414,10 +501,10 @@ hipError_t launch_int8_quantize(const uint16_t *x, int64_t x_stride, uint8_t *co
 // Measured, us: 28672 x 8192 of 32 rows 50.3 in tiles of 64, 54.3 split in two; 8192 x 28672 106.7, in four 44.8; 4096
 // x 4096 17.7 and 11.2. 28672 x 8192 of 200 rows 118, 74.6 and 101 in tiles of 64, 128 and 256, of 512 rows 193, 150 and
 // 114, of 1000 360, 292 and 239; 8192 x 28672 of 512 rows 131 in tiles of 256 split in four, 164 in tiles of 128 split
-// in two. Up to 16 rows the kernel without tiles is the faster one while w is small (4096 x 4096 of 13 rows 6.7, in
-// tiles 10.4) or the rows are few (28672 x 8192 of one row 44.3, of 13 63.4 and 50.1): each of its workgroups reads all
-// rows' codes.
-void plan_int8_linear(Int8Linear *p, int cus, int xcds) {
+// in two. Up to 16 rows whose codes fit LDS have the kernel without tiles: 28672 x 8192 of 1, 4, 8 and 16 rows 41, 44, 45
+// and 47, in tiles 49 and 50; 4096 x 4096 6, 7, 9 and 10, in tiles 13 and 14. Rows of fewer windows than waves leave
+// some of these idle: 28672 x 1024 of one row 10.9 (tiles: 11.5), of 16, whose codes take a launch, 13.5 and 11.9.
+void plan_int8_linear(Int8Linear *p, bool from_x, int cus, int xcds) {
   p->xcds = std::max(1, xcds);
   p->part_stride = (p->n + 3) / 4 * 4;
   const int64_t steps = std::max(1, (p->k + 127) / 128);
@@ -442,13 +529,22 @@ void plan_int8_linear(Int8Linear *p, int cus, int xcds) {
   weigh(64, 128, 45, 41, 400);
   if (p->m > 64) weigh(128, 128, 95, 64, 700);
   if (p->m > 128) weigh(256, 256, 150, 190, 1000);
-  if (p->m <= 16 && reading * (1000 + 35 * p->m) / 1000 + 250 <= best) {
+  const int64_t code_bytes = p->m * (p->code_stride + 16), windows = p->code_stride / kWindow;
+  p->one_launch = from_x && p->m <= 16 && p->m * ((p->k + kHeldRow - 1) / kHeldRow) <= kHeldRows;
+  if (p->m <= 16 && p->k > 0 && code_bytes <= kMostCodes &&
+      reading * (16 - std::min<int64_t>(8, windows)) / 8 + (p->one_launch ? 0 : 250) <= best) {
     p->tile_m = 16;
     p->splits = 1;
     p->items = static_cast<uint32_t>((p->n + 15) / 16);
+    // Two workgroups a CU take every place there is (10240 x 8192 of one row 18.4, in equal rounds 21.8), one a CU
+    // equal rounds (of 16 rows 21.8, 23.1 with every place taken).
+    const bool two = code_bytes <= kSomeCodes;
+    const uint32_t slots = cus * (two ? 2 : 1), rounds = (p->items + slots - 1) / slots;
+    p->groups = two ? std::min(slots, p->items) : (p->items + rounds - 1) / rounds;
     p->part_bytes = 0;
     return;
   }
+  p->one_launch = false;
   p->m_tiles = static_cast<uint32_t>((p->m + p->tile_m - 1) / p->tile_m);
   p->n_tiles = static_cast<uint32_t>((p->n + p->tile_n - 1) / p->tile_n);
   // An XCD walks a run of up to 12 tiles of tokens before its next tile of channels, equal runs: their codes and the
@@ -464,7 +560,12 @@ void plan_int8_linear(Int8Linear *p, int cus, int xcds) {
 
 hipError_t launch_int8_linear(const Int8Linear &p, hipStream_t stream) {
   switch (p.tile_m) {
-    case 16: hipLaunchKernelGGL(int8_rows_kernel, dim3(p.items), dim3(512), 0, stream, p); break;
+    case 16:
+      if (p.x) hipLaunchKernelGGL((int8_rows_kernel<true, kFusedCodes>), dim3(p.groups), dim3(512), 0, stream, p);
+      else if (p.m * (p.code_stride + 16) <= kSomeCodes)
+        hipLaunchKernelGGL((int8_rows_kernel<false, kSomeCodes>), dim3(p.groups), dim3(512), 0, stream, p);
+      else hipLaunchKernelGGL((int8_rows_kernel<false, kMostCodes>), dim3(p.groups), dim3(512), 0, stream, p);
+      break;
     case 64: start_tiles<64, 128, 1, 4, 3>(p, stream); break;
     case 128: start_tiles<128, 128, 2, 2, 2>(p, stream); break;
     default: start_tiles<256, 256, 2, 4, 2>(p, stream); break;

@@ -238,6 +238,8 @@ hipError_t launch_kv8_copy(const Kv8Copy &p, hipStream_t stream);
 constexpr int64_t kInt8MaxK = 131072;  // 127^2 K fits 32-bit sums
 constexpr int64_t int8_code_stride(int64_t k) { return (k + 255) / 256 * 256; }  // bytes of a row of codes
 struct Int8Linear {
+  const uint16_t *x;      // bf16 [m] rows x_stride apart: one_launch, in place of codes and x_scale; else null
+  int64_t x_stride;
   const uint8_t *codes;   // [m][code_stride], 0 from k on
   const float *x_scale;   // [m]
   const uint8_t *w;       // [n][k]
@@ -248,10 +250,11 @@ struct Int8Linear {
   int k, code_stride;
   // planned
   int tile_m, tile_n, splits, split_steps, band, xcds;  // tile_m 16: the kernel of up to 16 rows
-  uint32_t m_tiles, n_tiles, items;
+  uint32_t m_tiles, n_tiles, items, groups;  // groups: workgroups of the kernel of up to 16 rows
   size_t part_bytes;
+  bool one_launch;        // the product rounds x itself
 };
-void plan_int8_linear(Int8Linear *p, int cus, int xcds);
+void plan_int8_linear(Int8Linear *p, bool from_x, int cus, int xcds);  // from_x: x may be given in place of codes
 hipError_t launch_int8_linear(const Int8Linear &p, hipStream_t stream);
 hipError_t launch_int8_quantize(const uint16_t *x, int64_t x_stride, uint8_t *codes, int64_t code_stride, float *scales,
                                 int64_t m, int k, hipStream_t stream);

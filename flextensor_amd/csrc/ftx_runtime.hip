@@ -1654,7 +1654,7 @@ int check_int8(int64_t m, int64_t n, int64_t k) {
   return FTX_OK;
 }
 
-int plan_int8(int64_t m, int64_t n, int64_t k, ftx::Int8Linear *p) {
+int plan_int8(int64_t m, int64_t n, int64_t k, bool from_x, ftx::Int8Linear *p) {
   int rc = check_int8(m, n, k);
   if (rc != FTX_OK) return rc;
   p->m = m;
@@ -1668,7 +1668,7 @@ int plan_int8(int64_t m, int64_t n, int64_t k, ftx::Int8Linear *p) {
     cus = st->cu_count;
     xcds = st->xcd_count;
   }
-  ftx::plan_int8_linear(p, cus, xcds);
+  ftx::plan_int8_linear(p, from_x, cus, xcds);
   if (static_cast<int64_t>(p->items) + p->xcds > ftx::kMaxThreads / 512 ||
       (p->splits > 1 && m * p->part_stride > (int64_t(1) << 33)))
     return ftx::fail(FTX_ERR_UNSUPPORTED, "int8 linear: more workgroups than one launch holds");
@@ -1697,7 +1697,7 @@ int ftx_int8_quantize(const void *x, int64_t x_stride, void *codes, float *scale
 int ftx_int8_matmul_workspace(int64_t m, int64_t n, int64_t k, size_t *bytes) {
   if (!bytes) return ftx::fail(FTX_ERR_INVALID, "bytes is null");
   ftx::Int8Linear p{};
-  int rc = plan_int8(m, n, k, &p);
+  int rc = plan_int8(m, n, k, false, &p);
   if (rc == FTX_OK) *bytes = p.part_bytes;
   return rc;
 }
@@ -1726,7 +1726,7 @@ int ftx_int8_matmul(const void *codes, const float *x_scale, const void *w, cons
                     int64_t n, int64_t k, void *workspace, size_t workspace_bytes, void *stream) {
   FTX_REQUIRE_LIVE();
   ftx::Int8Linear p{};
-  int rc = plan_int8(m, n, k, &p);
+  int rc = plan_int8(m, n, k, false, &p);
   if (rc != FTX_OK) return rc;
   if (m == 0 || n == 0) return FTX_OK;
   if (k > 0) rc = check_operand(codes, m * p.code_stride, 1, "int8 codes");
@@ -1749,8 +1749,8 @@ int ftx_int8_matmul(const void *codes, const float *x_scale, const void *w, cons
 int ftx_int8_linear_workspace(int64_t m, int64_t n, int64_t k, size_t *bytes) {
   if (!bytes) return ftx::fail(FTX_ERR_INVALID, "bytes is null");
   ftx::Int8Linear p{};
-  int rc = plan_int8(m, n, k, &p);
-  if (rc == FTX_OK) *bytes = m == 0 || n == 0 ? 0 : int8_part_offset(p) + p.part_bytes;
+  int rc = plan_int8(m, n, k, true, &p);
+  if (rc == FTX_OK) *bytes = m == 0 || n == 0 || p.one_launch ? 0 : int8_part_offset(p) + p.part_bytes;
   return rc;
 }
 
@@ -1758,7 +1758,7 @@ int ftx_int8_linear(const void *x, int64_t x_stride, const void *w, const float 
                     int64_t k, void *workspace, size_t workspace_bytes, void *stream) {
   FTX_REQUIRE_LIVE();
   ftx::Int8Linear p{};
-  int rc = plan_int8(m, n, k, &p);
+  int rc = plan_int8(m, n, k, true, &p);
   if (rc != FTX_OK) return rc;
   if (x_stride < k || x_stride % 8 != 0 || x_stride > int64_t(1) << 38)
     return ftx::fail(FTX_ERR_INVALID, "int8 linear: rows of x must not overlap and start at multiples of 8 elements");
@@ -1766,6 +1766,12 @@ int ftx_int8_linear(const void *x, int64_t x_stride, const void *w, const float 
   if (k > 0) rc = check_operand(x, (m - 1) * x_stride + k, 2, "int8 input");
   if (rc == FTX_OK) rc = check_int8_product(&p, w, w_scale, y);
   if (rc != FTX_OK) return rc;
+  if (p.one_launch) {
+    p.x = static_cast<const uint16_t *>(x);
+    p.x_stride = x_stride;
+    FTX_HIP(ftx::launch_int8_linear(p, static_cast<hipStream_t>(stream)));
+    return FTX_OK;
+  }
   const size_t need = int8_part_offset(p) + p.part_bytes;
   if (workspace_bytes < need)
     return ftx::fail(FTX_ERR_INVALID, "the int8 linear needs a workspace of " + std::to_string(need) +

@@ -416,7 +416,8 @@ int ftx_silu_mul(const void *g, const void *u, void *y, int64_t n, void *stream)
  * w_scale[n]) of such rows and int8 w [n, k] (-127 .. 127, contiguous); the sums
  * are exact. workspace: ftx_int8_matmul_workspace bytes (0 unless K is split).
  * ftx_int8_linear: the one, then the other, with the codes in its workspace
- * (ftx_int8_linear_workspace bytes). Pointers are 16-byte aligned. */
+ * (ftx_int8_linear_workspace bytes; 0 for a few rows of few values, whose codes
+ * the product's workgroups make for themselves). Pointers are 16-byte aligned. */
 #define FTX_INT8_CODE_STRIDE(k) (((int64_t)(k) + 255) / 256 * 256)
 int ftx_int8_quantize(const void *x, int64_t x_stride, void *codes, float *scales, int64_t m, int64_t k, void *stream);
 int ftx_int8_matmul_workspace(int64_t m, int64_t n, int64_t k, size_t *bytes);

@@ -86,6 +86,29 @@ def test_linear_matches_exact_sums(gpu, m, n, k):
     assert ((got - want).abs() <= ONE_ROUNDING * want.abs()).all()
 
 
+@pytest.mark.parametrize("m,n,k", [
+    (1, 30000, 4112), (1, 300, 32768), (2, 20000, 8208), (4, 17, 272), (7, 9001, 272), (8, 8200, 4096),  # rounds x itself
+    (16, 40, 2048), (16, 9001, 3600), (3, 20000, 8208), (12, 9001, 8208), (1, 5000, 131072),              # codes from a launch
+])
+def test_rows_of_a_wider_tensor_as_codes_and_product(gpu, m, n, k):
+    """However the codes come to the product: the same numbers, of rows among others, one of them zeros, one with an
+    infinity."""
+    x, w, scale = _inputs(gpu, m, n, k)
+    wide = torch.full((m, k + 64), 3.0e38, device=gpu, dtype=torch.bfloat16)
+    wide[:, :k] = x
+    if m > 2:
+        wide[1, :k] = 0.0
+        wide[2, k - 1] = float("-inf")
+    codes, scales = _quantised(wide[:, :k])
+    want = codes.to(gpu).double() @ w.double().t() * scales[:, None].to(gpu).double() * scale.double()
+    got = hip.int8_linear(wide[:, :k], w, scale)
+    assert torch.equal(got.view(torch.int16), hip.int8_matmul(*hip.int8_quantize(wide[:, :k]), w, scale).view(torch.int16))
+    rest = [i for i in range(m) if m <= 2 or i != 2]
+    assert ((got.double() - want).abs() <= ONE_ROUNDING * want.abs())[rest].all()
+    if m > 2:
+        assert got[2].isnan().all()
+
+
 def test_linear_of_the_largest_sums(gpu):
     """Every product 127^2: the longest K reaches 2113929216 of the 2147483647 that 32 bits hold."""
     k = hip.INT8_LINEAR_MAX_K
