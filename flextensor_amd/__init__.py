@@ -4,7 +4,8 @@ Host logic (planning, scheduling, the offload phases) is Python over PyTorch;
 device work goes through the HIP C-ABI library ``libftx_hip.so``
 (``include/ftx.h``): pinned host arenas, host-to-device copy engines
 (hipMemcpyAsync and a zero-copy kernel), a batched scatter kernel and
-hipEvent gating, an fp8-weight MFMA GEMM, and a staged copy engine for
+hipEvent gating, an fp8-weight MFMA GEMM, a paged 8-bit KV cache
+(``kv_cache``) with int8 projections, and a staged copy engine for
 pageable and shared-memory sources. Models can be built straight from a
 saved profile and a safetensors checkpoint (``load_model_from_profile``).
 """
