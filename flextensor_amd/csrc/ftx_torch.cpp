@@ -2,7 +2,7 @@
 //
 // A decode step's kernels take 5 to 8 us; checking their tensors attribute by attribute in Python and packing the
 // C call's arguments took 13 to 18. Each function here looks at its arguments, allocates the result and the workspace
-// and calls the C ABI (6 to 10 us in all, the launches included). What it does not recognise as a plain call it leaves alone: it returns None,
+// and calls the C ABI (6 to 8 us in all, a launch included). What it does not recognise as a plain call it leaves alone: it returns None,
 // and the Python function goes through its own checks, which say what is wrong or arrange what can be (a copy of
 // strided rows, another stride of a table). A failed C call comes back as its status.
 #include <torch/csrc/autograd/python_variable.h>

@@ -109,6 +109,15 @@ def test_rows_of_a_wider_tensor_as_codes_and_product(gpu, m, n, k):
         assert got[2].isnan().all()
 
 
+@pytest.mark.parametrize("m,n,k", [(0, 5, 16), (3, 0, 16), (3, 5, 0), (20, 130, 0), (1, 1, 0)])
+def test_linear_of_nothing(gpu, m, n, k):
+    x = torch.ones(m, k, device=gpu, dtype=torch.bfloat16)
+    w = torch.ones(n, k, device=gpu, dtype=torch.int8)
+    scale = torch.ones(n, device=gpu)
+    for got in (hip.int8_linear(x, w, scale), hip.int8_matmul(*hip.int8_quantize(x), w, scale)):
+        assert got.shape == (m, n) and not got.any()
+
+
 def test_linear_of_the_largest_sums(gpu):
     """Every product 127^2: the longest K reaches 2113929216 of the 2147483647 that 32 bits hold."""
     k = hip.INT8_LINEAR_MAX_K
