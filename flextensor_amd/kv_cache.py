@@ -339,12 +339,14 @@ class PagedKVCache:
         return sequence
 
     def fork(self, sequence: int) -> int:
-        """A new sequence with the same tokens, on the same pages."""
-        pages = self._pages[sequence]
+        """A new sequence with the same tokens, on the same pages. Pages that a step not committed has reserved stay
+        the sequence's own."""
+        length = self._lengths[sequence]
+        pages = self._pages[sequence][: -(-length // self.page_tokens)]
         other = self.open()
         for p in pages:
             self._refs[p] += 1
-        self._pages[other], self._lengths[other] = list(pages), self._lengths[sequence]
+        self._pages[other], self._lengths[other] = pages, length
         return other
 
     def truncate(self, sequence: int, length: int) -> None:
@@ -387,9 +389,9 @@ class PagedKVCache:
         sharers: dict[int, int] = {}  # what is left of a shared page's references as this step's sequences leave it
         for s, c in zip(sequences, counts):
             length, held = self._lengths[s], self._pages[s]
-            need += max(0, -(-(length + c) // size) - len(held))
-            at = length // size
-            if c and at < len(held):
+            end = -(-(length + c) // size)
+            need += max(0, end - len(held))
+            for at in range(length // size, min(end, len(held)) if c else 0):  # held pages that the step writes
                 left = sharers.setdefault(held[at], self._refs[held[at]])
                 if left > 1:
                     sharers[held[at]] = left - 1

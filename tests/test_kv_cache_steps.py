@@ -1,0 +1,122 @@
+"""Steps of the paged cache that are not committed at once: what they reserve is theirs alone, and what a step may
+count. Without a GPU."""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+import torch
+
+from flextensor_amd import kv_cache as kvc
+
+PAGE = 32
+
+
+@pytest.fixture
+def pool(monkeypatch):
+    """A pool whose page copies are torch's."""
+
+    def copy(codes, scales, src, dst):
+        assert len(set(dst)) == len(dst) and not set(src) & set(dst)
+        codes.view(torch.uint8)[:, dst] = codes.view(torch.uint8)[:, src]
+        scales[:, dst] = scales[:, src]
+
+    monkeypatch.setattr(kvc, "copy_pages", copy)
+    return kvc.PagedKVCache(1, 1, 64, 16, page_tokens=PAGE, dtype=torch.int8, device="cpu")
+
+
+def _written(cache, step):
+    """The pages that a step's appends write, by its own table."""
+    pages = []
+    for row, start, count in zip(step.table.tolist(), step.starts.tolist(), step.new.tolist()):
+        if count:
+            pages += row[start // PAGE: (start + count - 1) // PAGE + 1]
+    return pages
+
+
+def test_a_fork_between_begin_and_commit_holds_committed_tokens_alone(pool):
+    a = pool.open()
+    step = pool.begin([a], 40)
+    b = pool.fork(a)
+    assert pool.table(b) == [] and pool.length(b) == 0
+    pool.commit(step)
+    other = pool.begin([b], 40)
+    assert not set(pool.table(a)) & set(_written(pool, other))
+
+
+def test_a_fork_shares_the_page_in_use_and_none_that_is_reserved(pool):
+    a = pool.open()
+    pool.commit(pool.begin([a], 10))
+    step = pool.begin([a], 100)
+    b = pool.fork(a)
+    assert pool.table(b) == pool.table(a)[:1]
+    pool.commit(step)
+    other = pool.begin([b], 100)
+    assert not set(pool.table(a)) & set(_written(pool, other)) and pool.table(a) == step.table[0].tolist()
+
+
+def test_forks_after_an_abandoned_step_write_pages_of_their_own(pool):
+    a = pool.open()
+    pool.begin([a], 100)  # a pass that failed
+    pool.commit(pool.begin([a], 10))
+    b = pool.fork(a)
+    step = pool.begin([a, b], 40)
+    pages = _written(pool, step)
+    assert len(pages) == 4 and len(set(pages)) == 4
+
+
+def test_every_shared_page_that_a_step_writes_is_copied(pool):
+    """Held pages past the one in use, however they came to be shared."""
+    a = pool.open()
+    pool.begin([a], 100)
+    b = pool.open()
+    pool._pages[b] = list(pool._pages[a])
+    for p in pool._pages[a]:
+        pool._refs[p] += 1
+    step = pool.begin([a, b], 70)
+    pages = _written(pool, step)
+    assert len(pages) == 6 and len(set(pages)) == 6
+    assert all(pool._refs[p] == 1 for p in pages)
+
+
+def test_a_long_run_with_steps_in_flight(pool):
+    """Random forks, truncations and closings between begin and commit, and steps that are given up: no page that a
+    step writes is held by another sequence when it begins, none that holds another's committed tokens is written."""
+    rng = random.Random(11)
+    held: list[int] = []
+    flight = []
+    for _ in range(1500):
+        move = rng.choice(["open", "begin", "begin", "commit", "fork", "fork", "truncate", "close", "give up"])
+        busy = {s for step in flight for s in step.sequences}
+        idle = [s for s in held if s not in busy]
+        try:
+            if move == "open" and len(held) < 6:
+                held.append(pool.open())
+            elif move == "begin" and idle:
+                some = rng.sample(idle, rng.randint(1, len(idle)))
+                step = pool.begin(some, [rng.randint(0, 70) for _ in some])
+                pages = _written(pool, step)
+                assert len(set(pages)) == len(pages) and all(pool._refs[p] == 1 for p in pages)
+                flight.append(step)
+            elif move == "commit" and flight:
+                pool.commit(flight.pop(rng.randrange(len(flight))))
+            elif move == "give up" and flight:
+                flight.pop(rng.randrange(len(flight)))
+            elif move == "fork" and held and len(held) < 8:
+                held.append(pool.fork(rng.choice(held)))
+            elif move == "truncate" and idle:
+                s = rng.choice(idle)
+                pool.truncate(s, rng.randint(0, pool.length(s)))
+            elif move == "close" and idle:
+                s = rng.choice(idle)
+                pool.close(s)
+                held.remove(s)
+        except kvc.KVCacheFull:
+            pass
+        for step in flight:  # committed tokens of a sequence stay out of the reach of the steps of others
+            for s, row, start, count in zip(step.sequences, step.table.tolist(), step.starts.tolist(), step.new.tolist()):
+                for at in range(start // PAGE, -(-(start + count) // PAGE)) if count else ():
+                    for other in held:
+                        if other != s and row[at] in pool.table(other):
+                            assert pool.table(other).index(row[at]) == at and pool.length(other) <= start
