@@ -398,16 +398,12 @@ class PagedKVCache:
                     shared.append((s, at))
         if need + len(shared) > len(self._free):
             raise KVCacheFull(f"{need + len(shared)} pages needed, {len(self._free)} of {self.pages} free")
-        src, dst = [], []
-        for s, at in shared:
-            old = self._pages[s][at]
-            new = self._take()
+        src = [self._pages[s][at] for s, at in shared]
+        if src:  # a copy that fails leaves the books as they were
+            copy_pages(self.codes, self.scales, src, self._free[: -len(src) - 1: -1])
+        for (s, at), old in zip(shared, src):
+            self._pages[s][at] = self._take()
             self._refs[old] -= 1
-            self._pages[s][at] = new
-            src.append(old)
-            dst.append(new)
-        if src:
-            copy_pages(self.codes, self.scales, src, dst)
         for s, c in zip(sequences, counts):
             held = self._pages[s]
             while len(held) * size < self._lengths[s] + c:

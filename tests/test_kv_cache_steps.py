@@ -120,3 +120,21 @@ def test_a_long_run_with_steps_in_flight(pool):
                     for other in held:
                         if other != s and row[at] in pool.table(other):
                             assert pool.table(other).index(row[at]) == at and pool.length(other) <= start
+
+
+def test_a_copy_that_fails_changes_nothing(pool, monkeypatch):
+    a = pool.open()
+    pool.commit(pool.begin([a], 10))
+    b = pool.fork(a)
+    before = pool.table(a), pool.table(b), list(pool._refs), list(pool._free)
+
+    def fails(*args):
+        raise RuntimeError("no copy")
+
+    with monkeypatch.context() as m:
+        m.setattr(kvc, "copy_pages", fails)
+        with pytest.raises(RuntimeError, match="no copy"):
+            pool.begin([a, b], 1)
+    assert (pool.table(a), pool.table(b), pool._refs, pool._free) == before
+    pages = _written(pool, pool.begin([a, b], 1))
+    assert len(set(pages)) == 2
