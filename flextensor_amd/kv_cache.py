@@ -251,6 +251,8 @@ class KVStep:
     new: torch.Tensor
     tokens: int
     max_tokens: int
+    held: tuple = ()  # of each sequence: its length, and the pages that its new tokens go to
+    moves: int = 0  # compactions of the cache before it
 
     def layer(self, index: int) -> "KVLayer":
         return KVLayer(self, index)
@@ -305,6 +307,7 @@ class PagedKVCache:
         self._pages: dict[int, list[int]] = {}
         self._lengths: dict[int, int] = {}
         self._next = 0
+        self._moves = 0
 
     def _tensors(self, pages: int) -> tuple[torch.Tensor, torch.Tensor]:
         shape = (self.layers, pages, 2, self.kv_heads, self.page_tokens // BLOCK)
@@ -415,10 +418,21 @@ class PagedKVCache:
         dev = host.to(self.device)  # one upload
         longest = max((self._lengths[s] + c for s, c in zip(sequences, counts)), default=0)
         return KVStep(self, tuple(sequences), tuple(counts), dev[2 * b:].view(b, width), dev[:b], dev[b: 2 * b],
-                      tokens, longest)
+                      tokens, longest, tuple(self._state(s, c) for s, c in zip(sequences, counts)), self._moves)
+
+    def _state(self, sequence: int, count: int) -> tuple[int, list[int]]:
+        """The length of a sequence, and the pages that its next tokens go to."""
+        length, size = self._lengths[sequence], self.page_tokens
+        return length, self._pages[sequence][length // size: -(-(length + count) // size) if count else 0]
 
     def commit(self, step: KVStep) -> None:
-        """Counts a step's tokens as cached."""
+        """Counts a step's tokens as cached. A step counts once, and only where its sequences are as they were when it
+        began: not truncated or closed, and the pages that it wrote still theirs (or moved by :meth:`compact`)."""
+        moved = step.moves != self._moves
+        if step.cache is not self or any(
+                self._lengths.get(s) != was[0] or not moved and self._state(s, c) != was
+                for s, c, was in zip(step.sequences, step.counts, step.held)):
+            raise ValueError("the step was committed before, or its sequences have changed since it began")
         for s, c in zip(step.sequences, step.counts):
             self._lengths[s] += c
 
@@ -435,6 +449,7 @@ class PagedKVCache:
                 self._refs[d], self._refs[s] = self._refs[s], 0
             for pages in self._pages.values():
                 pages[:] = [to.get(p, p) for p in pages]
+            self._moves += 1
         self._free = list(range(self.pages - 1, used - 1, -1))
         return len(src)
 

@@ -138,3 +138,51 @@ def test_a_copy_that_fails_changes_nothing(pool, monkeypatch):
     assert (pool.table(a), pool.table(b), pool._refs, pool._free) == before
     pages = _written(pool, pool.begin([a, b], 1))
     assert len(set(pages)) == 2
+
+
+def test_a_step_is_counted_once(pool):
+    a, b = pool.open(), pool.open()
+    step = pool.begin([a, b], [10, 0])
+    pool.commit(step)
+    with pytest.raises(ValueError, match="committed before"):
+        pool.commit(step)
+    assert pool.length(a) == 10 and pool.length(b) == 0
+
+
+def test_a_step_of_sequences_that_changed_is_not_counted(pool):
+    a, b = pool.open(), pool.open()
+    pool.commit(pool.begin([a, b], 40))
+
+    def refused(step):
+        lengths = dict(pool._lengths)
+        with pytest.raises(ValueError, match="changed"):
+            pool.commit(step)
+        assert pool._lengths == lengths
+
+    step = pool.begin([b, a], 3)
+    pool.truncate(a, 20)
+    refused(step)  # of neither of its sequences
+    step = pool.begin([a], 3)
+    c = pool.fork(a)
+    pool.begin([a], 3)  # writes a copy of the page that the first step would write
+    refused(step)
+    step = pool.begin([c], 3)
+    pool.close(c)
+    refused(step)
+    refused(kvc.PagedKVCache(1, 1, 64, 4, page_tokens=PAGE, dtype=torch.int8, device="cpu").begin([], []))
+    first, second = pool.begin([b], 3), pool.begin([b], 3)  # the same tokens again, in the same pages
+    pool.commit(second)
+    refused(first)
+    assert pool.length(b) == 43
+
+
+def test_a_compaction_after_the_pass_keeps_its_step(pool):
+    a, b = pool.open(), pool.open()
+    pool.commit(pool.begin([a], 40))
+    step = pool.begin([b], 40)
+    pool.close(a)
+    assert pool.compact() == 2
+    pool.commit(step)
+    assert pool.length(b) == 40 and pool.table(b) == [0, 1]
+    with pytest.raises(ValueError, match="committed before"):
+        pool.commit(step)
