@@ -134,8 +134,8 @@ def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
     Sequence b's token i (of ``new[b]``, None: t) gets position ``starts[b] + i``. A block's scale is the largest
     magnitude of its tokens over 448 (e4m3) or 127 (int8); it only grows while the block fills, and the block's
     older codes are rounded again when it does. Sequences with a negative start, tokens past the table or the rotary
-    positions, and holes are left out; the queries of tokens left out are 0. Two sequences of a call must not write
-    into one page.
+    positions, and holes are left out; the queries of tokens left out are 0. :func:`attention` has no positions: it
+    would see the places of tokens past the rotary tables. Two sequences of a call must not write into one page.
     """
     device = _device(q)
     if device >= 0 and torch.autograd.forward_ad._current_level < 0:
@@ -257,6 +257,15 @@ class KVStep:
     def layer(self, index: int) -> "KVLayer":
         return KVLayer(self, index)
 
+    def check(self, batch: int, tokens: int, positions: int) -> None:
+        """Refuses a pass of [batch, tokens] rows that does not hold the step's tokens, or whose rotary tables of so
+        many ``positions`` end before them."""
+        if batch != len(self.sequences) or tokens < max(self.counts, default=0):
+            raise ValueError(f"the step counts {self.counts} tokens of {len(self.sequences)} sequences, the pass has "
+                             f"{tokens} of {batch}")
+        if self.max_tokens > positions and any(c and was[0] + c > positions for c, was in zip(self.counts, self.held)):
+            raise ValueError(f"the step's sequences grow to {self.max_tokens} tokens, the model has {positions} positions")
+
 
 @dataclass(frozen=True)
 class KVLayer:
@@ -268,6 +277,7 @@ class KVLayer:
     def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
                sin: torch.Tensor) -> torch.Tensor:
         s = self.step
+        s.check(q.shape[0], q.shape[1], cos.shape[0])
         return append(q, k, v, cos, sin, s.cache.codes[self.index], s.cache.scales[self.index], s.table, s.starts, s.new)
 
     def attend(self, q: torch.Tensor) -> torch.Tensor:

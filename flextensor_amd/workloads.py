@@ -447,6 +447,8 @@ class LlamaModel(nn.Module):
     def forward(self, tokens: torch.Tensor, pos: int = 0, step: kv_cache.KVStep | None = None) -> torch.Tensor:
         """Logits of the last position, float32. With a ``step`` of a paged cache the tokens are its sequences' next
         ones (``pos`` does not matter), and the logits those of each sequence's last token in the step."""
+        if step is not None:
+            step.check(*tokens.shape, self.rope_cos.shape[0])
         x = self.embed(tokens)
         for i, layer in enumerate(self.layers):
             if step is not None:

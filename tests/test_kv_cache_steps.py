@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from flextensor_amd import kv_cache as kvc
+from flextensor_amd import workloads as W
 
 PAGE = 32
 
@@ -186,3 +187,29 @@ def test_a_compaction_after_the_pass_keeps_its_step(pool):
     assert pool.length(b) == 40 and pool.table(b) == [0, 1]
     with pytest.raises(ValueError, match="committed before"):
         pool.commit(step)
+
+
+def test_a_pass_holds_the_tokens_of_its_step_within_the_models_positions():
+    """Refused before anything is written, by the model and by a layer's append."""
+    shape = W.LlamaShape(n_layers=1, hidden=64, n_heads=1, n_kv_heads=1, head_dim=64, inter=96, vocab=50, max_seq=48)
+    model = W.build_llama(shape, seed=0)
+    cache = model.init_paged_cache(8, 32, torch.int8, "cpu")
+    a, b = cache.open(), cache.open()
+    cache.commit(cache.begin([a, b], [40, 3]))
+
+    def refused(step, b, t, match):
+        x = torch.zeros(b, t, 1, 64, dtype=torch.bfloat16)
+        with pytest.raises(ValueError, match=match):
+            model(torch.zeros(b, t, dtype=torch.long), step=step)
+        with pytest.raises(ValueError, match=match):
+            step.layer(0).append(x, x, x, model.rope_cos, model.rope_sin)
+
+    refused(cache.begin([a], 9), 1, 9, "48 positions")
+    refused(cache.begin([b, a], [1, 9]), 2, 9, "48 positions")
+    refused(cache.begin([a], 8), 1, 7, "the pass has 7 of 1")  # a row narrower than the tokens that commit would count
+    refused(cache.begin([a], 8), 2, 8, "the pass has 8 of 2")
+    refused(cache.begin([a, b], 1), 1, 1, "the pass has 1 of 1")
+    # up to the last position, in rows wider than the step's, beside a sequence that adds nothing: only the host's
+    # tensors are wrong
+    for step, shape in ((cache.begin([a], 8), (1, 12)), (cache.begin([a, b], [0, 45]), (2, 45))):
+        refused(step, *shape, "current GPU")
