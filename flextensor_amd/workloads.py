@@ -169,11 +169,41 @@ class Fp8Linear(nn.Module):
         return F.linear(x, w) * self.scale
 
 
+class _ThroughRounding(torch.autograd.Function):
+    """``y`` as it is, with the derivatives that ``x @ (weight * scale[:, None]).T`` has by x."""
+
+    generate_vmap_rule = True
+
+    @staticmethod
+    def forward(y: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+        return y.clone()
+
+    @staticmethod
+    def setup_context(ctx, inputs, output) -> None:
+        ctx.save_for_backward(*inputs[2:])
+        ctx.save_for_forward(*inputs[2:])
+        ctx.x_dtype = inputs[1].dtype
+
+    @staticmethod
+    def backward(ctx, grad: torch.Tensor):
+        weight, scale = ctx.saved_tensors
+        return grad, torch.matmul(grad.float() * scale, weight.float()).to(ctx.x_dtype), None, None
+
+    @staticmethod
+    def jvp(ctx, dy, dx, dweight, dscale):
+        weight, scale = ctx.saved_tensors
+        if dx is None:
+            return dy
+        through = (F.linear(dx.float(), weight.float()) * scale).to(ctx.x_dtype)
+        return through if dy is None else dy + through
+
+
 class Int8Linear(nn.Module):
     """y = x @ (W_int8 * scale[:, None])^T with x rounded to 8 bits, a scale for each row (token).
 
     On the GPU (bf16 inputs, K a multiple of 16) the library's integer kernels run; the sums of code products are
-    exact there. Other calls compute the same codes and their products in float32.
+    exact there. Other calls compute the same codes and their products in float32. Where x needs a gradient it gets
+    the one of x @ (W_int8 * scale[:, None])^T: that of the rounding is 0 almost everywhere.
     """
 
     def __init__(self, in_features: int, out_features: int) -> None:
@@ -193,11 +223,14 @@ class Int8Linear(nn.Module):
         if self.kernel_eligible(x):
             y = hip.int8_linear(x.reshape(x.numel() // k, k), self.weight, self.scale)
             return y.view(*x.shape[:-1], y.shape[-1])
-        xf = x.float()
+        xf = x.detach().float()
         scale = xf.abs().amax(-1, keepdim=True) * torch.tensor(1 / INT8_MAX, dtype=torch.float32)
         scale = torch.where(scale < 2.0 ** -100, 0.0, scale)
         codes = (xf * torch.where(scale > 0, 1.0 / scale, 0.0)).round().clamp(-INT8_MAX, INT8_MAX)
-        return (F.linear(codes, self.weight.float()) * scale * self.scale).to(x.dtype)
+        y = (F.linear(codes, self.weight.float()) * scale * self.scale).to(x.dtype)
+        if x.requires_grad or torch.autograd.forward_ad._current_level >= 0:
+            return _ThroughRounding.apply(y, x, self.weight, self.scale)
+        return y
 
 
 class Linear(nn.Linear):
