@@ -213,10 +213,12 @@ class Int8Linear(nn.Module):
 
     def kernel_eligible(self, x: torch.Tensor) -> bool:
         """Whether the library kernels take this call: non-empty bf16 rows, K a multiple of 16, and a contiguous,
-        16-byte aligned weight and scale (``raw_block_transfer`` packs weights back to back without alignment)."""
+        16-byte aligned weight and scale (``raw_block_transfer`` packs weights back to back without alignment), the
+        scale as it was made (``module.bfloat16()`` rounds it)."""
         k = x.shape[-1]
         return (x.numel() > 0 and k % 16 == 0 and k <= hip.INT8_LINEAR_MAX_K and hip.kernel_call(x)
-                and x.numel() // k < 1 << 24 and hip._packed(self.weight, self.scale))
+                and self.scale.dtype is torch.float32 and x.numel() // k < 1 << 24
+                and hip._packed(self.weight, self.scale))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         k = x.shape[-1]

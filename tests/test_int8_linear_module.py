@@ -97,3 +97,11 @@ def test_a_decoder_of_int8_projections_passes_gradients_on():
         mod(x, 0, torch.ones(8, 32), torch.zeros(8, 32), torch.zeros(1, 8, 1, 32), torch.zeros(1, 8, 1, 32)).backward(g)
         grads.append(x.grad - g)  # less the residual's own
     assert (grads[0] - grads[1]).norm() <= 0.1 * grads[1].norm()
+
+
+def test_a_scale_of_another_type_is_not_for_the_kernel(monkeypatch):
+    lin = _layer()
+    monkeypatch.setattr(W.hip, "kernel_call", lambda *tensors: True)
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    assert lin.kernel_eligible(x)
+    assert not lin.bfloat16().kernel_eligible(x)
