@@ -61,8 +61,8 @@ bool ints(PyObject *o, int64_t device, int64_t batch, const Tensor **out) {
 bool cache(PyObject *const *args, const Tensor &q, int64_t device, Cache *out) {
   out->codes = plain(args[0], device, at::kChar);
   const bool e4m3 = !out->codes;
-  if (e4m3) out->codes = plain(args[0], device, at::kFloat8_e4m3fn);
-  out->scales = plain(args[1], device, at::kFloat);
+  if (e4m3) out->codes = operand(args[0], device, at::kFloat8_e4m3fn);
+  out->scales = operand(args[1], device, at::kFloat);
   const Tensor *table = plain(args[2], device, at::kInt), *starts = nullptr, *news = nullptr;
   if (!out->codes || !out->scales || !table) return false;
   const Tensor &codes = *out->codes, &scales = *out->scales;
@@ -134,7 +134,7 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
       if (!heads(x[i], stride + 3 * i)) return other_way();
     }
     const Tensor &q = *x[0];
-    const Tensor *cos = plain(a[3], device, at::kFloat), *sin = plain(a[4], device, at::kFloat);
+    const Tensor *cos = operand(a[3], device, at::kFloat), *sin = operand(a[4], device, at::kFloat);
     Cache c;
     if (!cos || !sin || cos->dim() != 2 || cos->size(1) != q.size(3) || !cos->sizes().equals(sin->sizes()) ||
         !cos->is_contiguous() || !sin->is_contiguous() || !aligned(*cos) || !aligned(*sin) ||
@@ -201,8 +201,8 @@ PyObject *copy_pages(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return guarded([&]() -> PyObject * {
     if (n != 6 || !PyList_CheckExact(a[2]) || !PyList_CheckExact(a[3])) return other_way();
     const int64_t device = device_of(a[4]);
-    const Tensor *codes = plain(a[0], device, at::kChar), *scales = plain(a[1], device, at::kFloat);
-    if (!codes) codes = plain(a[0], device, at::kFloat8_e4m3fn);
+    const Tensor *codes = plain(a[0], device, at::kChar), *scales = operand(a[1], device, at::kFloat);
+    if (!codes) codes = operand(a[0], device, at::kFloat8_e4m3fn);
     if (!codes || !scales || codes->dim() != 6 || scales->dim() != 5 || !codes->is_contiguous() ||
         !scales->is_contiguous() || !aligned(*codes) || !aligned(*scales) || codes->size(2) != 2)
       return other_way();
@@ -242,7 +242,7 @@ PyObject *copy_pages(PyObject *, PyObject *const *a, Py_ssize_t n) {
 // An int8 weight [n, k] and its fp32 scale [n].
 bool weight(PyObject *w, PyObject *s, int64_t device, int64_t k, const Tensor **wt, const Tensor **st) {
   *wt = plain(w, device, at::kChar);
-  *st = plain(s, device, at::kFloat);
+  *st = operand(s, device, at::kFloat);
   return *wt && *st && (*wt)->dim() == 2 && (*wt)->size(1) == k && (*st)->dim() == 1 &&
          (*st)->size(0) == (*wt)->size(0) && (*wt)->is_contiguous() && (*st)->is_contiguous() && aligned(**wt) &&
          aligned(**st);
@@ -275,7 +275,7 @@ PyObject *int8_matmul(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return guarded([&]() -> PyObject * {
     if (n != 6) return other_way();
     const int64_t device = device_of(a[4]);
-    const Tensor *c = plain(a[0], device, at::kChar), *r = plain(a[1], device, at::kFloat), *w, *s;
+    const Tensor *c = plain(a[0], device, at::kChar), *r = operand(a[1], device, at::kFloat), *w, *s;
     const Tensor *shape = plain(a[2], device, at::kChar);
     if (!c || !r || !shape || shape->dim() != 2 || c->dim() != 2 || r->dim() != 1 || r->size(0) != c->size(0) ||
         !c->is_contiguous() || !r->is_contiguous() || !aligned(*c) || !aligned(*r))

@@ -433,9 +433,15 @@ def _check_operands(what: str, **tensors: torch.Tensor) -> None:
     for name, t in tensors.items():
         if not t.is_cuda or t.get_device() != torch._C._cuda_getDevice():
             raise ValueError(f"{what} runs on the current GPU, {name} is on {t.device}")
+    _check_underived(what, **tensors)
+
+
+def _check_underived(what: str, **tensors: torch.Tensor) -> None:
+    """Refuses tensors whose derivative the caller asks for."""
+    fwd = torch.autograd.forward_ad
+    for name, t in tensors.items():
         if torch.is_grad_enabled() and t.requires_grad:
             raise ValueError(f"{what} has no backward and {name} requires a gradient")
-        fwd = torch.autograd.forward_ad
         if fwd._current_level >= 0 and fwd.unpack_dual(t).tangent is not None:
             raise ValueError(f"{what} has no forward-mode derivative and {name} carries a tangent")
 
@@ -821,6 +827,7 @@ def _check_int8_weight(what: str, weight: torch.Tensor, scale: torch.Tensor, k: 
         raise ValueError(f"{what} needs weight and scale on cuda:{device}")
     if not _packed(weight, scale):
         raise ValueError(f"{what} needs a contiguous, 16-byte aligned weight and scale")
+    _check_underived(what, scale=scale)
     return shape[0]
 
 
@@ -846,6 +853,7 @@ def int8_matmul(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor,
         raise ValueError(f"int8_matmul runs on the current GPU, its input is on {codes.device} and {scales.device}")
     if not _packed(codes, scales):
         raise ValueError("int8_matmul needs contiguous, 16-byte aligned codes and scales")
+    _check_underived("int8_matmul", scales=scales)
     n = _check_int8_weight("int8_matmul", weight, scale, k, codes.get_device())
     m = codes.shape[0]
     y = torch.empty((m, n), dtype=torch.bfloat16, device=codes.device)

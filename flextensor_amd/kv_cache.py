@@ -105,6 +105,7 @@ def _cache(what: str, q: torch.Tensor, device: int, codes: torch.Tensor, scales:
             or not codes.is_contiguous() or not scales.is_contiguous() or shape[4] not in (2048, 4096)
             or shape[3] & (shape[3] - 1) or not 1 <= shape[3] <= MAX_PAGE_TOKENS // BLOCK):
         _check_pool(what, codes, scales, 5)
+    hip._check_underived(what, codes=codes, scales=scales)
     pages, _, kv, blocks, block_bytes = shape
     if block_bytes != BLOCK * d or h % kv:
         raise ValueError(f"{what}: queries {tuple(q.shape)} do not fit a cache of {kv} heads of {block_bytes // BLOCK}")
@@ -155,6 +156,7 @@ def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
         if x.dim() != 2 or x.shape != cos.shape or x.shape[1] != d or x.get_device() != device or not x.is_contiguous() or (
                 (cos_ptr | sin_ptr) % 16):
             raise ValueError(f"append needs cos and sin [positions, {d}], contiguous, 16-byte aligned and on {q.device}")
+    hip._check_underived("append", cos=cos, sin=sin)
     torch._C._increment_version((codes, scales))  # as an in-place operation, for what autograd saved
     out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
     nat.call("ftx_kv8_append", ctypes.byref(cache), q.data_ptr(), k.data_ptr(), v.data_ptr(), cos_ptr, sin_ptr,
@@ -211,6 +213,7 @@ def copy_pages(codes: torch.Tensor, scales: torch.Tensor, src: list[int], dst: l
             nat.result(got)
             return
     _check_pool("copy_pages", codes, scales, 6)
+    hip._check_underived("copy_pages", codes=codes, scales=scales)
     if len(src) != len(dst):
         raise ValueError(f"copy_pages takes as many sources as targets, got {len(src)} and {len(dst)}")
     layers, pages, _, kv, blocks, block_bytes = codes.shape

@@ -218,7 +218,8 @@ class Int8Linear(nn.Module):
         k = x.shape[-1]
         return (x.numel() > 0 and k % 16 == 0 and k <= hip.INT8_LINEAR_MAX_K and hip.kernel_call(x)
                 and self.scale.dtype is torch.float32 and x.numel() // k < 1 << 24
-                and hip._packed(self.weight, self.scale))
+                and hip._packed(self.weight, self.scale)
+                and not (self.scale.requires_grad and torch.is_grad_enabled()))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         k = x.shape[-1]

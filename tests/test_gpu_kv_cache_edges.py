@@ -6,6 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from flextensor_amd import hip, kv_cache as kvc
 from flextensor_amd import workloads as W
 
 pytestmark = pytest.mark.gpu
@@ -19,3 +20,57 @@ def test_a_layer_whose_scales_were_rounded_runs_in_torch(gpu):
     lin = lin.to(gpu)
     assert (lin(x).cpu().float() - want.float()).norm() <= 2.0 ** -8 * want.float().norm()
     assert W.int8_group(x, [lin, lin]) is None
+
+
+def _inputs(gpu, dtype=torch.int8):
+    """q, k, v, cos, sin, codes, scales, table and starts of one sequence of four tokens after three others."""
+    g = torch.Generator(device=gpu).manual_seed(1)
+    x = [torch.randn(1, 4, h, 64, device=gpu, generator=g).bfloat16() for h in (2, 1, 1)]
+    codes = torch.zeros(2, 2, 1, 1, 2048, device=gpu).to(dtype)
+    ints = [torch.tensor(v, dtype=torch.int32, device=gpu) for v in ([[0]], [3])]
+    return [*x, torch.ones(32, 64, device=gpu), torch.zeros(32, 64, device=gpu), codes, torch.ones(2, 2, 1, 1, device=gpu),
+            *ints]
+
+
+@pytest.mark.parametrize("at", [0, 1, 2, 3, 4, 6])
+def test_operands_of_the_cache_that_need_a_gradient_are_refused(gpu, at):
+    """q, k, v, cos, sin and the scales; without a gradient the call before and after it is the same."""
+    names = ["q", "k", "v", "cos", "sin", "codes", "scales"]
+    args = _inputs(gpu)
+    args[at].requires_grad_()
+    codes = args[5].clone()
+    with pytest.raises(ValueError, match=f"append has no backward and {names[at]} "):
+        kvc.append(*args)
+    assert torch.equal(args[5], codes)  # nothing was written
+    if at in (0, 6):
+        with pytest.raises(ValueError, match=f"attention has no backward and {names[at]} "):
+            kvc.attention(args[0], *args[5:])
+    if at == 6:
+        with pytest.raises(ValueError, match="copy_pages has no backward and scales "):
+            kvc.copy_pages(args[5][None], args[6][None], [0], [1])
+    with torch.no_grad():
+        got = kvc.append(*args)
+        out = kvc.attention(got, *args[5:])
+    plain = _inputs(gpu)
+    want = kvc.append(*plain)
+    assert torch.equal(got, want) and torch.equal(out, kvc.attention(want, *plain[5:]))
+
+
+def test_scales_of_the_int8_linear_that_need_a_gradient_are_refused(gpu):
+    x = torch.randn(3, 64, device=gpu, generator=torch.Generator(device=gpu).manual_seed(2)).bfloat16()
+    w, scale = torch.ones(8, 64, dtype=torch.int8, device=gpu), torch.ones(8, device=gpu)
+    codes, rows = hip.int8_quantize(x)
+    trained = scale.clone().requires_grad_()
+    with pytest.raises(ValueError, match="int8_linear has no backward and scale "):
+        hip.int8_linear(x, w, trained)
+    with pytest.raises(ValueError, match="int8_matmul has no backward and scale "):
+        hip.int8_matmul(codes, rows, w, trained)
+    with pytest.raises(ValueError, match="int8_matmul has no backward and scales "):
+        hip.int8_matmul(codes, rows.clone().requires_grad_(), w, scale)
+    with torch.no_grad():
+        assert torch.equal(hip.int8_linear(x, w, trained), hip.int8_linear(x, w, scale))
+    # the module's own scale: its gradient, in torch
+    lin = W.init_normal_(W.Int8Linear(64, 8), seed=3).to(gpu)
+    lin.scale.requires_grad_()
+    lin(x).float().sum().backward()
+    assert lin.scale.grad.isfinite().all() and lin.scale.grad.any()
