@@ -5,12 +5,14 @@
 // and calls the C ABI (6 to 8 us in all, a launch included). What it does not recognise as a plain call it leaves alone: it returns None,
 // and the Python function goes through its own checks, which say what is wrong or arrange what can be (a copy of
 // strided rows, another stride of a table). A failed C call comes back as its status.
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/torch.h>
 
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <exception>
 #include <vector>
 
 #include "../../include/ftx.h"
@@ -116,8 +118,8 @@ template <typename F>
 PyObject *guarded(F f) {
   try {
     return f();
-  } catch (const std::exception &e) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {  // as the Python type that torch gives it: memory that ran out is torch.OutOfMemoryError
+    torch::translate_exception_to_python(std::current_exception());
     return nullptr;
   }
 }

@@ -74,3 +74,26 @@ def test_scales_of_the_int8_linear_that_need_a_gradient_are_refused(gpu):
     lin.scale.requires_grad_()
     lin(x).float().sum().backward()
     assert lin.scale.grad.isfinite().all() and lin.scale.grad.any()
+
+
+def test_memory_that_runs_out_is_torchs_own_error(gpu):
+    """A result of 1 GiB where 64 MiB are left: no kernel has started when it is asked for."""
+    q = torch.zeros(1, 1 << 17, 64, 64, dtype=torch.bfloat16, device=gpu)
+    codes, scales = torch.zeros(1, 2, 1, 1, 2048, dtype=torch.int8, device=gpu), torch.zeros(1, 2, 1, 1, device=gpu)
+    table = torch.zeros(1, 1, dtype=torch.int32, device=gpu)
+    cos = torch.zeros(32, 64, device=gpu)
+    x, w = torch.zeros(1 << 13, 64, dtype=torch.bfloat16, device=gpu), torch.zeros(1 << 16, 64, dtype=torch.int8, device=gpu)
+    scale = torch.ones(1 << 16, device=gpu)
+    rows, row_scales = hip.int8_quantize(x)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(gpu).total_memory
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved(gpu) + (64 << 20)) / total)
+    try:
+        for call in (lambda: kvc.attention(q, codes, scales, table, table[0]),
+                     lambda: kvc.append(q, q[:, :, :1], q[:, :, :1], cos, cos, codes, scales, table, table[0]),
+                     lambda: hip.int8_linear(x, w, scale), lambda: hip.int8_matmul(rows, row_scales, w, scale)):
+            with pytest.raises(torch.OutOfMemoryError):
+                call()
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
