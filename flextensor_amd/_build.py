@@ -20,7 +20,7 @@ LIB_PATH = PKG_DIR / "libftx_hip.so"
 SOURCES = ("ftx_runtime.hip", "ftx_kernels.hip", "ftx_gemm.hip", "ftx_attention.hip", "ftx_layers.hip",
            "ftx_int8.hip", "ftx_kvcache.hip", "ftx_staged.hip", "ftx_expcode.hip")
 OFFLOAD_ARCH = "gfx950"
-# The same library's serving calls, taking torch tensors (a CPython extension, host code only).
+# The library's serving calls, taking torch tensors (a CPython extension, host code only); it is told which library.
 TORCH_SOURCE = CSRC / "ftx_torch.cpp"
 TORCH_LIB_PATH = PKG_DIR / "_ftx_torch.so"
 
@@ -76,14 +76,12 @@ def torch_command(output: Path = TORCH_LIB_PATH) -> list[str]:
         str(TORCH_SOURCE),
         "-o",
         str(output),
-        f"-L{PKG_DIR}",
-        f"-l:{LIB_PATH.name}",
         f"-L{torch_lib}",
         "-ltorch_python",
         "-ltorch",
         "-ltorch_cpu",
         "-lc10",
-        "-Wl,-rpath,$ORIGIN",
+        "-ldl",
         f"-Wl,-rpath,{torch_lib}",
     ]
 

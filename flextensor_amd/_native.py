@@ -276,10 +276,11 @@ def torch_calls():
     failed C call, or None for arguments that it leaves to the Python function of the same name."""
     global _torch_calls
     if _torch_calls is None:
-        load()
+        handle = load()._handle
         try:
             from . import _ftx_torch
-        except ImportError as e:
+            _ftx_torch.use(handle)
+        except (ImportError, AttributeError) as e:  # AttributeError: built from older sources
             raise FtxLibraryMissing(f"the torch binding of {LIB_PATH.name} is missing or does not load ({e}); build it "
                                     "with `python -m flextensor_amd._build`") from e
         _torch_calls = _ftx_torch

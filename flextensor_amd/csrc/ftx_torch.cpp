@@ -5,6 +5,7 @@
 // and calls the C ABI (6 to 8 us in all, a launch included). What it does not recognise as a plain call it leaves alone: it returns None,
 // and the Python function goes through its own checks, which say what is wrong or arrange what can be (a copy of
 // strided rows, another stride of a table). A failed C call comes back as its status.
+#include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/torch.h>
@@ -13,6 +14,7 @@
 #include <cmath>
 #include <cstdint>
 #include <exception>
+#include <type_traits>
 #include <vector>
 
 #include "../../include/ftx.h"
@@ -20,6 +22,20 @@
 namespace {
 
 using at::Tensor;
+
+// The entries of the one library that the process has loaded, from wherever it came: linked to the binding they would
+// be those of the library beside it, a second one with streams and buffers of its own.
+struct Library {
+  decltype(&ftx_kv8_append) kv8_append;
+  decltype(&ftx_kv8_attention_workspace) kv8_attention_workspace;
+  decltype(&ftx_kv8_attention) kv8_attention;
+  decltype(&ftx_kv8_copy_pages) kv8_copy_pages;
+  decltype(&ftx_int8_linear_workspace) int8_linear_workspace;
+  decltype(&ftx_int8_linear) int8_linear;
+  decltype(&ftx_int8_matmul_workspace) int8_matmul_workspace;
+  decltype(&ftx_int8_matmul) int8_matmul;
+};
+Library lib{};
 
 // The tensor behind an exact torch.Tensor or Parameter on `device` of this type, or nullptr: a subclass or a proxy is
 // not plain memory.
@@ -117,7 +133,9 @@ void *stream_of(PyObject *o) { return PyLong_AsVoidPtr(o); }
 template <typename F>
 PyObject *guarded(F f) {
   try {
-    return f();
+    if (lib.kv8_append) return f();
+    PyErr_SetString(PyExc_RuntimeError, "the binding has no library yet (use)");
+    return nullptr;
   } catch (...) {  // as the Python type that torch gives it: memory that ran out is torch.OutOfMemoryError
     torch::translate_exception_to_python(std::current_exception());
     return nullptr;
@@ -149,7 +167,7 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
     written(*c.codes);
     written(*c.scales);
-    const int rc = ftx_kv8_append(&c.c, q.data_ptr(), x[1]->data_ptr(), x[2]->data_ptr(), cos->data_ptr<float>(),
+    const int rc = lib.kv8_append(&c.c, q.data_ptr(), x[1]->data_ptr(), x[2]->data_ptr(), cos->data_ptr<float>(),
                                   sin->data_ptr<float>(), cos->size(0), out.data_ptr(), q.size(0), q.size(1),
                                   static_cast<int>(q.size(2)), stride, stream_of(a[11]));
     return result(rc, std::move(out));
@@ -187,11 +205,11 @@ PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (!heads(&out, stride + 3)) return other_way();
     const int h = static_cast<int>(q->size(2));
     size_t bytes = 0;
-    int rc = ftx_kv8_attention_workspace(q->size(0), q->size(1), h, c.c.kv_heads, c.c.d, longest, &bytes);
+    int rc = lib.kv8_attention_workspace(q->size(0), q->size(1), h, c.c.kv_heads, c.c.d, longest, &bytes);
     if (rc != FTX_OK) return result(rc, out);
     Tensor ws;
     if (bytes > 0) ws = at::empty({static_cast<int64_t>(bytes)}, q->options().dtype(at::kByte).requires_grad(false));
-    rc = ftx_kv8_attention(&c.c, q->data_ptr(), out.data_ptr(), q->size(0), q->size(1), h, stride,
+    rc = lib.kv8_attention(&c.c, q->data_ptr(), out.data_ptr(), q->size(0), q->size(1), h, stride,
                            static_cast<float>(scale), longest, bytes > 0 ? ws.data_ptr() : nullptr, bytes,
                            stream_of(a[9]));
     return result(rc, std::move(out));
@@ -233,7 +251,7 @@ PyObject *copy_pages(PyObject *, PyObject *const *a, Py_ssize_t n) {
     }
     written(*codes);
     written(*scales);
-    const int rc = ftx_kv8_copy_pages(codes->data_ptr(), scales->data_ptr<float>(), codes->size(0), codes->size(1),
+    const int rc = lib.kv8_copy_pages(codes->data_ptr(), scales->data_ptr<float>(), codes->size(0), codes->size(1),
                                       static_cast<int>(codes->size(3)), static_cast<int>(codes->size(4)) * FTX_KV8_BLOCK,
                                       static_cast<int>(d), pages[0].data(), pages[1].data(), count, stream_of(a[5]));
     if (rc != FTX_OK) return status(rc);
@@ -262,11 +280,11 @@ PyObject *int8_linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
       return other_way();
     const int64_t channels = w->size(0);
     size_t bytes = 0;
-    int rc = ftx_int8_linear_workspace(m, channels, k, &bytes);
+    int rc = lib.int8_linear_workspace(m, channels, k, &bytes);
     if (rc != FTX_OK) return other_way();
     Tensor y = at::empty({m, channels}, x->options().requires_grad(false));
     Tensor ws = at::empty({static_cast<int64_t>(bytes)}, x->options().dtype(at::kByte).requires_grad(false));
-    rc = ftx_int8_linear(x->data_ptr(), stride, w->data_ptr(), s->data_ptr<float>(), y.data_ptr(), m, channels, k,
+    rc = lib.int8_linear(x->data_ptr(), stride, w->data_ptr(), s->data_ptr<float>(), y.data_ptr(), m, channels, k,
                          ws.data_ptr(), bytes, stream_of(a[4]));
     return result(rc, std::move(y));
   });
@@ -286,11 +304,11 @@ PyObject *int8_matmul(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (k == 0 || c->size(1) != FTX_INT8_CODE_STRIDE(k) || !weight(a[2], a[3], device, k, &w, &s)) return other_way();
     const int64_t channels = w->size(0);
     size_t bytes = 0;
-    int rc = ftx_int8_matmul_workspace(m, channels, k, &bytes);
+    int rc = lib.int8_matmul_workspace(m, channels, k, &bytes);
     if (rc != FTX_OK) return other_way();
     Tensor y = at::empty({m, channels}, c->options().dtype(at::kBFloat16)), ws;
     if (bytes > 0) ws = at::empty({static_cast<int64_t>(bytes)}, c->options().dtype(at::kByte));
-    rc = ftx_int8_matmul(c->data_ptr(), r->data_ptr<float>(), w->data_ptr(), s->data_ptr<float>(), y.data_ptr(), m,
+    rc = lib.int8_matmul(c->data_ptr(), r->data_ptr<float>(), w->data_ptr(), s->data_ptr<float>(), y.data_ptr(), m,
                          channels, k, bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_of(a[5]));
     return result(rc, std::move(y));
   });
@@ -301,7 +319,33 @@ PyMethodDef method(const char *name) {
   return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)), METH_FASTCALL, nullptr};
 }
 
-PyMethodDef methods[] = {method<append>("append"),           method<attention>("attention"),
+// (the loaded library's handle)
+PyObject *use(PyObject *, PyObject *handle) {
+  void *from = PyLong_AsVoidPtr(handle);
+  if (!from) {
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "no library");
+    return nullptr;
+  }
+  Library found{};
+  const auto entry = [&](auto &to, const char *name) {
+    to = reinterpret_cast<std::remove_reference_t<decltype(to)>>(dlsym(from, name));
+    if (!to) PyErr_Format(PyExc_ImportError, "the library has no %s", name);
+    return to != nullptr;
+  };
+  if (!entry(found.kv8_append, "ftx_kv8_append") ||
+      !entry(found.kv8_attention_workspace, "ftx_kv8_attention_workspace") ||
+      !entry(found.kv8_attention, "ftx_kv8_attention") || !entry(found.kv8_copy_pages, "ftx_kv8_copy_pages") ||
+      !entry(found.int8_linear_workspace, "ftx_int8_linear_workspace") ||
+      !entry(found.int8_linear, "ftx_int8_linear") ||
+      !entry(found.int8_matmul_workspace, "ftx_int8_matmul_workspace") ||
+      !entry(found.int8_matmul, "ftx_int8_matmul"))
+    return nullptr;
+  lib = found;
+  Py_RETURN_NONE;
+}
+
+PyMethodDef methods[] = {{"use", use, METH_O, nullptr},
+                         method<append>("append"),           method<attention>("attention"),
                          method<copy_pages>("copy_pages"),   method<int8_linear>("int8_linear"),
                          method<int8_matmul>("int8_matmul"), {nullptr, nullptr, 0, nullptr}};
 

@@ -1,13 +1,17 @@
 """Steps of the paged cache that are not committed at once: what they reserve is theirs alone, and what a step may
-count. Without a GPU."""
+count. The binding that its calls go through. Without a GPU."""
 
 from __future__ import annotations
 
 import random
+import shutil
+import subprocess
+import sys
 
 import pytest
 import torch
 
+from flextensor_amd import _native as nat
 from flextensor_amd import kv_cache as kvc
 from flextensor_amd import workloads as W
 
@@ -213,3 +217,32 @@ def test_a_pass_holds_the_tokens_of_its_step_within_the_models_positions():
     # tensors are wrong
     for step, shape in ((cache.begin([a], 8), (1, 12)), (cache.begin([a, b], [0, 45]), (2, 45))):
         refused(step, *shape, "current GPU")
+
+
+def test_the_torch_binding_takes_the_library_that_is_loaded(tmp_path):
+    """A library loaded from another place is the only one in the process, and the binding's calls end in it."""
+    other = tmp_path / "libftx_elsewhere.so"
+    shutil.copy(nat.LIB_PATH, other)
+    code = f"""
+from flextensor_amd import _native as nat
+nat.load({str(other)!r})
+calls = nat.torch_calls()
+maps = open("/proc/self/maps").read()
+assert {str(other)!r} in maps and {nat.LIB_PATH.name!r} not in maps
+assert calls.append(*[None] * 12) is None
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=120, cwd=nat.LIB_PATH.parent.parent)
+
+
+def test_the_torch_binding_refuses_calls_before_it_has_a_library():
+    code = """
+import torch
+from flextensor_amd import _ftx_torch
+for call in (lambda: _ftx_torch.append(), lambda: _ftx_torch.use(0), lambda: _ftx_torch.use(None)):
+    try:
+        call()
+    except (RuntimeError, ValueError, TypeError):
+        continue
+    raise SystemExit("not refused")
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=120, cwd=nat.LIB_PATH.parent.parent)
