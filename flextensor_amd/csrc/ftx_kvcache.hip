@@ -746,7 +746,7 @@ hipError_t launch_attend(const Kv8Attention &p, hipStream_t stream) {
 // blocks under s = max(the block's scale if it holds older tokens, max |y| / top), top = 448 or 127, as the nearest
 // codes to y / s; where s grew, the older codes are rounded again to the nearest of c * (old s / s). Tokens of the
 // block past the new ones become 0. The maximum is over finite values (an infinity becomes the largest code, a NaN
-// the e4m3 NaN or the integer 0), and a scale below 2^-100 counts as 0, with codes of 0.
+// the e4m3 NaN or the integer 0), and a scale below 2^-100 counts as 0, with codes of 0 for all but a NaN.
 //
 // The sums are the ones elementary operations make, each product and sum rounded to fp32 on its own (no fused
 // multiply-add), so the codes do not depend on how a compiler contracts them.
@@ -914,9 +914,12 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
       for (int j = 0; j < 16; ++j)
         y[j] = code_value<FP8>(side == 0 ? tile[chunk * (16 * kKvBlock) + token * 16 + j]
                                          : tile[(16 * chunk + j) * kKvBlock + token]) * ratio;
-    } else {
+    } else if (scale > 0.f) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) y[j] = fresh ? y[j] * inverse : 0.f;
+    } else {  // an infinity is 0 like the block's other values; a NaN stays one
+#pragma unroll
+      for (int j = 0; j < 16; ++j) y[j] = fresh && y[j] != y[j] ? y[j] : 0.f;
     }
     u32x4 w;
 #pragma unroll

@@ -450,8 +450,9 @@ int ftx_int8_linear(const void *x, int64_t x_stride, const void *w, const float 
  *   s = max(the block's scale if it holds tokens before starts[b], max |y| / top)
  * over the new tokens' finite y, top = 448 or 127; a code is the nearest to
  * y / s, ties to even. Where s grew, the block's older codes are rounded again;
- * tokens of the block past the new ones become 0. A scale below 2^-100 is 0,
- * with codes of 0; an infinity becomes the largest code, a NaN the e4m3 NaN or
+ * tokens of the block past the new ones become 0. An infinity becomes the largest
+ * code; a scale below 2^-100 is 0, with codes of 0 (for an infinity too: the
+ * block's finite values make the scale). A NaN becomes the e4m3 NaN or
  * the integer 0. Tokens past the rotary tables are not written, and must not be
  * attended to: the attention knows no positions. strides: batch, token
  * and head of q, k and v, multiples of 8. No two sequences of a call may name

@@ -11,6 +11,10 @@ from flextensor_amd import workloads as W
 
 pytestmark = pytest.mark.gpu
 
+BLOCK = 32
+TOP = {torch.float8_e4m3fn: 448.0, torch.int8: 127.0}
+FORMATS = list(TOP)
+
 
 def test_a_layer_whose_scales_were_rounded_runs_in_torch(gpu):
     """``module.bfloat16()`` rounds the channel scales, which the kernels take in fp32."""
@@ -97,3 +101,34 @@ def test_memory_that_runs_out_is_torchs_own_error(gpu):
                 call()
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
+
+
+@pytest.mark.parametrize("dtype", FORMATS)
+@pytest.mark.parametrize("small", [0.0, 1e-36])
+def test_infinities_among_zeros_are_stored_as_zeros(gpu, dtype, small):
+    """A block whose finite values make no scale: all of its codes are 0 but those of NaN; what is appended to it
+    later has a scale of its own, and attention sees zeros."""
+    kv, d = 2, 64
+    codes, scales = torch.zeros(2, 2, kv, 1, BLOCK * d, device=gpu).to(dtype), torch.ones(2, 2, kv, 1, device=gpu)
+    table = torch.tensor([[1]], dtype=torch.int32, device=gpu)
+    cos, sin = torch.ones(BLOCK, d, device=gpu), torch.zeros(BLOCK, d, device=gpu)
+    q = torch.ones(1, 5, 2, d, dtype=torch.bfloat16, device=gpu)
+    k, v = (torch.full((1, 5, kv, d), small, dtype=torch.bfloat16, device=gpu) for _ in range(2))
+    v[0, 1, 0, 3], v[0, 2, 0, 40], v[0, 4, 1, 7] = float("inf"), float("-inf"), float("nan")
+    starts = torch.tensor([0], dtype=torch.int32, device=gpu)
+    kvc.append(q, k, v, cos, sin, codes, scales, table, starts)
+    assert not scales[1].any()
+    keys, values = kvc.read(codes, scales, table[0])
+    nan = torch.zeros(BLOCK, kv, d, dtype=torch.bool, device=gpu)
+    nan[4, 1, 7] = dtype != torch.int8
+    assert not keys.any() and torch.equal(values.isnan(), nan) and not values.nan_to_num(0.0).any()
+    out = kvc.attention(q, codes, scales, table, starts)
+    assert torch.equal(out[0, 4].isnan(), nan[4]) and not out[0].isnan()[:, ~nan[4]].any()
+    assert not out.nan_to_num(0.0).any()
+    # three more tokens, of ones: the scale that they make, the infinities' codes still 0
+    one = torch.ones(1, 3, kv, d, dtype=torch.bfloat16, device=gpu)
+    kvc.append(one, one, one, cos, sin, codes, scales, table, starts + 5)
+    keys, values = kvc.read(codes, scales, table[0])
+    want = torch.zeros(BLOCK, kv, d, device=gpu)
+    want[5:8] = TOP[dtype] * (torch.ones((), device=gpu) * (1 / TOP[dtype]))
+    assert torch.equal(keys, want) and torch.equal(values.nan_to_num(0.0), want)
