@@ -29,6 +29,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kWave = 64;
 constexpr float kSlack = 8.0f;
 constexpr int kTileWaves = 8;  // of an attention workgroup
+constexpr float kTiny = 0x1p-100f;  // a block whose scale is below this stands for zeros
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
@@ -68,6 +69,7 @@ __device__ __forceinline__ int64_t block_index(const KvPages &c, int page, int s
 
 // Pages and scales of 64 blocks, a lane each: a kernel reads them at once, and its loop over the blocks takes them
 // from the lanes without waiting for memory. Lane i holds block first + i * step; blocks past `last` are it again.
+// The value scale of a block that stands for zeros is 0.
 struct BlockList {
   int page;
   float key_scale, value_scale;
@@ -78,8 +80,10 @@ __device__ __forceinline__ BlockList block_list(const KvPages &c, int64_t b, int
   x.page = page_of(c, b, block);
   x.key_scale = c.scales[block_index(c, max(x.page, 0), 0, head, block)];
   x.value_scale = c.scales[block_index(c, max(x.page, 0), 1, head, block)];
+  if (fabsf(x.value_scale) < kTiny) x.value_scale = 0.f;
   return x;
 }
+__device__ __forceinline__ bool no_scale(float scale) { return __float_as_uint(scale) == 0; }  // a scalar comparison
 __device__ __forceinline__ float lane_float(float v, int lane) {
   return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(v)), lane)));
 }
@@ -117,6 +121,18 @@ __device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi) {
 __device__ __forceinline__ u32x2 keep_codes(u32x2 v, int n) {
   const uint64_t mask = n >= 8 ? ~0ull : n <= 0 ? 0ull : (1ull << (8 * n)) - 1;
   return (u32x2){v[0] & static_cast<uint32_t>(mask), v[1] & static_cast<uint32_t>(mask >> 32)};
+}
+
+// What is left of eight codes whose scale counts as 0: a NaN, which is one times 0 too.
+template <bool FP8>
+__device__ __forceinline__ u32x2 without_scale(u32x2 v) {
+  if constexpr (!FP8) return (u32x2){0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t nan = ((v[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // where all seven bits are set
+    v[i] &= (nan >> 7) * 255u;
+  }
+  return v;
 }
 
 // The maximum (or sum) of a value and its partner's in the other half of the wave, and over the four lanes that hold
@@ -252,7 +268,8 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
     }
     const int key0 = block * kKvBlock;
     float scale = a.scale_log2 * x.k_scale;
-    if (x.hole || key0 + kKvBlock > whole) {
+    const bool zeros = no_scale(x.v_scale);
+    if (x.hole || zeros || key0 + kKvBlock > whole) {
       const int kept = x.hole ? 0 : length - key0;
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
@@ -267,11 +284,15 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
 #pragma unroll
         for (int d = 0; d < kDTiles; ++d) x.v[d] = keep_codes(x.v[d], kept - 8 * g);
       }
+      if (zeros) {
+#pragma unroll
+        for (int d = 0; d < kDTiles; ++d) x.v[d] = without_scale<FP8>(x.v[d]);
+      }
     }
-    // p times the value scale in one operation: 2^(s - m + log2(scale)); the sum of the p takes it out again. A
-    // scale of 0 stands beside codes of 0, whose weight does not matter. The products take it in two parts of eight
-    // bits: these kernels wait for memory, and have the time for a result that is only rounded at its end.
-    const float factor = x.v_scale == 0.f || x.hole ? 1.0f : x.v_scale;
+    // p times the value scale in one operation: 2^(s - m + log2(scale)); the sum of the p takes it out again. A block
+    // of zeros has been given codes of 0 and takes any. The products take p in two parts of eight bits: these kernels
+    // wait for memory, and have the time for a result that is only rounded at its end.
+    const float factor = zeros || x.hole ? 1.0f : x.v_scale;
     const float log_factor = __builtin_amdgcn_logf(factor), inverse = __builtin_amdgcn_rcpf(factor);
     u32x4 p[RT], rest[RT];
 #pragma unroll
@@ -430,7 +451,7 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
   };
   struct Unit {  // 16 bytes of codes on their way to LDS
     u32x4 w;
-    int keep;    // values: the tokens of them that the sequence has
+    int keep;    // values: the tokens of them that the sequence has; less 64 where they have no scale
   };
   Unit units[kUnits];
   struct Scales {
@@ -459,7 +480,8 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
       const uint8_t *from =
           a.kv.codes + block_index(a.kv, max(own, 0), side, kvh, min(block, end - 1)) * kBlockBytes;
       units[i].w = *reinterpret_cast<const u32x4 *>(from + (u0 % kBlockUnits + lane) * 16);
-      units[i].keep = own < 0 || block >= end ? 0 : length - block * kKvBlock;
+      units[i].keep = own < 0 || block >= end ? 0 : min(length - block * kKvBlock, kKvBlock);
+      if (side != 0 && no_scale(sub == 0 ? x.value[0] : x.value[1])) units[i].keep -= 64;
     }
     return x;
   };
@@ -478,8 +500,9 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
       const int side = side_of(i);
       u32x4 w = units[i].w;
       if (side != 0 && units[i].keep < kKvBlock) {
-        const int n = units[i].keep - lane % 2 * 16;
-        const u32x2 lo = keep_codes((u32x2){w[0], w[1]}, n), hi = keep_codes((u32x2){w[2], w[3]}, n - 8);
+        const int n = (units[i].keep < 0 ? units[i].keep + 64 : units[i].keep) - lane % 2 * 16;
+        u32x2 lo = keep_codes((u32x2){w[0], w[1]}, n), hi = keep_codes((u32x2){w[2], w[3]}, n - 8);
+        if (units[i].keep < 0) lo = without_scale<FP8>(lo), hi = without_scale<FP8>(hi);
         w = (u32x4){lo[0], lo[1], hi[0], hi[1]};
       }
       uint8_t *to = lds + (side == 0 ? t & 1 : 2 + (t & 1)) * kSide + store_at[i];
@@ -573,7 +596,7 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
     bf16x8 p[2 * kSub];  // times the value scale, as above
 #pragma unroll
     for (int j = 0; j < kSub; ++j) {
-      const float factor = x.value[j] == 0.f || x.hole[j] ? 1.0f : x.value[j];
+      const float factor = no_scale(x.value[j]) || x.hole[j] ? 1.0f : x.value[j];
       const float offset = __builtin_amdgcn_logf(factor) - m;
       float sum = 0.f;
       uint32_t w[8];
@@ -750,8 +773,6 @@ hipError_t launch_attend(const Kv8Attention &p, hipStream_t stream) {
 //
 // The sums are the ones elementary operations make, each product and sum rounded to fp32 on its own (no fused
 // multiply-add), so the codes do not depend on how a compiler contracts them.
-constexpr float kTiny = 0x1p-100f;
-
 template <bool FP8>
 __device__ __forceinline__ uint32_t code4(const float *y) {
   if constexpr (FP8) {

@@ -431,7 +431,7 @@ int ftx_int8_linear(const void *x, int64_t x_stride, const void *w, const float 
  * No reference counterpart. One layer is codes, bytes [pages][2][kv_heads]
  * [page_tokens / 32][32 d] (keys, then values), and scales, fp32 [pages][2]
  * [kv_heads][page_tokens / 32]: a block of 32 tokens of a head shares a scale,
- * and a code c stands for c * scale. format: FTX_KV8_E4M3 or FTX_KV8_INT8
+ * and a code c stands for c * scale (not negative; 0 below 2^-100). format: FTX_KV8_E4M3 or FTX_KV8_INT8
  * (-127 .. 127). A block's keys are stored as [d / 16][32][16], its values as
  * [d][32]. page_tokens: 32 times a power of two, at most 4096; d: 64 or 128.
  *

@@ -3,6 +3,8 @@ numbers, gradients that are asked for, memory that runs out. Against float64, an
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -132,3 +134,78 @@ def test_infinities_among_zeros_are_stored_as_zeros(gpu, dtype, small):
     want = torch.zeros(BLOCK, kv, d, device=gpu)
     want[5:8] = TOP[dtype] * (torch.ones((), device=gpu) * (1 / TOP[dtype]))
     assert torch.equal(keys, want) and torch.equal(values.nan_to_num(0.0), want)
+
+
+def _pool(gpu, pages, kv, page, d, dtype, seed=0):
+    g = torch.Generator(device=gpu).manual_seed(seed + pages)
+    top = TOP[dtype]
+    y = torch.randn(pages, 2, kv, page // BLOCK, BLOCK * d, device=gpu, generator=g).mul_(top / 4).clamp_(-top, top)
+    return (y.round() if dtype == torch.int8 else y).to(dtype), \
+        torch.exp(0.3 * torch.randn(y.shape[:-1], device=gpu, generator=g)) * (4 / top)
+
+
+def _attend64(q, codes, scales, table, start):
+    """One sequence in float64, head by head over what :func:`kvc.read` says that the codes stand for."""
+    _, t, h, d = q.shape
+    kv = codes.shape[2]
+    keys, values = (x[0, : start + t].double() for x in kvc.read(codes, scales, table))
+    seen = torch.arange(start + t, device=q.device) <= start + torch.arange(t, device=q.device)[:, None]
+    out = torch.zeros(1, t, h, d, dtype=torch.float64, device=q.device)
+    for head in range(h):
+        k, v = (x[:, head // (h // kv)].contiguous() for x in (keys, values))
+        s = (q[0, :, head].double() @ k.t().contiguous() / math.sqrt(d)).masked_fill(~seen, -math.inf)
+        out[0, :, head] = torch.softmax(s, -1) @ v
+    return out
+
+
+# tokens, heads, kv heads, d, page, start: a row, a tile of 16 rows over split keys, tiles of 32, tiles of 256 unsplit and
+# split
+SHAPES = [(1, 2, 2, 64, 32, 100), (1, 8, 1, 128, 64, 9000), (20, 4, 2, 64, 32, 70), (300, 64, 64, 128, 64, 0),
+          (64, 64, 8, 64, 64, 30000)]
+TWO_ROUNDINGS = 2.0 ** -7  # of the probabilities (2^-8 of each at most, less in a sum of many) and of the output
+
+
+def _case(gpu, dtype, t, h, kv, d, page, start):
+    pages = -(-(start + t) // page)
+    codes, scales = _pool(gpu, pages, kv, page, d, dtype)
+    g = torch.Generator(device=gpu).manual_seed(t + h)
+    table = torch.randperm(pages, device=gpu, generator=g).view(1, pages).int()
+    q = torch.randn(1, t, h, d, device=gpu, generator=g).mul(2.0).bfloat16()
+    return q, codes, scales, table, torch.tensor([start], dtype=torch.int32, device=gpu)
+
+
+def _check(got, want):
+    got = got.double()
+    assert got.isfinite().all()
+    assert (got - want).norm() <= TWO_ROUNDINGS * want.norm()
+    assert ((got - want).norm(dim=-1) <= 4 * TWO_ROUNDINGS * want.norm(dim=-1)).all()
+
+
+@pytest.mark.parametrize("dtype", FORMATS)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -101])
+def test_blocks_without_a_scale_stand_for_zeros(gpu, dtype, shape, scale):
+    """Their codes, which are none of them 0, weigh in the sum and add nothing: the first and every third block."""
+    q, codes, scales, table, starts = _case(gpu, dtype, *shape)
+    start = shape[-1]
+    for block in range(0, table.shape[1] * codes.shape[3], 3):
+        scales[int(table[0, block // codes.shape[3]]), 1, :, block % codes.shape[3]] = scale
+    want = _attend64(q, codes, scales, table, start)
+    if start == 0:  # the first tokens see the first block alone
+        assert not kvc.attention(q, codes, scales, table, starts)[0, :BLOCK].float().abs().gt(1e-25).any()
+        got = kvc.attention(q, codes, scales, table, starts)[:, BLOCK:]
+        _check(got, want[:, BLOCK:])
+        return
+    _check(kvc.attention(q, codes, scales, table, starts), want)
+
+
+def test_a_nan_code_without_a_scale_is_a_nan(gpu):
+    """c * 0 of a NaN."""
+    q, codes, scales, table, starts = _case(gpu, torch.float8_e4m3fn, 1, 2, 2, 64, 32, 100)
+    page = int(table[0, 1])
+    scales[page, 1] = 0.0
+    codes.view(torch.uint8)[page, 1, 1, 0, 5 * BLOCK + 9] = 0x7F
+    out = kvc.attention(q, codes, scales, table, starts)
+    nan = torch.zeros(1, 1, 2, 64, dtype=torch.bool, device=gpu)
+    nan[0, 0, 1, 5] = True
+    assert torch.equal(out.isnan(), nan)
