@@ -94,8 +94,12 @@ __device__ __forceinline__ float lane_float(float v, int lane) {
 //
 // over the cached tokens p of the head that the group of `rep` query heads shares; a row that sees no token is 0.
 // Scores, the running maximum and the running sum are fp32. A code is exact in bf16 and enters the products as it
-// is: a block's key scale multiplies its scores, its value scale the probabilities. Prompts round those to bf16
-// (2^-9 of each at most, as in the attention over a bf16 cache), few rows do not.
+// is: a block's key scale multiplies its scores, its value scale the probabilities. Few rows take a probability into the
+// products in two parts of eight bits, as exact as fp32 to the output's rounding. Prompts round it to bf16 (2^-8 of each
+// at most, as the attention over a bf16 cache does): the matrix cores are what they wait for, and a second part makes
+// 2048 tokens over 8148 (64 / 8 heads) 647 us where one takes 483, for an error of 0.0017 of the result in 64 bits
+// (relative norm; the output's own rounding) where one gives 0.0024. A probability may be 2^kSlack and the sums are
+// divided at the end, so fp32 holds them for values of up to about 2^112 (5e33).
 
 // Eight codes as bf16.
 template <bool FP8>

@@ -209,3 +209,18 @@ def test_a_nan_code_without_a_scale_is_a_nan(gpu):
     nan = torch.zeros(1, 1, 2, 64, dtype=torch.bool, device=gpu)
     nan[0, 0, 1, 5] = True
     assert torch.equal(out.isnan(), nan)
+
+
+@pytest.mark.parametrize("dtype", FORMATS)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("near", ["large", "small", "both"])
+def test_values_over_the_range_that_the_sums_hold(gpu, dtype, shape, near):
+    """Values of up to 2^100, and down to the smallest scale, alone and in turn by block."""
+    q, codes, scales, table, starts = _case(gpu, dtype, *shape)
+    start = shape[-1]
+    spread = scales[:, 1].clamp(max=4 / TOP[dtype]) * (TOP[dtype] / 4)  # exp(0.3 n), 1 at most
+    scales[:, 1] = (spread * 2.0 ** -99).clamp(min=2.0 ** -100) if near == "small" else spread * (2.0 ** 100 / TOP[dtype])
+    if near == "both":
+        for block in range(1, table.shape[1] * codes.shape[3], 2):
+            scales[int(table[0, block // codes.shape[3]]), 1, :, block % codes.shape[3]] = 2.0 ** -99
+    _check(kvc.attention(q, codes, scales, table, starts), _attend64(q, codes, scales, table, start))
