@@ -64,7 +64,8 @@ __device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t bytes,
 //
 // The largest magnitude's bits order as integers, and a NaN's are above all: a row that holds an infinity or a NaN
 // gets the scale NaN, and codes of 0. A row of up to 8192 values is held in the registers of 256 threads, of up to
-// 32768 of 1024 (one row of 28672: 7.6 us with 256 threads that read it twice); what is longer is read twice.
+// 32768 of 1024 (one row of 28672: 7.6 us with 256 threads that read it twice); what is longer is read twice, and so are
+// the long rows of a call with too many of them for one launch of 1024 threads each.
 
 __device__ __forceinline__ uint32_t largest8(u32x4 v, uint32_t top) {
 #pragma unroll
@@ -482,7 +483,7 @@ void start_tiles(const Int8Linear &p, hipStream_t stream) {
 hipError_t launch_int8_quantize(const uint16_t *x, int64_t x_stride, uint8_t *codes, int64_t code_stride, float *scales,
                                 int64_t m, int k, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(m));
-  if (k <= 8192)
+  if (k <= 8192 || m > kMaxThreads / 1024)
     hipLaunchKernelGGL(int8_quantize_kernel<256>, grid, dim3(256), kLdsToken, stream, x, x_stride, codes, code_stride,
                        scales, k);
   else

@@ -224,3 +224,24 @@ def test_values_over_the_range_that_the_sums_hold(gpu, dtype, shape, near):
         for block in range(1, table.shape[1] * codes.shape[3], 2):
             scales[int(table[0, block // codes.shape[3]]), 1, :, block % codes.shape[3]] = 2.0 ** -99
     _check(kvc.attention(q, codes, scales, table, starts), _attend64(q, codes, scales, table, start))
+
+
+def test_more_long_rows_than_a_launch_of_wide_workgroups_holds(gpu):
+    """2^22 rows of 8208 values: 2^32 threads would be one too many where a row has 1024."""
+    m, k = 1 << 22, 8208
+    need = m * (2 * k + 8448 + 4)
+    if torch.cuda.mem_get_info(gpu)[0] + torch.cuda.memory_reserved(gpu) - torch.cuda.memory_allocated(gpu) < need + (8 << 30):
+        pytest.skip(f"needs {need >> 30} GiB")
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device=gpu)
+    rows = [0, 1, m // 2 + 5, m - 1]
+    some = torch.randn(4, k, device=gpu, generator=torch.Generator(device=gpu).manual_seed(0)).bfloat16()
+    x[rows] = some
+    try:
+        codes, scales = hip.int8_quantize(x)
+        want, want_scales = hip.int8_quantize(some)
+        assert torch.equal(codes[rows], want) and torch.equal(scales[rows], want_scales)
+        assert not scales[2: m // 2].any() and not codes[m // 2 + 6: m // 2 + 5000].any()
+    finally:
+        del x
+        codes = None
+        torch.cuda.empty_cache()
