@@ -8,6 +8,7 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <new>
 #include <unordered_set>
 #include <vector>
 
@@ -1608,14 +1609,18 @@ int ftx_kv8_copy_pages(void *codes, float *scales, int64_t layers, int64_t pages
   if (layers < 0 || n < 0 || layers > 65536) return ftx::fail(FTX_ERR_INVALID, "page copy dimensions");
   if (layers == 0 || n == 0) return FTX_OK;
   if (!src || !dst) return ftx::fail(FTX_ERR_INVALID, "null pointer");
-  std::unordered_set<int32_t> targets;
-  for (int64_t i = 0; i < n; ++i) {
-    if (src[i] < 0 || src[i] >= pages || dst[i] < 0 || dst[i] >= pages)
-      return ftx::fail(FTX_ERR_INVALID, "page copy: a page number outside the pool");
-    if (!targets.insert(dst[i]).second) return ftx::fail(FTX_ERR_INVALID, "page copy: a page is written twice");
+  try {
+    std::unordered_set<int32_t> targets;
+    for (int64_t i = 0; i < n; ++i) {
+      if (src[i] < 0 || src[i] >= pages || dst[i] < 0 || dst[i] >= pages)
+        return ftx::fail(FTX_ERR_INVALID, "page copy: a page number outside the pool");
+      if (!targets.insert(dst[i]).second) return ftx::fail(FTX_ERR_INVALID, "page copy: a page is written twice");
+    }
+    for (int64_t i = 0; i < n; ++i)
+      if (targets.count(src[i])) return ftx::fail(FTX_ERR_INVALID, "page copy: a page is read and written");
+  } catch (const std::bad_alloc &) {
+    return ftx::fail(FTX_ERR_OOM, "page copy: no memory to compare the pages in");
   }
-  for (int64_t i = 0; i < n; ++i)
-    if (targets.count(src[i])) return ftx::fail(FTX_ERR_INVALID, "page copy: a page is read and written");
   ftx::Kv8Copy p;
   const int64_t page_scales = static_cast<int64_t>(2) * kv_heads * (page_tokens / ftx::kKvBlock);
   const int64_t page_bytes = page_scales * ftx::kKvBlock * d;

@@ -246,3 +246,22 @@ for call in (lambda: _ftx_torch.append(), lambda: _ftx_torch.use(0), lambda: _ft
     raise SystemExit("not refused")
 """
     subprocess.run([sys.executable, "-c", code], check=True, timeout=120, cwd=nat.LIB_PATH.parent.parent)
+
+
+def test_a_page_list_too_long_for_the_memory_left_is_an_error():
+    """Of the C entry, which no exception may leave: a list that takes hundreds of MiB to check where 128 are left."""
+    code = """
+import ctypes, resource
+from flextensor_amd import _native as nat
+lib = nat.load()
+n = 20_000_000
+src, dst = ((ctypes.c_int32 * n)() for _ in range(2))
+import numpy as np
+np.frombuffer(dst, dtype=np.int32)[:] = np.arange(1, n + 1, dtype=np.int32)
+size = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (size + (128 << 20),) * 2)
+rc = lib.ftx_kv8_copy_pages(None, None, 1, n + 1, 1, 32, 64, src, dst, n, None)
+assert rc == nat.FTX_ERR_OOM, rc
+assert b"page copy" in lib.ftx_last_error()
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=120, cwd=nat.LIB_PATH.parent.parent)
