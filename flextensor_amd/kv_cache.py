@@ -230,10 +230,12 @@ def copy_pages(codes: torch.Tensor, scales: torch.Tensor, src: list[int], dst: l
 
 def read(codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """The keys and values that pages stand for, fp32 [..., tokens, kv heads, d] for a table [..., pages] of one
-    layer (torch operations: for inspection and export, not for a step)."""
+    layer (torch operations: for inspection and export, not for a step). Holes are zeros."""
     d, blocks, kv = codes.shape[-1] // BLOCK, codes.shape[-2], codes.shape[-3]
-    table = table.long()
+    hole = (table < 0) | (table >= codes.shape[0])
+    table = table.long().masked_fill(hole, 0)
     c = codes.view(torch.uint8)[table].view(codes.dtype).float() * scales[table].unsqueeze(-1)
+    c = c.masked_fill_(hole.view(*hole.shape, *[1] * 4), 0.0)
     lead = table.shape[:-1]
     c = c.movedim(-4, 0)  # [2, ..., pages, kv, blocks, 32 d]
     keys = c[0].unflatten(-1, (d // 16, BLOCK, 16)).transpose(-3, -2).flatten(-2)

@@ -265,3 +265,16 @@ assert rc == nat.FTX_ERR_OOM, rc
 assert b"page copy" in lib.ftx_last_error()
 """
     subprocess.run([sys.executable, "-c", code], check=True, timeout=120, cwd=nat.LIB_PATH.parent.parent)
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.float8_e4m3fn])
+def test_read_gives_zeros_for_holes(dtype):
+    """Numbers outside the pool on either side, as a ragged step's table holds them: not the last page's tokens."""
+    codes = torch.full((3, 2, 2, 1, 32 * 64), 5.0).to(dtype)
+    codes.view(torch.uint8)[2] = 0x7F  # a NaN in e4m3
+    scales = torch.full((3, 2, 2, 1), 2.0)
+    table = torch.tensor([[0, -1], [3, 1], [1 << 30, -7]], dtype=torch.int32)
+    for got in kvc.read(codes, scales, table):
+        assert got.shape == (3, 64, 2, 64)
+        assert (got[0, :32] == 10.0).all() and (got[1, 32:] == 10.0).all()
+        assert not got[0, 32:].any() and not got[1, :32].any() and not got[2].any()
