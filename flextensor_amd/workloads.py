@@ -491,7 +491,7 @@ class LlamaModel(nn.Module):
                 x = layer(x, pos, self.rope_cos, self.rope_sin, step.layer(i), None)
             else:
                 x = layer(x, pos, self.rope_cos, self.rope_sin, self.cache_k[i], self.cache_v[i])
-        if step is not None and min(step.counts) < x.shape[1]:
+        if step is not None and min(step.counts, default=x.shape[1]) < x.shape[1]:
             last = (step.new.long() - 1).clamp_min(0).view(-1, 1, 1).expand(-1, 1, x.shape[2])
             x = x.gather(1, last)
         return self.lm_head(self.norm(x[:, -1:])).float()

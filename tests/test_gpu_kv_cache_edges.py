@@ -245,3 +245,15 @@ def test_more_long_rows_than_a_launch_of_wide_workgroups_holds(gpu):
         del x
         codes = None
         torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_a_decoder_step_of_no_sequences(gpu, int8):
+    shape = W.LlamaShape(n_layers=2, hidden=128, n_heads=2, n_kv_heads=1, head_dim=64, inter=192, vocab=50, max_seq=64,
+                         int8=int8)
+    model = W.build_llama(shape, seed=0).to(gpu)
+    cache = model.init_paged_cache(4, 32, torch.int8, gpu)
+    step = cache.begin([], [], tokens=2)
+    with torch.no_grad():
+        assert model(torch.zeros(0, 2, dtype=torch.long, device=gpu), step=step).shape == (0, 1, 50)
+    cache.commit(step)

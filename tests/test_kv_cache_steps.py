@@ -278,3 +278,12 @@ def test_read_gives_zeros_for_holes(dtype):
         assert got.shape == (3, 64, 2, 64)
         assert (got[0, :32] == 10.0).all() and (got[1, 32:] == 10.0).all()
         assert not got[0, 32:].any() and not got[1, :32].any() and not got[2].any()
+
+
+def test_a_step_of_no_sequences_is_an_empty_pass():
+    shape = W.LlamaShape(n_layers=0, hidden=64, n_heads=1, n_kv_heads=1, head_dim=64, inter=96, vocab=50, max_seq=48)
+    model = W.build_llama(shape, seed=0)
+    cache = kvc.PagedKVCache(1, 1, 64, 4, page_tokens=PAGE, dtype=torch.int8, device="cpu")
+    step = cache.begin([], [], tokens=3)
+    assert model(torch.zeros(0, 3, dtype=torch.long), step=step).shape == (0, 1, 50)
+    cache.commit(step)
