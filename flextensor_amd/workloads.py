@@ -535,26 +535,34 @@ def generate_paged(model: LlamaModel, cache: kv_cache.PagedKVCache, prompts: lis
     """Greedy decoding of prompts of different lengths over a paged 8-bit cache.
 
     The prompts are one ragged pass. Each is then forked into ``samples`` sequences that share its pages; sample j
-    starts from its j-th likeliest token. Returns the sequences (in the cache until closed), their tokens
-    ``[prompts * samples, steps]`` and the logits of every step.
+    starts from its j-th likeliest token. Returns the sequences (in the cache until closed; closed already where an
+    error ends the run), their tokens ``[prompts * samples, steps]`` and the logits of every step.
     """
     longest = max(len(p) for p in prompts)
     device = model.rope_cos.device
     tokens = torch.tensor([p + [0] * (longest - len(p)) for p in prompts], device=device)
     roots = [cache.open() for _ in prompts]
-    step = cache.begin(roots, [len(p) for p in prompts])
-    logits = model(tokens, step=step)
-    cache.commit(step)
-    sequences = [s for root in roots for s in [root, *(cache.fork(root) for _ in range(samples - 1))]]
-    tok = logits[:, -1].topk(samples, -1).indices.reshape(-1, 1)
-    out, all_logits = [tok], [logits]
-    for _ in range(steps - 1):
-        step = cache.begin(sequences, 1)
-        logits = model(tok, step=step)
+    sequences = roots
+    try:
+        step = cache.begin(roots, [len(p) for p in prompts])
+        logits = model(tokens, step=step)
         cache.commit(step)
-        all_logits.append(logits)
-        tok = logits.argmax(-1)
-        out.append(tok)
+        sequences = []
+        for root in roots:
+            sequences += [root, *(cache.fork(root) for _ in range(samples - 1))]
+        tok = logits[:, -1].topk(samples, -1).indices.reshape(-1, 1)
+        out, all_logits = [tok], [logits]
+        for _ in range(steps - 1):
+            step = cache.begin(sequences, 1)
+            logits = model(tok, step=step)
+            cache.commit(step)
+            all_logits.append(logits)
+            tok = logits.argmax(-1)
+            out.append(tok)
+    except BaseException:  # the caller has no numbers to close them by
+        for s in sequences:
+            cache.close(s)
+        raise
     return sequences, torch.cat(out, dim=1), all_logits
 
 

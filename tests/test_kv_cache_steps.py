@@ -287,3 +287,27 @@ def test_a_step_of_no_sequences_is_an_empty_pass():
     step = cache.begin([], [], tokens=3)
     assert model(torch.zeros(0, 3, dtype=torch.long), step=step).shape == (0, 1, 50)
     cache.commit(step)
+
+
+@pytest.mark.parametrize("fails_at", ["the pool", "the prompts", "a step"])
+def test_a_run_that_ends_early_leaves_no_sequences_behind(pool, monkeypatch, fails_at):
+    shape = W.LlamaShape(n_layers=0, hidden=64, n_heads=1, n_kv_heads=1, head_dim=64, inter=96, vocab=50, max_seq=4096)
+    model = W.build_llama(shape, seed=0)
+    kept = pool.open()
+    pool.commit(pool.begin([kept], 40))
+    before, passes = pool.free_pages, []
+    if fails_at != "the pool":
+        forward = model.forward
+
+        def fails(tokens, step):
+            passes.append(step)
+            if len(passes) == (1 if fails_at == "the prompts" else 3):
+                raise RuntimeError("lost")
+            return forward(tokens, step=step)
+
+        monkeypatch.setattr(model, "forward", fails)
+    prompts = [[1] * (400 if fails_at == "the pool" else 40)] * 2
+    with pytest.raises((RuntimeError, kvc.KVCacheFull)):
+        W.generate_paged(model, pool, prompts, 5, samples=2)
+    assert pool.free_pages == before and list(pool._lengths) == [kept]
+    monkeypatch.undo()
