@@ -923,7 +923,6 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
     }
 #pragma unroll
     for (int m = 1; m < kWave; m *= 2) largest = fmaxf(largest, __shfl_xor(largest, m));
-    if (head > h0) __syncthreads();  // the head before is through with the shared arrays
     if ((threadIdx.x & (kWave - 1)) == 0) wave_max[threadIdx.x / kWave] = largest;
     if (before > 0 && threadIdx.x * 16 < kKvBlock * D)
       *reinterpret_cast<u32x4 *>(tile + threadIdx.x * 16) = *reinterpret_cast<const u32x4 *>(codes + threadIdx.x * 16);
@@ -974,7 +973,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
       if (threadIdx.x * 16 < kKvBlock * D)
         *reinterpret_cast<u32x4 *>(codes + threadIdx.x * 16) = *reinterpret_cast<const u32x4 *>(tile + threadIdx.x * 16);
     }
-    __syncthreads();  // every thread has read the old scale
+    __syncthreads();  // every thread has read the old scale and is through with the shared arrays
     if (threadIdx.x == 0) a.scales[index] = scale;
   }
 }
