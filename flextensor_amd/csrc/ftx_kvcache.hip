@@ -99,7 +99,7 @@ __device__ __forceinline__ float lane_float(float v, int lane) {
 // at most, as the attention over a bf16 cache does): the matrix cores are what they wait for, and a second part makes
 // 2048 tokens over 8148 (64 / 8 heads) 647 us where one takes 483, for an error of 0.0017 of the result in 64 bits
 // (relative norm; the output's own rounding) where one gives 0.0024. A probability may be 2^kSlack and the sums are
-// divided at the end, so fp32 holds them for values of up to about 2^112 (5e33).
+// divided at the end: 2^19 keys of values of 2^100 (1e30) stay within fp32.
 
 // Eight codes as bf16.
 template <bool FP8>

@@ -177,7 +177,7 @@ def attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, table:
     cached one), the rounding of the probabilities: prompts in tiles of 256 rows round each to bf16 for the matrix cores
     (0.0024 of the result in relative norm, 0.0017 being the output's own rounding), fewer rows do not. ``scale``:
     1 / sqrt(d) if None. A NaN that a sequence holds may reach earlier tokens of the same call. The sums are fp32: values
-    of up to about 5e33 stay finite.
+    of up to about 1e30 stay finite.
     """
     device = _device(q)
     if device >= 0 and torch.autograd.forward_ad._current_level < 0:
@@ -472,7 +472,8 @@ class PagedKVCache:
         return len(src)
 
     def resize(self, pages: int) -> None:
-        """Changes the number of pages; those in use must be among the first ``pages`` (:meth:`compact`)."""
+        """Changes the number of pages; those in use must be among the first ``pages`` (:meth:`compact`). The pool is
+        other tensors then: what holds the old ones (a captured graph) does not follow."""
         if pages < 1 or any(self._refs[pages:]):
             raise ValueError(f"a pool of {pages} pages does not hold the pages in use")
         codes, scales = self._tensors(pages)
