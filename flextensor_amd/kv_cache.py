@@ -261,6 +261,7 @@ class KVStep:
     max_tokens: int
     held: tuple = ()  # of each sequence: its length, and the pages that its new tokens go to
     moves: int = 0  # compactions of the cache before it
+    most: int = 0  # the largest count
 
     def layer(self, index: int) -> "KVLayer":
         return KVLayer(self, index)
@@ -268,7 +269,7 @@ class KVStep:
     def check(self, batch: int, tokens: int, positions: int) -> None:
         """Refuses a pass of [batch, tokens] rows that does not hold the step's tokens, or whose rotary tables of so
         many ``positions`` end before them."""
-        if batch != len(self.sequences) or tokens < max(self.counts, default=0):
+        if batch != len(self.sequences) or tokens < self.most:
             raise ValueError(f"the step counts {self.counts} tokens of {len(self.sequences)} sequences, the pass has "
                              f"{tokens} of {batch}")
         if self.max_tokens > positions and any(c and was[0] + c > positions for c, was in zip(self.counts, self.held)):
@@ -436,7 +437,8 @@ class PagedKVCache:
         dev = host.to(self.device)  # one upload
         longest = max((self._lengths[s] + c for s, c in zip(sequences, counts)), default=0)
         return KVStep(self, tuple(sequences), tuple(counts), dev[2 * b:].view(b, width), dev[:b], dev[b: 2 * b],
-                      tokens, longest, tuple(self._state(s, c) for s, c in zip(sequences, counts)), self._moves)
+                      tokens, longest, tuple(self._state(s, c) for s, c in zip(sequences, counts)), self._moves,
+                      max(counts, default=0))
 
     def _state(self, sequence: int, count: int) -> tuple[int, list[int]]:
         """The length of a sequence, and the pages that its next tokens go to."""

@@ -257,3 +257,36 @@ def test_a_decoder_step_of_no_sequences(gpu, int8):
     with torch.no_grad():
         assert model(torch.zeros(0, 2, dtype=torch.long, device=gpu), step=step).shape == (0, 1, 50)
     cache.commit(step)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_a_query_that_is_not_finite_spoils_its_own_row(gpu, shape, value):
+    """An infinity gives scores of both infinities or NaN: no softmax of them is a number."""
+    q, codes, scales, table, starts = _case(gpu, torch.int8, *shape)
+    want = _attend64(q, codes, scales, table, shape[-1])
+    t, h = shape[:2]
+    bad = torch.zeros(1, t, h, dtype=torch.bool, device=gpu)
+    bad[0, t // 2, h - 1] = bad[0, t - 1, 0] = True
+    q[bad] = torch.where(torch.arange(q.shape[3], device=gpu) % 17 == 3, value, q[bad])
+    got = kvc.attention(q, codes, scales, table, starts)
+    assert got[bad].isnan().all()
+    if not bad.all():
+        _check(got[~bad], want[~bad])
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_a_key_that_is_not_a_number_spoils_the_rows_that_see_it(gpu, shape):
+    """An e4m3 NaN among a head's keys: rows from its token on, of the queries that share the head."""
+    q, codes, scales, table, starts = _case(gpu, torch.float8_e4m3fn, *shape)
+    t, h, kv, d, page, start = shape
+    want = _attend64(q, codes, scales, table, start)
+    at = start + t // 2
+    cell = codes.view(torch.uint8)[int(table[0, at // page]), 0, kv - 1, at % page // BLOCK]
+    cell.view(d // 16, BLOCK, 16)[1, at % BLOCK, 5] = 0x7F
+    got = kvc.attention(q, codes, scales, table, starts)
+    bad = torch.zeros(1, t, h, dtype=torch.bool, device=gpu)
+    bad[0, t // 2:, (kv - 1) * (h // kv):] = True
+    assert got[bad].isnan().all()
+    if not bad.all():
+        _check(got[~bad], want[~bad])
