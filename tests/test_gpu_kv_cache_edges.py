@@ -290,3 +290,25 @@ def test_a_key_that_is_not_a_number_spoils_the_rows_that_see_it(gpu, shape):
     assert got[bad].isnan().all()
     if not bad.all():
         _check(got[~bad], want[~bad])
+
+
+def test_a_decoder_ends_at_its_last_position_on_pages_used_before(gpu):
+    """Every page holds NaN codes of an earlier sequence. Up to the last position the logits are numbers; a step past it
+    is refused, writes nothing and counts nothing."""
+    shape = W.LlamaShape(n_layers=2, hidden=128, n_heads=2, n_kv_heads=1, head_dim=64, inter=192, vocab=50, max_seq=40)
+    model = W.build_llama(shape, seed=0).to(gpu)
+    cache = model.init_paged_cache(4, 32, torch.float8_e4m3fn, gpu)
+    cache.codes.view(torch.uint8).fill_(0x7F)
+    cache.scales.fill_(1.0)
+    seq = cache.open()
+    with torch.no_grad():
+        for n in (37, 3):
+            step = cache.begin([seq], n)
+            assert model(torch.ones(1, n, dtype=torch.long, device=gpu), step=step).isfinite().all()
+            cache.commit(step)
+        before = cache.codes.view(torch.uint8).clone(), cache.scales.clone()
+        step = cache.begin([seq], 1)
+        with pytest.raises(ValueError, match="40 positions"):
+            model(torch.ones(1, 1, dtype=torch.long, device=gpu), step=step)
+    assert torch.equal(cache.codes.view(torch.uint8), before[0]) and torch.equal(cache.scales, before[1])
+    assert cache.length(seq) == 40
