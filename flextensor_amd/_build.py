@@ -18,7 +18,7 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libftx_hip.so"
 SOURCES = ("ftx_runtime.hip", "ftx_kernels.hip", "ftx_gemm.hip", "ftx_attention.hip", "ftx_layers.hip",
-           "ftx_int8.hip", "ftx_kvcache.hip", "ftx_staged.hip", "ftx_expcode.hip")
+           "ftx_int8.hip", "ftx_int4.hip", "ftx_kvcache.hip", "ftx_logprobs.hip", "ftx_staged.hip", "ftx_expcode.hip")
 OFFLOAD_ARCH = "gfx950"
 # The library's serving calls, taking torch tensors (a CPython extension, host code only); it is told which library.
 TORCH_SOURCE = CSRC / "ftx_torch.cpp"

@@ -190,6 +190,17 @@ _SIGNATURES: dict[str, list] = {
                                     ctypes.POINTER(_sz)],
     "ftx_kv8_attention": [ctypes.POINTER(Kv8Cache), _vp, _vp, ctypes.c_int64, ctypes.c_int64, _int, _vp,
                           ctypes.c_float, ctypes.c_int64, _vp, _sz, _vp],
+    "ftx_kv8_append_norm": [ctypes.POINTER(Kv8Cache), _vp, _vp, _vp, _vp, _vp, ctypes.c_float, _vp, _vp, ctypes.c_int64,
+                            _vp, ctypes.c_int64, _vp, ctypes.c_int64, ctypes.c_int64, _int, _vp, _vp],
+    "ftx_kv8_tree_attention": [ctypes.POINTER(Kv8Cache), _vp, _vp, _vp, ctypes.c_int64, _int, ctypes.c_int64,
+                               ctypes.c_int64, _int, _vp, ctypes.c_float, ctypes.c_int64, _vp, _sz, _vp],
+    "ftx_kv8_keep": [ctypes.POINTER(Kv8Cache), ctypes.c_int64, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp],
+    "ftx_int4_linear_workspace": [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _int, ctypes.POINTER(_sz)],
+    "ftx_int4_linear": [_vp, ctypes.c_int64, _vp, _vp, _vp, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _int, _vp,
+                        _sz, _vp],
+    "ftx_token_logprobs_workspace": [ctypes.c_int64, ctypes.c_int64, _int, _int, ctypes.POINTER(_sz)],
+    "ftx_token_logprobs": [_vp, ctypes.c_int64, _int, _vp, ctypes.c_int64, ctypes.c_int64, _int, _vp, _vp, _vp, _vp, _vp,
+                           _sz, _vp],
     "ftx_kv8_copy_pages": [_vp, _vp, ctypes.c_int64, ctypes.c_int64, _int, _int, _int, _vp, _vp, ctypes.c_int64, _vp],
     "ftx_silu_mul": [_vp, _vp, _vp, ctypes.c_int64, _vp],
     "ftx_fp8_linear_fused": [_vp, ctypes.c_int, _vp, _vp, _vp, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, _vp,
@@ -203,6 +214,14 @@ FP8_EPILOGUE_RESIDUAL = 2
 KV8_BLOCK = 32
 KV8_E4M3 = 0
 KV8_INT8 = 1
+KV8_TREE_NODES = 64
+
+INT4_TILE = 16
+INT4_UNIT = 128
+
+LOGITS_BF16 = 0
+LOGITS_FP16 = 1
+LOGITS_FP32 = 2
 
 NORM_NONE = 0
 NORM_RMS = 1

@@ -197,6 +197,9 @@ struct Kv8Attention {
   int64_t q_stride[3], o_stride[3];  // batch, token, head, in elements
   int batch, t, heads;
   float scale_log2;
+  const int64_t *tree;    // of a call over a tree: the nodes that each row sees, a bit each [batch][t]; else null
+  int64_t tree_stride;
+  int nodes;              // cached after the starts, 64 at most
   // planned
   int rep, rows, row_tiles, splits, chunk, xcds;  // chunk: blocks of a split
   int tile_rows;          // up to 16 or 32: the kernel of few rows; else the prompts'
@@ -216,6 +219,10 @@ struct Kv8Append {
   int64_t positions;
   int64_t q_stride[3], k_stride[3], v_stride[3];
   int batch, t, heads;
+  const int32_t *at;      // rows of cos and sin [batch][t], at_stride apart; null: a token's own place
+  int64_t at_stride;
+  const uint16_t *q_weight, *k_weight;  // bf16 [d], or null: no norm
+  float eps;
   // planned
   int seq_blocks;         // blocks that t tokens touch at most
   int heads_each;         // heads of a workgroup
@@ -223,6 +230,16 @@ struct Kv8Append {
 };
 void plan_kv8_append(Kv8Append *p, int cus);
 hipError_t launch_kv8_append(const Kv8Append &p, hipStream_t stream);
+struct Kv8Keep {
+  KvPages kv;             // news: the tokens that a path keeps
+  uint8_t *codes;         // of all layers
+  float *scales;
+  int64_t layers;
+  const int32_t *path;    // [batch][n], path_stride apart
+  int64_t path_stride;
+  int batch, n;
+};
+hipError_t launch_kv8_keep(const Kv8Keep &p, hipStream_t stream);
 constexpr int kKvCopyPairs = 256;  // of one launch: they travel as its argument
 struct Kv8Copy {
   uint8_t *codes;
@@ -258,6 +275,48 @@ void plan_int8_linear(Int8Linear *p, bool from_x, int cus, int xcds);  // from_x
 hipError_t launch_int8_linear(const Int8Linear &p, hipStream_t stream);
 hipError_t launch_int8_quantize(const uint16_t *x, int64_t x_stride, uint8_t *codes, int64_t code_stride, float *scales,
                                 int64_t m, int k, hipStream_t stream);
+
+// The matrix product with 4-bit weights (ftx_int4.hip).
+constexpr int kInt4Unit = 128;  // inputs of 1 KB of codes
+constexpr int64_t kInt4MaxK = int64_t(1) << 20;
+constexpr int64_t kInt4MaxStride = int64_t(1) << 21;  // 256 rows of x are within 32-bit byte offsets
+struct Int4Linear {
+  const uint16_t *x;      // bf16 [m] rows x_stride apart
+  int64_t x_stride;
+  const uint8_t *w;       // [tiles][units][1024]
+  const uint16_t *scale, *zero;  // bf16 [tiles][units][16][parts]; zero may be null
+  uint16_t *y;            // bf16 [m][n]
+  float *part;            // [splits][m][part_stride] sums, when splits > 1
+  int64_t m, n, part_stride;
+  int k, parts;           // parts: groups of a unit
+  // planned
+  int64_t tiles;          // of 16 channels
+  int units, tile_m, row_tiles, splits, split_units, band, xcds;  // tile_m 16: the kernel of up to 16 rows
+  uint32_t m_tiles, n_tiles, items;
+  size_t part_bytes;
+};
+void plan_int4_linear(Int4Linear *p, int cus, int xcds);
+hipError_t launch_int4_linear(const Int4Linear &p, hipStream_t stream);
+
+// Log probabilities, entropy and likeliest tokens of rows of logits (ftx_logprobs.hip).
+constexpr int64_t kLogprobsMaxVocab = int64_t(1) << 28;
+constexpr int kLogprobsMaxTop = 64;  // a wave's lanes
+struct Logprobs {
+  const void *logits;     // [rows] of vocab values, row_stride values apart
+  int64_t row_stride;
+  const int64_t *tokens;  // [rows]
+  int64_t rows, vocab;
+  int type, top;
+  float *logprob, *entropy, *top_logprob;
+  int64_t *top_token;
+  float4 *part;           // [rows][splits] sums, when splits > 1
+  unsigned long long *part_keys;  // [rows][splits][64], when there is a top
+  // planned
+  int threads, splits, split_units;  // of a workgroup: threads, parts of a row, 16-byte units of a part
+  size_t part_bytes;
+};
+void plan_logprobs(Logprobs *p, int cus);
+hipError_t launch_logprobs(const Logprobs &p, hipStream_t stream);
 
 // Staged copies from pageable host memory and the parallel host memcpy
 // (ftx_staged.hip).

@@ -158,10 +158,42 @@ __device__ __forceinline__ float row_sum(float v) {
   return half_sum(__uint_as_float(s[0]) + __uint_as_float(s[1]));
 }
 
+// A call over a tree of drafted tokens: `count` rows that see the `start` first tokens and, of the `nodes` after them,
+// the ones in their set.
+__device__ __forceinline__ Span tree_span(const Kv8Attention &a, int64_t b) {
+  const int start = a.kv.starts[b];
+  if (start < 0 || start > a.kv.width * a.kv.page_blocks * kKvBlock) return {0, 0};
+  return {start, max(0, a.kv.news ? min(a.kv.news[b], a.t) : a.t)};
+}
+template <bool TREE>
+__device__ __forceinline__ Span rows_of(const Kv8Attention &a, int64_t b) {
+  if constexpr (TREE) return tree_span(a, b);
+  return span_of(a.kv, b, a.t);
+}
+// The tokens that any row may see.
+template <bool TREE>
+__device__ __forceinline__ int length_of(const Kv8Attention &a, Span s) {
+  if constexpr (TREE) return min(s.start + a.nodes, a.kv.width * a.kv.page_blocks * kKvBlock);
+  return s.start + s.count;
+}
+// The nodes that a row sees.
+__device__ __forceinline__ uint64_t node_set(const Kv8Attention &a, int64_t b, int token, int held) {
+  const uint64_t set = static_cast<uint64_t>(a.tree[b * a.tree_stride + token]);
+  return held >= 64 ? set : set & ((1ull << max(held, 0)) - 1);
+}
+// Of the 32 tokens from `at` on (counted from the nodes' first one), the ones that a row with this set sees.
+__device__ __forceinline__ uint32_t tokens_seen(uint64_t set, int at) {
+  if (at >= 64) return 0;
+  if (at >= 0) return static_cast<uint32_t>(set >> at);
+  return at <= -32 ? ~0u : static_cast<uint32_t>(set << -at) | ((1u << -at) - 1);
+}
+
 // The blocks that the rows of a tile see.
+template <bool TREE>
 __device__ __forceinline__ int tile_blocks(const Kv8Attention &a, Span s, int tile) {
   const int row0 = tile * a.tile_rows;
   if (row0 / a.rep >= s.count) return 0;
+  if (TREE) return (length_of<TREE>(a, s) + kKvBlock - 1) / kKvBlock;
   const int last = min(min(row0 + a.tile_rows, a.rows) - 1, s.count * a.rep - 1) / a.rep;
   return (s.start + last) / kKvBlock + 1;
 }
@@ -169,7 +201,7 @@ __device__ __forceinline__ int tile_blocks(const Kv8Attention &a, Span s, int ti
 // Few rows: RT tiles of 16 (row = token * rep + head of the group) over one chunk of the keys; the eight waves take its
 // blocks in turn and join their sums through LDS. Nothing is staged: each wave loads the next block's codes into
 // registers while it works on this one, and widens a code once for all its rows.
-template <int D, bool FP8, int RT>
+template <int D, bool FP8, int RT, bool TREE>
 __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Attention a) {
   constexpr int kWaves = 8;
   constexpr int kKLoads = D / 64;   // 16 bytes a lane, of each 16 keys of a block
@@ -186,8 +218,8 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
   item /= static_cast<uint32_t>(a.row_tiles);
   const int kvh = uniform(item % static_cast<uint32_t>(a.kv.kv_heads));
   const int64_t b = uniform(item / static_cast<uint32_t>(a.kv.kv_heads));
-  const Span span = span_of(a.kv, b, a.t);
-  const int blocks = tile_blocks(a, span, tile);
+  const Span span = rows_of<TREE>(a, b);
+  const int blocks = tile_blocks<TREE>(a, span, tile);
   const int first = split * a.chunk;
   if (a.splits > 1 && first >= blocks) return;
   const int end = split == a.splits - 1 ? blocks : min(blocks, first + a.chunk);
@@ -196,10 +228,12 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 15, g = lane >> 4;
   const int row0 = tile * (16 * RT);
-  const int length = span.start + span.count;
+  const int length = length_of<TREE>(a, span);
   const int last_token = (min(row0 + 16 * RT, a.rows) - 1) / a.rep;
-  const int whole = last_token < span.count ? span.start + row0 / a.rep + 1 : 0;  // every row sees keys below this
-  int seen[RT];  // keys this lane's rows see
+  // every row sees keys below this
+  const int whole = last_token >= span.count ? 0 : TREE ? span.start : span.start + row0 / a.rep + 1;
+  int seen[RT];       // keys this lane's rows see
+  uint64_t sets[RT];  // nodes, after them
   bf16x8 qf[RT][D / 32];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
@@ -207,6 +241,7 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
     const int token = row / a.rep;
     const int head = kvh * a.rep + (row - token * a.rep);
     seen[t] = token < span.count ? span.start + token + 1 : 0;
+    if (TREE) sets[t] = token < span.count ? node_set(a, b, token, length - span.start) : 0;
     const uint16_t *qp = a.q + b * a.q_stride[0] + token * a.q_stride[1] + head * a.q_stride[2] + 16 * g;
 #pragma unroll
     for (int i = 0; i < kKLoads; ++i)
@@ -278,6 +313,12 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
         const int limit = x.hole ? 0 : seen[t] - key0;
+        if (TREE) {
+          const uint32_t in = x.hole || seen[t] == 0 ? 0 : tokens_seen(sets[t], key0 + 8 * g - span.start);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[t][e / 4][e % 4] = in >> e & 1 ? s[t][e / 4][e % 4] * scale : -INFINITY;
+          continue;
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -406,7 +447,7 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
 //
 // S^T = K Q^T gives a lane 16 of a block's 32 scores of one row, keys 8 a + 4 g + c (g the half of the wave); V's
 // operands are written in that order.
-template <int D, bool FP8, bool SPLIT>
+template <int D, bool FP8, bool SPLIT, bool TREE>
 __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Attention a) {
   constexpr int kThreads = kTileWaves * kWave;
   constexpr int kKeys = 64, kSub = 2;
@@ -429,8 +470,8 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
   const int64_t tile_item = static_cast<int64_t>(bkv) * a.row_tiles + tile;
   const int64_t b = uniform(bkv / static_cast<uint32_t>(a.kv.kv_heads));
   const int kvh = uniform(bkv % static_cast<uint32_t>(a.kv.kv_heads));
-  const Span span = span_of(a.kv, b, a.t);
-  const int blocks = tile_blocks(a, span, tile);
+  const Span span = rows_of<TREE>(a, b);
+  const int blocks = tile_blocks<TREE>(a, span, tile);
   const int first = SPLIT ? split * a.chunk : 0;
   if (SPLIT && first >= blocks) return;
   const int end = !SPLIT || split == a.splits - 1 ? blocks : min(blocks, first + a.chunk);
@@ -443,12 +484,17 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
   const int row = min(row0 + r, a.rows - 1);
   const int token = row / a.rep;
   const int head = kvh * a.rep + (row - token * a.rep);
-  const int length = span.start + span.count;
-  const int seen = row0 + r < a.rows && token < span.count ? span.start + token + 1 : 0;  // keys this lane's row sees
+  const int length = length_of<TREE>(a, span);
+  const bool live = row0 + r < a.rows && token < span.count;
+  const int seen = live ? span.start + token + 1 : 0;  // keys this lane's row sees
+  const uint64_t set = TREE && live ? node_set(a, b, token, length - span.start) : 0;  // of a tree: the nodes
   const int last_row = min(row0 + 32, a.rows) - 1;
-  const int wave_end = row0 < a.rows && row0 / a.rep < span.count ? min(span.start + last_row / a.rep + 1, length) : 0;
+  const int wave_end = row0 >= a.rows || row0 / a.rep >= span.count ? 0
+                       : TREE                                       ? length
+                                                                    : min(span.start + last_row / a.rep + 1, length);
   // every row of the wave sees keys below this
-  const int whole = row0 + 32 <= a.rows && last_row / a.rep < span.count ? span.start + row0 / a.rep + 1 : 0;
+  const bool all_live = row0 + 32 <= a.rows && last_row / a.rep < span.count;
+  const int whole = !all_live ? 0 : TREE ? span.start : span.start + row0 / a.rep + 1;
 
   const auto side_of = [&](int i) {  // known when compiled where a unit of all waves is of one side
     return kSideUnits >= kThreads ? i * kThreads / kSideUnits : (i * kThreads + wave * kWave) / kSideUnits;
@@ -572,6 +618,14 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
       scale[j] = a.scale_log2 * x.key[j];
       const int block = first + t * kSub + j;
       if (x.hole[j] || (block + 1) * kKvBlock > whole) {
+        if (TREE) {
+          const uint32_t in = x.hole[j] || !live ? 0 : tokens_seen(set, block * kKvBlock - span.start) >> (4 * g);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            s[j][e] = in >> (8 * (e >> 2) + (e & 3)) & 1 ? s[j][e] * scale[j] : -INFINITY;
+          scale[j] = 1.0f;
+          continue;
+        }
         const int limit = x.hole[j] ? 0 : seen - block * kKvBlock;
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[j][e] = 8 * (e >> 2) + 4 * g + (e & 3) < limit ? s[j][e] * scale[j] : -INFINITY;
@@ -685,7 +739,7 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
 // o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the chunks that hold keys the tile sees, M the largest
 // m_i. A workgroup a row: groups of D / 4 lanes take the chunks in turn, so that few rows over many chunks wait for
 // a few loads and not for one after the other, and meet in LDS.
-template <int D>
+template <int D, bool TREE>
 __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8Attention a) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes, kBatch = 4;
   __shared__ f32x4 part_o[kGroups][kLanes];
@@ -697,7 +751,7 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8Attention a) {
   if (row >= a.rows) return;
   const uint32_t bkv = uniform(tile_item / static_cast<uint32_t>(a.row_tiles));
   const int64_t b = uniform(bkv / static_cast<uint32_t>(a.kv.kv_heads));
-  const int used = min(a.splits, (tile_blocks(a, span_of(a.kv, b, a.t), tile) + a.chunk - 1) / a.chunk);
+  const int used = min(a.splits, (tile_blocks<TREE>(a, rows_of<TREE>(a, b), tile) + a.chunk - 1) / a.chunk);
   const float *pm = a.part + a.splits * slots * D;
   const float *pl = pm + a.splits * slots;
   const int c = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
@@ -753,16 +807,16 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8Attention a) {
       (u32x2){pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
 }
 
-template <int D, bool FP8>
+template <int D, bool FP8, bool TREE>
 hipError_t launch_attend(const Kv8Attention &p, hipStream_t stream) {
   const dim3 block(kTileWaves * kWave), grid(p.items), xcd_grid((p.items + p.xcds - 1) / p.xcds * p.xcds);
-  if (p.tile_rows <= 16) hipLaunchKernelGGL((kv8_rows_kernel<D, FP8, 1>), grid, block, 0, stream, p);
-  else if (p.tile_rows == 32) hipLaunchKernelGGL((kv8_rows_kernel<D, FP8, 2>), grid, block, 0, stream, p);
-  else if (p.splits > 1) hipLaunchKernelGGL((kv8_tile_kernel<D, FP8, true>), xcd_grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((kv8_tile_kernel<D, FP8, false>), xcd_grid, block, 0, stream, p);
+  if (p.tile_rows <= 16) hipLaunchKernelGGL((kv8_rows_kernel<D, FP8, 1, TREE>), grid, block, 0, stream, p);
+  else if (p.tile_rows == 32) hipLaunchKernelGGL((kv8_rows_kernel<D, FP8, 2, TREE>), grid, block, 0, stream, p);
+  else if (p.splits > 1) hipLaunchKernelGGL((kv8_tile_kernel<D, FP8, true, TREE>), xcd_grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((kv8_tile_kernel<D, FP8, false, TREE>), xcd_grid, block, 0, stream, p);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || p.splits == 1) return err;
-  hipLaunchKernelGGL((kv8_join_kernel<D>), dim3(static_cast<unsigned>(p.tile_items * p.tile_rows)), dim3(256), 0,
+  hipLaunchKernelGGL((kv8_join_kernel<D, TREE>), dim3(static_cast<unsigned>(p.tile_items * p.tile_rows)), dim3(256), 0,
                      stream, p);
   return hipGetLastError();
 }
@@ -804,9 +858,12 @@ __device__ __forceinline__ float code_value(uint32_t byte) {
 
 // What rotates a thread's N values from d0 on: a row of the tables. x cos + rot(x) sin, rot(x) = (-upper half, lower
 // half).
-template <int D, int N>
+//
+// NORM: the values are x * f * w first, f = 1 / sqrt(mean x^2 + eps) of their head's row and w the weights.
+template <int D, int N, bool NORM>
 struct Rotation {
   float cos[N], sin[N];
+  float own_w[NORM ? N : 1], other_w[NORM ? N : 1];  // of the values, and of the ones they turn against
   __device__ __forceinline__ void load(const float *c, const float *s, int d0) {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
@@ -814,7 +871,39 @@ struct Rotation {
       *reinterpret_cast<f32x4 *>(sin + i) = *reinterpret_cast<const f32x4 *>(s + d0 + i);
     }
   }
-  __device__ __forceinline__ void apply(const uint16_t *x, int d0, float *y) const {
+  __device__ __forceinline__ void load_weights(const uint16_t *w, int d0) {
+    const int other = d0 < D / 2 ? d0 + D / 2 : d0 - D / 2;
+#pragma unroll
+    for (int v = 0; v < N; v += 8) {
+      const u32x4 a = *reinterpret_cast<const u32x4 *>(w + d0 + v), b = *reinterpret_cast<const u32x4 *>(w + other + v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        own_w[v + i] = bf16_value(a[i / 2] >> (16 * (i & 1)));
+        other_w[v + i] = bf16_value(b[i / 2] >> (16 * (i & 1)));
+      }
+    }
+  }
+  // The D / N lanes of a row: its f. The sum is one of 64 bits, in which the squares are exact, and f the nearest fp32
+  // number: the codes made from it depend on no order of the sum.
+  __device__ __forceinline__ float factor(const uint16_t *x, int d0, float eps) const {
+    double sum = 0.0;
+#pragma unroll
+    for (int v = 0; v < N; v += 8) {
+      const u32x4 a = *reinterpret_cast<const u32x4 *>(x + d0 + v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const double value = bf16_value(a[i / 2] >> (16 * (i & 1)));
+        sum = fma(value, value, sum);
+      }
+    }
+#pragma unroll
+    for (int j = 1; j < D / N; j *= 2) sum += __shfl_xor(sum, j);
+    const double mean = sum * (1.0 / D) + static_cast<double>(eps);
+    const double rough = __builtin_amdgcn_rsq(mean);  // 2^-23 off or less; a step of Newton's: 2^-45
+    const double better = fma(0.5 * rough, fma(-mean * rough, rough, 1.0), rough);
+    return static_cast<float>(mean > 0.0 && mean < INFINITY ? better : rough);
+  }
+  __device__ __forceinline__ void apply(const uint16_t *x, int d0, float *y, float f) const {
 #pragma clang fp contract(off)
     const int other = d0 < D / 2 ? d0 + D / 2 : d0 - D / 2;
 #pragma unroll
@@ -822,8 +911,12 @@ struct Rotation {
       const u32x4 a = *reinterpret_cast<const u32x4 *>(x + d0 + v), b = *reinterpret_cast<const u32x4 *>(x + other + v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float va = bf16_value(a[i / 2] >> (16 * (i & 1)));
-        const float vb = bf16_value(b[i / 2] >> (16 * (i & 1)));
+        float va = bf16_value(a[i / 2] >> (16 * (i & 1)));
+        float vb = bf16_value(b[i / 2] >> (16 * (i & 1)));
+        if (NORM) {
+          va = va * f * own_w[v + i];
+          vb = vb * f * other_w[v + i];
+        }
         const float turned = d0 < D / 2 ? -vb : vb;
         const float p = va * cos[v + i], q = turned * sin[v + i];
         y[v + i] = p + q;
@@ -836,7 +929,11 @@ struct Rotation {
 // the same number of heads each. The heads share their tokens' rows of the tables, 4 d bytes each of cos and sin where
 // a head's own values are 2 d; with that, and a token's values side by side in a wave, a prompt of 2048 tokens (32 heads
 // of 128, int8) takes 20.7 us, 4.1 TB/s, and took 31 before. A decode step needs the workgroups and has one head each.
-template <int D, bool FP8>
+//
+// AT: a token's row of the tables may be another than its place's, `a.at`; one outside the tables makes the token 0, in
+// the cache too. NORM: queries and keys are normalised head by head first, by the lanes that share the row; the prompt
+// above takes 27.8 us then.
+template <int D, bool FP8, bool AT, bool NORM>
 __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
 #pragma clang fp contract(off)
   constexpr int kChunks = D / 16;
@@ -852,15 +949,20 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
     const int64_t b = bt / static_cast<uint32_t>(a.t);
     const int i = static_cast<int>(bt % static_cast<uint32_t>(a.t));
     const Span span = span_of(a.kv, b, a.t);
-    const int64_t pos = static_cast<int64_t>(span.start) + i;
-    const bool here = i < span.count && pos < a.positions;
-    Rotation<D, 8> turn;
+    int64_t pos = static_cast<int64_t>(span.start) + i;
+    if (AT && a.at && i < span.count) pos = a.at[b * a.at_stride + i];
+    const bool here = i < span.count && pos < a.positions && (!AT || pos >= 0);
+    Rotation<D, 8, NORM> turn;
     if (here) turn.load(a.cos + pos * D, a.sin + pos * D, d0);
+    if (NORM) turn.load_weights(a.q_weight, d0);
     const uint16_t *from = a.q + b * a.q_stride[0] + i * a.q_stride[1];
     uint16_t *to = a.q_out + static_cast<int64_t>(bt) * a.heads * D + d0;
     for (int head = h0; head < min(h0 + a.heads_each, a.heads); ++head) {
       float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (here) turn.apply(from + head * a.q_stride[2], d0, y);
+      if (here) {
+        const uint16_t *x = from + head * a.q_stride[2];
+        turn.apply(x, d0, y, NORM ? turn.factor(x, d0, a.eps) : 1.f);
+      }
       *reinterpret_cast<u32x4 *>(to + head * D) =
           (u32x4){pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7])};
     }
@@ -879,7 +981,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
   const int nth = uniform(rest % static_cast<uint32_t>(a.seq_blocks));
   const int64_t b = uniform(rest / static_cast<uint32_t>(a.seq_blocks));
   Span span = span_of(a.kv, b, a.t);
-  span.count = static_cast<int>(least(span.count, a.positions > span.start ? a.positions - span.start : 0));
+  if (!AT || !a.at)
+    span.count = static_cast<int>(least(span.count, a.positions > span.start ? a.positions - span.start : 0));
   const int block = span.start / kKvBlock + nth;
   const int lo = max(span.start, block * kKvBlock);  // the new tokens of this block: lo .. hi - 1
   const int hi = min(span.start + span.count, (block + 1) * kKvBlock);
@@ -895,20 +998,27 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
   const bool fresh = here && pos >= lo && pos < hi;
   const bool older = here && pos < lo;
   const int64_t i = pos - span.start;
+  int64_t at = pos;
+  if (AT && a.at && fresh) at = a.at[b * a.at_stride + i];
+  const bool placed = !AT || (at >= 0 && at < a.positions);  // has a row of the tables
   const uint16_t *x = side == 0 ? a.k + b * a.k_stride[0] + i * a.k_stride[1] : a.v + b * a.v_stride[0] + i * a.v_stride[1];
   const int64_t head_stride = side == 0 ? a.k_stride[2] : a.v_stride[2];
-  Rotation<D, 16> turn;
-  if (fresh && side == 0)
-    turn.load(a.cos + static_cast<int64_t>(pos) * D, a.sin + static_cast<int64_t>(pos) * D, 16 * chunk);
+  Rotation<D, 16, NORM> turn;
+  if (fresh && side == 0 && placed) turn.load(a.cos + at * D, a.sin + at * D, 16 * chunk);
+  if (NORM && side == 0) turn.load_weights(a.k_weight, 16 * chunk);
 
   for (int head = h0; head < min(h0 + a.heads_each, a.kv.kv_heads); ++head) {
     const int64_t index = block_index(a.kv, page, side, head, block);
     uint8_t *codes = a.codes + index * (kKvBlock * D);
     float y[16];
     float largest = 0.f;
-    if (fresh) {
+    if (AT && fresh && !placed) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) y[j] = 0.f;
+    } else if (fresh) {
       if (side == 0) {
-        turn.apply(x + head * head_stride, 16 * chunk, y);
+        const uint16_t *from = x + head * head_stride;
+        turn.apply(from, 16 * chunk, y, NORM ? turn.factor(from, 16 * chunk, a.eps) : 1.f);
       } else {
         const uint16_t *from = x + head * head_stride + 16 * chunk;
         const u32x4 w0 = *reinterpret_cast<const u32x4 *>(from), w1 = *reinterpret_cast<const u32x4 *>(from + 8);
@@ -975,6 +1085,102 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
     }
     __syncthreads();  // every thread has read the old scale and is through with the shared arrays
     if (threadIdx.x == 0) a.scales[index] = scale;
+  }
+}
+
+// ---- keeping the accepted nodes of a tree ---------------------------------------------------------------------------
+//
+// Token i of a sequence's path, which lies at start + path[i], moves to start + i, in every layer. The blocks that the
+// path reaches into are read into LDS, three at most, and the ones that its tokens move to are made from there, so that
+// none is read after it was written. A block's new scale is the largest of those that its tokens had (of the older ones
+// too); codes that had another are rounded again, and what lies behind the last token becomes 0. A workgroup a head and
+// side of a layer. 32 sequences x 80 layers (8 heads of 128, int8) take 163 us, 4.2 TB/s of the blocks read and written.
+template <int D, bool FP8>
+__global__ __launch_bounds__(2 * D) void kv8_keep_kernel(Kv8Keep a) {
+#pragma clang fp contract(off)
+  constexpr int kBytes = kKvBlock * D, kSources = 3;
+  __shared__ __align__(16) uint8_t from[kSources][kBytes];
+  __shared__ int16_t place[kSources][kKvBlock];  // where a token's codes begin in `from`, or -1
+  uint32_t item = blockIdx.x;
+  const int side = static_cast<int>(item & 1);
+  item >>= 1;
+  const int head = uniform(item % static_cast<uint32_t>(a.kv.kv_heads));
+  item /= static_cast<uint32_t>(a.kv.kv_heads);
+  const int64_t b = uniform(item % static_cast<uint32_t>(a.batch));
+  const int64_t layer = uniform(item / static_cast<uint32_t>(a.batch));
+  const int lane = threadIdx.x & (kWave - 1);
+  const Span span = span_of(a.kv, b, a.n);
+  // the path ends where it does not ascend or leaves the tree or the table
+  const int node = lane < span.count ? a.path[b * a.path_stride + lane] : 0;
+  const int before = __shfl_up(node, 1);
+  const int capacity = a.kv.width * a.kv.page_blocks * kKvBlock;
+  const bool good = lane < span.count && node >= lane && node < 64 && node < capacity - span.start &&
+                    (lane == 0 || node > before);
+  const uint64_t stop = __ballot(!good);
+  const int count = stop ? __builtin_ctzll(stop) : 64;
+  if (count == 0) return;
+  const int first = span.start / kKvBlock, last = (span.start + count - 1) / kKvBlock;
+  const int reach = (span.start + __builtin_amdgcn_readlane(node, count - 1)) / kKvBlock;
+  const int64_t layer_block = layer * a.kv.pages * 2 * a.kv.kv_heads * a.kv.page_blocks;
+
+  int64_t index[kSources];
+  float scale[kSources];
+#pragma unroll
+  for (int j = 0; j < kSources; ++j) {
+    const int page = first + j <= reach ? page_of(a.kv, b, first + j) : -1;
+    index[j] = page < 0 ? -1 : layer_block + block_index(a.kv, page, side, head, first + j);
+    scale[j] = index[j] < 0 ? 0.f : a.scales[index[j]];
+    u32x4 w = {0u, 0u, 0u, 0u};  // a hole holds zeros
+    if (index[j] >= 0) w = *reinterpret_cast<const u32x4 *>(a.codes + index[j] * kBytes + threadIdx.x * 16);
+    *reinterpret_cast<u32x4 *>(from[j] + threadIdx.x * 16) = w;
+  }
+  // a lane a token of the block (both halves of the wave the same ones)
+  float largest[kSources];
+#pragma unroll
+  for (int j = 0; j < kSources; ++j) {
+    const int token = (first + j) * kKvBlock + lane % kKvBlock, nth = token - span.start;
+    const int moved = span.start + __shfl(node, min(max(nth, 0), 63));
+    const int source = nth < 0 ? token : moved;
+    const bool used = nth < count;
+    const int block = source / kKvBlock - first;
+    float of = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSources; ++i)
+      if (used && block == i) of = scale[i];
+#pragma unroll
+    for (int m = 1; m < kKvBlock; m *= 2) of = fmaxf(of, __shfl_xor(of, m));
+    largest[j] = of;
+    if (threadIdx.x < kKvBlock)
+      place[j][lane] = static_cast<int16_t>(used ? block * kBytes + source % kKvBlock * (side == 0 ? 16 : 1) : -1);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kSources; ++j) {
+    if (first + j > last || index[j] < 0) continue;
+    const float made = largest[j], inverse = made > 0.f ? 1.0f / made : 0.f;
+    float ratio[kSources];
+#pragma unroll
+    for (int i = 0; i < kSources; ++i) ratio[i] = made > scale[i] ? scale[i] * inverse : 1.0f;
+    const auto ratio_of = [&](int at) { return at < kBytes ? ratio[0] : at < 2 * kBytes ? ratio[1] : ratio[2]; };
+    const uint8_t *codes = &from[0][0];
+    float y[16];
+    if (side == 0) {  // 16 values of one token
+      const int at = place[j][threadIdx.x % kKvBlock];
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        y[e] = at < 0 ? 0.f : code_value<FP8>(codes[at + threadIdx.x / kKvBlock * (16 * kKvBlock) + e]) * ratio_of(at);
+    } else {  // one value of 16 tokens
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int at = place[j][threadIdx.x % 2 * 16 + e];
+        y[e] = at < 0 ? 0.f : code_value<FP8>(codes[at + threadIdx.x / 2 * kKvBlock]) * ratio_of(at);
+      }
+    }
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = code4<FP8>(y + 4 * e);
+    *reinterpret_cast<u32x4 *>(a.codes + index[j] * kBytes + threadIdx.x * 16) = w;
+    if (threadIdx.x == 0) a.scales[index[j]] = made;
   }
 }
 
@@ -1060,9 +1266,15 @@ void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, int cus, int xcds) 
   p->part_bytes = p->splits > 1 ? static_cast<size_t>(items) * p->tile_rows * (p->kv.d + 2) * sizeof(float) : 0;
 }
 
+template <bool TREE>
+hipError_t launch_attention_over(const Kv8Attention &p, hipStream_t stream) {
+  if (p.kv.d == 128)
+    return p.kv.fp8 ? launch_attend<128, true, TREE>(p, stream) : launch_attend<128, false, TREE>(p, stream);
+  return p.kv.fp8 ? launch_attend<64, true, TREE>(p, stream) : launch_attend<64, false, TREE>(p, stream);
+}
+
 hipError_t launch_kv8_attention(const Kv8Attention &p, hipStream_t stream) {
-  if (p.kv.d == 128) return p.kv.fp8 ? launch_attend<128, true>(p, stream) : launch_attend<128, false>(p, stream);
-  return p.kv.fp8 ? launch_attend<64, true>(p, stream) : launch_attend<64, false>(p, stream);
+  return p.tree ? launch_attention_over<true>(p, stream) : launch_attention_over<false>(p, stream);
 }
 
 void plan_kv8_append(Kv8Append *p, int cus) {
@@ -1075,21 +1287,40 @@ void plan_kv8_append(Kv8Append *p, int cus) {
   p->query_items = row_items * ((p->heads + p->heads_each - 1) / p->heads_each);
 }
 
+template <bool AT, bool NORM>
+void start_append(const Kv8Append &p, dim3 grid, dim3 block, hipStream_t stream) {
+  if (p.kv.d == 128) {
+    if (p.kv.fp8) hipLaunchKernelGGL((kv8_append_kernel<128, true, AT, NORM>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((kv8_append_kernel<128, false, AT, NORM>), grid, block, 0, stream, p);
+  } else {
+    if (p.kv.fp8) hipLaunchKernelGGL((kv8_append_kernel<64, true, AT, NORM>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((kv8_append_kernel<64, false, AT, NORM>), grid, block, 0, stream, p);
+  }
+}
+
 hipError_t launch_kv8_append(const Kv8Append &p, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(p.block_items + p.query_items)), block(256);
-  if (p.kv.d == 128) {
-    if (p.kv.fp8) hipLaunchKernelGGL((kv8_append_kernel<128, true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((kv8_append_kernel<128, false>), grid, block, 0, stream, p);
-  } else {
-    if (p.kv.fp8) hipLaunchKernelGGL((kv8_append_kernel<64, true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((kv8_append_kernel<64, false>), grid, block, 0, stream, p);
-  }
+  if (p.q_weight) start_append<true, true>(p, grid, block, stream);
+  else if (p.at) start_append<true, false>(p, grid, block, stream);
+  else start_append<false, false>(p, grid, block, stream);
   return hipGetLastError();
 }
 
 hipError_t launch_kv8_copy(const Kv8Copy &p, hipStream_t stream) {
   hipLaunchKernelGGL(kv8_copy_kernel, dim3(static_cast<unsigned>(p.layers) * p.n * p.pieces), dim3(256), kLdsToken,
                      stream, p);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv8_keep(const Kv8Keep &p, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(p.layers * p.batch * p.kv.kv_heads * 2)), block(2 * p.kv.d);
+  if (p.kv.d == 128) {
+    if (p.kv.fp8) hipLaunchKernelGGL((kv8_keep_kernel<128, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((kv8_keep_kernel<128, false>), grid, block, 0, stream, p);
+  } else {
+    if (p.kv.fp8) hipLaunchKernelGGL((kv8_keep_kernel<64, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((kv8_keep_kernel<64, false>), grid, block, 0, stream, p);
+  }
   return hipGetLastError();
 }
 

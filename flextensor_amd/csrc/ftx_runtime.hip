@@ -1478,6 +1478,16 @@ int kv8_pages(const ftx_kv8_cache *c, int64_t batch, int64_t t, int heads, ftx::
   return FTX_OK;
 }
 
+// Rows [batch][n] of integers, `stride` apart; 0, where `shared`, is one row for all.
+int check_rows(const void *ptr, int64_t stride, int64_t batch, int64_t n, int64_t item, const char *what,
+               bool shared = false) {
+  if (!ptr || reinterpret_cast<uintptr_t>(ptr) % item != 0)
+    return ftx::fail(FTX_ERR_INVALID, std::string(what) + " is null or not aligned");
+  if ((stride < n && !(shared && stride == 0)) || stride > (int64_t(1) << 32))
+    return ftx::fail(FTX_ERR_INVALID, std::string(what) + ": rows must not overlap");
+  return ftx::check_device_range(ptr, static_cast<size_t>(((batch - 1) * stride + n) * item), what);
+}
+
 int check_view(const void *ptr, const int64_t *stride, int64_t n0, int64_t n1, int64_t n2, int64_t d, const char *what,
                int64_t *out) {
   const int64_t extent = view_extent(stride, n0, n1, n2, d);
@@ -1506,11 +1516,21 @@ int plan_kv8(int64_t max_tokens, ftx::Kv8Attention *p) {
 int ftx_kv8_append(const ftx_kv8_cache *cache, const void *q, const void *k, const void *v, const float *cos,
                    const float *sin, int64_t positions, void *q_out, int64_t batch, int64_t t, int heads,
                    const int64_t *strides, void *stream) {
+  return ftx_kv8_append_norm(cache, q, k, v, nullptr, nullptr, 0.f, cos, sin, positions, nullptr, 0, q_out, batch, t,
+                             heads, strides, stream);
+}
+
+int ftx_kv8_append_norm(const ftx_kv8_cache *cache, const void *q, const void *k, const void *v, const void *q_weight,
+                        const void *k_weight, float eps, const float *cos, const float *sin, int64_t positions,
+                        const int32_t *at, int64_t at_stride, void *q_out, int64_t batch, int64_t t, int heads,
+                        const int64_t *strides, void *stream) {
   FTX_REQUIRE_LIVE();
   ftx::Kv8Append p{};
   int rc = kv8_pages(cache, batch, t, heads, &p.kv);
   if (rc != FTX_OK) return rc;
   if (positions < 0 || positions > (int64_t(1) << 40)) return ftx::fail(FTX_ERR_INVALID, "rotary positions");
+  if (!q_weight != !k_weight) return ftx::fail(FTX_ERR_INVALID, "append takes norm weights for both q and k, or none");
+  if (q_weight && !(eps >= 0.f && eps < INFINITY)) return ftx::fail(FTX_ERR_INVALID, "append needs a finite eps, not negative");
   if (batch == 0 || t == 0) return FTX_OK;
   if (!strides) return ftx::fail(FTX_ERR_INVALID, "strides is null");
   const int d = cache->d, kv = cache->kv_heads;
@@ -1520,7 +1540,15 @@ int ftx_kv8_append(const ftx_kv8_cache *cache, const void *q, const void *k, con
   if (rc == FTX_OK) rc = check_operand(q_out, batch * t * heads * d, 2, "append q output");
   if (rc == FTX_OK && positions > 0) rc = check_operand(cos, positions * d, 4, "rotary cos");
   if (rc == FTX_OK && positions > 0) rc = check_operand(sin, positions * d, 4, "rotary sin");
+  if (rc == FTX_OK && q_weight) rc = check_operand(q_weight, d, 2, "append q norm weight");
+  if (rc == FTX_OK && k_weight) rc = check_operand(k_weight, d, 2, "append k norm weight");
+  if (rc == FTX_OK && at) rc = check_rows(at, at_stride, batch, t, 4, "rotary rows");
   if (rc != FTX_OK) return rc;
+  p.q_weight = static_cast<const uint16_t *>(q_weight);
+  p.k_weight = static_cast<const uint16_t *>(k_weight);
+  p.eps = eps;
+  p.at = at;
+  p.at_stride = at_stride;
   p.codes = static_cast<uint8_t *>(cache->codes);
   p.scales = cache->scales;
   p.q = static_cast<const uint16_t *>(q);
@@ -1567,9 +1595,12 @@ int ftx_kv8_attention_workspace(int64_t batch, int64_t t, int heads, int kv_head
   return rc;
 }
 
-int ftx_kv8_attention(const ftx_kv8_cache *cache, const void *q, void *o, int64_t batch, int64_t t, int heads,
-                      const int64_t *strides, float scale, int64_t max_tokens, void *workspace, size_t workspace_bytes,
-                      void *stream) {
+namespace {
+
+// tree: null, or the rows' sets of nodes.
+int kv8_attention(const ftx_kv8_cache *cache, const void *q, void *o, const int64_t *tree, int64_t tree_stride, int nodes,
+                  int64_t batch, int64_t t, int heads, const int64_t *strides, float scale, int64_t max_tokens,
+                  void *workspace, size_t workspace_bytes, void *stream) {
   FTX_REQUIRE_LIVE();
   ftx::Kv8Attention p{};
   int rc = kv8_pages(cache, batch, t, heads, &p.kv);
@@ -1580,7 +1611,11 @@ int ftx_kv8_attention(const ftx_kv8_cache *cache, const void *q, void *o, int64_
   if (!strides) return ftx::fail(FTX_ERR_INVALID, "strides is null");
   rc = check_view(q, strides, batch, t, heads, cache->d, "attention q", p.q_stride);
   if (rc == FTX_OK) rc = check_view(o, strides + 3, batch, t, heads, cache->d, "attention o", p.o_stride);
+  if (rc == FTX_OK && tree) rc = check_rows(tree, tree_stride, batch, t, 8, "tree", true);
   if (rc != FTX_OK) return rc;
+  p.tree = tree;
+  p.tree_stride = tree_stride;
+  p.nodes = nodes;
   p.q = static_cast<const uint16_t *>(q);
   p.o = static_cast<uint16_t *>(o);
   p.batch = static_cast<int>(batch);
@@ -1598,6 +1633,50 @@ int ftx_kv8_attention(const ftx_kv8_cache *cache, const void *q, void *o, int64_
     p.part = static_cast<float *>(workspace);
   }
   FTX_HIP(ftx::launch_kv8_attention(p, static_cast<hipStream_t>(stream)));
+  return FTX_OK;
+}
+
+}  // namespace
+
+int ftx_kv8_attention(const ftx_kv8_cache *cache, const void *q, void *o, int64_t batch, int64_t t, int heads,
+                      const int64_t *strides, float scale, int64_t max_tokens, void *workspace, size_t workspace_bytes,
+                      void *stream) {
+  return kv8_attention(cache, q, o, nullptr, 0, 0, batch, t, heads, strides, scale, max_tokens, workspace,
+                       workspace_bytes, stream);
+}
+
+int ftx_kv8_tree_attention(const ftx_kv8_cache *cache, const void *q, void *o, const int64_t *tree, int64_t tree_stride,
+                           int nodes, int64_t batch, int64_t t, int heads, const int64_t *strides, float scale,
+                           int64_t max_tokens, void *workspace, size_t workspace_bytes, void *stream) {
+  if (nodes < 0 || nodes > 64) return ftx::fail(FTX_ERR_INVALID, "a tree has 0 to 64 nodes");
+  if (!tree && batch > 0 && t > 0) return ftx::fail(FTX_ERR_INVALID, "tree is null");
+  return kv8_attention(cache, q, o, tree, tree_stride, nodes, batch, t, heads, strides, scale, max_tokens, workspace,
+                       workspace_bytes, stream);
+}
+
+int ftx_kv8_keep(const ftx_kv8_cache *cache, int64_t layers, const int32_t *path, int64_t path_stride, int64_t batch,
+                 int64_t n, void *stream) {
+  FTX_REQUIRE_LIVE();
+  ftx::Kv8Keep p{};
+  int rc = kv8_pages(cache, layers == 0 ? 0 : batch, n, cache ? cache->kv_heads : 0, &p.kv);
+  if (rc != FTX_OK) return rc;
+  if (layers < 0 || layers > 65536 || n > 64) return ftx::fail(FTX_ERR_INVALID, "keep takes up to 65536 layers and 64 nodes");
+  if (layers == 0 || batch == 0 || n == 0) return FTX_OK;
+  if (layers > ftx::kMaxThreads / 256 / (batch * cache->kv_heads * 2))
+    return ftx::fail(FTX_ERR_UNSUPPORTED, "keep: more workgroups than one launch holds");
+  const int64_t blocks = layers * cache->pages * 2 * cache->kv_heads * p.kv.page_blocks;
+  rc = check_operand(cache->codes, blocks, ftx::kKvBlock * cache->d, "cache codes");
+  if (rc == FTX_OK) rc = check_operand(cache->scales, blocks, 4, "cache scales");
+  if (rc == FTX_OK) rc = check_rows(path, path_stride, batch, n, 4, "path");
+  if (rc != FTX_OK) return rc;
+  p.codes = static_cast<uint8_t *>(cache->codes);
+  p.scales = cache->scales;
+  p.layers = layers;
+  p.path = path;
+  p.path_stride = path_stride;
+  p.batch = static_cast<int>(batch);
+  p.n = static_cast<int>(n);
+  FTX_HIP(ftx::launch_kv8_keep(p, static_cast<hipStream_t>(stream)));
   return FTX_OK;
 }
 
@@ -1643,6 +1722,156 @@ int ftx_kv8_copy_pages(void *codes, float *scales, int64_t layers, int64_t pages
     for (uint32_t i = 0; i < p.n; ++i) p.pair[i] = {src[i0 + i], dst[i0 + i]};
     FTX_HIP(ftx::launch_kv8_copy(p, static_cast<hipStream_t>(stream)));
   }
+  return FTX_OK;
+}
+
+namespace {
+
+int plan_int4(int64_t m, int64_t n, int64_t k, int group, ftx::Int4Linear *p) {
+  if (group != 32 && group != 64 && group != 128)
+    return ftx::fail(FTX_ERR_UNSUPPORTED, "the int4 linear has groups of 32, 64 or 128 inputs");
+  if (m < 0 || n < 0 || k < 1) return ftx::fail(FTX_ERR_INVALID, "int4 linear dimensions");
+  if (k % group != 0 || k > ftx::kInt4MaxK)
+    return ftx::fail(FTX_ERR_UNSUPPORTED, "the int4 linear needs k to be a multiple of the group, at most 2^20");
+  if (m > (int64_t(1) << 40) || n > (int64_t(1) << 36) || (n > 0 && m > (int64_t(1) << 40) / n))
+    return ftx::fail(FTX_ERR_INVALID, "int4 linear dimensions too large");
+  p->m = m;
+  p->n = n;
+  p->k = static_cast<int>(k);
+  p->parts = ftx::kInt4Unit / group;
+  int cus = 256, xcds = 8;
+  ftx::DeviceState *st = nullptr;
+  if (ftx::device_state(&st) == FTX_OK) {
+    cus = st->cu_count;
+    xcds = st->xcd_count;
+  }
+  ftx::plan_int4_linear(p, cus, xcds);
+  const int64_t join = p->splits > 1 ? m * p->part_stride / 4 : 0;
+  if (static_cast<int64_t>(p->items) + p->xcds > ftx::kMaxThreads / 512 || join > ftx::kMaxThreads - 256)
+    return ftx::fail(FTX_ERR_UNSUPPORTED, "int4 linear: more workgroups than one launch holds");
+  return FTX_OK;
+}
+
+}  // namespace
+
+int ftx_int4_linear_workspace(int64_t m, int64_t n, int64_t k, int group, size_t *bytes) {
+  if (!bytes) return ftx::fail(FTX_ERR_INVALID, "bytes is null");
+  ftx::Int4Linear p{};
+  int rc = plan_int4(m, n, k, group, &p);
+  if (rc == FTX_OK) *bytes = m == 0 || n == 0 ? 0 : p.part_bytes;
+  return rc;
+}
+
+int ftx_int4_linear(const void *x, int64_t x_stride, const void *w, const void *scale, const void *zero, void *y,
+                    int64_t m, int64_t n, int64_t k, int group, void *workspace, size_t workspace_bytes, void *stream) {
+  FTX_REQUIRE_LIVE();
+  ftx::Int4Linear p{};
+  int rc = plan_int4(m, n, k, group, &p);
+  if (rc != FTX_OK) return rc;
+  if (x_stride < k || x_stride % 8 != 0 || x_stride > ftx::kInt4MaxStride)
+    return ftx::fail(FTX_ERR_INVALID, "int4 linear: rows of x must not overlap and start at multiples of 8 elements, at "
+                                      "most 2^21");
+  if (m == 0 || n == 0) return FTX_OK;
+  const int64_t cells = p.tiles * p.units;
+  rc = check_operand(x, (m - 1) * x_stride + k, 2, "int4 input");
+  if (rc == FTX_OK) rc = check_operand(w, cells, FTX_INT4_TILE * FTX_INT4_UNIT / 2, "int4 weight");
+  if (rc == FTX_OK) rc = check_operand(scale, cells * FTX_INT4_TILE * p.parts, 2, "int4 scales");
+  if (rc == FTX_OK && zero) rc = check_operand(zero, cells * FTX_INT4_TILE * p.parts, 2, "int4 zeros");
+  if (rc == FTX_OK) rc = check_operand(y, m * n, 2, "int4 output");
+  if (rc != FTX_OK) return rc;
+  if (p.part_bytes > 0) {
+    if (workspace_bytes < p.part_bytes)
+      return ftx::fail(FTX_ERR_INVALID, "the int4 linear needs a workspace of " + std::to_string(p.part_bytes) +
+                                            " bytes (ftx_int4_linear_workspace)");
+    rc = check_operand(workspace, static_cast<int64_t>(p.part_bytes), 1, "int4 workspace");
+    if (rc != FTX_OK) return rc;
+    p.part = static_cast<float *>(workspace);
+  }
+  p.x = static_cast<const uint16_t *>(x);
+  p.x_stride = x_stride;
+  p.w = static_cast<const uint8_t *>(w);
+  p.scale = static_cast<const uint16_t *>(scale);
+  p.zero = static_cast<const uint16_t *>(zero);
+  p.y = static_cast<uint16_t *>(y);
+  FTX_HIP(ftx::launch_int4_linear(p, static_cast<hipStream_t>(stream)));
+  return FTX_OK;
+}
+
+namespace {
+
+int plan_token_logprobs(int64_t rows, int64_t vocab, int type, int top, ftx::Logprobs *p) {
+  if (type != FTX_LOGITS_BF16 && type != FTX_LOGITS_FP16 && type != FTX_LOGITS_FP32)
+    return ftx::fail(FTX_ERR_INVALID, "unknown type of logits");
+  if (rows < 0 || vocab < 1 || vocab > ftx::kLogprobsMaxVocab || rows > (int64_t(1) << 40) / vocab)
+    return ftx::fail(FTX_ERR_INVALID, "token logprobs dimensions");
+  if (top < 0 || top > ftx::kLogprobsMaxTop || top > vocab)
+    return ftx::fail(FTX_ERR_INVALID, "token logprobs give the 0 to 64 likeliest tokens, no more than the vocabulary");
+  p->rows = rows;
+  p->vocab = vocab;
+  p->type = type;
+  p->top = top;
+  int cus = 256;
+  ftx::DeviceState *st = nullptr;
+  if (ftx::device_state(&st) == FTX_OK) cus = st->cu_count;
+  if (rows == 0) return FTX_OK;
+  ftx::plan_logprobs(p, cus);
+  if (rows > ftx::kMaxThreads / p->threads / p->splits)
+    return ftx::fail(FTX_ERR_UNSUPPORTED, "token logprobs: more rows than one launch holds");
+  return FTX_OK;
+}
+
+}  // namespace
+
+int ftx_token_logprobs_workspace(int64_t rows, int64_t vocab, int type, int top, size_t *bytes) {
+  if (!bytes) return ftx::fail(FTX_ERR_INVALID, "bytes is null");
+  ftx::Logprobs p{};
+  int rc = plan_token_logprobs(rows, vocab, type, top, &p);
+  if (rc == FTX_OK) *bytes = p.part_bytes;
+  return rc;
+}
+
+int ftx_token_logprobs(const void *logits, int64_t row_stride, int type, const int64_t *tokens, int64_t rows,
+                       int64_t vocab, int top, float *logprob, float *entropy, float *top_logprob, int64_t *top_token,
+                       void *workspace, size_t workspace_bytes, void *stream) {
+  FTX_REQUIRE_LIVE();
+  ftx::Logprobs p{};
+  int rc = plan_token_logprobs(rows, vocab, type, top, &p);
+  if (rc != FTX_OK) return rc;
+  if (rows == 0) return FTX_OK;
+  if (row_stride < 0 || row_stride > (int64_t(1) << 40) / rows)
+    return ftx::fail(FTX_ERR_INVALID, "token logprobs: the stride of the rows");
+  const int item = type == FTX_LOGITS_FP32 ? 4 : 2;
+  const struct { const void *p; int64_t n, item; const char *what; } parts[6] = {
+      {logits, (rows - 1) * row_stride + vocab, item, "logits"},
+      {tokens, rows, 8, "tokens"},
+      {logprob, rows, 4, "log probabilities"},
+      {entropy, rows, 4, "entropies"},
+      {top_logprob, rows * top, 4, "top log probabilities"},
+      {top_token, rows * top, 8, "top tokens"}};
+  for (const auto &v : parts) {
+    if (v.n == 0) continue;
+    if (!v.p || reinterpret_cast<uintptr_t>(v.p) % v.item != 0)
+      return ftx::fail(FTX_ERR_INVALID, std::string(v.what) + " is null or not aligned");
+    rc = ftx::check_device_range(v.p, static_cast<size_t>(v.n * v.item), v.what);
+    if (rc != FTX_OK) return rc;
+  }
+  if (p.part_bytes > 0) {
+    if (workspace_bytes < p.part_bytes)
+      return ftx::fail(FTX_ERR_INVALID, "token logprobs need a workspace of " + std::to_string(p.part_bytes) +
+                                            " bytes (ftx_token_logprobs_workspace)");
+    rc = check_operand(workspace, static_cast<int64_t>(p.part_bytes), 1, "logprobs workspace");
+    if (rc != FTX_OK) return rc;
+    p.part = static_cast<float4 *>(workspace);
+    p.part_keys = reinterpret_cast<unsigned long long *>(p.part + rows * p.splits);
+  }
+  p.logits = logits;
+  p.row_stride = row_stride;
+  p.tokens = tokens;
+  p.logprob = logprob;
+  p.entropy = entropy;
+  p.top_logprob = top_logprob;
+  p.top_token = top_token;
+  FTX_HIP(ftx::launch_logprobs(p, static_cast<hipStream_t>(stream)));
   return FTX_OK;
 }
 

@@ -892,6 +892,163 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor) -> t
     return y
 
 
+INT4_GROUPS = (32, 64, 128)
+INT4_MAX_K = 1 << 20
+_INT4_MAX_STRIDE = 1 << 21
+
+
+def int4_pack(codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None = None
+              ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """``(weight, scale, zero)`` as :func:`int4_linear` takes them, of codes [n, k] (0 .. 15, any integer type) and bf16
+    scales and zeros [n, k / group]: weights ``scale * (code - zero)``, a zero of None standing for 8.
+
+    The codes lie in tiles of 16 channels and units of 128 inputs, in the order of the matrix cores' operands
+    (``include/ftx.h``); what fills the last ones is 0.
+    """
+    if codes.dim() != 2 or scale.dim() != 2 or codes.is_floating_point():
+        raise ValueError(f"int4_pack takes codes [n, k] and scales [n, k / group], got {tuple(codes.shape)} "
+                         f"{codes.dtype} and {tuple(scale.shape)}")
+    n, k = codes.shape
+    group = k // max(1, scale.shape[1])
+    if group not in INT4_GROUPS or scale.shape != (n, k // group) or k % group:
+        raise ValueError(f"int4_pack needs scales [{n}, {k} / group] for a group of 32, 64 or 128, got {tuple(scale.shape)}")
+    for name, t in (("scale", scale), ("zero", zero)):
+        if t is not None and (t.dtype != torch.bfloat16 or t.shape != scale.shape):
+            raise ValueError(f"int4_pack needs a bf16 {name} {tuple(scale.shape)}, got {tuple(t.shape)} {t.dtype}")
+    if n and (int(codes.min()) < 0 or int(codes.max()) > 15):
+        raise ValueError("int4_pack needs codes of 0 to 15")
+    tiles, units = -(-n // nat.INT4_TILE), -(-k // nat.INT4_UNIT)
+    c = torch.zeros(tiles * nat.INT4_TILE, units * nat.INT4_UNIT, dtype=torch.uint8, device=codes.device)
+    c[:n, :k] = codes.to(torch.uint8)
+    # [tile, channel, unit, i, q, j / 2, j % 2, half] -> bytes of [tile, unit, q, channel, i, half, j / 2]
+    c = c.view(tiles, 16, units, 4, 4, 2, 2, 2).permute(0, 2, 4, 1, 3, 7, 5, 6)
+    weight = (c[..., 0] | c[..., 1] << 4).reshape(tiles, units, 1024)
+
+    def of_units(t: torch.Tensor) -> torch.Tensor:
+        parts = nat.INT4_UNIT // group
+        full = torch.zeros(tiles * 16, units * parts, dtype=torch.bfloat16, device=t.device)
+        full[:n, : k // group] = t
+        return full.view(tiles, 16, units, parts).transpose(1, 2).contiguous()
+
+    return weight, of_units(scale), of_units(zero) if zero is not None else None
+
+
+def int4_dequantize(weight: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None, n: int, k: int) -> torch.Tensor:
+    """The fp32 weights [n, k] that :func:`int4_pack`'s tensors stand for (torch operations, on any device)."""
+    tiles, units, parts = weight.shape[0], weight.shape[1], scale.shape[3]
+    c = torch.stack((weight & 15, weight >> 4), -1).view(tiles, units, 4, 16, 4, 2, 2, 2)
+    c = c.permute(0, 3, 1, 4, 2, 6, 7, 5).reshape(tiles, 16, units, parts, nat.INT4_UNIT // parts).float()
+    z = zero.float().transpose(1, 2).unsqueeze(-1) if zero is not None else 8.0
+    w = (c - z) * scale.float().transpose(1, 2).unsqueeze(-1)
+    return w.reshape(tiles * 16, units * nat.INT4_UNIT)[:n, :k]
+
+
+def int4_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None = None,
+                n: int | None = None) -> torch.Tensor:
+    """``x @ w.T`` of bf16 rows [m, k] and the 4-bit weights ``w = scale * (code - zero)`` of :func:`int4_pack`
+    (``ftx_int4_linear``), ``n`` channels of them (None: all that the tiles hold).
+
+    Up to 16 rows take the weights as they are; for more rows they are rounded to bf16, as a dequantised copy would be.
+    ``k`` is a multiple of the group; rows may be strided. A row that holds an infinity or a NaN gives infinities or NaNs.
+    No backward.
+    """
+    if x.is_cuda and torch.autograd.forward_ad._current_level < 0:
+        device = torch._C._cuda_getDevice()
+        got = nat.torch_calls().int4_linear(x, weight, scale, zero, n, device, _stream(device))
+        if got is not None:
+            return nat.result(got)
+    if x.dim() != 2:
+        raise ValueError(f"int4_linear takes rows [m, k], got {tuple(x.shape)}")
+    _check_operands("int4_linear", x=x)
+    for name, t, dtype, dims in (("weight", weight, torch.uint8, 3), ("scale", scale, torch.bfloat16, 4),
+                                 ("zero", zero, torch.bfloat16, 4)):
+        if t is None:
+            continue
+        if type(t) not in _PLAIN_TYPES or t.dtype != dtype:
+            raise TypeError(f"int4_linear needs a plain {dtype} {name}, got a {t.dtype} {type(t).__name__}")
+        if t.dim() != dims or not _packed(t) or t.get_device() != x.get_device():
+            raise ValueError(f"int4_linear needs a contiguous, 16-byte aligned {name} of {dims} dimensions on {x.device}, "
+                             f"got {tuple(t.shape)} on {t.device}")
+        _check_underived("int4_linear", **{name: t})
+    m, k = x.shape
+    tiles, units, _ = weight.shape
+    group = nat.INT4_UNIT // max(1, scale.shape[3])
+    if (weight.shape[2] != 1024 or group not in INT4_GROUPS or scale.shape != (tiles, units, 16, nat.INT4_UNIT // group)
+            or (zero is not None and zero.shape != scale.shape)):
+        raise ValueError(f"int4_linear takes what int4_pack returns, not a weight {tuple(weight.shape)} with scales "
+                         f"{tuple(scale.shape)}" + (f" and zeros {tuple(zero.shape)}" if zero is not None else ""))
+    if not 0 < k <= INT4_MAX_K or k % group or units != -(-k // nat.INT4_UNIT):
+        raise ValueError(f"int4_linear: rows of {k} values do not fit weights of {units} units in groups of {group}")
+    n = tiles * 16 if n is None else n
+    if -(-n // 16) != tiles or n < 0:
+        raise ValueError(f"int4_linear: {n} channels are not what {tiles} tiles of 16 hold")
+    stride, inner = x.stride()
+    if m <= 1:
+        stride = k
+    if inner != 1 or stride < k or stride % 8 or stride > _INT4_MAX_STRIDE or x.data_ptr() % 16:
+        x, stride = x.clone(memory_format=torch.contiguous_format), k
+    y = torch.empty((m, n), dtype=torch.bfloat16, device=x.device)
+    b = ctypes.c_size_t(0)
+    nat.call("ftx_int4_linear_workspace", m, n, k, group, ctypes.byref(b))
+    ws_bytes = int(b.value)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
+    nat.call("ftx_int4_linear", x.data_ptr(), stride, weight.data_ptr(), scale.data_ptr(),
+             zero.data_ptr() if zero is not None else None, y.data_ptr(), m, n, k, group,
+             ws.data_ptr() if ws is not None else None, ws_bytes, _stream())
+    return y
+
+
+LOGITS_TYPES = {torch.bfloat16: nat.LOGITS_BF16, torch.float16: nat.LOGITS_FP16, torch.float32: nat.LOGITS_FP32}
+LOGPROBS_MAX_TOP = 64
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0
+                   ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(logprob, entropy, top_logprobs, top_tokens)`` of rows of logits [rows, vocab] in one pass over them
+    (``ftx_token_logprobs``).
+
+    ``logprob``: log softmax of each row at its token (int64 [rows]); 0 for a negative token, NaN for one past the
+    vocabulary. ``entropy``: of each row, in nats. ``top_logprobs`` and ``top_tokens`` [rows, top]: the ``top`` (up to 64)
+    likeliest, the lowest index first among equal logits. Logits are bf16, fp16 or fp32, rows may be strided; the results
+    are fp32 and int64. Logits of -inf have no part in the sums; rows of nothing else, or with a NaN or +inf, have NaN for
+    log probabilities and entropy. No backward.
+    """
+    if logits.is_cuda and torch.autograd.forward_ad._current_level < 0:
+        device = torch._C._cuda_getDevice()
+        got = nat.torch_calls().token_logprobs(logits, tokens, top, device, _stream(device))
+        if got is not None:
+            return nat.result(got)
+    for name, t in (("logits", logits), ("tokens", tokens)):
+        if type(t) not in _PLAIN_TYPES:
+            raise TypeError(f"token_logprobs takes plain tensors, {name} is a {type(t).__name__}")
+    if logits.dtype not in LOGITS_TYPES or tokens.dtype != torch.int64:
+        raise TypeError(f"token_logprobs takes bf16, fp16 or fp32 logits and int64 tokens, got {logits.dtype} and "
+                        f"{tokens.dtype}")
+    if logits.dim() != 2 or tokens.shape != logits.shape[:1] or not logits.shape[1]:
+        raise ValueError(f"token_logprobs takes logits [rows, vocab] and a token for each row, got {tuple(logits.shape)} "
+                         f"and {tuple(tokens.shape)}")
+    if not isinstance(top, int) or not 0 <= top <= min(LOGPROBS_MAX_TOP, logits.shape[1]):
+        raise ValueError(f"token_logprobs gives the 0 to {LOGPROBS_MAX_TOP} likeliest of {logits.shape[1]} tokens, not {top}")
+    if not logits.is_cuda or logits.get_device() != torch._C._cuda_getDevice() or tokens.device != logits.device:
+        raise ValueError(f"token_logprobs runs on the current GPU, its input is on {logits.device} and {tokens.device}")
+    _check_underived("token_logprobs", logits=logits)
+    rows, vocab = logits.shape
+    if logits.stride(1) != 1 and vocab > 1:
+        logits = logits.contiguous()
+    tokens = tokens.contiguous()
+    kind, where = LOGITS_TYPES[logits.dtype], logits.device
+    out = [torch.empty(s, dtype=torch.float32, device=where) for s in ((rows,), (rows,), (rows, top))]
+    index = torch.empty((rows, top), dtype=torch.int64, device=where)
+    b = ctypes.c_size_t(0)
+    nat.call("ftx_token_logprobs_workspace", rows, vocab, kind, top, ctypes.byref(b))
+    ws_bytes = int(b.value)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=where) if ws_bytes else None
+    nat.call("ftx_token_logprobs", logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, kind, tokens.data_ptr(), rows,
+             vocab, top, *[t.data_ptr() or None for t in (*out, index)], ws.data_ptr() if ws is not None else None, ws_bytes,
+             _stream())
+    return (*out, index)
+
+
 BF16_LINEAR_MAX_ROWS = 16
 
 

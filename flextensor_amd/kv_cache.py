@@ -128,7 +128,8 @@ def _cache(what: str, q: torch.Tensor, device: int, codes: torch.Tensor, scales:
 
 def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
            codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor, starts: torch.Tensor,
-           new: torch.Tensor | None = None) -> torch.Tensor:
+           new: torch.Tensor | None = None, *, positions: torch.Tensor | None = None, q_norm: torch.Tensor | None = None,
+           k_norm: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
     """Writes new tokens into the cache and returns the rotated queries, in one launch (``ftx_kv8_append``).
 
     ``q``, ``k``, ``v``: bf16 [batch, t, heads or kv heads, d]; ``cos``, ``sin``: fp32 [positions, d], both halves.
@@ -137,10 +138,21 @@ def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
     older codes are rounded again when it does. Sequences with a negative start, tokens past the table or the rotary
     positions, and holes are left out; the queries of tokens left out are 0. :func:`attention` has no positions: it
     would see the places of tokens past the rotary tables. Two sequences of a call must not write into one page.
+
+    ``q_norm``, ``k_norm``: bf16 [d]; queries and keys are first normalised head by head, ``x / sqrt(mean(x^2) + eps)``
+    times these, in the same launch (``ftx_kv8_append_norm``). ``positions``: int32 [batch, t], the rows of the rotary
+    tables that tokens are turned by in place of their places' (nodes of a tree: the prefix's length and their depth); a
+    token of a position outside the tables becomes 0, in the cache too, and must not be attended to.
     """
     device = _device(q)
+    plain = positions is None and q_norm is None and k_norm is None
     if device >= 0 and torch.autograd.forward_ad._current_level < 0:
-        got = nat.torch_calls().append(q, k, v, cos, sin, codes, scales, table, starts, new, device, hip._stream(device))
+        stream = hip._stream(device)
+        if plain:
+            got = nat.torch_calls().append(q, k, v, cos, sin, codes, scales, table, starts, new, device, stream)
+        else:
+            got = nat.torch_calls().append_norm(q, k, v, cos, sin, codes, scales, table, starts, new, positions, q_norm,
+                                                k_norm, eps, device, stream)
         if got is not None:
             return nat.result(got)
     strides = _heads("append", device, q, k, v)
@@ -157,8 +169,28 @@ def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
                 (cos_ptr | sin_ptr) % 16):
             raise ValueError(f"append needs cos and sin [positions, {d}], contiguous, 16-byte aligned and on {q.device}")
     hip._check_underived("append", cos=cos, sin=sin)
+    if (q_norm is None) != (k_norm is None):
+        raise ValueError("append takes norm weights for both q and k, or none")
+    if q_norm is not None:
+        hip._check_operands("append", q_norm=q_norm, k_norm=k_norm)
+        if q_norm.shape != (d,) or k_norm.shape != (d,) or not hip._packed(q_norm, k_norm):
+            raise ValueError(f"append needs norm weights [{d}], contiguous and 16-byte aligned, got {tuple(q_norm.shape)} "
+                             f"and {tuple(k_norm.shape)}")
+        if not 0.0 <= eps < float("inf"):
+            raise ValueError(f"append needs a finite eps that is not negative, not {eps}")
+    if positions is not None:
+        _check_ints("append", "positions", positions, 2, b, device)
+        if positions.shape[1] != t:
+            raise ValueError(f"append needs a position for each of {t} tokens, got {tuple(positions.shape)}")
     torch._C._increment_version((codes, scales))  # as an in-place operation, for what autograd saved
     out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
+    if not plain:
+        nat.call("ftx_kv8_append_norm", ctypes.byref(cache), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                 *[w.data_ptr() if w is not None else None for w in (q_norm, k_norm)], eps, cos_ptr, sin_ptr, cos.shape[0],
+                 (positions.data_ptr() or None) if positions is not None else None,
+                 max(positions.stride(0), t) if positions is not None else 0, out.data_ptr(), b, t, h,
+                 _Strides9(*strides), hip._stream(device))
+        return out
     nat.call("ftx_kv8_append", ctypes.byref(cache), q.data_ptr(), k.data_ptr(), v.data_ptr(), cos_ptr, sin_ptr,
              cos.shape[0], out.data_ptr(), b, t, h, _Strides9(*strides), hip._stream(device))
     return out
@@ -203,6 +235,92 @@ def attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, table:
              _Strides6(*strides), d ** -0.5 if scale is None else scale, longest,
              ws.data_ptr() if ws is not None else None, ws_bytes, hip._stream(device))
     return out
+
+
+def tree_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor, starts: torch.Tensor,
+                   tree: torch.Tensor, new: torch.Tensor | None = None, *, nodes: int | None = None,
+                   max_tokens: int | None = None, scale: float | None = None) -> torch.Tensor:
+    """:func:`attention` of drafted tokens that form a tree (``ftx_kv8_tree_attention``).
+
+    ``starts[b]``: the first tokens of a sequence, which every row sees. The ``nodes`` tokens (None: t; at most 64) cached
+    after them are the tree's nodes, and ``tree`` (int64 [batch, t]) says which of them a row sees: bit j of
+    ``tree[b, i]`` the token ``starts[b] + j`` (one tree may be expanded over the batch). A row's own node is one of its bits, its ancestors the others; rows may be
+    a part of the nodes (a level of the tree). Rows from ``new[b]`` on, and rows that see no token, are 0. ``max_tokens``
+    counts the nodes. A NaN that a sequence's nodes hold may reach rows that do not see it.
+    """
+    device = _device(q)
+    if device >= 0 and torch.autograd.forward_ad._current_level < 0:
+        got = nat.torch_calls().tree_attention(q, codes, scales, table, starts, tree, new, nodes, max_tokens, scale, device,
+                                               hip._stream(device))
+        if got is not None:
+            return nat.result(got)
+    strides = _heads("tree_attention", device, q)
+    cache = _cache("tree_attention", q, device, codes, scales, table, starts, new)
+    b, t, h, d = q.shape
+    if type(tree) is not torch.Tensor or tree.dtype != torch.int64:
+        raise TypeError("tree_attention takes tree as an int64 tensor")
+    if tree.shape != (b, t) or tree.get_device() != device or (t > 1 and tree.stride(1) != 1) or (
+            b > 1 and tree.stride(0) != 0 and tree.stride(0) < t):
+        raise ValueError(f"tree_attention needs a set of nodes for each of [{b}, {t}] rows on cuda:{device}, in rows that do "
+                         f"not overlap, got {tuple(tree.shape)} of strides {tree.stride()} on {tree.device}")
+    nodes = t if nodes is None else nodes
+    if not 0 <= nodes <= nat.KV8_TREE_NODES:
+        raise ValueError(f"a tree has 0 to {nat.KV8_TREE_NODES} nodes, not {nodes}")
+    longest = cache.width * cache.page_tokens
+    if max_tokens is not None:
+        if max_tokens < 0:
+            raise ValueError(f"max_tokens must not be negative, got {max_tokens}")
+        longest = min(longest, max_tokens)
+    out = torch.empty_like(q)
+    strides += hip._head_strides(out)
+    got = ctypes.c_size_t(0)
+    nat.call("ftx_kv8_attention_workspace", b, t, h, cache.kv_heads, d, longest, ctypes.byref(got))
+    ws_bytes = int(got.value)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    nat.call("ftx_kv8_tree_attention", ctypes.byref(cache), q.data_ptr(), out.data_ptr(), tree.data_ptr(),
+             tree.stride(0) if b > 1 else t, nodes, b, t, h, _Strides6(*strides), d ** -0.5 if scale is None else scale, longest,
+             ws.data_ptr() if ws is not None else None, ws_bytes, hip._stream(device))
+    return out
+
+
+def keep(codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, path: torch.Tensor,
+         counts: torch.Tensor | None = None) -> None:
+    """Moves the accepted nodes of drafted trees behind their sequences' first tokens, in every layer of a pool
+    [layers, pages, ...], in one launch (``ftx_kv8_keep``).
+
+    Token ``starts[b] + path[b, i]`` moves to ``starts[b] + i``, for i below ``counts[b]`` (None: all of path's n, at most
+    64). ``path``: int32 [batch, n], ascending; it ends before an entry that does not ascend or is 64 or more. Keys and
+    values stay what they are, but for tokens that move into a block of another scale: a block's scale becomes the largest
+    that its tokens had, and codes of another one are rounded again. What lies behind the last kept token of its block
+    becomes 0. Two sequences must not write into one page.
+    """
+    device = _device(codes)
+    if device >= 0 and torch.autograd.forward_ad._current_level < 0:
+        got = nat.torch_calls().keep(codes, scales, table, starts, path, counts, device, hip._stream(device))
+        if got is not None:
+            nat.result(got)
+            return
+    _check_pool("keep", codes, scales, 6)
+    hip._check_underived("keep", codes=codes, scales=scales)
+    if path.dim() != 2:
+        raise ValueError(f"keep takes a path [batch, n], got {tuple(path.shape)}")
+    b, n = path.shape
+    _check_ints("keep", "path", path, 2, b, device)
+    _check_ints("keep", "table", table, 2, b, device)
+    _check_ints("keep", "starts", starts, 1, b, device)
+    if counts is not None:
+        _check_ints("keep", "counts", counts, 1, b, device)
+    if n > nat.KV8_TREE_NODES:
+        raise ValueError(f"keep moves up to {nat.KV8_TREE_NODES} nodes of a sequence, not {n}")
+    layers, pages, _, kv, blocks, block_bytes = codes.shape
+    torch._C._increment_version((codes, scales))
+    if not layers:
+        return
+    width = table.shape[1]
+    cache = nat.Kv8Cache(codes.data_ptr(), scales.data_ptr(), pages, table.data_ptr() or None, max(table.stride(0), width),
+                         starts.data_ptr(), counts.data_ptr() if counts is not None else None, width, kv, blocks * BLOCK,
+                         block_bytes // BLOCK, FORMATS[codes.dtype])
+    nat.call("ftx_kv8_keep", ctypes.byref(cache), layers, path.data_ptr(), max(path.stride(0), n), b, n, hip._stream(device))
 
 
 def copy_pages(codes: torch.Tensor, scales: torch.Tensor, src: list[int], dst: list[int]) -> None:

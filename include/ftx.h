@@ -427,6 +427,44 @@ int ftx_int8_linear_workspace(int64_t m, int64_t n, int64_t k, size_t *bytes);
 int ftx_int8_linear(const void *x, int64_t x_stride, const void *w, const float *w_scale, void *y, int64_t m, int64_t n,
                     int64_t k, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- matrix product with 4-bit weights ----------------------------------------
+ * No reference counterpart. y[m, n] = bf16(sum_k x[m, k] s[n, k / G] (c[n, k] -
+ * z[n, k / G])) of bf16 rows x (x_stride elements apart, a multiple of 8, at most
+ * 2^21; k a multiple of the group G = 32, 64 or 128, at most 2^20). w holds the
+ * codes c (0 .. 15) in tiles of 16 channels and units of 128 inputs, 1024 bytes
+ * each, [ceil(n / 16)][ceil(k / 128)]: the 16 bytes at 16 (16 q + r) are channel r,
+ * their 32-bit word i inputs 32 i + 8 q + (0 .. 7), input 2 j at bit 4 j and 2 j + 1
+ * at bit 16 + 4 j. scale and zero are bf16 [tile][unit][16][128 / G]; zero NULL is 8
+ * for all. What lies past n and k is finite. Up to 16 rows use the weights as they
+ * are; for more rows s (c - z) is rounded to bf16. Sums are fp32: they stay finite
+ * while 256 sum |x| does, and a row that holds an infinity or a NaN has NaN or
+ * infinite results. workspace: ftx_int4_linear_workspace bytes (0 unless K is split).
+ * Pointers are 16-byte aligned. */
+#define FTX_INT4_TILE 16
+#define FTX_INT4_UNIT 128
+int ftx_int4_linear_workspace(int64_t m, int64_t n, int64_t k, int group, size_t *bytes);
+int ftx_int4_linear(const void *x, int64_t x_stride, const void *w, const void *scale, const void *zero, void *y,
+                    int64_t m, int64_t n, int64_t k, int group, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- log probabilities of tokens ----------------------------------------------
+ * No reference counterpart. Of each row of logits [rows, vocab] (bf16, fp16 or fp32,
+ * row_stride values apart, any alignment of their own size): logprob = x[token] -
+ * log sum exp x, entropy = -sum p log p, and the `top` (0 .. 64) largest logits' log
+ * probabilities and indices, the lowest index first among equal ones. A negative
+ * token has the log probability 0, one of vocab or more NaN. Logits of -inf have no
+ * part in the sums; a row of nothing else, or with a NaN or +inf, has NaN for its
+ * log probabilities and entropy (its largest logits are found all the same, a NaN
+ * above all). fp32 arithmetic. workspace: ftx_token_logprobs_workspace bytes,
+ * 16-byte aligned (0 unless rows are split). tokens and the outputs are
+ * contiguous; top_logprob and top_token may be NULL for a top of 0. */
+#define FTX_LOGITS_BF16 0
+#define FTX_LOGITS_FP16 1
+#define FTX_LOGITS_FP32 2
+int ftx_token_logprobs_workspace(int64_t rows, int64_t vocab, int type, int top, size_t *bytes);
+int ftx_token_logprobs(const void *logits, int64_t row_stride, int type, const int64_t *tokens, int64_t rows,
+                       int64_t vocab, int top, float *logprob, float *entropy, float *top_logprob, int64_t *top_token,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- a KV cache in pages of 8-bit codes --------------------------------------
  * No reference counterpart. One layer is codes, bytes [pages][2][kv_heads]
  * [page_tokens / 32][32 d] (keys, then values), and scales, fp32 [pages][2]
@@ -465,6 +503,29 @@ int ftx_int8_linear(const void *x, int64_t x_stride, const void *w, const float 
  * sequence, new tokens included, as far as the caller knows; it shapes the
  * launch, not the result. workspace: ftx_kv8_attention_workspace bytes.
  *
+ * ftx_kv8_append_norm: ftx_kv8_append of normalised queries and keys: x becomes
+ * x f w first, f = 1 / sqrt(mean x^2 + eps) over its head's row, w the bf16 [d]
+ * weights q_weight and k_weight (both NULL: no norm). at: int32 [batch][t], rows
+ * at_stride apart, the rows of cos and sin that tokens are turned by (NULL: each
+ * its own place). A token whose `at` lies outside the tables becomes 0, its query
+ * and in the cache, and must not be attended to.
+ *
+ * ftx_kv8_tree_attention: attention of t rows over the starts[b] first tokens of a
+ * sequence (all of them) and those of the `nodes` (at most 64) tokens after them
+ * whose bit is set in the row's set tree[b][i] (int64, rows tree_stride apart, 0
+ * for one tree of all sequences).
+ * news: the rows that take part; the others, and rows that see no token, are 0.
+ * The rest as ftx_kv8_attention; max_tokens counts the nodes.
+ *
+ * ftx_kv8_keep: in each of `layers` layers that lie back to back, the token
+ * starts[b] + path[b][i] moves to starts[b] + i, for i below news[b] (NULL: n, at
+ * most 64). A path ascends; it ends before an entry that does not, that is 64 or
+ * more, or past the table. A block that tokens move to gets the largest of the
+ * scales that its tokens (older ones too) had before; codes of another scale are
+ * rounded again, and what lies behind the last kept token becomes 0. Tokens in
+ * holes are zeros. path: int32, rows path_stride apart. cache->codes and scales
+ * are the first layer's. No two sequences may name one page for these tokens.
+ *
  * ftx_kv8_copy_pages: in each of `layers` layers that lie back to back, pages
  * src[i] are copied to dst[i] (host arrays). No dst occurs twice or as a src. */
 #define FTX_KV8_BLOCK 32
@@ -488,6 +549,15 @@ int ftx_kv8_attention_workspace(int64_t batch, int64_t t, int heads, int kv_head
 int ftx_kv8_attention(const ftx_kv8_cache *cache, const void *q, void *o, int64_t batch, int64_t t, int heads,
                       const int64_t *strides, float scale, int64_t max_tokens, void *workspace, size_t workspace_bytes,
                       void *stream);
+int ftx_kv8_append_norm(const ftx_kv8_cache *cache, const void *q, const void *k, const void *v, const void *q_weight,
+                        const void *k_weight, float eps, const float *cos, const float *sin, int64_t positions,
+                        const int32_t *at, int64_t at_stride, void *q_out, int64_t batch, int64_t t, int heads,
+                        const int64_t *strides, void *stream);
+int ftx_kv8_tree_attention(const ftx_kv8_cache *cache, const void *q, void *o, const int64_t *tree, int64_t tree_stride,
+                           int nodes, int64_t batch, int64_t t, int heads, const int64_t *strides, float scale,
+                           int64_t max_tokens, void *workspace, size_t workspace_bytes, void *stream);
+int ftx_kv8_keep(const ftx_kv8_cache *cache, int64_t layers, const int32_t *path, int64_t path_stride, int64_t batch,
+                 int64_t n, void *stream);
 int ftx_kv8_copy_pages(void *codes, float *scales, int64_t layers, int64_t pages, int kv_heads, int page_tokens, int d,
                        const int32_t *src, const int32_t *dst, int64_t n, void *stream);
 
