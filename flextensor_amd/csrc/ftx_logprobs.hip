@@ -4,15 +4,17 @@
 //
 // over rows of bf16, fp16 or fp32 logits, all statistics in fp32. One pass: a thread keeps a running maximum, the sum of
 // the exponentials and the sum of their products with the exponents, in units of log2, and rescales both sums when a
-// batch of its values exceeds the maximum. An exponent is clamped before it multiplies an exponential of 0, so logits
-// of -inf add nothing; a NaN or +inf makes the row's sums NaN.
+// batch of its values exceeds the maximum. An exponent is one fused multiply-add, y = x log2(e) - fl(m log2(e)); what the
+// rounding of m's product puts into every y comes out of the sums at the end. Bound by the exponentials and their sums,
+// some nine cycles of a SIMD a value, close to what memory takes for bf16.
 //
 // The likeliest tokens are keys (the logit's bits in the order of unsigned integers, then the complement of the index):
-// the largest keys are the largest logits, the lowest index first among equal ones, a NaN above all. Each wave keeps the
-// 64 largest keys it has met sorted over its lanes, and the value of the last one that counts as a threshold: a batch
-// whose largest value is not above it (nearly all of them) costs one comparison. The first threshold is the `top`
-// largest of the lanes' first maxima, so that only a few values pass it. What passes is read again (it is in the cache),
-// collected in LDS and merged 64 at a time.
+// the largest keys are the largest logits, the lowest index first among equal ones, a NaN above all. The pass over the
+// row keeps no more for them than each thread's maximum. The threads form 64 groups (128 for a top of more than 32): as
+// many values as groups' maxima reach the `top`th largest of these, so no token below it counts, and some 1.2 `top` values
+// reach it. The threads whose own maximum does read their values again (from the cache) and collect the keys in LDS,
+// where one wave sorts them. Rows that more keys pass than LDS holds (many equal ones), or that are not finite, take
+// another way: each wave keeps the 64 largest keys of what it reads sorted over its lanes.
 #include <algorithm>
 #include <cfloat>
 
@@ -25,7 +27,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWave = 64;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-constexpr int kVecs = 4;  // 16-byte loads of a thread's batch
+constexpr int kVecs = 2;  // 16-byte loads of a thread's batch
 
 // A quotient or remainder of a workgroup's number, computed on the vector unit, as the scalar that it is.
 __device__ __forceinline__ int uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(static_cast<int>(v)); }
@@ -63,29 +65,66 @@ __device__ __forceinline__ Key key_of(float x, int64_t index) {
   return static_cast<Key>(ordered(x)) << 32 | static_cast<uint32_t>(~static_cast<uint32_t>(index));
 }
 
+// The value of lane ^ J, by moves within the vector registers.
+template <int J>
+__device__ __forceinline__ uint32_t across(uint32_t v, int lane) {
+  const int x = static_cast<int>(v);
+  if constexpr (J == 1) return __builtin_amdgcn_mov_dpp(x, 0xb1, 15, 15, true);  // quad_perm 1 0 3 2
+  if constexpr (J == 2) return __builtin_amdgcn_mov_dpp(x, 0x4e, 15, 15, true);  // quad_perm 2 3 0 1
+  if constexpr (J == 4)                                                          // eights mirrored, then quads
+    return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(x, 0x141, 15, 15, true), 0x1b, 15, 15, true);
+  if constexpr (J == 8) return __builtin_amdgcn_mov_dpp(x, 0x128, 15, 15, true);  // row_ror 8
+  if constexpr (J == 16) {
+    const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return lane & 16 ? s[0] : s[1];
+  }
+  const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return lane & 32 ? s[0] : s[1];
+}
+template <int J>
+__device__ __forceinline__ Key across(Key v, int lane) {
+  return static_cast<Key>(across<J>(static_cast<uint32_t>(v >> 32), lane)) << 32 |
+         across<J>(static_cast<uint32_t>(v), lane);
+}
+template <int J>
+__device__ __forceinline__ float across(float v, int lane) {
+  return __uint_as_float(across<J>(__float_as_uint(v), lane));
+}
+
 // Sorts the lanes' keys, the largest first; clean() where they are bitonic.
-template <typename K>
-__device__ __forceinline__ K exchange(K key, int distance, bool larger) {
-  const K other = __shfl_xor(key, distance);
+template <int J, typename K>
+__device__ __forceinline__ K exchange(K key, int lane, bool larger) {
+  const K other = across<J>(key, lane);
+  if constexpr (sizeof(K) == 4) return larger ? max(key, other) : min(key, other);
   return (key > other) == larger ? key : other;
 }
 template <typename K>
 __device__ __forceinline__ K clean(K key, int lane) {
-#pragma unroll
-  for (int j = 32; j > 0; j /= 2) key = exchange(key, j, (lane & j) == 0);
+  key = exchange<32>(key, lane, !(lane & 32));
+  key = exchange<16>(key, lane, !(lane & 16));
+  key = exchange<8>(key, lane, !(lane & 8));
+  key = exchange<4>(key, lane, !(lane & 4));
+  key = exchange<2>(key, lane, !(lane & 2));
+  return exchange<1>(key, lane, !(lane & 1));
+}
+template <int K2, int J, typename K>
+__device__ __forceinline__ K sort_step(K key, int lane) {
+  key = exchange<J>(key, lane, !(lane & J) == !(lane & K2));
+  if constexpr (J > 1) return sort_step<K2, J / 2>(key, lane);
   return key;
 }
 template <typename K>
 __device__ __forceinline__ K sorted(K key, int lane) {
-#pragma unroll
-  for (int k = 2; k < 64; k *= 2)
-#pragma unroll
-    for (int j = k / 2; j > 0; j /= 2) key = exchange(key, j, ((lane & j) == 0) == ((lane & k) == 0));
+  key = sort_step<2, 1>(key, lane);
+  key = sort_step<4, 2>(key, lane);
+  key = sort_step<8, 4>(key, lane);
+  key = sort_step<16, 8>(key, lane);
+  key = sort_step<32, 16>(key, lane);
   return clean(key, lane);
 }
 // The 64 largest of two sorted lists.
 __device__ __forceinline__ Key merged(Key a, Key b, int lane) {
-  const Key other = __shfl(b, 63 - lane);
+  const Key other = __shfl(b, kWave - 1 - lane);
   return clean(a > other ? a : other, lane);
 }
 
@@ -104,10 +143,27 @@ __device__ __forceinline__ Sums joined(Sums a, Sums b) {
   to(b);
   return {m, a.s + b.s, a.t + b.t};
 }
-__device__ __forceinline__ Sums wave_joined(Sums x) {
-#pragma unroll
-  for (int j = 1; j < kWave; j *= 2) x = joined(x, {__shfl_xor(x.m, j), __shfl_xor(x.s, j), __shfl_xor(x.t, j)});
-  return x;
+// The lanes' maximum (a NaN is left out) and sum, in every lane.
+__device__ __forceinline__ float wave_max(float v, int lane) {
+  v = fmaxf(v, across<1>(v, lane));
+  v = fmaxf(v, across<2>(v, lane));
+  v = fmaxf(v, across<4>(v, lane));
+  v = fmaxf(v, across<8>(v, lane));
+  v = fmaxf(v, across<16>(v, lane));
+  return fmaxf(v, across<32>(v, lane));
+}
+__device__ __forceinline__ float wave_sum(float v, int lane) {
+  v += across<1>(v, lane);
+  v += across<2>(v, lane);
+  v += across<4>(v, lane);
+  v += across<8>(v, lane);
+  v += across<16>(v, lane);
+  return v + across<32>(v, lane);
+}
+__device__ __forceinline__ Sums wave_joined(Sums x, int lane) {
+  const float m = wave_max(x.m, lane);
+  x = joined(x, {m, 0.f, 0.f});
+  return {m, wave_sum(x.s, lane), wave_sum(x.t, lane)};
 }
 
 // A wave writes a row's results.
@@ -127,154 +183,291 @@ __device__ __forceinline__ void write_row(const Logprobs &p, int64_t row, const 
   }
 }
 
+// A part of a row as 16-byte units, counted from the boundary before the row: the values of the first and last one that
+// are not the row's are left out (an aligned unit with a value of the row lies in its memory page). A thread's units are
+// THREADS apart, and a batch of it kVecs of them.
+template <int TYPE, int THREADS>
+struct Part {
+  static constexpr int kValues = Vec<TYPE>::kValues, kBatch = kVecs * kValues;
+  const void *row;
+  const u32x4 *units;
+  int lead, vocab, end, plain;  // plain: units below it (but for the first after a lead) are the row's altogether
+
+  // Whether the workgroup's batch from u on is of such units; the thread's first unit of it is u + its number.
+  __device__ __forceinline__ bool is_plain(int u) const {
+    return u + kVecs * THREADS <= plain && (u > 0 || lead == 0);
+  }
+  __device__ __forceinline__ void load(Vec<TYPE> (&v)[kVecs], int u) const {
+    if (is_plain(u)) {
+      const u32x4 *from = units + u;
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) v[i].w = from[threadIdx.x + i * THREADS];
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+      v[i].w = units[min(u + static_cast<int>(threadIdx.x) + i * THREADS, end - 1)];
+  }
+  __device__ __forceinline__ int index(int u0, int value) const {
+    return (u0 + value / kValues * THREADS) * kValues - lead + value % kValues;
+  }
+  static __device__ __forceinline__ void drop(Vec<TYPE> &v, int e) {
+    if constexpr (TYPE == FTX_LOGITS_FP32) v.w[e] = 0xff800000u;
+    else v.w[e / 2] = (v.w[e / 2] & (e % 2 ? 0xffffu : 0xffff0000u)) |
+                      (TYPE == FTX_LOGITS_BF16 ? 0xff80u : 0xfc00u) << (16 * (e % 2));
+  }
+  // Which of a batch's values are the row's, a bit each; the others become -inf.
+  __device__ __forceinline__ uint32_t trim(Vec<TYPE> (&v)[kVecs], int u) const {
+    if (is_plain(u)) return kBatch == 32 ? ~0u : (1u << (kBatch % 32)) - 1;
+    uint32_t valid = 0;
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int unit = u + static_cast<int>(threadIdx.x) + i * THREADS;
+      uint32_t here = unit < end ? (1u << kValues) - 1 : 0;
+      if (unit == 0) here = here >> lead << lead;
+      if ((unit + 1) * kValues - lead > vocab) here &= (1u << max(0, vocab + lead - unit * kValues)) - 1;
+      valid |= here << (i * kValues);
+      if (__any(here != 0 && here != (1u << kValues) - 1)) {  // the first or last one
+#pragma unroll
+        for (int e = 0; e < kValues; ++e)
+          if (!(here >> e & 1)) drop(v[i], e);
+      } else {
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          if (!here) v[i].w[w] = TYPE == FTX_LOGITS_FP32 ? 0xff800000u : TYPE == FTX_LOGITS_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+      }
+    }
+    return valid;
+  }
+};
+
+// The 64 largest keys of a part, sorted in wave 0's lanes: every wave those of its units, 64 candidates at a time in its
+// part of LDS, then two waves' lists at a time.
+template <int TYPE, int THREADS>
+__device__ __forceinline__ Key largest_keys(const Part<TYPE, THREADS> &part, int first, int top, Key *lists, int wave,
+                                            int lane) {
+  constexpr int kWaves = THREADS / kWave;
+  Key *mine = lists + wave * 2 * kWave, list = 0;
+  uint32_t threshold = 0;
+  int held = 0;
+  const auto merge = [&]() {
+    const Key fresh = lane < held ? mine[lane] : 0;
+    list = merged(list, sorted(fresh, lane), lane);
+    const Key rest = mine[kWave + lane];
+    held = max(held - kWave, 0);
+    if (lane < held) mine[lane] = rest;
+    threshold = static_cast<uint32_t>(__shfl(list, top - 1) >> 32);
+  };
+  for (int u = first; u < part.end; u += kVecs * THREADS) {
+    const int u0 = u + wave * kWave + lane;
+    Vec<TYPE> v[kVecs];
+    part.load(v, u);
+    uint32_t passed = part.trim(v, u);
+#pragma unroll
+    for (int i = 0; i < part.kBatch; ++i)
+      if (ordered(v[i / part.kValues][i % part.kValues]) <= threshold) passed &= ~(1u << i);
+    while (uint64_t some = __ballot(passed != 0)) {
+      const int slot = held + static_cast<int>(__builtin_amdgcn_mbcnt_hi(
+                                  static_cast<uint32_t>(some >> 32),
+                                  __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(some), 0)));
+      if (passed) {
+        const int at = part.index(u0, __builtin_ctz(passed));
+        mine[slot] = key_of(value_at<TYPE>(part.row, at), at);
+        passed &= passed - 1;
+      }
+      held += __popcll(some);
+      __builtin_amdgcn_wave_barrier();
+      if (held >= kWave) merge();
+    }
+  }
+  if (held > 0) merge();
+  mine[lane] = list;
+  __syncthreads();
+  for (int step = 1; step < kWaves; step *= 2) {
+    if (wave % (2 * step) == 0) {
+      list = merged(list, lists[(wave + step) * 2 * kWave + lane], lane);
+      mine[lane] = list;
+    }
+    __syncthreads();
+  }
+  return list;
+}
+
+constexpr float kFar = -0x1p126f;  // below this, or above its negative, a logit's product with log2(e) may overflow
+
 template <int TYPE, int THREADS, bool TOP>
-__global__ __launch_bounds__(THREADS) void logprobs_kernel(Logprobs p) {
+__global__ __launch_bounds__(THREADS, THREADS == 256 ? 8 : 4) void logprobs_kernel(Logprobs p) {
   constexpr int kWaves = THREADS / kWave, kValues = Vec<TYPE>::kValues, kItem = 16 / kValues;
-  __shared__ Key lists[TOP ? kWaves : 1][TOP ? 2 * kWave : 1];
+  constexpr int kKeys = kWaves * 2 * kWave, kGroups = 2 * kWave;
+  __shared__ Key lists[TOP ? kKeys : 1];
+  __shared__ uint32_t group_max[TOP ? kGroups : 1];
+  __shared__ int collected;
   __shared__ Sums parts[kWaves];
   const int64_t row = uniform(blockIdx.x / static_cast<uint32_t>(p.splits));
   const int split = uniform(blockIdx.x % static_cast<uint32_t>(p.splits));
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const uint8_t *x = static_cast<const uint8_t *>(p.logits) + row * p.row_stride * kItem;
-  // 16-byte units from the boundary before the row: the values of the first and last one that are not the row's are
-  // left out (an aligned unit with a value of the row lies in its memory page)
-  const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16) / kItem;
-  const u32x4 *units = reinterpret_cast<const u32x4 *>(x - lead * kItem);
-  const int vocab = static_cast<int>(p.vocab);
-  const int all = (lead + vocab + kValues - 1) / kValues;
-  const int first = split * p.split_units, end = min(all, first + p.split_units);
+  Part<TYPE, THREADS> part;
+  part.row = x;
+  part.lead = static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16) / kItem;
+  part.units = reinterpret_cast<const u32x4 *>(x - part.lead * kItem);
+  part.vocab = static_cast<int>(p.vocab);
+  const int all = (part.lead + part.vocab + kValues - 1) / kValues;
+  const int first = split * p.split_units;
+  part.end = min(all, first + p.split_units);
+  part.plain = min(part.end, (part.lead + part.vocab) / kValues);
+  if (TOP && threadIdx.x == 0) collected = 0;
 
-  Sums mine = {-FLT_MAX, 0.f, 0.f};
-  Key list = 0;            // lane i: the wave's ith largest key
-  uint32_t threshold = 0;  // values up to this need not be looked at
-  int held = 0;            // keys in LDS that have not been merged
-
-  Vec<TYPE> now[kVecs], next[kVecs];
-  const auto load = [&](Vec<TYPE> (&v)[kVecs], int u0) {
+  float top = -INFINITY, c = -kFar * kLog2e, s = 0.f, t = 0.f;  // y = x log2(e) + c
+  const auto work = [&](Vec<TYPE> (&v)[kVecs], int u) {
+    part.trim(v, u);
+    float high = v[0][0], low = v[0][0];
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) v[i].w = units[min(u0 + i * THREADS, end - 1)];
-  };
-  const auto merge = [&]() {
-    const Key fresh = lane < held ? lists[wave][lane] : 0;
-    list = merged(list, sorted(fresh, lane), lane);
-    const Key rest = lists[wave][kWave + lane];
-    held = max(held - kWave, 0);
-    if (lane < held) lists[wave][lane] = rest;
-    threshold = max(threshold, static_cast<uint32_t>(__shfl(list, p.top - 1) >> 32));
-  };
-  const auto work = [&](Vec<TYPE> (&v)[kVecs], int u0, bool start) {
-    // which of the batch's values are the row's: all but at its ends
-    const int u1 = u0 + (kVecs - 1) * THREADS;
-    uint32_t valid = ~0u;
-    if (__any((lead > 0 && u0 == 0) || u1 >= end || (u1 + 1) * kValues - lead > vocab)) {
-      valid = 0;
-#pragma unroll
-      for (int i = 0; i < kVecs; ++i)
-#pragma unroll
-        for (int e = 0; e < kValues; ++e) {
-          const int u = u0 + i * THREADS, at = u * kValues - lead + e;
-          if (u < end && at >= 0 && at < vocab) valid |= 1u << (i * kValues + e);
-        }
-#pragma unroll
-      for (int i = 0; i < kVecs; ++i)
-#pragma unroll
-        for (int e = 0; e < kValues; ++e) {
-          if (valid >> (i * kValues + e) & 1) continue;
-          if constexpr (TYPE == FTX_LOGITS_FP32) v[i].w[e] = 0xff800000u;
-          else v[i].w[e / 2] = (v[i].w[e / 2] & (e % 2 ? 0xffffu : 0xffff0000u)) |
-                               (TYPE == FTX_LOGITS_BF16 ? 0xff80u : 0xfc00u) << (16 * (e % 2));
-        }
+    for (int i = 0; i < kVecs * kValues; i += 2) {  // three operands at a time
+      const float a = v[i / kValues][i % kValues], b = v[i / kValues][i % kValues + 1];
+      high = fmaxf(fmaxf(high, a), b);
+      low = fminf(fminf(low, a), b);
     }
-    float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i)
-#pragma unroll
-      for (int e = 0; e < kValues; ++e) top = fmaxf(top, v[i][e]);
-    if (top > mine.m) {
-      const float y = (mine.m - top) * kLog2e, w = __builtin_amdgcn_exp2f(y);
-      mine.t = (mine.t + fmaxf(y, -1000.f) * mine.s) * w;
-      mine.s *= w;
-      mine.m = top;
+    if (high > top) {
+      top = high;
+      const float now = -__builtin_amdgcn_fmed3f(top, kFar, -kFar) * kLog2e, y = now - c, w = __builtin_amdgcn_exp2f(y);
+      t = (t + fmaxf(y, -1000.f) * s) * w;
+      s *= w;
+      c = now;
     }
+    if (__any(low < kFar)) {  // an exponent may be -inf, and its exponential is 0
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i)
-#pragma unroll
-      for (int e = 0; e < kValues; ++e) {
-        const float y = (v[i][e] - mine.m) * kLog2e, w = __builtin_amdgcn_exp2f(y);
-        mine.s += w;
-        mine.t = fmaf(fmaxf(y, -1000.f), w, mine.t);
+      for (int i = 0; i < kVecs * kValues; ++i) {
+        const float y = fmaf(v[i / kValues][i % kValues], kLog2e, c), w = __builtin_amdgcn_exp2f(y);
+        s += w;
+        t = fmaf(fmaxf(y, -1000.f), w, t);
       }
-    if constexpr (TOP) {
-      uint32_t best = valid ? ordered(top) : 0;
-      uint32_t least = threshold;
-      if (start) {  // as many lanes as tokens are asked for have a value of at least this
-        const uint32_t seed = __shfl(sorted(best, lane), p.top - 1);
-        threshold = seed;
-        least = seed == 0 ? 0 : seed - 1;  // and in this batch the values equal to it count
-      }
-      if (mine.s != mine.s) best = valid ? 0xffffffffu : 0;  // a NaN, which the maximum leaves out
-      if (__any(best > least)) {
-        uint32_t passed = 0;
+    } else {
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i)
-#pragma unroll
-          for (int e = 0; e < kValues; ++e)
-            if (ordered(v[i][e]) > least) passed |= 1u << (i * kValues + e);
-        passed &= valid;
-        while (uint64_t some = __ballot(passed != 0)) {
-          const int slot = held + static_cast<int>(__builtin_amdgcn_mbcnt_hi(
-                                      static_cast<uint32_t>(some >> 32),
-                                      __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(some), 0)));
-          if (passed) {
-            const int bit = __builtin_ctz(passed);
-            const int at = (u0 + bit / kValues * THREADS) * kValues - lead + bit % kValues;
-            lists[wave][slot] = key_of(value_at<TYPE>(x, at), at);
-            passed &= passed - 1;
-          }
-          held += __popcll(some);
-          __builtin_amdgcn_wave_barrier();
-          if (held >= kWave) merge();
-        }
+      for (int i = 0; i < kVecs * kValues; ++i) {
+        const float y = fmaf(v[i / kValues][i % kValues], kLog2e, c), w = __builtin_amdgcn_exp2f(y);
+        s += w;
+        t = fmaf(y, w, t);
       }
     }
   };
-
-  if (first < end) {
-    int u0 = first + static_cast<int>(threadIdx.x);
-    load(now, u0);
-    for (bool start = true;; start = false) {
-      const int u1 = u0 + kVecs * THREADS;
-      const bool more = u1 - static_cast<int>(threadIdx.x) < end;
-      if (more) load(next, u1);
-      work(now, u0, start);
-      if (!more) break;
-#pragma unroll
-      for (int i = 0; i < kVecs; ++i) now[i] = next[i];
-      u0 = u1;
+  const int mine0 = first + static_cast<int>(threadIdx.x);
+  if (first < part.end) {
+    Vec<TYPE> a[kVecs], b[kVecs];
+    part.load(a, first);
+    for (int u = first;;) {
+      constexpr int kNext = kVecs * THREADS;
+      part.load(b, u + kNext);
+      work(a, u);
+      if ((u += kNext) >= part.end) break;
+      part.load(a, u + kNext);
+      work(b, u);
+      if ((u += kNext) >= part.end) break;
     }
   }
-  if constexpr (TOP) {
-    if (held > 0) merge();
+  const auto all_parts = [&]() {  // a wave a lane
+    Sums x = parts[lane % kWaves];
+    if (lane >= kWaves) x.s = x.t = 0.f;
+    return wave_joined(x, lane);
+  };
+  Sums mine = {fmaxf(top, -FLT_MAX), s, t};
+  if (s != 0.f && top > kFar) {  // every y is too large by what fl(m log2(e)) is too small
+    const float more = fmaf(top, kLog2e, c);
+    mine.s = fmaf(-more * kLn2, s, s);
+    mine.t = fmaf(-more, s, fmaf(-more * kLn2, t, t));
   }
-  mine = wave_joined(mine);
+  mine = wave_joined(mine, lane);
   if (lane == 0) parts[wave] = mine;
-  if constexpr (TOP) lists[wave][lane] = list;
-  __syncthreads();
+  // the groups' maxima: a quad of 256 threads or a sixteen of 1024, or half of these
+  const bool fine = p.top > kWave / 2;
   if constexpr (TOP) {
+    uint32_t most = mine0 < part.end ? ordered(top) : 0;
+    most = max(most, across<1>(most, lane));
+    if constexpr (kWaves == 16) {
+      most = max(most, across<2>(most, lane));
+      most = max(most, across<4>(most, lane));
+    }
+    if (fine) {
+      if (threadIdx.x % (THREADS / 128) == 0) group_max[threadIdx.x / (THREADS / 128)] = most;
+    } else {
+      most = max(most, kWaves == 16 ? across<8>(most, lane) : across<2>(most, lane));
+      if (threadIdx.x % (THREADS / 64) == 0) group_max[threadIdx.x / (THREADS / 64)] = most;
+    }
+  }
+  __syncthreads();
+  mine = all_parts();
+  if (!(fabsf(mine.m) < -0.5f * kFar) && first < part.end) {  // the products may have overflowed: the differences first
+    Sums far = {mine.m, 0.f, 0.f};
+    for (int u = first; u < part.end; u += kVecs * THREADS) {
+      Vec<TYPE> v[kVecs];
+      part.load(v, u);
+      part.trim(v, u);
 #pragma unroll
-    for (int step = 1; step < kWaves; step *= 2) {
-      if (wave % (2 * step) == 0) {
-        list = merged(list, lists[wave + step][lane], lane);
-        lists[wave][lane] = list;
+      for (int i = 0; i < kVecs * kValues; ++i) {
+        const float y = (v[i / kValues][i % kValues] - mine.m) * kLog2e, w = __builtin_amdgcn_exp2f(y);
+        far.s += w;
+        far.t = fmaf(fmaxf(y, -1000.f), w, far.t);
+      }
+    }
+    far = wave_joined(far, lane);
+    __syncthreads();
+    if (lane == 0) parts[wave] = far;
+    __syncthreads();
+    mine = all_parts();
+  }
+
+  Key list = 0;
+  if constexpr (TOP) {
+    uint32_t groups = sorted(group_max[lane], lane);
+    if (fine) {
+      const uint32_t others = __shfl(sorted(group_max[kWave + lane], lane), kWave - 1 - lane);
+      groups = clean(max(groups, others), lane);
+    }
+    const uint32_t least = __builtin_amdgcn_readlane(static_cast<int>(groups), p.top - 1);
+    bool exact = mine.s == mine.s;  // else a NaN may be among the values, which no maximum shows
+    if (exact) {
+      const float bound = least == 0 ? -INFINITY : unordered(least);
+      // four of the threads at a time, a unit a lane
+      uint64_t those = __ballot(mine0 < part.end && top >= bound);
+      while (those) {
+        int whose[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          whose[i] = those ? __builtin_ctzll(those) : -1;
+          those &= those - 1;
+        }
+        const int thread = lane < 16 ? whose[0] : lane < 32 ? whose[1] : lane < 48 ? whose[2] : whose[3];
+        if (thread < 0) continue;
+        for (int u = first + wave * kWave + thread + lane % 16 * THREADS; u < part.end; u += 16 * THREADS) {
+          const Vec<TYPE> v = {part.units[u]};
+          uint32_t passed = 0;
+#pragma unroll
+          for (int e = 0; e < kValues; ++e) passed |= v[e] >= bound ? 1u << e : 0;
+          while (passed) {
+            const int e = __builtin_ctz(passed), at = u * kValues - part.lead + e;
+            passed &= passed - 1;
+            if (at < 0 || at >= part.vocab) continue;
+            const int slot = atomicAdd(&collected, 1);
+            if (slot < kKeys) lists[slot] = key_of(value_at<TYPE>(x, at), at);
+          }
+        }
       }
       __syncthreads();
+      exact = collected <= kKeys;
+    }
+    if (exact) {
+      if (wave == 0)
+        for (int i = 0; i < collected; i += kWave) {
+          const Key fresh = sorted(i + lane < collected ? lists[i + lane] : 0, lane);
+          list = i == 0 ? fresh : merged(list, fresh, lane);
+        }
+    } else {
+      __syncthreads();
+      list = largest_keys<TYPE, THREADS>(part, first, p.top, lists, wave, lane);
     }
   }
   if (wave > 0) return;
-  mine = parts[0];
-#pragma unroll
-  for (int i = 1; i < kWaves; ++i) mine = joined(mine, parts[i]);
   if (p.splits == 1) {
     write_row<TYPE>(p, row, x, mine, list, lane);
     return;
@@ -296,7 +489,7 @@ __global__ __launch_bounds__(kWave) void logprobs_join_kernel(Logprobs p) {
       sums = joined(sums, {v.x, v.y, v.z});
     }
   }
-  sums = wave_joined(sums);
+  sums = wave_joined(sums, lane);
   if (p.top > 0) {
     list = p.part_keys[row * p.splits * kWave + lane];
     for (int i = 1; i < p.splits; ++i) list = merged(list, p.part_keys[(row * p.splits + i) * kWave + lane], lane);
