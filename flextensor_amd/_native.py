@@ -192,6 +192,8 @@ _SIGNATURES: dict[str, list] = {
                           ctypes.c_float, ctypes.c_int64, _vp, _sz, _vp],
     "ftx_kv8_append_norm": [ctypes.POINTER(Kv8Cache), _vp, _vp, _vp, _vp, _vp, ctypes.c_float, _vp, _vp, ctypes.c_int64,
                             _vp, ctypes.c_int64, _vp, ctypes.c_int64, ctypes.c_int64, _int, _vp, _vp],
+    "ftx_kv8_tree_attention_workspace": [ctypes.c_int64, ctypes.c_int64, _int, _int, _int, ctypes.c_int64,
+                                         ctypes.POINTER(_sz)],
     "ftx_kv8_tree_attention": [ctypes.POINTER(Kv8Cache), _vp, _vp, _vp, ctypes.c_int64, _int, ctypes.c_int64,
                                ctypes.c_int64, _int, _vp, ctypes.c_float, ctypes.c_int64, _vp, _sz, _vp],
     "ftx_kv8_keep": [ctypes.POINTER(Kv8Cache), ctypes.c_int64, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp],

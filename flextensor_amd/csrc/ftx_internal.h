@@ -207,7 +207,7 @@ struct Kv8Attention {
   uint32_t items;         // times the splits
   size_t part_bytes;
 };
-void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, int cus, int xcds);
+void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, bool tree, int cus, int xcds);
 hipError_t launch_kv8_attention(const Kv8Attention &p, hipStream_t stream);
 struct Kv8Append {
   KvPages kv;

@@ -30,6 +30,7 @@ constexpr int kWave = 64;
 constexpr float kSlack = 8.0f;
 constexpr int kTileWaves = 8;  // of an attention workgroup
 constexpr float kTiny = 0x1p-100f;  // a block whose scale is below this stands for zeros
+constexpr int kRowJoinSplits = 16;  // chunks that a group of lanes joins one after the other
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
@@ -807,6 +808,59 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8Attention a) {
       (u32x2){pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
 }
 
+// The same for few chunks of many rows, as trees have them: a group of D / 4 lanes a row, which takes its chunks one after
+// the other, four loads at a time (12800 rows in four chunks: 6.4 us, a workgroup a row 20.8).
+template <int D>
+__global__ __launch_bounds__(256) void kv8_join_rows_kernel(Kv8Attention a) {
+  constexpr int kLanes = D / 4, kBatch = 4;
+  const int64_t slots = a.tile_items * a.tile_rows;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+  if (at >= slots) return;
+  const uint32_t tile_item = static_cast<uint32_t>(at) / static_cast<uint32_t>(a.tile_rows);
+  const int tile = static_cast<int>(tile_item % static_cast<uint32_t>(a.row_tiles));
+  const int row = tile * a.tile_rows + static_cast<int>(static_cast<uint32_t>(at) % static_cast<uint32_t>(a.tile_rows));
+  if (row >= a.rows) return;
+  const uint32_t bkv = tile_item / static_cast<uint32_t>(a.row_tiles);
+  const int64_t b = bkv / static_cast<uint32_t>(a.kv.kv_heads);
+  const int used = min(a.splits, (tile_blocks<true>(a, rows_of<true>(a, b), tile) + a.chunk - 1) / a.chunk);
+  const float *pm = a.part + a.splits * slots * D;
+  const float *pl = pm + a.splits * slots;
+  const int c = threadIdx.x % kLanes;
+  float mx = -FLT_MAX, l = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int i0 = 0; i0 < used; i0 += kBatch) {
+    float m[kBatch], part[kBatch];
+    f32x4 o[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {  // past the last chunk it again, with a weight of zero below
+      const int64_t s = min(i0 + i, used - 1) * slots + at;
+      m[i] = pm[s];
+      part[i] = pl[s];
+      o[i] = *reinterpret_cast<const f32x4 *>(a.part + s * D + 4 * c);
+    }
+    float m_new = mx;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) m_new = fmaxf(m_new, m[i]);
+    const float alpha = __builtin_amdgcn_exp2f(mx - m_new);
+    l *= alpha;
+    acc *= alpha;
+    mx = m_new;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (i0 + i >= used) break;
+      const float w = __builtin_amdgcn_exp2f(m[i] - m_new);
+      l += w * part[i];
+      acc += w * o[i];
+    }
+  }
+  const float inv = l != 0.f ? 1.0f / l : 0.f;
+  const int token = row / a.rep;
+  const int head = static_cast<int>(bkv % static_cast<uint32_t>(a.kv.kv_heads)) * a.rep + (row - token * a.rep);
+  uint16_t *op = a.o + b * a.o_stride[0] + token * a.o_stride[1] + head * a.o_stride[2] + 4 * c;
+  *reinterpret_cast<u32x2 *>(op) =
+      (u32x2){pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
+}
+
 template <int D, bool FP8, bool TREE>
 hipError_t launch_attend(const Kv8Attention &p, hipStream_t stream) {
   const dim3 block(kTileWaves * kWave), grid(p.items), xcd_grid((p.items + p.xcds - 1) / p.xcds * p.xcds);
@@ -816,6 +870,11 @@ hipError_t launch_attend(const Kv8Attention &p, hipStream_t stream) {
   else hipLaunchKernelGGL((kv8_tile_kernel<D, FP8, false, TREE>), xcd_grid, block, 0, stream, p);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || p.splits == 1) return err;
+  if (TREE && p.splits <= kRowJoinSplits) {
+    const int64_t groups = (p.tile_items * p.tile_rows * (D / 4) + 255) / 256;
+    hipLaunchKernelGGL((kv8_join_rows_kernel<D>), dim3(static_cast<unsigned>(groups)), dim3(256), 0, stream, p);
+    return hipGetLastError();
+  }
   hipLaunchKernelGGL((kv8_join_kernel<D, TREE>), dim3(static_cast<unsigned>(p.tile_items * p.tile_rows)), dim3(256), 0,
                      stream, p);
   return hipGetLastError();
@@ -1231,7 +1290,9 @@ __global__ __launch_bounds__(256) void kv8_copy_kernel(Kv8Copy) {
 // 32 splits, 21.9 in 63, 36 in 4; 256 heads over 4096 keys 48.5 unsplit, 56 in two. 512 rows over 500 keys 10.9 in
 // tiles of 32 and 26.8 in tiles of 256, over 4000 31.4 and 38.0, over 30000 132 and 98; 128 heads of 512 rows over
 // 2000 keys 205 and 111, 32 heads 52.5 and 62. Up to 64 rows tiles of 32 were never slower (14.6 and 18.7 over 4000).
-void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, int cus, int xcds) {
+// Trees join their chunks at less cost: 128 rows over 32000 keys (16 heads) 68.5 in tiles of 256 split in 16, 79.3 in
+// tiles of 32 split in four.
+void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, bool tree, int cus, int xcds) {
   p->xcds = std::max(1, xcds);
   p->rep = p->heads / p->kv.kv_heads;
   p->rows = p->t * p->rep;
@@ -1244,7 +1305,7 @@ void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, int cus, int xcds) 
       const int64_t s = rounds == 0 ? 1 : std::min(rounds * cus / items, blocks / 8);
       if (s < 1 || (rounds > 0 && s == 1)) continue;
       const int64_t cost = (items * s + cus - 1) / cus * ((blocks + s - 1) / s * block_cost + start_cost) +
-                           (s > 1 ? 30 + items * tile_rows * s / 385 : 0);
+                           (s == 1 ? 0 : 30 + items * tile_rows * s / (tree && s <= kRowJoinSplits ? 900 : 385));
       if (cost >= best) continue;
       best = cost;
       splits = s;

@@ -1497,14 +1497,14 @@ int check_view(const void *ptr, const int64_t *stride, int64_t n0, int64_t n1, i
   return check_operand(ptr, extent, 2, what);
 }
 
-int plan_kv8(int64_t max_tokens, ftx::Kv8Attention *p) {
+int plan_kv8(int64_t max_tokens, bool tree, ftx::Kv8Attention *p) {
   int cus = 256, xcds = 8;
   ftx::DeviceState *st = nullptr;
   if (ftx::device_state(&st) == FTX_OK) {
     cus = st->cu_count;
     xcds = st->xcd_count;
   }
-  ftx::plan_kv8_attention(p, std::min<int64_t>(max_tokens, int64_t(1) << 30), cus, xcds);
+  ftx::plan_kv8_attention(p, std::min<int64_t>(max_tokens, int64_t(1) << 30), tree, cus, xcds);
   const int64_t join_rows = p->splits > 1 ? p->tile_items * p->tile_rows : 0;
   if (static_cast<int64_t>(p->items) + p->xcds > ftx::kMaxThreads / 512 || join_rows > ftx::kMaxThreads / 256)
     return ftx::fail(FTX_ERR_UNSUPPORTED, "cache attention: more workgroups than one launch holds");
@@ -1571,8 +1571,10 @@ int ftx_kv8_append_norm(const ftx_kv8_cache *cache, const void *q, const void *k
   return FTX_OK;
 }
 
-int ftx_kv8_attention_workspace(int64_t batch, int64_t t, int heads, int kv_heads, int d, int64_t max_tokens,
-                                size_t *bytes) {
+namespace {
+
+int kv8_workspace(int64_t batch, int64_t t, int heads, int kv_heads, int d, int64_t max_tokens, bool tree,
+                  size_t *bytes) {
   if (!bytes) return ftx::fail(FTX_ERR_INVALID, "bytes is null");
   int rc = check_kv8_shape(1, kv_heads, ftx::kKvBlock, d);
   if (rc != FTX_OK) return rc;
@@ -1590,12 +1592,10 @@ int ftx_kv8_attention_workspace(int64_t batch, int64_t t, int heads, int kv_head
   p.batch = static_cast<int>(batch);
   p.t = static_cast<int>(t);
   p.heads = heads;
-  rc = plan_kv8(max_tokens, &p);
+  rc = plan_kv8(max_tokens, tree, &p);
   if (rc == FTX_OK) *bytes = p.part_bytes;
   return rc;
 }
-
-namespace {
 
 // tree: null, or the rows' sets of nodes.
 int kv8_attention(const ftx_kv8_cache *cache, const void *q, void *o, const int64_t *tree, int64_t tree_stride, int nodes,
@@ -1622,7 +1622,7 @@ int kv8_attention(const ftx_kv8_cache *cache, const void *q, void *o, const int6
   p.t = static_cast<int>(t);
   p.heads = heads;
   p.scale_log2 = scale * 1.44269504088896340736f;
-  rc = plan_kv8(max_tokens, &p);
+  rc = plan_kv8(max_tokens, tree != nullptr, &p);
   if (rc != FTX_OK) return rc;
   if (p.part_bytes > 0) {
     if (workspace_bytes < p.part_bytes)
@@ -1637,6 +1637,16 @@ int kv8_attention(const ftx_kv8_cache *cache, const void *q, void *o, const int6
 }
 
 }  // namespace
+
+int ftx_kv8_attention_workspace(int64_t batch, int64_t t, int heads, int kv_heads, int d, int64_t max_tokens,
+                                size_t *bytes) {
+  return kv8_workspace(batch, t, heads, kv_heads, d, max_tokens, false, bytes);
+}
+
+int ftx_kv8_tree_attention_workspace(int64_t batch, int64_t t, int heads, int kv_heads, int d, int64_t max_tokens,
+                                     size_t *bytes) {
+  return kv8_workspace(batch, t, heads, kv_heads, d, max_tokens, true, bytes);
+}
 
 int ftx_kv8_attention(const ftx_kv8_cache *cache, const void *q, void *o, int64_t batch, int64_t t, int heads,
                       const int64_t *strides, float scale, int64_t max_tokens, void *workspace, size_t workspace_bytes,

@@ -35,6 +35,7 @@ struct Library {
   decltype(&ftx_int8_matmul_workspace) int8_matmul_workspace;
   decltype(&ftx_int8_matmul) int8_matmul;
   decltype(&ftx_kv8_append_norm) kv8_append_norm;
+  decltype(&ftx_kv8_tree_attention_workspace) kv8_tree_attention_workspace;
   decltype(&ftx_kv8_tree_attention) kv8_tree_attention;
   decltype(&ftx_kv8_keep) kv8_keep;
   decltype(&ftx_int4_linear_workspace) int4_linear_workspace;
@@ -244,7 +245,8 @@ PyObject *attend(const Tensor &q, int64_t *stride, const Cache &c, const Tensor 
   if (!heads(&out, stride + 3)) return other_way();
   const int h = static_cast<int>(q.size(2));
   size_t bytes = 0;
-  int rc = lib.kv8_attention_workspace(q.size(0), q.size(1), h, c.c.kv_heads, c.c.d, longest, &bytes);
+  int rc = (tree ? lib.kv8_tree_attention_workspace : lib.kv8_attention_workspace)(q.size(0), q.size(1), h, c.c.kv_heads,
+                                                                                  c.c.d, longest, &bytes);
   if (rc != FTX_OK) return result(rc, out);
   Tensor ws;
   if (bytes > 0) ws = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte).requires_grad(false));
@@ -537,6 +539,7 @@ PyObject *use(PyObject *, PyObject *handle) {
       !entry(found.int8_linear, "ftx_int8_linear") ||
       !entry(found.int8_matmul_workspace, "ftx_int8_matmul_workspace") ||
       !entry(found.int8_matmul, "ftx_int8_matmul") || !entry(found.kv8_append_norm, "ftx_kv8_append_norm") ||
+      !entry(found.kv8_tree_attention_workspace, "ftx_kv8_tree_attention_workspace") ||
       !entry(found.kv8_tree_attention, "ftx_kv8_tree_attention") || !entry(found.kv8_keep, "ftx_kv8_keep") ||
       !entry(found.int4_linear_workspace, "ftx_int4_linear_workspace") ||
       !entry(found.int4_linear, "ftx_int4_linear") ||

@@ -274,7 +274,7 @@ def tree_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, t
     out = torch.empty_like(q)
     strides += hip._head_strides(out)
     got = ctypes.c_size_t(0)
-    nat.call("ftx_kv8_attention_workspace", b, t, h, cache.kv_heads, d, longest, ctypes.byref(got))
+    nat.call("ftx_kv8_tree_attention_workspace", b, t, h, cache.kv_heads, d, longest, ctypes.byref(got))
     ws_bytes = int(got.value)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     nat.call("ftx_kv8_tree_attention", ctypes.byref(cache), q.data_ptr(), out.data_ptr(), tree.data_ptr(),

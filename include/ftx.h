@@ -515,7 +515,8 @@ int ftx_token_logprobs(const void *logits, int64_t row_stride, int type, const i
  * whose bit is set in the row's set tree[b][i] (int64, rows tree_stride apart, 0
  * for one tree of all sequences).
  * news: the rows that take part; the others, and rows that see no token, are 0.
- * The rest as ftx_kv8_attention; max_tokens counts the nodes.
+ * The rest as ftx_kv8_attention; max_tokens counts the nodes. workspace:
+ * ftx_kv8_tree_attention_workspace bytes.
  *
  * ftx_kv8_keep: in each of `layers` layers that lie back to back, the token
  * starts[b] + path[b][i] moves to starts[b] + i, for i below news[b] (NULL: n, at
@@ -553,6 +554,8 @@ int ftx_kv8_append_norm(const ftx_kv8_cache *cache, const void *q, const void *k
                         const void *k_weight, float eps, const float *cos, const float *sin, int64_t positions,
                         const int32_t *at, int64_t at_stride, void *q_out, int64_t batch, int64_t t, int heads,
                         const int64_t *strides, void *stream);
+int ftx_kv8_tree_attention_workspace(int64_t batch, int64_t t, int heads, int kv_heads, int d, int64_t max_tokens,
+                                     size_t *bytes);
 int ftx_kv8_tree_attention(const ftx_kv8_cache *cache, const void *q, void *o, const int64_t *tree, int64_t tree_stride,
                            int nodes, int64_t batch, int64_t t, int heads, const int64_t *strides, float scale,
                            int64_t max_tokens, void *workspace, size_t workspace_bytes, void *stream);
