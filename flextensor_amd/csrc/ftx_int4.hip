@@ -19,7 +19,6 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kWave = 64;
@@ -177,35 +176,36 @@ __global__ __launch_bounds__(512) void int4_rows_kernel(Int4Linear p) {
 
 // ---- tiles -----------------------------------------------------------------------------------------------------------
 //
-// TM tokens x TN channels a workgroup, K in steps of 64. A step's x goes straight from memory into one of two stages of
-// LDS, its weights from codes in registers through (c - z) s in fp32, rounded to bf16, into the same stage, once for all
-// the tile's rows; both while the other stage is multiplied, with one barrier a step. Row R's 16-byte chunk c lies at slot
-// c ^ (R / 2 % 8), which spreads the 16 rows that a phase of ds_read_b128 touches over all banks. AHEAD units of codes
-// are in registers or on their way.
+// Up to TM tokens x TN channels a workgroup, K in units of 128: the tokens are dealt evenly to the tiles, in 16s, and
+// products of 16s that a tile does not have are left out (777 rows in four tiles of 208). A unit's x goes straight from memory into one of STAGES stages
+// of LDS while another is multiplied, with one barrier a unit; row R's 16-byte chunk c lies at slot c ^ (R % 16), so the
+// 16 rows that a read touches lie in different banks. The codes go from memory into the registers of the wave that
+// multiplies by them, as the operands that they are, DEPTH units ahead: they take no LDS and no barrier. A wave makes the
+// weights of its channels for the next 32 inputs, (c - z) s in fp32 rounded to bf16, between the products of these ones.
 //
-// Rounding the weights is what lets the matrix cores sum over groups: an error of 2^-9 of each at most, 0.0022 of the
-// result in relative norm where the output's own rounding is 0.0017.
-// v_mfma_f32_32x32x16_bf16 takes the channels as rows and the tokens as columns, so a lane ends with four neighbouring
-// channels of a token at a time; they reach y through LDS, in whole lines.
+// Rounding the weights is what lets the matrix cores sum over groups: an error of 2^-8 of each at most, 0.0022 of the
+// result in relative norm where the output's own rounding is 0.0017. v_mfma_f32_16x16x32_bf16 takes the channels as rows
+// and the tokens as columns, so a lane ends with four neighbouring channels of a token; they reach y through LDS, in whole
+// lines.
 
 // Eight codes as weights, s c + b.
-__device__ __forceinline__ u32x4 weights(uint32_t w, float s, float b) {
+__device__ __forceinline__ bf16x8 weights(uint32_t w, float s, float b) {
   const uint32_t lo = w & 0x0f0f0f0fu, hi = w >> 4 & 0x0f0f0f0fu;
   const auto value = [&](uint32_t v, int byte) { return fmaf(static_cast<float>(v >> (8 * byte) & 255u), s, b); };
-  return (u32x4){pack_bf16(value(lo, 0), value(lo, 2)), pack_bf16(value(hi, 0), value(hi, 2)),
-                 pack_bf16(value(lo, 1), value(lo, 3)), pack_bf16(value(hi, 1), value(hi, 3))};
+  return __builtin_bit_cast(bf16x8, (u32x4){pack_bf16(value(lo, 0), value(lo, 2)), pack_bf16(value(hi, 0), value(hi, 2)),
+                                            pack_bf16(value(lo, 1), value(lo, 3)), pack_bf16(value(hi, 1), value(hi, 3))});
 }
 
-template <int TM, int TN, int WM, int WN, int AHEAD, int PARTS, bool ZERO, bool SPLIT>
-__global__ __launch_bounds__(WM * WN * kWave, 2) void int4_tile_kernel(Int4Linear p) {
-  constexpr int kWaves = WM * WN;
-  constexpr int kStep = 128;                       // bytes of a row: 64 inputs
-  constexpr int kStage = (TM + TN) * kStep;
-  constexpr int kLoads = TM / 8 / kWaves;          // of one wave, 8 rows of x each
-  constexpr int kUnits = TN / 16 / kWaves;         // tiles of 16 channels that one wave makes the weights of
-  constexpr int kMT = TM / WM / 32, kNT = TN / WN / 32;
-  static_assert(TM / 8 % kWaves == 0 && TN / 16 % kWaves == 0, "every wave has the same to load");
-  __shared__ __align__(1024) uint8_t lds[2 * kStage];
+template <int TM, int TN, int WN, int STAGES, int DEPTH, int PARTS, bool ZERO, bool SPLIT>
+__global__ __launch_bounds__(WN * kWave, 2) void int4_tile_kernel(Int4Linear p) {
+  constexpr int kWaves = WN;
+  constexpr int kRow = kUnit * 2;                    // bytes of a row of x in a stage
+  constexpr int kStage = TM * kRow;
+  constexpr int kLoads = kStage / 1024 / kWaves;     // of one wave, four rows of x each
+  constexpr int kMT = TM / 16, kNT = TN / WN / 16;
+  constexpr int kCodeLoads = kNT * (ZERO ? 3 : 2);
+  static_assert(kStage / 1024 % kWaves == 0, "every wave has the same to load");
+  __shared__ __align__(1024) uint8_t lds[STAGES * kStage];
   const uint32_t per_xcd = (p.items + p.xcds - 1) / p.xcds;
   uint32_t item = (blockIdx.x % p.xcds) * per_xcd + blockIdx.x / p.xcds;
   if (blockIdx.x / p.xcds >= per_xcd || item >= p.items) return;
@@ -213,169 +213,149 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void int4_tile_kernel(Int4Linea
   if (SPLIT) item /= static_cast<uint32_t>(p.splits);
   const uint32_t run = item / (p.band * p.n_tiles), at = item - run * p.band * p.n_tiles;
   const uint32_t rows = min(static_cast<uint32_t>(p.band), p.m_tiles - run * p.band);
-  const int64_t m0 = static_cast<int64_t>(uniform(run * p.band + at % rows)) * TM;
+  const int64_t m0 = static_cast<int64_t>(uniform(run * p.band + at % rows)) * p.tile_rows;
   const int64_t n0 = static_cast<int64_t>(uniform(at / rows)) * TN;
 
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int r = lane & 31, g = lane >> 5;
-  const int wm = wave / WN, wn = wave % WN;
+  const int r = lane & 15, q = lane >> 4;
+  const int live = (static_cast<int>(least(p.m - m0, p.tile_rows)) + 15) / 16;  // 16s of tokens that the tile has
 
-  // Load i of a wave brings rows 8 (i kWaves + wave) .. + 7 of 128 bytes; rows past the last and inputs past K are 0.
+  // Load i of a wave brings rows 4 (i kWaves + wave) .. + 3 of 256 bytes; rows past the last and inputs past K are 0.
   const uint8_t *tokens = reinterpret_cast<const uint8_t *>(p.x + m0 * p.x_stride);
   const uint32_t token_bytes = static_cast<uint32_t>(
-      least(((least(p.m - m0, TM) - 1) * p.x_stride + p.k) * 2, 0x7fffffff));
-  uint32_t offset[kLoads];
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int R = (i * kWaves + wave) * 8 + lane / 8;
-    offset[i] = R * static_cast<uint32_t>(p.x_stride * 2) + ((lane % 8) ^ (R / 2 % 8)) * 16;
-  }
-  const auto issue = [&](int step) {
-    uint8_t *base = lds + step % 2 * kStage + wave * 1024;
-    const bool whole = (step + 1) * 64 <= p.k;
+      least(((least(p.m - m0, p.tile_rows) - 1) * p.x_stride + p.k) * 2, 0x7fffffff));
+  const auto issue = [&](int u, int stage) {
+    uint8_t *base = lds + stage * kStage + wave * 1024;
+    const bool whole = (u + 1) * kUnit <= p.k;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int R = (i * kWaves + wave) * 8 + lane / 8;
-      const int chunk = (lane % 8) ^ (R / 2 % 8);
-      load_to_lds(tokens, token_bytes, whole || step * 64 + chunk * 8 < p.k ? offset[i] : 0xf0000000u, step * kStep,
+      const int R = (i * kWaves + wave) * 4 + lane / 16;
+      const int chunk = (lane % 16) ^ (R % 16);
+      const uint32_t offset = R * static_cast<uint32_t>(p.x_stride * 2) + chunk * 16;
+      load_to_lds(tokens, token_bytes, whole || u * kUnit + chunk * 8 < p.k ? offset : 0xf0000000u, u * kRow,
                   base + i * kWaves * 1024);
     }
   };
 
-  struct Unit {  // 128 inputs of a channel each
-    u32x4 w[kUnits];
-    Scales<PARTS> s[kUnits], z[ZERO ? kUnits : 1];
+  struct Unit {  // 128 inputs of the wave's channels
+    u32x4 w[kNT];
+    Scales<PARTS> s[kNT], z[ZERO ? kNT : 1];
   };
-  Unit units[AHEAD];
-  const int64_t tile0 = n0 / 16 + wave;
-  const int cr = lane & 15, cq = lane >> 4;
+  const int64_t tile0 = n0 / 16 + wave * kNT;
   const auto load = [&](Unit &v, int u) {
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-      const int64_t of = least(tile0 + i * kWaves, p.tiles - 1) * p.units + u;
-      v.w[i] = *reinterpret_cast<const u32x4 *>(p.w + of * kUnitBytes + lane * 16);
-      v.s[i].load(p.scale + (of * 16 + cr) * PARTS);
-      if (ZERO) v.z[i].load(p.zero + (of * 16 + cr) * PARTS);
+    for (int t = 0; t < kNT; ++t) {
+      const int64_t of = least(tile0 + t, p.tiles - 1) * p.units + u;
+      v.w[t] = *reinterpret_cast<const u32x4 *>(p.w + of * kUnitBytes + lane * 16);
+      v.s[t].load(p.scale + (of * 16 + r) * PARTS);
+      if (ZERO) v.z[t].load(p.zero + (of * 16 + r) * PARTS);
     }
   };
-  const auto store = [&](const Unit &v, int half) {  // the weights of one step
-#pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-      const int R = (i * kWaves + wave) * 16 + cr;
-      uint8_t *to = lds + half * kStage + (TM + R) * kStep;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int word = 2 * half + j, part = word * PARTS / 4;
-        const float s = v.s[i][part], b = -s * (ZERO ? v.z[i][part] : 8.f);
-        *reinterpret_cast<u32x4 *>(to + ((4 * j + cq) ^ (R / 2 % 8)) * 16) = weights(v.w[i][word], s, b);
-      }
-    }
+  const auto make = [&](const Unit &v, int t, int word) {
+    const int part = word * PARTS / 4;
+    const float s = v.s[t][part];
+    return weights(v.w[t][word], s, -s * (ZERO ? v.z[t][part] : 8.f));
   };
 
-  uint32_t a_at[kNT], b_at[kMT];
+  f32x4 acc[kMT][kNT];
 #pragma unroll
-  for (int i = 0; i < kNT; ++i) a_at[i] = (TM + wn * kNT * 32 + i * 32 + r) * kStep;
+  for (int j = 0; j < kMT; ++j)
 #pragma unroll
-  for (int j = 0; j < kMT; ++j) b_at[j] = (wm * kMT * 32 + j * 32 + r) * kStep;
-  const uint32_t swizzle = r / 2 % 8;
-  f32x16 acc[kNT][kMT];
-#pragma unroll
-  for (int i = 0; i < kNT; ++i)
-#pragma unroll
-    for (int j = 0; j < kMT; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  const auto multiply = [&](int half) {
-    const uint8_t *stage = lds + half * kStage;
-    bf16x8 a[2][kNT], b[2][kMT];  // operands of 16 inputs, the next ones read during this one's products
-    const auto read = [&](int ks) {
-      const uint32_t chunk = ((2 * ks + g) ^ swizzle) * 16;
-#pragma unroll
-      for (int i = 0; i < kNT; ++i) a[ks & 1][i] = *reinterpret_cast<const bf16x8 *>(stage + a_at[i] + chunk);
-#pragma unroll
-      for (int j = 0; j < kMT; ++j) b[ks & 1][j] = *reinterpret_cast<const bf16x8 *>(stage + b_at[j] + chunk);
+    for (int t = 0; t < kNT; ++t) acc[j][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  const uint32_t b_at = r * kRow;
+  const auto multiply = [&](const Unit &v, int stage) {
+    const uint8_t *from = lds + stage * kStage + b_at;
+    const auto read = [&](int n) {  // the nth of the unit's operands: a tile of tokens, 32 inputs
+      return *reinterpret_cast<const bf16x8 *>(from + n % kMT * 16 * kRow + ((n / kMT * 4 + q) ^ r) * 16);
     };
-    read(0);
+    constexpr int kAhead = kMT > 8 ? 5 : 3;
+    bf16x8 a[2][kNT], b[kAhead + 1];
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      if (ks < 3) read(ks + 1);
+    for (int n = 0; n < kAhead; ++n) b[n] = read(n);
 #pragma unroll
-      for (int j = 0; j < kMT; ++j)
+    for (int t = 0; t < kNT; ++t) a[0][t] = make(v, t, 0);
 #pragma unroll
-        for (int i = 0; i < kNT; ++i)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[ks & 1][i], b[ks & 1][j], acc[i][j], 0, 0, 0);
+    for (int n = 0; n < 4 * kMT; ++n) {
+      const int word = n / kMT, j = n % kMT;
+      if (n + kAhead < 4 * kMT) b[(n + kAhead) % (kAhead + 1)] = read(n + kAhead);
+      if (word < 3) {  // a part of the next weights
+#pragma unroll
+        for (int t = j * kNT / kMT; t < (j + 1) * kNT / kMT; ++t) a[(word + 1) % 2][t] = make(v, t, word + 1);
+      }
+      if (j < live) {
+#pragma unroll
+        for (int t = 0; t < kNT; ++t)
+          acc[j][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[word % 2][t], b[n % (kAhead + 1)], acc[j][t], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  // A unit is two steps, the first in stage 0. Weights are made a step ahead: the unit's second half during its first
-  // step, the next unit's first half during its second one.
+  // x of unit u lies in stage u - first modulo STAGES and is on its way STAGES - 1 units ahead, its codes DEPTH - 1 and
+  // a little. Past the last unit it again, so that every round has the same loads in flight.
   const int first = SPLIT ? split * p.split_units : 0;
   const int end = SPLIT ? min(p.units, first + p.split_units) : p.units;
   const auto at_most = [&](int u) { return min(u, end - 1); };
+  Unit units[DEPTH];
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) load(units[i], at_most(first + i));
-  issue(2 * first);
-  store(units[0], 0);
-  for (int u0 = first; u0 < end; u0 += AHEAD) {
+  for (int i = 0; i < STAGES - 1; ++i) issue(at_most(first + i), i);
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const int u = u0 + i;
-      if (u >= end) break;
-      wait_vmcnt<0>();
-      ring_barrier();
-      issue(2 * u + 1);
-      store(units[i], 1);
-      load(units[i], at_most(u + AHEAD));
-      multiply(0);
-      wait_vmcnt<0>();
-      ring_barrier();
-      if (u + 1 < end) {
-        issue(2 * u + 2);
-        store(units[(i + 1) % AHEAD], 0);
-      }
-      multiply(1);
-    }
+  for (int i = 0; i < DEPTH; ++i) load(units[i], at_most(first + i));
+  asm volatile("" ::: "memory");
+  int stage = 0, next = STAGES - 1;
+  const auto round = [&](Unit &v, int u) {
+    // in flight behind x of this unit: the x of STAGES - 2 more, and the codes loaded since
+    if (u == first) wait_vmcnt<0>();
+    else wait_vmcnt<(STAGES - 2) * kLoads + (STAGES - 1) * kCodeLoads>();
+    ring_barrier();
+    issue(at_most(u + STAGES - 1), next);
+    asm volatile("" ::: "memory");
+    multiply(v, stage);
+    load(v, at_most(u + DEPTH));
+    asm volatile("" ::: "memory");
+    stage = stage == STAGES - 1 ? 0 : stage + 1;
+    next = next == STAGES - 1 ? 0 : next + 1;
+  };
+  for (int u0 = first; u0 < end; u0 += DEPTH) {
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i)
+      if (u0 + i < end) round(units[i], u0 + i);
   }
 
   if (SPLIT) {  // sums [split][m][n]
 #pragma unroll
     for (int j = 0; j < kMT; ++j) {
-      const int64_t t = m0 + wm * kMT * 32 + j * 32 + r;
-      if (t >= p.m) continue;
+      const int64_t row = m0 + j * 16 + r;
+      if (j >= live || row >= p.m) continue;
 #pragma unroll
-      for (int i = 0; i < kNT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int64_t ch = n0 + wn * kNT * 32 + i * 32 + 8 * e + 4 * g;
-          if (ch < p.part_stride)
-            *reinterpret_cast<f32x4 *>(p.part + (split * p.m + t) * p.part_stride + ch) =
-                (f32x4){acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
-        }
+      for (int t = 0; t < kNT; ++t) {
+        const int64_t ch = n0 + (wave * kNT + t) * 16 + 4 * q;
+        if (ch < p.part_stride)
+          *reinterpret_cast<f32x4 *>(p.part + (split * p.m + row) * p.part_stride + ch) = acc[j][t];
+      }
     }
     return;
   }
-  // 32 tokens x the wave's channels at a time through this wave's part of LDS, 16 bytes between rows against conflicts
-  constexpr int kPitch = kNT * 64 + 16;
-  static_assert(32 * kPitch * kWaves <= 2 * kStage, "the epilogue fits the stages");
-  __syncthreads();  // the last step has been read
-  uint8_t *mine = lds + wave * 32 * kPitch;
+  // 16 tokens x the wave's channels at a time through this wave's part of LDS, 16 bytes between rows against conflicts
+  constexpr int kPitch = kNT * 32 + 16;
+  static_assert(16 * kPitch * kWaves <= STAGES * kStage, "the epilogue fits the stages");
+  wait_vmcnt<0>();  // what was loaded past the last unit has arrived
+  __syncthreads();  // and the last one has been read
+  uint8_t *mine = lds + wave * 16 * kPitch;
 #pragma unroll
   for (int j = 0; j < kMT; ++j) {
-    const int64_t t0 = m0 + wm * kMT * 32 + j * 32;
-    const int64_t c0 = n0 + wn * kNT * 32;
+    if (j >= live) continue;
+    const int64_t t0 = m0 + j * 16, c0 = n0 + wave * kNT * 16;
 #pragma unroll
-    for (int i = 0; i < kNT; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        *reinterpret_cast<u32x2 *>(mine + r * kPitch + (i * 32 + 8 * e + 4 * g) * 2) =
-            (u32x2){pack_bf16(acc[i][j][4 * e], acc[i][j][4 * e + 1]),
-                    pack_bf16(acc[i][j][4 * e + 2], acc[i][j][4 * e + 3])};
+    for (int t = 0; t < kNT; ++t)
+      *reinterpret_cast<u32x2 *>(mine + r * kPitch + (t * 16 + 4 * q) * 2) =
+          (u32x2){pack_bf16(acc[j][t][0], acc[j][t][1]), pack_bf16(acc[j][t][2], acc[j][t][3])};
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_s_waitcnt(0xc07f);
-    constexpr int kLanes = kNT * 4;  // 16 bytes each, of one token
+    constexpr int kLanes = kNT * 2;  // 16 bytes each, of one token
 #pragma unroll
-    for (int i = 0; i < 32 * kLanes / kWave; ++i) {
+    for (int i = 0; i < (16 * kLanes + kWave - 1) / kWave; ++i) {
       const int row = i * (kWave / kLanes) + lane / kLanes, col = lane % kLanes;
       const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + row * kPitch + col * 16);
       if (t0 + row >= p.m) continue;
@@ -411,12 +391,12 @@ void start_rows(const Int4Linear &p, hipStream_t stream) {
   hipLaunchKernelGGL((int4_rows_kernel<NT, PARTS, ZERO>), dim3(p.items), dim3(512), 0, stream, p);
 }
 
-template <int PARTS, bool ZERO, int TM, int TN, int WM, int WN, int AHEAD>
+template <int PARTS, bool ZERO, int TM, int TN, int WN, int STAGES, int DEPTH>
 void start_tiles(const Int4Linear &p, hipStream_t stream) {
-  const dim3 grid((p.items + p.xcds - 1) / p.xcds * p.xcds), block(WM * WN * kWave);
+  const dim3 grid((p.items + p.xcds - 1) / p.xcds * p.xcds), block(WN * kWave);
   if (p.splits > 1)
-    hipLaunchKernelGGL((int4_tile_kernel<TM, TN, WM, WN, AHEAD, PARTS, ZERO, true>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((int4_tile_kernel<TM, TN, WM, WN, AHEAD, PARTS, ZERO, false>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((int4_tile_kernel<TM, TN, WN, STAGES, DEPTH, PARTS, ZERO, true>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((int4_tile_kernel<TM, TN, WN, STAGES, DEPTH, PARTS, ZERO, false>), grid, block, 0, stream, p);
 }
 
 template <int PARTS, bool ZERO>
@@ -427,14 +407,22 @@ void start(const Int4Linear &p, hipStream_t stream) {
       else if (p.row_tiles == 2) start_rows<PARTS, ZERO, 2>(p, stream);
       else start_rows<PARTS, ZERO, 4>(p, stream);
       break;
-    case 64: start_tiles<PARTS, ZERO, 64, 128, 1, 4, 4>(p, stream); break;
-    case 128: start_tiles<PARTS, ZERO, 128, 128, 2, 2, 2>(p, stream); break;
-    default: start_tiles<PARTS, ZERO, 256, 256, 2, 4, 2>(p, stream); break;
+    case 64: start_tiles<PARTS, ZERO, 64, 128, 4, 3, 4>(p, stream); break;
+    default: start_tiles<PARTS, ZERO, 256, 256, 8, 2, 2>(p, stream); break;
   }
 }
 
 }  // namespace
 
+// Which tiles and how often K is split, by what it costs in 0.01 us: a unit of a tile, more for each 16 tokens that it
+// has; tiles of 256 have a CU to themselves, so theirs come in whole rounds, tiles of 64 share one; reading w; a start,
+// and the join of the splits.
+//                    a unit   a 16   start
+//   64 x 128             65      8     500
+//   256 x 256           120     15    1000
+// Measured, us: 8192 x 28672 of 777 rows 382 in tiles of 256 split in two, 530 in tiles of 64; 28672 x 8192 of 100 rows
+// 103 and 93, of 200 128 and 161, of 512 220 and 308, of 64 rows 60 split in three and 64 unsplit; 4096 x 4096 of 17
+// rows 13.5 split in eight, 20 in four.
 void plan_int4_linear(Int4Linear *p, int cus, int xcds) {
   p->xcds = std::max(1, xcds);
   p->tiles = (p->n + 15) / 16;
@@ -450,15 +438,14 @@ void plan_int4_linear(Int4Linear *p, int cus, int xcds) {
   }
   int64_t best = INT64_MAX, splits = 1;
   int tile_n = 128;
-  const int64_t reading = p->n * p->k / 100000;
-  const auto weigh = [&](int tm, int tn, int64_t alone, int64_t shared, int64_t start_cost) {
-    const int64_t tiles = ((p->m + tm - 1) / tm) * ((p->n + tn - 1) / tn);
-    for (int64_t s = 1; s <= 16 && (s == 1 || p->units / s >= 2); s *= 2) {
-      const int64_t items = tiles * s, length = (p->units + s - 1) / s;
-      const int64_t rounds = (items + cus - 1) / cus;
-      const int64_t products = tm == 256 ? rounds * length * (rounds == 1 ? alone : shared)
-                                         : length * std::max(alone, shared * items / cus);
-      const int64_t cost = std::max(products, reading) + start_cost + (s > 1 ? 250 + p->m * p->n * s / 5000 : 0);
+  const int64_t reading = p->n * p->k / 106000;
+  const auto weigh = [&](int tm, int tn, int64_t unit, int64_t per16, int64_t start) {
+    const int64_t m_tiles = (p->m + tm - 1) / tm, live = ((p->m + 15) / 16 + m_tiles - 1) / m_tiles;
+    const int64_t tiles = m_tiles * ((p->n + tn - 1) / tn);
+    for (int64_t s = 1; s <= 16 && (s == 1 || p->units / s >= 2); s += s < 4 ? 1 : s / 2) {
+      const int64_t items = tiles * s, each = (unit + per16 * live) * ((p->units + s - 1) / s);
+      const int64_t products = tm == 256 ? (items + cus - 1) / cus * each : std::max(each, each * 9 / 10 * items / cus);
+      const int64_t cost = std::max(products, reading) + start + (s > 1 ? 300 + p->m * p->n * s / 10000 : 0);
       if (cost >= best) continue;
       best = cost;
       splits = s;
@@ -466,10 +453,10 @@ void plan_int4_linear(Int4Linear *p, int cus, int xcds) {
       tile_n = tn;
     }
   };
-  weigh(64, 128, 60, 45, 400);
-  if (p->m > 64) weigh(128, 128, 110, 90, 700);
-  if (p->m > 128) weigh(256, 256, 280, 320, 1000);
+  weigh(64, 128, 65, 8, 500);
+  if (p->m > 64) weigh(256, 256, 120, 15, 1000);
   p->m_tiles = static_cast<uint32_t>((p->m + p->tile_m - 1) / p->tile_m);
+  p->tile_rows = static_cast<int>(((p->m + 15) / 16 + p->m_tiles - 1) / p->m_tiles * 16);
   p->n_tiles = static_cast<uint32_t>((p->n + tile_n - 1) / tile_n);
   const uint32_t runs = (p->m_tiles + 11) / 12;
   p->band = static_cast<int>((p->m_tiles + runs - 1) / runs);
