@@ -75,8 +75,11 @@ struct Scales {
 
 // ---- up to 16 rows -------------------------------------------------------------------------------------------------
 //
-// A workgroup owns NT tiles of channels over the whole of K; its eight waves take units in turn, codes and x straight
-// into registers as operands, the next units' on their way, and join their sums through LDS. Bound by the bytes of w.
+// A workgroup a CU walks its share of the tiles of channels, up to NT at a time, over the whole of K; its eight waves take
+// units in turn, codes and x straight into registers as operands, three units in flight across the ends of the chunks, and
+// join their sums through LDS. Bound by the bytes of w: 28672 x 8192 (G 128) of four rows 28 us, 4.3 TB/s where plain
+// reads of as many bytes reach 6.2 (without the products 27); with G 64 and zeros 31 us for one row, 33 for 13; 4096 x 4096
+// of one row 5.5 us.
 //
 // A code becomes the bf16 number 128 + c by an AND and an OR of two codes at a time, exact in the seven bits below the
 // leading one. What that adds comes out again for each group: with a column of ones the matrix cores sum the rows' x in
@@ -85,20 +88,26 @@ struct Scales {
 template <int NT, int PARTS, bool ZERO>
 __global__ __launch_bounds__(512) void int4_rows_kernel(Int4Linear p) {
   constexpr int kWaves = 8, kSteps = 4 / PARTS;  // products of 32 inputs in a group
-  __shared__ f32x4 part[kWaves][NT][kWave];
+  __shared__ f32x4 part[2][kWaves][NT][kWave];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 15, q = lane >> 4;
   const int m = static_cast<int>(p.m);
-  const int64_t tile0 = static_cast<int64_t>(blockIdx.x) * NT;
+  const int64_t tile0 = static_cast<int64_t>(blockIdx.x) * p.tiles / p.items;
+  const int count = static_cast<int>(static_cast<int64_t>(blockIdx.x + 1) * p.tiles / p.items - tile0);
+  const int chunks = (count + NT - 1) / NT, steps = (p.units + kWaves - 1) / kWaves;
+  const auto chunk_at = [&](int i) { return static_cast<int>(static_cast<uint32_t>(i * count) / static_cast<uint32_t>(chunks)); };
   const uint16_t *xr = p.x + min(r, m - 1) * p.x_stride + 8 * q;
 
   struct Unit {
     u32x4 x[4], w[NT];
     Scales<PARTS> s[NT], z[ZERO ? NT : 1];
   };
-  const auto load = [&](Unit &v, int u) {
-    const uint16_t *from = xr + u * kUnit;
+  int load_chunk = 0, load_step = 0, load_first = 0, load_tiles = chunk_at(1);
+  const auto load = [&](Unit &v) {  // the wave's next unit; past K, x is 0 and w the last one
+    if (load_chunk >= chunks) return;
+    const int u = load_step * kWaves + wave, held = min(u, p.units - 1);
+    const uint16_t *from = xr + held * kUnit;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       v.x[i] = (u32x4){0u, 0u, 0u, 0u};
@@ -106,71 +115,80 @@ __global__ __launch_bounds__(512) void int4_rows_kernel(Int4Linear p) {
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int64_t at = least(tile0 + t, p.tiles - 1) * p.units + u;
+      if (t >= load_tiles) continue;
+      const int64_t at = (tile0 + load_first + t) * p.units + held;
       v.w[t] = *reinterpret_cast<const u32x4 *>(p.w + at * kUnitBytes + lane * 16);
       v.s[t].load(p.scale + (at * 16 + r) * PARTS);
       if (ZERO) v.z[t].load(p.zero + (at * 16 + r) * PARTS);
+    }
+    if (++load_step == steps) {
+      load_step = 0;
+      ++load_chunk;
+      load_first += load_tiles;
+      load_tiles = chunk_at(load_chunk + 1) - load_first;
     }
   };
   f32x4 y[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) y[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
   const bf16x8 ones = __builtin_bit_cast(bf16x8, (u32x4){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
-  const auto work = [&](const Unit &v) {
+  int chunk = 0, step = 0, first = 0, tiles = chunk_at(1), side = 0;
+  const auto work = [&](const Unit &v) {  // returns whether it was the last one
 #pragma unroll
     for (int g = 0; g < PARTS; ++g) {
-      f32x4 sum = {0.f, 0.f, 0.f, 0.f}, acc[NT];
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int t = 0; t < NT; ++t) acc[t] = sum;
+      for (int i = g * kSteps; i < (g + 1) * kSteps; ++i)
+        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v.x[i]), ones, sum, 0, 0, 0);
 #pragma unroll
-      for (int i = g * kSteps; i < (g + 1) * kSteps; ++i) {
-        const bf16x8 x = __builtin_bit_cast(bf16x8, v.x[i]);
-        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, ones, sum, 0, 0, 0);
+      for (int t = 0; t < NT; ++t) {
+        if (t >= tiles) continue;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
+        for (int i = g * kSteps; i < (g + 1) * kSteps; ++i) {
           u32x4 c;
 #pragma unroll
           for (int j = 0; j < 4; ++j) c[j] = (v.w[t][i] >> (4 * j) & 0x000f000fu) | 0x43004300u;
-          acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, c), acc[t], 0, 0, 0);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v.x[i]), __builtin_bit_cast(bf16x8, c),
+                                                        acc, 0, 0, 0);
         }
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
         const float s = v.s[t][g], offset = ZERO ? -128.f - v.z[t][g] : -136.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[t][e] = fmaf(s, fmaf(offset, sum[e], acc[t][e]), y[t][e]);
+        for (int e = 0; e < 4; ++e) y[t][e] = fmaf(s, fmaf(offset, sum[e], acc[e]), y[t][e]);
       }
     }
-  };
-  const int n = (p.units - wave + kWaves - 1) / kWaves;  // the wave's units
-  if (n > 0) {
-    const auto nth = [&](int i) { return wave + min(i, n - 1) * kWaves; };  // past the last one it again
-    Unit a, b, c;
-    load(a, nth(0));
-    load(b, nth(1));
-    for (int i = 0;;) {
-      load(c, nth(i + 2));
-      work(a);
-      if (++i >= n) break;
-      load(a, nth(i + 2));
-      work(b);
-      if (++i >= n) break;
-      load(b, nth(i + 2));
-      work(c);
-      if (++i >= n) break;
+    if (++step < steps) return false;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      part[side][wave][t][lane] = y[t];
+      y[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
-  }
+    ring_barrier();  // the other side's sums have been read by all
+    for (int i = threadIdx.x; i < 16 * 16 * tiles; i += 512) {
+      const int ch = i % 16, row = i / 16 % 16, t = i / 256;
+      const int64_t at = (tile0 + first + t) * 16 + ch;
+      if (row >= m || at >= p.n) continue;
+      float all = 0.f;
 #pragma unroll
-  for (int t = 0; t < NT; ++t) part[wave][t][lane] = y[t];
-  __syncthreads();
-  for (int i = threadIdx.x; i < 16 * 16 * NT; i += 512) {
-    const int row = i / (16 * NT), t = i / 16 % NT, ch = i % 16;
-    const int64_t at = (tile0 + t) * 16 + ch;
-    if (row >= m || at >= p.n) continue;
-    float sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) sum += part[w][t][ch + 16 * (row / 4)][row % 4];
-    p.y[row * p.n + at] = static_cast<uint16_t>(pack_bf16(sum, 0.f));
+      for (int w = 0; w < kWaves; ++w) all += part[side][w][t][ch + 16 * (row / 4)][row % 4];
+      p.y[row * p.n + at] = static_cast<uint16_t>(pack_bf16(all, 0.f));
+    }
+    step = 0;
+    side ^= 1;
+    first += tiles;
+    tiles = chunk_at(++chunk + 1) - first;
+    return chunk >= chunks;
+  };
+  Unit a, b, c;
+  load(a);
+  load(b);
+  for (;;) {
+    load(c);
+    if (work(a)) break;
+    load(a);
+    if (work(b)) break;
+    load(b);
+    if (work(c)) break;
   }
 }
 
@@ -432,8 +450,9 @@ void plan_int4_linear(Int4Linear *p, int cus, int xcds) {
   p->part_bytes = 0;
   if (p->m <= 16) {
     p->tile_m = 16;
-    p->row_tiles = p->m > 8 && p->tiles >= 4 * cus ? 4 : p->m > 2 && p->tiles >= 2 * cus ? 2 : 1;
-    p->items = static_cast<uint32_t>((p->tiles + p->row_tiles - 1) / p->row_tiles);
+    p->items = static_cast<uint32_t>(std::min<int64_t>(p->tiles, cus));
+    const int64_t each = p->items > 0 ? (p->tiles + p->items - 1) / p->items : 0;
+    p->row_tiles = each == 1 ? 1 : each == 2 ? 2 : 4;
     return;
   }
   int64_t best = INT64_MAX, splits = 1;
