@@ -919,10 +919,38 @@ __device__ __forceinline__ float code_value(uint32_t byte) {
 // half).
 //
 // NORM: the values are x * f * w first, f = 1 / sqrt(mean x^2 + eps) of their head's row and w the weights.
+template <int D, int N>
+struct Row {  // a thread's values, and the ones that they turn against
+  u32x4 own[N / 8], other[N / 8];
+  __device__ __forceinline__ void load(const uint16_t *x, int d0) {
+    const int from = d0 < D / 2 ? d0 + D / 2 : d0 - D / 2;
+#pragma unroll
+    for (int v = 0; v < N; v += 8) {
+      own[v / 8] = *reinterpret_cast<const u32x4 *>(x + d0 + v);
+      other[v / 8] = *reinterpret_cast<const u32x4 *>(x + from + v);
+    }
+  }
+};
+// v of lane ^ J in a row of 16 lanes, by moves within the vector registers.
+template <int J>
+__device__ __forceinline__ int row_xor(int v) {
+  if constexpr (J == 1) return __builtin_amdgcn_mov_dpp(v, 0xb1, 15, 15, true);  // quad_perm 1 0 3 2
+  if constexpr (J == 2) return __builtin_amdgcn_mov_dpp(v, 0x4e, 15, 15, true);  // quad_perm 2 3 0 1
+  if constexpr (J == 4)                                                          // eights mirrored, then quads
+    return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(v, 0x141, 15, 15, true), 0x1b, 15, 15, true);
+  return __builtin_amdgcn_mov_dpp(v, 0x128, 15, 15, true);  // row_ror 8
+}
+template <int J>
+__device__ __forceinline__ double row_xor(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = row_xor<J>(static_cast<int>(b)), hi = row_xor<J>(static_cast<int>(b >> 32));
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
 template <int D, int N, bool NORM>
 struct Rotation {
   float cos[N], sin[N];
-  float own_w[NORM ? N : 1], other_w[NORM ? N : 1];  // of the values, and of the ones they turn against
+  Row<D, NORM ? N : 8> w;  // the weights
   __device__ __forceinline__ void load(const float *c, const float *s, int d0) {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
@@ -930,51 +958,36 @@ struct Rotation {
       *reinterpret_cast<f32x4 *>(sin + i) = *reinterpret_cast<const f32x4 *>(s + d0 + i);
     }
   }
-  __device__ __forceinline__ void load_weights(const uint16_t *w, int d0) {
-    const int other = d0 < D / 2 ? d0 + D / 2 : d0 - D / 2;
-#pragma unroll
-    for (int v = 0; v < N; v += 8) {
-      const u32x4 a = *reinterpret_cast<const u32x4 *>(w + d0 + v), b = *reinterpret_cast<const u32x4 *>(w + other + v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        own_w[v + i] = bf16_value(a[i / 2] >> (16 * (i & 1)));
-        other_w[v + i] = bf16_value(b[i / 2] >> (16 * (i & 1)));
-      }
-    }
-  }
   // The D / N lanes of a row: its f. The sum is one of 64 bits, in which the squares are exact, and f the nearest fp32
   // number: the codes made from it depend on no order of the sum.
-  __device__ __forceinline__ float factor(const uint16_t *x, int d0, float eps) const {
+  __device__ __forceinline__ float factor(const Row<D, N> &x, float eps) const {
     double sum = 0.0;
 #pragma unroll
-    for (int v = 0; v < N; v += 8) {
-      const u32x4 a = *reinterpret_cast<const u32x4 *>(x + d0 + v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const double value = bf16_value(a[i / 2] >> (16 * (i & 1)));
-        sum = fma(value, value, sum);
-      }
+    for (int i = 0; i < N; ++i) {
+      const double value = bf16_value(x.own[i / 8][i % 8 / 2] >> (16 * (i & 1)));
+      sum = fma(value, value, sum);
     }
-#pragma unroll
-    for (int j = 1; j < D / N; j *= 2) sum += __shfl_xor(sum, j);
+    static_assert(D / N == 4 || D / N == 8 || D / N == 16, "the lanes of a row are within 16");
+    sum += row_xor<1>(sum);
+    sum += row_xor<2>(sum);
+    if constexpr (D / N >= 8) sum += row_xor<4>(sum);
+    if constexpr (D / N >= 16) sum += row_xor<8>(sum);
     const double mean = sum * (1.0 / D) + static_cast<double>(eps);
     const double rough = __builtin_amdgcn_rsq(mean);  // 2^-23 off or less; a step of Newton's: 2^-45
     const double better = fma(0.5 * rough, fma(-mean * rough, rough, 1.0), rough);
     return static_cast<float>(mean > 0.0 && mean < INFINITY ? better : rough);
   }
-  __device__ __forceinline__ void apply(const uint16_t *x, int d0, float *y, float f) const {
+  __device__ __forceinline__ void apply(const Row<D, N> &x, int d0, float *y, float f) const {
 #pragma clang fp contract(off)
-    const int other = d0 < D / 2 ? d0 + D / 2 : d0 - D / 2;
 #pragma unroll
     for (int v = 0; v < N; v += 8) {
-      const u32x4 a = *reinterpret_cast<const u32x4 *>(x + d0 + v), b = *reinterpret_cast<const u32x4 *>(x + other + v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float va = bf16_value(a[i / 2] >> (16 * (i & 1)));
-        float vb = bf16_value(b[i / 2] >> (16 * (i & 1)));
+        float va = bf16_value(x.own[v / 8][i / 2] >> (16 * (i & 1)));
+        float vb = bf16_value(x.other[v / 8][i / 2] >> (16 * (i & 1)));
         if (NORM) {
-          va = va * f * own_w[v + i];
-          vb = vb * f * other_w[v + i];
+          va = va * f * bf16_value(w.own[v / 8][i / 2] >> (16 * (i & 1)));
+          vb = vb * f * bf16_value(w.other[v / 8][i / 2] >> (16 * (i & 1)));
         }
         const float turned = d0 < D / 2 ? -vb : vb;
         const float p = va * cos[v + i], q = turned * sin[v + i];
@@ -1013,14 +1026,15 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
     const bool here = i < span.count && pos < a.positions && (!AT || pos >= 0);
     Rotation<D, 8, NORM> turn;
     if (here) turn.load(a.cos + pos * D, a.sin + pos * D, d0);
-    if (NORM) turn.load_weights(a.q_weight, d0);
+    if constexpr (NORM) turn.w.load(a.q_weight, d0);
     const uint16_t *from = a.q + b * a.q_stride[0] + i * a.q_stride[1];
     uint16_t *to = a.q_out + static_cast<int64_t>(bt) * a.heads * D + d0;
+    Row<D, 8> x;
     for (int head = h0; head < min(h0 + a.heads_each, a.heads); ++head) {
       float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (here) {
-        const uint16_t *x = from + head * a.q_stride[2];
-        turn.apply(x, d0, y, NORM ? turn.factor(x, d0, a.eps) : 1.f);
+        x.load(from + head * a.q_stride[2], d0);
+        turn.apply(x, d0, y, NORM ? turn.factor(x, a.eps) : 1.f);
       }
       *reinterpret_cast<u32x4 *>(to + head * D) =
           (u32x4){pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7])};
@@ -1064,7 +1078,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
   const int64_t head_stride = side == 0 ? a.k_stride[2] : a.v_stride[2];
   Rotation<D, 16, NORM> turn;
   if (fresh && side == 0 && placed) turn.load(a.cos + at * D, a.sin + at * D, 16 * chunk);
-  if (NORM && side == 0) turn.load_weights(a.k_weight, 16 * chunk);
+  if constexpr (NORM)
+    if (side == 0) turn.w.load(a.k_weight, 16 * chunk);
 
   for (int head = h0; head < min(h0 + a.heads_each, a.kv.kv_heads); ++head) {
     const int64_t index = block_index(a.kv, page, side, head, block);
@@ -1076,8 +1091,9 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
       for (int j = 0; j < 16; ++j) y[j] = 0.f;
     } else if (fresh) {
       if (side == 0) {
-        const uint16_t *from = x + head * head_stride;
-        turn.apply(from, 16 * chunk, y, NORM ? turn.factor(from, 16 * chunk, a.eps) : 1.f);
+        Row<D, 16> row;
+        row.load(x + head * head_stride, 16 * chunk);
+        turn.apply(row, 16 * chunk, y, NORM ? turn.factor(row, a.eps) : 1.f);
       } else {
         const uint16_t *from = x + head * head_stride + 16 * chunk;
         const u32x4 w0 = *reinterpret_cast<const u32x4 *>(from), w1 = *reinterpret_cast<const u32x4 *>(from + 8);
