@@ -1169,13 +1169,29 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
 // path reaches into are read into LDS, three at most, and the ones that its tokens move to are made from there, so that
 // none is read after it was written. A block's new scale is the largest of those that its tokens had (of the older ones
 // too); codes that had another are rounded again, and what lies behind the last token becomes 0. A workgroup a head and
-// side of a layer. 32 sequences x 80 layers (8 heads of 128, int8) take 163 us, 4.2 TB/s of the blocks read and written.
+// side of a layer; each thread keeps its part of a block and only takes the moved tokens from LDS, one after the other
+// (gathering all 32 byte by byte: 22 us for one sequence in 32 layers of 32 heads, 8.5 now). 32 sequences x 80 layers (8
+// heads of 128, int8) take 131 us, 5.3 TB/s of the blocks read and written.
+template <bool FP8>
+__device__ __forceinline__ u32x4 again(u32x4 w, float ratio) {  // 16 codes under another scale
+#pragma clang fp contract(off)
+  if (ratio == 1.0f) return w;
+  u32x4 out;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = code_value<FP8>(w[i] >> (8 * e) & 255u) * ratio;
+    out[i] = code4<FP8>(y);
+  }
+  return out;
+}
+
 template <int D, bool FP8>
 __global__ __launch_bounds__(2 * D) void kv8_keep_kernel(Kv8Keep a) {
 #pragma clang fp contract(off)
   constexpr int kBytes = kKvBlock * D, kSources = 3;
   __shared__ __align__(16) uint8_t from[kSources][kBytes];
-  __shared__ int16_t place[kSources][kKvBlock];  // where a token's codes begin in `from`, or -1
   uint32_t item = blockIdx.x;
   const int side = static_cast<int>(item & 1);
   item >>= 1;
@@ -1184,9 +1200,17 @@ __global__ __launch_bounds__(2 * D) void kv8_keep_kernel(Kv8Keep a) {
   const int64_t b = uniform(item % static_cast<uint32_t>(a.batch));
   const int64_t layer = uniform(item / static_cast<uint32_t>(a.batch));
   const int lane = threadIdx.x & (kWave - 1);
+  // three waits for memory: for the sequence, its pages, their codes
+  const int path = a.path[b * a.path_stride + min(lane, a.n - 1)];
   const Span span = span_of(a.kv, b, a.n);
+  if (span.count == 0) return;
+  const int first = span.start / kKvBlock;
+  int pages[kSources];
+#pragma unroll
+  for (int j = 0; j < kSources; ++j)
+    pages[j] = page_of(a.kv, b, min(first + j, a.kv.width * a.kv.page_blocks - 1));
   // the path ends where it does not ascend or leaves the tree or the table
-  const int node = lane < span.count ? a.path[b * a.path_stride + lane] : 0;
+  int node = lane < span.count ? path : 0;
   const int before = __shfl_up(node, 1);
   const int capacity = a.kv.width * a.kv.page_blocks * kKvBlock;
   const bool good = lane < span.count && node >= lane && node < 64 && node < capacity - span.start &&
@@ -1194,66 +1218,82 @@ __global__ __launch_bounds__(2 * D) void kv8_keep_kernel(Kv8Keep a) {
   const uint64_t stop = __ballot(!good);
   const int count = stop ? __builtin_ctzll(stop) : 64;
   if (count == 0) return;
-  const int first = span.start / kKvBlock, last = (span.start + count - 1) / kKvBlock;
+  node = lane < count ? node : 0;
+  const int last = (span.start + count - 1) / kKvBlock;
   const int reach = (span.start + __builtin_amdgcn_readlane(node, count - 1)) / kKvBlock;
   const int64_t layer_block = layer * a.kv.pages * 2 * a.kv.kv_heads * a.kv.page_blocks;
 
   int64_t index[kSources];
   float scale[kSources];
+  u32x4 held[kSources];
 #pragma unroll
   for (int j = 0; j < kSources; ++j) {
-    const int page = first + j <= reach ? page_of(a.kv, b, first + j) : -1;
-    index[j] = page < 0 ? -1 : layer_block + block_index(a.kv, page, side, head, first + j);
-    scale[j] = index[j] < 0 ? 0.f : a.scales[index[j]];
-    u32x4 w = {0u, 0u, 0u, 0u};  // a hole holds zeros
-    if (index[j] >= 0) w = *reinterpret_cast<const u32x4 *>(a.codes + index[j] * kBytes + threadIdx.x * 16);
-    *reinterpret_cast<u32x4 *>(from[j] + threadIdx.x * 16) = w;
+    index[j] = first + j > reach || pages[j] < 0 ? -1 : layer_block + block_index(a.kv, pages[j], side, head, first + j);
+    scale[j] = 0.f;
+    held[j] = (u32x4){0u, 0u, 0u, 0u};  // a hole holds zeros
+    if (index[j] < 0) continue;
+    scale[j] = a.scales[index[j]];
+    held[j] = *reinterpret_cast<const u32x4 *>(a.codes + index[j] * kBytes + threadIdx.x * 16);
   }
-  // a lane a token of the block (both halves of the wave the same ones)
+#pragma unroll
+  for (int j = 0; j < kSources; ++j) *reinterpret_cast<u32x4 *>(from[j] + threadIdx.x * 16) = held[j];
+  // The largest scale of each block's tokens, a lane a token (both halves of the wave the same ones). A thread's 16
+  // bytes are 16 values of a token (keys) or a value of 16 tokens (values): the older tokens' are the ones that it holds.
   float largest[kSources];
+  int source[kSources];  // where the lane's token comes from
 #pragma unroll
   for (int j = 0; j < kSources; ++j) {
     const int token = (first + j) * kKvBlock + lane % kKvBlock, nth = token - span.start;
     const int moved = span.start + __shfl(node, min(max(nth, 0), 63));
-    const int source = nth < 0 ? token : moved;
-    const bool used = nth < count;
-    const int block = source / kKvBlock - first;
+    source[j] = (nth < 0 ? token : moved) - first * kKvBlock;
     float of = 0.f;
 #pragma unroll
     for (int i = 0; i < kSources; ++i)
-      if (used && block == i) of = scale[i];
+      if (nth < count && source[j] / kKvBlock == i) of = scale[i];
 #pragma unroll
     for (int m = 1; m < kKvBlock; m *= 2) of = fmaxf(of, __shfl_xor(of, m));
     largest[j] = of;
-    if (threadIdx.x < kKvBlock)
-      place[j][lane] = static_cast<int16_t>(used ? block * kBytes + source % kKvBlock * (side == 0 ? 16 : 1) : -1);
   }
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kSources; ++j) {
     if (first + j > last || index[j] < 0) continue;
     const float made = largest[j], inverse = made > 0.f ? 1.0f / made : 0.f;
-    float ratio[kSources];
+    const auto ratio = [&](int block) {
+      const float was = block == 0 ? scale[0] : block == 1 ? scale[1] : scale[2];
+      return made > was ? was * inverse : 1.0f;
+    };
+    const int base = (first + j) * kKvBlock;
+    const int lo = max(span.start - base, 0), hi = min(span.start + count - base, kKvBlock);  // moved tokens: lo .. hi - 1
+    u32x4 w = held[j];
+    if (side == 0) {
+      const int token = threadIdx.x % kKvBlock, chunk = threadIdx.x / kKvBlock;
+      if (token >= lo)
+        w = *reinterpret_cast<const u32x4 *>(from[0] + source[j] / kKvBlock * kBytes + chunk * (16 * kKvBlock) +
+                                             source[j] % kKvBlock * 16);
+      w = again<FP8>(w, ratio(source[j] / kKvBlock));
+      if (token >= hi) w = (u32x4){0u, 0u, 0u, 0u};
+    } else {
+      const int half = threadIdx.x % 2 * 16, row = threadIdx.x / 2 * kKvBlock;
+      w = again<FP8>(w, ratio(j));
 #pragma unroll
-    for (int i = 0; i < kSources; ++i) ratio[i] = made > scale[i] ? scale[i] * inverse : 1.0f;
-    const auto ratio_of = [&](int at) { return at < kBytes ? ratio[0] : at < 2 * kBytes ? ratio[1] : ratio[2]; };
-    const uint8_t *codes = &from[0][0];
-    float y[16];
-    if (side == 0) {  // 16 values of one token
-      const int at = place[j][threadIdx.x % kKvBlock];
+      for (int k = 0; k < 4; ++k) {  // the older tokens
+        const int n = lo - half - 4 * k;
+        w[k] &= n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1;
+      }
+      for (int token = lo; token < hi; ++token) {
+        const int s = __builtin_amdgcn_readlane(source[j], token);
+        uint32_t code = from[0][s / kKvBlock * kBytes + row + s % kKvBlock];
+        const float r = ratio(s / kKvBlock);
+        if (r != 1.0f) {
+          const float y[4] = {code_value<FP8>(code) * r, 0.f, 0.f, 0.f};
+          code = code4<FP8>(y) & 255u;
+        }
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        y[e] = at < 0 ? 0.f : code_value<FP8>(codes[at + threadIdx.x / kKvBlock * (16 * kKvBlock) + e]) * ratio_of(at);
-    } else {  // one value of 16 tokens
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int at = place[j][threadIdx.x % 2 * 16 + e];
-        y[e] = at < 0 ? 0.f : code_value<FP8>(codes[at + threadIdx.x / 2 * kKvBlock]) * ratio_of(at);
+        for (int k = 0; k < 4; ++k)
+          if ((token - half) >> 2 == k) w[k] |= code << (8 * (token & 3));
       }
     }
-    u32x4 w;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = code4<FP8>(y + 4 * e);
     *reinterpret_cast<u32x4 *>(a.codes + index[j] * kBytes + threadIdx.x * 16) = w;
     if (threadIdx.x == 0) a.scales[index[j]] = made;
   }
