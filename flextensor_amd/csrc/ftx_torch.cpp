@@ -76,11 +76,6 @@ struct Cache {
   const Tensor *codes, *scales;
 };
 
-// A tensor of rows [batch][n] that are contiguous.
-bool rows_of(const Tensor *t, int64_t batch, int64_t n) {
-  return t && t->dim() == 2 && t->size(0) == batch && t->size(1) == n && t->is_contiguous();
-}
-
 // None, or a whole number that is not negative.
 bool whole(PyObject *o, int64_t *out) {
   if (o == Py_None) return true;
@@ -190,10 +185,14 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
         return other_way();
     const Tensor *positions = nullptr, *weight[2] = {nullptr, nullptr};
     double eps = 0.0;
+    int64_t apart = q.size(1);
     if (n == 16) {
       if (a[10] != Py_None) {
         positions = plain(a[10], device, at::kInt);
-        if (!rows_of(positions, q.size(0), q.size(1))) return other_way();
+        if (!positions || positions->dim() != 2 || positions->size(0) != q.size(0) || positions->size(1) != q.size(1) ||
+            (q.size(1) > 1 && positions->stride(1) != 1) || (q.size(0) > 1 && positions->stride(0) < q.size(1)))
+          return other_way();
+        if (q.size(0) > 1) apart = positions->stride(0);
       }
       if ((a[11] == Py_None) != (a[12] == Py_None)) return other_way();
       for (int i = 0; i < 2 && a[11] != Py_None; ++i) {
@@ -220,7 +219,7 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
       rc = lib.kv8_append_norm(&c.c, q.data_ptr(), x[1]->data_ptr(), x[2]->data_ptr(),
                                weight[0] ? weight[0]->data_ptr() : nullptr, weight[1] ? weight[1]->data_ptr() : nullptr,
                                static_cast<float>(eps), cos->data_ptr<float>(), sin->data_ptr<float>(), cos->size(0),
-                               positions ? positions->data_ptr<int32_t>() : nullptr, q.size(1), out.data_ptr(), q.size(0),
+                               positions ? positions->data_ptr<int32_t>() : nullptr, apart, out.data_ptr(), q.size(0),
                                q.size(1), static_cast<int>(q.size(2)), stride, stream_of(a[15]));
     return result(rc, std::move(out));
   });

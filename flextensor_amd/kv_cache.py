@@ -8,11 +8,13 @@ would otherwise stream. One layer is two tensors:
   [d, 32], the order in which the matrix cores take them.
 * ``scales`` [pages, 2, kv heads, blocks of a page], fp32: a code ``c`` of a block stands for ``c * scale``.
 
-:func:`append` rotates new queries and keys and writes keys and values, :func:`attention` attends over the cache,
-:func:`copy_pages` copies pages; each takes the sequences' page ``table`` (int32; a number outside the pool is a hole
-whose tokens are not seen), the tokens that each has cached (``starts``) and the new ones it adds (``new``) as device
-tensors, so a captured graph follows them. :class:`PagedKVCache` owns the pool of all layers and its bookkeeping:
-sequences, shared pages, forks, truncation and compaction.
+:func:`append` rotates new queries and keys (normalised head by head first, where a model does so) and writes keys and
+values, :func:`attention` attends over the cache, :func:`tree_attention` lets drafted tokens that form a tree attend over
+it and their ancestors, :func:`keep` moves the accepted ones up, :func:`copy_pages` copies pages; each takes the
+sequences' page ``table`` (int32; a number outside the pool is a hole whose tokens are not seen), the tokens that each has
+cached (``starts``) and the new ones it adds (``new``) as device tensors, so a captured graph follows them.
+:class:`PagedKVCache` owns the pool of all layers and its bookkeeping: sequences, shared pages, forks, drafted trees,
+truncation and compaction.
 """
 
 from __future__ import annotations
@@ -401,16 +403,91 @@ class KVLayer:
     step: KVStep
     index: int
 
-    def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
-               sin: torch.Tensor) -> torch.Tensor:
+    def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+               **norms) -> torch.Tensor:
+        """``norms``: q_norm, k_norm and eps of :func:`append`."""
         s = self.step
         s.check(q.shape[0], q.shape[1], cos.shape[0])
-        return append(q, k, v, cos, sin, s.cache.codes[self.index], s.cache.scales[self.index], s.table, s.starts, s.new)
+        return append(q, k, v, cos, sin, s.cache.codes[self.index], s.cache.scales[self.index], s.table, s.starts, s.new,
+                      **norms)
 
     def attend(self, q: torch.Tensor) -> torch.Tensor:
         s = self.step
         return attention(q, s.cache.codes[self.index], s.cache.scales[self.index], s.table, s.starts, s.new,
                          max_tokens=s.max_tokens)
+
+
+@dataclass(frozen=True)
+class KVTree:
+    """Drafted tokens behind the cached ones of some sequences, a tree of one shape each: what the passes over them share.
+    :meth:`nodes` is the step of some of the nodes."""
+
+    cache: "PagedKVCache"
+    step: KVStep  # of all the nodes, as if they were a chain
+    parents: tuple[int, ...]
+    depths: tuple[int, ...]
+    sets: torch.Tensor  # int64 [1, nodes]: the nodes that each one sees
+    starts: torch.Tensor  # int32 [nodes, batch]: how many first tokens and nodes come before each
+    positions: torch.Tensor  # int32 [batch, nodes]
+
+    def nodes(self, first: int = 0, last: int | None = None) -> "KVNodes":
+        """The step of nodes ``first`` .. ``last - 1`` (None: all that follow); the ones before are in the cache."""
+        last = len(self.parents) if last is None else last
+        if not 0 <= first < last <= len(self.parents):
+            raise ValueError(f"nodes {first} to {last} of a tree of {len(self.parents)}")
+        return KVNodes(self, first, last)
+
+    def levels(self) -> list[tuple[int, int]]:
+        """The nodes of each depth as ranges, where the tree lists them so."""
+        if list(self.depths) != sorted(self.depths):
+            raise ValueError("the tree does not list its nodes level by level")
+        return [(self.depths.index(d), self.depths.index(d) + self.depths.count(d)) for d in sorted(set(self.depths))]
+
+
+@dataclass(frozen=True)
+class KVNodes:
+    """Some nodes of drafted trees as the step of a forward pass."""
+
+    tree: KVTree
+    first: int
+    last: int
+
+    @property
+    def counts(self) -> tuple[int, ...]:
+        return (self.last - self.first,) * len(self.tree.step.sequences)
+
+    def layer(self, index: int) -> "KVTreeLayer":
+        return KVTreeLayer(self, index)
+
+    def check(self, batch: int, tokens: int, positions: int) -> None:
+        """Refuses a pass of [batch, tokens] rows that are not the nodes, or whose rotary tables end before them."""
+        step = self.tree.step
+        if (batch, tokens) != (len(step.sequences), self.last - self.first):
+            raise ValueError(f"the step has nodes {self.first} to {self.last} of {len(step.sequences)} trees, the pass "
+                             f"{tokens} of {batch}")
+        deepest = max((was[0] for was in step.held), default=0) + max(self.tree.depths[self.first: self.last])
+        if deepest >= positions:
+            raise ValueError(f"the trees reach position {deepest}, the model has {positions}")
+
+
+@dataclass(frozen=True)
+class KVTreeLayer(KVLayer):
+    """One layer of the cache in a step of a tree's nodes."""
+
+    step: KVNodes
+
+    def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+               **norms) -> torch.Tensor:
+        s, t = self.step, self.step.tree
+        s.check(q.shape[0], q.shape[1], cos.shape[0])
+        return append(q, k, v, cos, sin, t.cache.codes[self.index], t.cache.scales[self.index], t.step.table,
+                      t.starts[s.first], positions=t.positions[:, s.first: s.last], **norms)
+
+    def attend(self, q: torch.Tensor) -> torch.Tensor:
+        s, t = self.step, self.step.tree
+        return tree_attention(q, t.cache.codes[self.index], t.cache.scales[self.index], t.step.table, t.starts[0],
+                              t.sets[:, s.first: s.last].expand(q.shape[0], -1), nodes=s.last,
+                              max_tokens=t.step.max_tokens - len(t.parents) + s.last)
 
 
 class PagedKVCache:
@@ -419,8 +496,9 @@ class PagedKVCache:
     A sequence is a number from :meth:`open`. :meth:`begin` reserves pages for its next tokens and returns the
     :class:`KVStep` that the layers' calls take; :meth:`commit` counts those tokens as cached once the pass has been
     queued. :meth:`fork` gives a sequence's pages to another one too: full pages stay shared, and the page that one
-    of them writes into next is copied first. :meth:`truncate` drops a sequence's last tokens, :meth:`close` all of
-    it. :meth:`compact` moves the pages in use to the pool's start and :meth:`resize` then gives the rest back.
+    of them writes into next is copied first. :meth:`draft` reserves pages for a tree of drafted tokens behind each
+    sequence, and :meth:`accept` keeps one path of each. :meth:`truncate` drops a sequence's last tokens, :meth:`close`
+    all of it. :meth:`compact` moves the pages in use to the pool's start and :meth:`resize` then gives the rest back.
 
     The bookkeeping is the host's; every device operation runs on torch's current stream, which must be the same
     one, or ordered, from call to call.
@@ -566,13 +644,59 @@ class PagedKVCache:
     def commit(self, step: KVStep) -> None:
         """Counts a step's tokens as cached. A step counts once, and only where its sequences are as they were when it
         began: not truncated or closed, and the pages that it wrote still theirs (or moved by :meth:`compact`)."""
+        self._check_step(step)
+        for s, c in zip(step.sequences, step.counts):
+            self._lengths[s] += c
+
+    def _check_step(self, step: KVStep) -> None:
         moved = step.moves != self._moves
         if step.cache is not self or any(
                 self._lengths.get(s) != was[0] or not moved and self._state(s, c) != was
                 for s, c, was in zip(step.sequences, step.counts, step.held)):
             raise ValueError("the step was committed before, or its sequences have changed since it began")
-        for s, c in zip(step.sequences, step.counts):
-            self._lengths[s] += c
+
+    def draft(self, sequences: list[int], parents: list[int]) -> KVTree:
+        """Reserves pages for a tree of drafted tokens behind each sequence. ``parents[i]``: the node before node i, a
+        lower number, or -1 for one that follows the cached tokens; 64 nodes at most. A node sees the cached tokens, its
+        ancestors and itself, and has the position that its depth gives it."""
+        parents = list(parents)
+        n, b = len(parents), len(sequences)
+        if not 1 <= n <= nat.KV8_TREE_NODES or any(not -1 <= p < i for i, p in enumerate(parents)):
+            raise ValueError(f"a tree has 1 to {nat.KV8_TREE_NODES} nodes, each behind its parent, got {parents}")
+        sets, depths = [], []
+        for i, p in enumerate(parents):
+            sets.append(1 << i | (sets[p] if p >= 0 else 0))
+            depths.append(depths[p] + 1 if p >= 0 else 0)
+        step = self.begin(sequences, n)
+        lengths = [self._lengths[s] for s in sequences]
+        host = torch.tensor([x + d for x in lengths for d in depths] + [x + i for i in range(n) for x in lengths],
+                            dtype=torch.int32)
+        masks = torch.tensor([[s - (1 << 64) if s >> 63 else s for s in sets]], dtype=torch.int64)
+        at = host.to(self.device)
+        return KVTree(self, step, tuple(parents), tuple(depths), masks.to(self.device), at[b * n:].view(n, b),
+                      at[: b * n].view(b, n))
+
+    def accept(self, tree: KVTree, paths: list[list[int]]) -> None:
+        """Counts one path of each tree as cached, in the order of its nodes (each the child of the one before; empty:
+        none), and moves its keys and values to follow the sequence's tokens. Conditions as for :meth:`commit`."""
+        step = tree.step
+        if len(paths) != len(step.sequences):
+            raise ValueError(f"{len(paths)} paths for {len(step.sequences)} sequences")
+        for path in paths:
+            if any(not 0 <= n < len(tree.parents) or tree.parents[n] != before for n, before in zip(path, [-1, *path])):
+                raise ValueError(f"{path} is no path of the tree {list(tree.parents)}")
+        self._check_step(step)
+        b, n, width = len(paths), max(map(len, paths), default=0), step.table.shape[1]
+        if any(path != list(range(len(path))) for path in paths):  # others are where they belong
+            pages = [p for s in step.sequences  # as they are now: compact may have moved them
+                     for p in self._pages[s][:width] + [-1] * (width - len(self._pages[s]))]
+            host = torch.tensor([len(p) for p in paths] + [x for p in paths for x in [*p, *[0] * (n - len(p))]] + pages,
+                                dtype=torch.int32)
+            dev = host.to(self.device)  # one upload
+            keep(self.codes, self.scales, dev[b + b * n:].view(b, width), tree.starts[0], dev[b: b + b * n].view(b, n),
+                 dev[:b])
+        for s, path in zip(step.sequences, paths):
+            self._lengths[s] += len(path)
 
     def compact(self) -> int:
         """Moves pages in use to the pool's start, the fewest that leave no free page before them, and returns how

@@ -39,7 +39,8 @@ def init_normal_(model: nn.Module, seed: int, std: float = 0.02, init_device: st
     An ``Fp8Linear`` draws its weight the same way, then stores it as
     float8_e4m3fn with a per-output-channel scale ``absmax / 448`` (bf16); the
     quantised weight is ``round_e4m3(w / scale)``. An ``Int8Linear``'s is
-    ``round(w / scale)`` with ``absmax / 127`` (fp32).
+    ``round(w / scale)`` with ``absmax / 127`` (fp32), an ``Int4Linear``'s the
+    same with ``absmax / 7`` of each group of inputs (bf16).
     """
     gen = torch.Generator(device=init_device).manual_seed(seed)
     with torch.no_grad():
@@ -57,6 +58,10 @@ def init_normal_(model: nn.Module, seed: int, std: float = 0.02, init_device: st
                 scale = (w.abs().amax(dim=1) / INT8_MAX).clamp_min(1e-12)
                 mod.weight.copy_((w / scale[:, None]).round().to(torch.int8))
                 mod.scale.copy_(scale)
+                continue
+            if isinstance(mod, Int4Linear):
+                w = torch.empty(mod.out_features, mod.in_features, dtype=torch.float32, device=init_device)
+                mod.quantize_(w.normal_(0.0, std, generator=gen))
                 continue
             for p in mod.parameters(recurse=False):
                 w = torch.empty(p.shape, dtype=torch.float32, device=init_device)
@@ -116,14 +121,21 @@ class LlamaShape:
     rope_theta: float = 10000.0
     fp8: bool = False  # projection weights in float8_e4m3fn with per-output-channel bf16 scales
     int8: bool = False  # projection weights and their inputs in 8-bit integers, fp32 scales per channel and per token
+    int4: bool = False  # projection weights in 4 bits with bf16 scales for groups of a channel's inputs
+    qk_norm: bool = False  # queries and keys normalised head by head before they are rotated
 
     def layer_bytes(self, itemsize: int = 2) -> int:
         h, d = self.hidden, self.head_dim
         mats = h * self.n_heads * d + 2 * h * self.n_kv_heads * d + self.n_heads * d * h + 3 * h * self.inter
+        norms = 2 * h + (2 * d if self.qk_norm else 0)
+        if self.int4:
+            shapes = [(h, self.n_heads * d), *[(h, self.n_kv_heads * d)] * 2, (self.n_heads * d, h),
+                      *[(h, self.inter)] * 2, (self.inter, h)]
+            return sum(Int4Linear.nbytes(*shape) for shape in shapes) + 2 * norms
         if self.fp8 or self.int8:
             outs = self.n_heads * d + 2 * self.n_kv_heads * d + h + 2 * self.inter + h
-            return mats + (2 if self.fp8 else 4) * outs + 2 * 2 * h
-        return itemsize * (mats + 2 * h)
+            return mats + (2 if self.fp8 else 4) * outs + 2 * norms
+        return itemsize * (mats + norms)
 
 
 LLAMA_7B = LlamaShape()
@@ -236,6 +248,74 @@ class Int8Linear(nn.Module):
         return y
 
 
+class Int4Linear(nn.Module):
+    """y = x @ W^T with W = scale * (code - zero): 4-bit codes, a bf16 scale (and zero, 8 without) for each group of 128
+    (64 or 32, as they divide) inputs of a channel, packed as :func:`hip.int4_pack` does.
+
+    On the GPU (bf16 inputs) the library's kernels run. Other calls multiply by the weights in float32, through which x
+    gets its gradient.
+    """
+
+    def __init__(self, in_features: int, out_features: int, zeros: bool = False) -> None:
+        super().__init__()
+        self.in_features, self.out_features = in_features, out_features
+        tiles, units, parts = self._cells(in_features, out_features)
+        self.weight = nn.Parameter(torch.empty(tiles, units, 1024, dtype=torch.uint8), requires_grad=False)
+        self.scale = nn.Parameter(torch.ones(tiles, units, 16, parts, dtype=torch.bfloat16), requires_grad=False)
+        zero = torch.full((tiles, units, 16, parts), 8.0, dtype=torch.bfloat16)
+        self.register_parameter("zero", nn.Parameter(zero, requires_grad=False) if zeros else None)
+
+    @staticmethod
+    def _cells(in_features: int, out_features: int) -> tuple[int, int, int]:
+        """Tiles, units and groups of a unit; the groups are the largest that divide the inputs."""
+        group = next((g for g in reversed(hip.INT4_GROUPS) if in_features > 0 and in_features % g == 0), 0)
+        if not group:
+            raise ValueError(f"4-bit weights have groups of 32 inputs or more, {in_features} are no multiple")
+        return -(-out_features // hip.nat.INT4_TILE), -(-in_features // hip.nat.INT4_UNIT), hip.nat.INT4_UNIT // group
+
+    @classmethod
+    def nbytes(cls, in_features: int, out_features: int) -> int:
+        """Bytes of a layer without zeros."""
+        tiles, units, parts = cls._cells(in_features, out_features)
+        return tiles * units * (1024 + 2 * 16 * parts)
+
+    @torch.no_grad()
+    def quantize_(self, w: torch.Tensor) -> None:
+        """Takes weights [out_features, in_features]: the nearest codes under a scale of ``absmax / 7`` for each group, or
+        with zeros under ``(max - min) / 15`` and the zero that gives the least weight code 0."""
+        if w.shape != (self.out_features, self.in_features):
+            raise ValueError(f"weights [{self.out_features}, {self.in_features}] expected, got {tuple(w.shape)}")
+        grouped = w.float().unflatten(1, (-1, hip.nat.INT4_UNIT // self.scale.shape[3]))
+        zero: torch.Tensor | float = 8.0
+        if self.zero is None:
+            scale = (grouped.abs().amax(-1) / 7.0).clamp_min(1e-12).to(torch.bfloat16)
+        else:
+            least = grouped.amin(-1)
+            scale = ((grouped.amax(-1) - least) / 15.0).clamp_min(1e-12).to(torch.bfloat16)
+            zero = (-least / scale.float()).to(torch.bfloat16)
+        shift = zero.float()[..., None] if isinstance(zero, torch.Tensor) else zero
+        codes = (grouped / scale.float()[..., None] + shift).round().clamp_(0, 15).flatten(1).to(torch.uint8)
+        packed = hip.int4_pack(codes, scale, zero if isinstance(zero, torch.Tensor) else None)
+        for held, new in zip((self.weight, self.scale, self.zero), packed):
+            if held is not None:
+                held.copy_(new)
+
+    def kernel_eligible(self, x: torch.Tensor) -> bool:
+        """Whether the library kernels take this call: non-empty bf16 rows, and a contiguous, 16-byte aligned weight, scale
+        and zero (``raw_block_transfer`` packs weights back to back without alignment)."""
+        held = (self.scale,) if self.zero is None else (self.scale, self.zero)
+        k = x.shape[-1]
+        return (x.numel() > 0 and k == self.in_features and k <= hip.INT4_MAX_K and hip.kernel_call(x, *held)
+                and x.numel() // k < 1 << 24 and hip._packed(self.weight, *held))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.kernel_eligible(x):
+            y = hip.int4_linear(x.reshape(-1, self.in_features), self.weight, self.scale, self.zero, self.out_features)
+            return y.view(*x.shape[:-1], self.out_features)
+        w = hip.int4_dequantize(self.weight, self.scale, self.zero, self.out_features, self.in_features)
+        return F.linear(x.float(), w).to(x.dtype)
+
+
 class Linear(nn.Linear):
     """``nn.Linear`` whose forward on a few bf16 GPU rows (a decode batch) is the library's one-launch kernel."""
 
@@ -340,6 +420,8 @@ def linear_residual(x: torch.Tensor, lin: nn.Module, residual: torch.Tensor) -> 
 
 
 def _proj(s: LlamaShape, n_in: int, n_out: int, dtype: torch.dtype) -> nn.Module:
+    if s.int4:
+        return Int4Linear(n_in, n_out)
     if s.int8:
         return Int8Linear(n_in, n_out)
     return Fp8Linear(n_in, n_out) if s.fp8 else Linear(n_in, n_out, bias=False, dtype=dtype)
@@ -376,6 +458,8 @@ class Attention(nn.Module):
         self.wk = _proj(s, s.hidden, s.n_kv_heads * s.head_dim, dtype)
         self.wv = _proj(s, s.hidden, s.n_kv_heads * s.head_dim, dtype)
         self.wo = _proj(s, s.n_heads * s.head_dim, s.hidden, dtype)
+        self.q_norm = RMSNorm(s.head_dim, s.eps, dtype) if s.qk_norm else None
+        self.k_norm = RMSNorm(s.head_dim, s.eps, dtype) if s.qk_norm else None
 
     def forward(self, x: torch.Tensor, pos: int, cos: torch.Tensor, sin: torch.Tensor,
                 cache_k: torch.Tensor | kv_cache.KVLayer, cache_v: torch.Tensor | None,
@@ -390,8 +474,17 @@ class Attention(nn.Module):
         q = q.view(b, t, s.n_heads, s.head_dim)
         k = k.view(b, t, s.n_kv_heads, s.head_dim)
         v = v.view(b, t, s.n_kv_heads, s.head_dim)
+        norms = {}
+        if self.q_norm is not None and self.k_norm is not None:
+            # The paged cache's launch normalises too, where calling the norms would run nothing else.
+            weights = self.q_norm.weight, self.k_norm.weight
+            if (isinstance(cache_k, kv_cache.KVLayer) and _plain_call(self.q_norm) and _plain_call(self.k_norm)
+                    and hip.kernel_call(q, *weights) and hip._packed(*weights)):
+                norms = {"q_norm": weights[0], "k_norm": weights[1], "eps": s.eps}
+            else:
+                q, k = self.q_norm(q), self.k_norm(k)
         if isinstance(cache_k, kv_cache.KVLayer):
-            o = cache_k.attend(cache_k.append(q, k, v, cos, sin))
+            o = cache_k.attend(cache_k.append(q, k, v, cos, sin, **norms))
             return self._output(o.view(b, t, s.n_heads * s.head_dim), residual)
         o = hip.rope_attention(q, k, v, cos, sin, pos, cache_k, cache_v)
         if o is not None:
@@ -480,9 +573,11 @@ class LlamaModel(nn.Module):
         s = self.shape
         return kv_cache.PagedKVCache(s.n_layers, s.n_kv_heads, s.head_dim, pages, page_tokens, dtype, device)
 
-    def forward(self, tokens: torch.Tensor, pos: int = 0, step: kv_cache.KVStep | None = None) -> torch.Tensor:
+    def forward(self, tokens: torch.Tensor, pos: int = 0, step: kv_cache.KVStep | kv_cache.KVNodes | None = None,
+                every: bool = False) -> torch.Tensor:
         """Logits of the last position, float32. With a ``step`` of a paged cache the tokens are its sequences' next
-        ones (``pos`` does not matter), and the logits those of each sequence's last token in the step."""
+        ones, or nodes of their trees (``pos`` does not matter), and the logits those of each sequence's last token in the
+        step. With ``every`` the logits of all positions, in the weights' type."""
         if step is not None:
             step.check(*tokens.shape, self.rope_cos.shape[0])
         x = self.embed(tokens)
@@ -491,6 +586,8 @@ class LlamaModel(nn.Module):
                 x = layer(x, pos, self.rope_cos, self.rope_sin, step.layer(i), None)
             else:
                 x = layer(x, pos, self.rope_cos, self.rope_sin, self.cache_k[i], self.cache_v[i])
+        if every:
+            return self.lm_head(self.norm(x))
         if step is not None and min(step.counts, default=x.shape[1]) < x.shape[1]:
             last = (step.new.long() - 1).clamp_min(0).view(-1, 1, 1).expand(-1, 1, x.shape[2])
             x = x.gather(1, last)
@@ -564,6 +661,107 @@ def generate_paged(model: LlamaModel, cache: kv_cache.PagedKVCache, prompts: lis
             cache.close(s)
         raise
     return sequences, torch.cat(out, dim=1), all_logits
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0
+                   ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """:func:`hip.token_logprobs` of logits [..., vocab] and tokens [...]; the results have the tokens' shape, the last two
+    with [top] behind it. On the host torch operations."""
+    shape, vocab = tokens.shape, logits.shape[-1]
+    rows, flat = logits.reshape(-1, vocab), tokens.reshape(-1)
+    if rows.is_cuda:
+        given, entropy, best, index = hip.token_logprobs(rows, flat, top)
+    else:
+        logp = torch.log_softmax(rows.float(), -1)
+        given = logp.gather(1, flat.clamp(0, vocab - 1)[:, None])[:, 0]
+        given = torch.where(flat < 0, 0.0, torch.where(flat < vocab, given, float("nan")))
+        entropy = -(logp.exp() * torch.where(logp == float("-inf"), 0.0, logp)).sum(-1)
+        index = torch.sort(rows, dim=-1, descending=True, stable=True).indices[:, :top]
+        best = logp.gather(1, index)
+    return given.view(shape), entropy.view(shape), best.reshape(*shape, top), index.reshape(*shape, top)
+
+
+@torch.no_grad()
+def score(model: LlamaModel, tokens: torch.Tensor, top: int = 0
+          ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """What the model makes of tokens [batch, t], as :func:`token_logprobs` returns it for the places [batch, t - 1] behind
+    the first: the log probability of the token there, the entropy, and the ``top`` likeliest tokens. Uses the model's own
+    cache (:meth:`LlamaModel.init_cache`)."""
+    logits = model(tokens, 0, every=True)
+    return token_logprobs(logits[:, :-1], tokens[:, 1:], top)
+
+
+DRAFT_TREE = (-1, 0, 0, 1, 1, 2, 3, 3, 5, 6, 9)  # the likeliest chain of five, and siblings near the root
+
+
+@torch.no_grad()
+def generate_drafted(model: LlamaModel, draft: LlamaModel, cache: kv_cache.PagedKVCache,
+                     draft_cache: kv_cache.PagedKVCache, prompts: list[list[int]], steps: int,
+                     parents: tuple[int, ...] = DRAFT_TREE) -> tuple[torch.Tensor, torch.Tensor, int]:
+    """Greedy decoding over paged 8-bit caches, several tokens for each pass of ``model``: ``draft``, a smaller model of
+    the same vocabulary, proposes a tree of tokens behind each sequence, and one pass of ``model`` checks all of its nodes.
+
+    ``parents``: the tree. Node 0 is a sequence's newest token, the others follow level by level; the children of a node
+    are the likeliest tokens behind it, in this order. Returns the tokens [prompts, steps], their log probabilities under
+    ``model``, and how many passes it made, the prompts' included. Caches and rotary tables need room for a tree's nodes
+    beyond the last token; the sequences are closed at the end.
+    """
+    device = model.rope_cos.device
+    n = len(parents)
+    if not parents or parents[0] != -1 or -1 in parents[1:]:
+        raise ValueError(f"a tree has one root, its first node, got {list(parents)}")
+    children = [[c for c, p in enumerate(parents) if p == node] for node in range(n)]
+    width = max(map(len, children))
+    rank = [children[p].index(c) for c, p in enumerate(parents) if p >= 0]
+    before, rank_of = torch.tensor([[-1, *parents[1:]], [0, *rank]], device=device)
+    tokens = torch.tensor([p + [0] * (max(map(len, prompts)) - len(p)) for p in prompts], device=device)
+    opened: list[tuple[kv_cache.PagedKVCache, int]] = []
+
+    def prompt_pass(m: LlamaModel, c: kv_cache.PagedKVCache) -> tuple[list[int], torch.Tensor]:
+        sequences = [c.open() for _ in prompts]
+        opened.extend((c, s) for s in sequences)
+        step = c.begin(sequences, [len(p) for p in prompts])
+        logits = m(tokens, step=step)
+        c.commit(step)
+        return sequences, logits
+
+    def likeliest(logits: torch.Tensor, top: int) -> tuple[torch.Tensor, torch.Tensor]:
+        return token_logprobs(logits, torch.full(logits.shape[:2], -1, device=device), top)[2:]
+
+    try:
+        drafted, _ = prompt_pass(draft, draft_cache)
+        sequences, logits = prompt_pass(model, cache)
+        logp, best = likeliest(logits, 1)
+        out, logps = best[:, 0].tolist(), logp[:, 0].tolist()
+        passes = 1
+        while active := [i for i in range(len(prompts)) if len(out[i]) < steps]:
+            nodes = torch.zeros(len(active), n, dtype=torch.int64, device=device)
+            nodes[:, 0] = torch.tensor([out[i][-1] for i in active], device=device)
+            proposed = draft_cache.draft([drafted[i] for i in active], parents)
+            levels = proposed.levels()
+            for (lo, hi), (_, end) in zip(levels, [*levels[1:], (n, n)]):  # the last level too: its tokens may be kept
+                logits = draft(nodes[:, lo:hi], step=proposed.nodes(lo, hi), every=True)
+                if end > hi:
+                    _, best = likeliest(logits, width)
+                    nodes[:, hi:end] = best[:, before[hi:end] - lo, rank_of[hi:end]]
+            checked = cache.draft([sequences[i] for i in active], parents)
+            logp, best = likeliest(model(nodes, step=checked.nodes(), every=True), 1)
+            passes += 1
+            guesses, answers, scores = nodes.tolist(), best[..., 0].tolist(), logp[..., 0].tolist()
+            paths = []
+            for row, i in enumerate(active):
+                path = [0]
+                while match := [c for c in children[path[-1]] if guesses[row][c] == answers[row][path[-1]]]:
+                    path.append(match[0])
+                out[i] += [answers[row][node] for node in path]  # the tokens behind the path's nodes; the last is new
+                logps[i] += [scores[row][node] for node in path]
+                paths.append(path)
+            cache.accept(checked, paths)
+            draft_cache.accept(proposed, paths)
+    finally:
+        for c, s in opened:
+            c.close(s)
+    return torch.tensor([o[:steps] for o in out]), torch.tensor([x[:steps] for x in logps]), passes
 
 
 def prompt_tokens(batch: int, length: int, vocab: int, seed: int = 0) -> torch.Tensor:
