@@ -203,6 +203,7 @@ struct Kv8Attention {
   // planned
   int rep, rows, row_tiles, splits, chunk, xcds;  // chunk: blocks of a split
   int tile_rows;          // up to 16 or 32: the kernel of few rows; else the prompts'
+  int part_rows;          // of a tile that exist
   int64_t tile_items;     // batch * kv heads * row tiles
   uint32_t items;         // times the splits
   size_t part_bytes;

@@ -199,6 +199,87 @@ __device__ __forceinline__ int tile_blocks(const Kv8Attention &a, Span s, int ti
   return (s.start + last) / kKvBlock + 1;
 }
 
+// How a batch's trees are dealt to workgroups, in tiles of 64 keys: sequence by sequence, of each its heads, of a head
+// its tiles of rows, of those the keys. `before`: the tiles of the sequences before b; `own`: b's.
+struct Share {
+  uint32_t at, end, before, own;
+  int64_t b;
+};
+struct Piece {  // the part of a share in one head and tile of rows
+  Span span;
+  int kvh, tile, blocks, tiles, offset, n;
+};
+struct Join {  // what a share leaves to be joined: the pieces of the head that it begins and does not end, or 0
+  int b, kvh, tile, pieces;
+};
+__device__ __forceinline__ Join *joins_of(const Kv8Attention &a, int64_t slots, int d) {  // behind the sums
+  return reinterpret_cast<Join *>(a.part + slots * (d + 2));
+}
+constexpr uint32_t kLeastShare = 4;  // tiles that are worth a workgroup's start
+__device__ __forceinline__ int live_tiles(const Kv8Attention &a, Span s) {
+  return (min(s.count * a.rep, a.rows) + a.tile_rows - 1) / a.tile_rows;
+}
+__device__ __forceinline__ int key_tiles(int blocks) { return (blocks + 1) / 2; }
+__device__ __forceinline__ uint32_t tiles_of(const Kv8Attention &a, int64_t b) {
+  if (b >= a.batch) return 0;
+  const Span s = tree_span(a, b);
+  return a.kv.kv_heads * live_tiles(a, s) * key_tiles(tile_blocks<true>(a, s, 0));
+}
+__device__ __forceinline__ uint32_t sums_before(uint32_t v) {  // of the lanes up to each
+#pragma unroll
+  for (int i = 1; i < kWave; i *= 2) {
+    const uint32_t lower = __shfl_up(v, i);
+    if (static_cast<int>(threadIdx.x & (kWave - 1)) >= i) v += lower;
+  }
+  return v;
+}
+__device__ __forceinline__ uint32_t tiles_each(const Kv8Attention &a) {
+  uint32_t total = 0;
+  for (int base = 0; base < a.batch; base += kWave)
+    total += __builtin_amdgcn_readlane(sums_before(tiles_of(a, base + (threadIdx.x & (kWave - 1)))), kWave - 1);
+  return max((total + a.items - 1) / a.items, kLeastShare);
+}
+// `each` tiles from `at` on, as far as there are any.
+__device__ __forceinline__ Share share_at(const Kv8Attention &a, uint32_t at, uint32_t each) {
+  uint32_t before = 0;
+  Share s{at, at, 0, 0, 0};
+  for (int base = 0; base < a.batch; base += kWave) {
+    const uint32_t own = tiles_of(a, base + (threadIdx.x & (kWave - 1))), upto = sums_before(own) + before;
+    const uint32_t total = __builtin_amdgcn_readlane(upto, kWave - 1);
+    if (s.end == at && total > at) {
+      const int lane = uniform(__popcll(__ballot(upto <= at)));
+      s.b = base + lane;
+      s.own = __builtin_amdgcn_readlane(own, lane);
+      s.before = __builtin_amdgcn_readlane(upto, lane) - s.own;
+    }
+    if (total > at) s.end = min(total, at + each);
+    if (s.end == at + each) break;
+    before = total;
+  }
+  return s;
+}
+__device__ __forceinline__ Piece piece_at(const Kv8Attention &a, const Share &s) {
+  Piece p;
+  p.span = tree_span(a, s.b);
+  p.blocks = tile_blocks<true>(a, p.span, 0);
+  p.tiles = key_tiles(p.blocks);
+  const uint32_t inner = s.at - s.before;
+  const int item = uniform(inner / static_cast<uint32_t>(p.tiles));
+  p.offset = inner - item * p.tiles;
+  const int live = live_tiles(a, p.span);
+  p.kvh = uniform(item / static_cast<uint32_t>(live));
+  p.tile = item - p.kvh * live;
+  p.n = min(static_cast<uint32_t>(p.tiles - p.offset), s.end - s.at);
+  return p;
+}
+__device__ __forceinline__ void advance(const Kv8Attention &a, Share &s, int n) {
+  s.at += n;
+  while (s.at < s.end && s.at == s.before + s.own) {
+    s.before += s.own;
+    s.own = uniform(tiles_of(a, ++s.b));
+  }
+}
+
 // Few rows: RT tiles of 16 (row = token * rep + head of the group) over one chunk of the keys; the eight waves take its
 // blocks in turn and join their sums through LDS. Nothing is staged: each wave loads the next block's codes into
 // registers while it works on this one, and widens a code once for all its rows.
@@ -448,6 +529,10 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
 //
 // S^T = K Q^T gives a lane 16 of a block's 32 scores of one row, keys 8 a + 4 g + c (g the half of the wave); V's
 // operands are written in that order.
+//
+// Trees: the sequences' lengths are known on the device alone, so a workgroup a CU reads them all and takes an equal
+// share of the batch's tiles. Where a share ends inside a head's tiles, its sums go to `part`, one place for the head it
+// begins and one for the head that it goes on with (kv8_join_shares_kernel); SPLIT does not matter.
 template <int D, bool FP8, bool SPLIT, bool TREE>
 __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Attention a) {
   constexpr int kThreads = kTileWaves * kWave;
@@ -464,18 +549,42 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
   const uint32_t per_xcd = (a.items + a.xcds - 1) / a.xcds;
   uint32_t item = (blockIdx.x % a.xcds) * per_xcd + blockIdx.x / a.xcds;
   if (item >= a.items) return;
-  const int split = SPLIT ? uniform(item % static_cast<uint32_t>(a.splits)) : 0;
-  if (SPLIT) item /= static_cast<uint32_t>(a.splits);
-  const uint32_t bkv = uniform(item / static_cast<uint32_t>(a.row_tiles));
-  const int tile = uniform(a.row_tiles - 1 - (item - bkv * a.row_tiles));  // the longest first
-  const int64_t tile_item = static_cast<int64_t>(bkv) * a.row_tiles + tile;
-  const int64_t b = uniform(bkv / static_cast<uint32_t>(a.kv.kv_heads));
-  const int kvh = uniform(bkv % static_cast<uint32_t>(a.kv.kv_heads));
-  const Span span = rows_of<TREE>(a, b);
-  const int blocks = tile_blocks<TREE>(a, span, tile);
-  const int first = SPLIT ? split * a.chunk : 0;
-  if (SPLIT && first >= blocks) return;
-  const int end = !SPLIT || split == a.splits - 1 ? blocks : min(blocks, first + a.chunk);
+  [[maybe_unused]] const uint32_t group = item;
+  [[maybe_unused]] Share share{};
+  [[maybe_unused]] uint32_t each = 0;
+  [[maybe_unused]] Join join{};
+  if constexpr (TREE) {
+    each = tiles_each(a);
+    share = share_at(a, group * each, each);
+  }
+  while (!TREE || share.at < share.end) {
+  int split = 0, tile, kvh, blocks, first = 0, end;
+  [[maybe_unused]] bool alone = true;  // the share holds all of the head's tiles
+  int64_t b, tile_item;
+  Span span;
+  if constexpr (TREE) {
+    const Piece piece = piece_at(a, share);
+    b = share.b, kvh = piece.kvh, tile = piece.tile, span = piece.span, blocks = piece.blocks;
+    first = piece.offset * kSub, end = min(blocks, (piece.offset + piece.n) * kSub);
+    alone = piece.n == piece.tiles;
+    tile_item = piece.offset == 0 ? a.items + group : group;  // the place of its sums
+    if (piece.offset == 0 && !alone)
+      join = {static_cast<int>(b), kvh, tile, 1 + static_cast<int>((piece.tiles - piece.n + each - 1) / each)};
+    advance(a, share, piece.n);
+  } else {
+    split = SPLIT ? uniform(item % static_cast<uint32_t>(a.splits)) : 0;
+    if (SPLIT) item /= static_cast<uint32_t>(a.splits);
+    const uint32_t bkv = uniform(item / static_cast<uint32_t>(a.row_tiles));
+    tile = uniform(a.row_tiles - 1 - (item - bkv * a.row_tiles));  // the longest first
+    tile_item = static_cast<int64_t>(bkv) * a.row_tiles + tile;
+    b = uniform(bkv / static_cast<uint32_t>(a.kv.kv_heads));
+    kvh = uniform(bkv % static_cast<uint32_t>(a.kv.kv_heads));
+    span = rows_of<TREE>(a, b);
+    blocks = tile_blocks<TREE>(a, span, tile);
+    first = SPLIT ? split * a.chunk : 0;
+    if (SPLIT && first >= blocks) return;
+    end = !SPLIT || split == a.splits - 1 ? blocks : min(blocks, first + a.chunk);
+  }
   const int n_tiles = (end - first + kSub - 1) / kSub;
 
   const int lane = threadIdx.x & (kWave - 1);
@@ -707,11 +816,12 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
     }
   }
 
-  if (row0 + r >= a.rows) return;
+  if (!TREE && row0 + r >= a.rows) return;
   l = half_sum(l);
-  if (SPLIT) {
-    const int64_t slots = a.tile_items * a.tile_rows;
-    const int64_t slot = split * slots + tile_item * a.tile_rows + wave * 32 + r;
+  if (row0 + r >= a.rows) {
+  } else if (TREE ? !alone : SPLIT) {
+    const int64_t slots = TREE ? 2 * static_cast<int64_t>(a.items) * a.part_rows : a.tile_items * a.tile_rows;
+    const int64_t slot = (TREE ? tile_item * a.part_rows : split * slots + tile_item * a.tile_rows) + wave * 32 + r;
     float *po = a.part + slot * D;
 #pragma unroll
     for (int d = 0; d < kDTiles; ++d)
@@ -720,21 +830,96 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
         *reinterpret_cast<f32x4 *>(po + d * 32 + q * 8 + 4 * g) =
             (f32x4){o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
     if (g == 0) {
-      float *pm = a.part + a.splits * slots * D;
+      const int64_t all = TREE ? slots : a.splits * slots;
+      float *pm = a.part + all * D;
       pm[slot] = m;
-      pm[a.splits * slots + slot] = l;
+      pm[all + slot] = l;
     }
-    return;
+  } else {
+    const float inv = l != 0.f ? 1.0f / l : 0.f;  // no key, no weight: the row is 0
+    uint16_t *op = a.o + b * a.o_stride[0] + token * a.o_stride[1] + head * a.o_stride[2] + 4 * g;
+#pragma unroll
+    for (int d = 0; d < kDTiles; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<u32x2 *>(op + d * 32 + q * 8) =
+            (u32x2){pack_bf16(o[d][4 * q] * inv, o[d][4 * q + 1] * inv),
+                    pack_bf16(o[d][4 * q + 2] * inv, o[d][4 * q + 3] * inv)};
   }
-  const float inv = l != 0.f ? 1.0f / l : 0.f;  // no key, no weight: the row is 0
-  uint16_t *op = a.o + b * a.o_stride[0] + token * a.o_stride[1] + head * a.o_stride[2] + 4 * g;
+  if (!TREE) return;
+  __syncthreads();  // the next piece's first tiles go where waves may still read the last ones
+  }
+  if constexpr (TREE) {
+    if (threadIdx.x == 0) joins_of(a, 2 * static_cast<int64_t>(a.items) * a.part_rows, D)[group] = join;
+    // Rows that see nothing, and have no tiles.
+    for (uint32_t i = group; i < a.tile_items; i += a.items) {
+      const uint32_t bkv = i / static_cast<uint32_t>(a.row_tiles);
+      const int tile = uniform(i - bkv * a.row_tiles);
+      const int64_t b = uniform(bkv / static_cast<uint32_t>(a.kv.kv_heads));
+      if (tile_blocks<TREE>(a, rows_of<TREE>(a, b), tile) > 0) continue;
+      const int kvh = uniform(bkv % static_cast<uint32_t>(a.kv.kv_heads));
+      const int rows = min(a.rows - tile * a.tile_rows, a.tile_rows);
+      for (int j = threadIdx.x; j < rows * (D / 8); j += kThreads) {
+        const int row = tile * a.tile_rows + j / (D / 8), token = row / a.rep;
+        const int head = kvh * a.rep + (row - token * a.rep);
+        uint16_t *op = a.o + b * a.o_stride[0] + token * a.o_stride[1] + head * a.o_stride[2] + j % (D / 8) * 8;
+        *reinterpret_cast<u32x2 *>(op) = (u32x2){0, 0};
+        *reinterpret_cast<u32x2 *>(op + 4) = (u32x2){0, 0};
+      }
+    }
+  }
+}
+
+// The join of the shares: the head's tiles that a share begins and does not end are joined by the workgroups of that
+// share, 256 / (D / 4) rows each.
+template <int D>
+__global__ __launch_bounds__(256) void kv8_join_shares_kernel(Kv8Attention a) {
+  constexpr int kLanes = D / 4, kBatch = 4;
+  const uint32_t parts = (a.part_rows + 256 / kLanes - 1) / (256 / kLanes);
+  const uint32_t left = uniform(blockIdx.x / parts);
+  const int64_t slots = 2 * static_cast<int64_t>(a.items) * a.part_rows;
+  const Join join = joins_of(a, slots, D)[left];
+  const int used = uniform(join.pieces);
+  if (used == 0) return;
+  const int in_tile = (blockIdx.x - left * parts) * (256 / kLanes) + threadIdx.x / kLanes;
+  const int row = join.tile * a.tile_rows + in_tile;
+  if (in_tile >= a.part_rows || row >= a.rows) return;
+  const float *pm = a.part + slots * D, *pl = pm + slots;
+  const int c = threadIdx.x % kLanes;
+  float mx = -FLT_MAX, l = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int i0 = 0; i0 < used; i0 += kBatch) {
+    float m[kBatch], part[kBatch];
+    f32x4 o[kBatch];
 #pragma unroll
-  for (int d = 0; d < kDTiles; ++d)
+    for (int i = 0; i < kBatch; ++i) {  // past the last piece it again, with a weight of zero below
+      const int64_t n = min(i0 + i, used - 1);
+      const int64_t s = (n == 0 ? a.items + left : left + n) * a.part_rows + in_tile;
+      m[i] = pm[s];
+      part[i] = pl[s];
+      o[i] = *reinterpret_cast<const f32x4 *>(a.part + s * D + 4 * c);
+    }
+    float m_new = mx;
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      *reinterpret_cast<u32x2 *>(op + d * 32 + q * 8) =
-          (u32x2){pack_bf16(o[d][4 * q] * inv, o[d][4 * q + 1] * inv),
-                  pack_bf16(o[d][4 * q + 2] * inv, o[d][4 * q + 3] * inv)};
+    for (int i = 0; i < kBatch; ++i) m_new = fmaxf(m_new, m[i]);
+    const float alpha = __builtin_amdgcn_exp2f(mx - m_new);
+    l *= alpha;
+    acc *= alpha;
+    mx = m_new;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (i0 + i >= used) break;
+      const float w = __builtin_amdgcn_exp2f(m[i] - m_new);
+      l += w * part[i];
+      acc += w * o[i];
+    }
+  }
+  const float inv = l != 0.f ? 1.0f / l : 0.f;
+  const int token = row / a.rep;
+  const int head = join.kvh * a.rep + (row - token * a.rep);
+  uint16_t *op = a.o + join.b * a.o_stride[0] + token * a.o_stride[1] + head * a.o_stride[2] + 4 * c;
+  *reinterpret_cast<u32x2 *>(op) =
+      (u32x2){pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
 }
 
 // o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the chunks that hold keys the tile sees, M the largest
@@ -866,8 +1051,16 @@ hipError_t launch_attend(const Kv8Attention &p, hipStream_t stream) {
   const dim3 block(kTileWaves * kWave), grid(p.items), xcd_grid((p.items + p.xcds - 1) / p.xcds * p.xcds);
   if (p.tile_rows <= 16) hipLaunchKernelGGL((kv8_rows_kernel<D, FP8, 1, TREE>), grid, block, 0, stream, p);
   else if (p.tile_rows == 32) hipLaunchKernelGGL((kv8_rows_kernel<D, FP8, 2, TREE>), grid, block, 0, stream, p);
-  else if (p.splits > 1) hipLaunchKernelGGL((kv8_tile_kernel<D, FP8, true, TREE>), xcd_grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((kv8_tile_kernel<D, FP8, false, TREE>), xcd_grid, block, 0, stream, p);
+  else if (TREE || p.splits == 1)
+    hipLaunchKernelGGL((kv8_tile_kernel<D, FP8, false, TREE>), xcd_grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((kv8_tile_kernel<D, FP8, !TREE, TREE>), xcd_grid, block, 0, stream, p);
+  if (TREE && p.tile_rows > 32) {
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess || p.items == 1) return err;
+    const unsigned parts = (p.part_rows * (D / 4) + 255) / 256;
+    hipLaunchKernelGGL((kv8_join_shares_kernel<D>), dim3((p.items - 1) * parts), dim3(256), 0, stream, p);
+    return hipGetLastError();
+  }
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || p.splits == 1) return err;
   if (TREE && p.splits <= kRowJoinSplits) {
@@ -1372,10 +1565,23 @@ void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, bool tree, int cus,
     weigh(p->rows, 1, 16);
   } else {
     weigh(32, 2, 30);
-    if (p->rows > 64) weigh(32 * kTileWaves, 10, 40);
+    if (p->rows > 64 && !tree) weigh(32 * kTileWaves, 10, 40);
+    if (p->rows > 64 && tree) {  // dealt: no rounds, but a start for each piece
+      const int64_t items = heads * ((p->rows + 32 * kTileWaves - 1) / (32 * kTileWaves));
+      const int64_t cost = (items * blocks * 10 + (items + cus) * 40) / cus + 30 +
+                           (items + cus) * std::min(p->rows, 32 * kTileWaves) / 900;
+      if (cost < best) p->tile_rows = 32 * kTileWaves;
+    }
   }
   p->row_tiles = (p->rows + p->tile_rows - 1) / p->tile_rows;
   p->tile_items = heads * p->row_tiles;
+  p->part_rows = std::min(p->rows, p->tile_rows);
+  if (tree && p->tile_rows > 32) {  // dealt: a workgroup a CU
+    p->splits = p->chunk = 1;
+    p->items = static_cast<uint32_t>(std::max(1, cus / p->xcds) * p->xcds);
+    p->part_bytes = p->items * (static_cast<size_t>(2) * p->part_rows * (p->kv.d + 2) + 4) * sizeof(float);
+    return;
+  }
   p->chunk = static_cast<int>((blocks + splits - 1) / splits);  // the last one goes on to the end of the sequence,
   p->splits = static_cast<int>((blocks + p->chunk - 1) / p->chunk);  // whatever max_tokens says
   const int64_t items = p->tile_items * p->splits;

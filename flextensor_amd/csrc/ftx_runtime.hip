@@ -1624,6 +1624,9 @@ int kv8_attention(const ftx_kv8_cache *cache, const void *q, void *o, const int6
   p.scale_log2 = scale * 1.44269504088896340736f;
   rc = plan_kv8(max_tokens, tree != nullptr, &p);
   if (rc != FTX_OK) return rc;
+  if (tree && p.tile_rows > 32 &&  // dealt in numbers of 32 bits
+      p.tile_items > INT32_MAX / ((int64_t(p.kv.width) * p.kv.page_blocks + 1) / 2 + 1))
+    return ftx::fail(FTX_ERR_UNSUPPORTED, "cache attention: more than 2^31 tiles of keys");
   if (p.part_bytes > 0) {
     if (workspace_bytes < p.part_bytes)
       return ftx::fail(FTX_ERR_INVALID, "cache attention needs a workspace of " + std::to_string(p.part_bytes) +
