@@ -1547,8 +1547,11 @@ __global__ __launch_bounds__(256) void kv8_copy_kernel(Kv8Copy) {
 // 32 splits, 21.9 in 63, 36 in 4; 256 heads over 4096 keys 48.5 unsplit, 56 in two. 512 rows over 500 keys 10.9 in
 // tiles of 32 and 26.8 in tiles of 256, over 4000 31.4 and 38.0, over 30000 132 and 98; 128 heads of 512 rows over
 // 2000 keys 205 and 111, 32 heads 52.5 and 62. Up to 64 rows tiles of 32 were never slower (14.6 and 18.7 over 4000).
-// Trees join their chunks at less cost: 128 rows over 32000 keys (16 heads) 68.5 in tiles of 256 split in 16, 79.3 in
-// tiles of 32 split in four.
+// Trees in tiles of 256 rows are dealt to the CUs, without rounds but with two starts for many, in units again:
+//   a block 10, with more than 128 rows 12 (two waves of a SIMD at work); a start 80; 32 rows of the other kernel 3
+// Measured, us, int8, in tiles of 32 and of 256: 80 rows of 64 heads over 4096 keys at most 39.5 and 32.1, of 128 heads
+// over 8000 145 and 121; 128 rows of 16 heads over 32000 82.3 and 76.7, of 64 over 1000 19.7 and 27.7, over 4096 48.4 and
+// 48.4; 150 of 12 over 20000 54.2 and 58.0; 512 of 8 over 4096 30.8 and 39.5; 96 of 256 over 1000 at most 34.0 and 56.0.
 void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, bool tree, int cus, int xcds) {
   p->xcds = std::max(1, xcds);
   p->rep = p->heads / p->kv.kv_heads;
@@ -1572,11 +1575,11 @@ void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, bool tree, int cus,
   if (p->rows <= 16) {
     weigh(p->rows, 1, 16);
   } else {
-    weigh(32, 2, 30);
+    weigh(32, tree && p->rows > 64 ? 3 : 2, 30);
     if (p->rows > 64 && !tree) weigh(32 * kTileWaves, 10, 40);
     if (p->rows > 64 && tree) {  // dealt: no rounds, but a start for each piece
       const int64_t items = heads * ((p->rows + 32 * kTileWaves - 1) / (32 * kTileWaves));
-      const int64_t cost = (items * blocks * 10 + (items + cus) * 40) / cus + 30 +
+      const int64_t cost = (items * blocks * (p->rows > 128 ? 12 : 10) + (items + cus) * 80) / cus + 30 +
                            (items + cus) * std::min(p->rows, 32 * kTileWaves) / 900;
       if (cost < best) p->tile_rows = 32 * kTileWaves;
     }
