@@ -5,7 +5,8 @@ device work goes through the HIP C-ABI library ``libftx_hip.so``
 (``include/ftx.h``): pinned host arenas, host-to-device copy engines
 (hipMemcpyAsync and a zero-copy kernel), a batched scatter kernel and
 hipEvent gating, an fp8-weight MFMA GEMM, a paged 8-bit KV cache
-(``kv_cache``) with int8 projections, and a staged copy engine for
+(``kv_cache``) with int8 projections, drafted token trees over it with
+4-bit projections and token log probabilities, and a staged copy engine for
 pageable and shared-memory sources. Models can be built straight from a
 saved profile and a safetensors checkpoint (``load_model_from_profile``).
 """

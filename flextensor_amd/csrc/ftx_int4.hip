@@ -438,9 +438,9 @@ void start(const Int4Linear &p, hipStream_t stream) {
 //                    a unit   a 16   start
 //   64 x 128             65      8     500
 //   256 x 256           120     15    1000
-// Measured, us: 8192 x 28672 of 777 rows 382 in tiles of 256 split in two, 530 in tiles of 64; 28672 x 8192 of 100 rows
-// 103 and 93, of 200 128 and 161, of 512 220 and 308, of 64 rows 60 split in three and 64 unsplit; 4096 x 4096 of 17
-// rows 13.5 split in eight, 20 in four.
+// Measured, us: 8192 x 28672 of 777 rows 366 in tiles of 256 split in two, 585 unsplit and as much in tiles of 64; 28672 x
+// 8192 of 100 rows 98 and 94, of 200 119 and 167, of 512 217 and 302, of 64 rows 60 split in three and 74 unsplit; 4096 x
+// 4096 of 17 rows 13.1 split in eight, 36 unsplit.
 void plan_int4_linear(Int4Linear *p, int cus, int xcds) {
   p->xcds = std::max(1, xcds);
   p->tiles = (p->n + 15) / 16;

@@ -1538,7 +1538,8 @@ __global__ __launch_bounds__(256) void kv8_copy_kernel(Kv8Copy) {
 }  // namespace
 
 // Which kernel runs, and how often the keys are split, by what it costs in units of 0.1 us: a round of workgroups, one
-// a CU, takes a start and its blocks; the join a launch and the partial values' way through memory and back.
+// a CU, takes a start and its blocks; the join a launch and the partial values' way through memory and back, shorter for
+// trees of up to 16 chunks (kv8_join_rows_kernel).
 //                                 a block  a start
 //   up to 16 rows                       1       16
 //   tiles of 32 rows                    2       30
