@@ -3,9 +3,12 @@ a GPU: page moves are torch's."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
+from flextensor_amd import _native as nat
 from flextensor_amd import hip
 from flextensor_amd import kv_cache as kvc
 from flextensor_amd import workloads as W
@@ -287,3 +290,9 @@ def test_layer_bytes_are_those_of_the_parameters():
                              **change)
         layer = W.build_llama(shape).layers[0]
         assert sum(p.numel() * p.element_size() for p in layer.parameters()) == shape.layer_bytes()
+
+
+def test_more_channels_than_a_launch_tells_apart_are_refused():
+    lib, b = nat.load(), ctypes.c_size_t(0)
+    assert lib.ftx_int4_linear_workspace(1, 1 << 27, 128, 128, ctypes.byref(b)) == nat.FTX_OK and b.value == 0
+    assert lib.ftx_int4_linear_workspace(1, 1 << 33, 128, 128, ctypes.byref(b)) == nat.FTX_ERR_UNSUPPORTED

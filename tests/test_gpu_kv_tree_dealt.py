@@ -164,3 +164,15 @@ def test_a_captured_call_deals_by_the_lengths_of_each_replay(gpu):
         torch.cuda.synchronize()
         graph.replay()
         assert torch.equal(out, want)
+
+
+def test_more_tiles_of_keys_than_are_counted_are_refused(gpu):
+    """Tiles are dealt in 32-bit numbers: 4096 tables of two million tokens hold too many. Nothing is launched."""
+    b, t, h, kv, d = 4096, 64, 64, 8, 64
+    codes, scales = _cache(gpu, _gen(gpu, 0), 1, kv, 64, d, torch.int8)
+    table = torch.zeros(b, 1 << 15, dtype=torch.int32, device=gpu)
+    starts = torch.zeros(b, dtype=torch.int32, device=gpu)
+    q = torch.empty(b, t, h, d, dtype=torch.bfloat16, device=gpu)
+    sets = torch.ones(1, t, dtype=torch.int64, device=gpu).expand(b, t)
+    with pytest.raises(nat.FtxError, match="tiles of keys"):
+        kvc.tree_attention(q, codes, scales, table, starts, sets, max_tokens=64)
