@@ -10,11 +10,12 @@
 //
 // The likeliest tokens are keys (the logit's bits in the order of unsigned integers, then the complement of the index):
 // the largest keys are the largest logits, the lowest index first among equal ones, a NaN above all. The pass over the
-// row keeps no more for them than each thread's maximum. The threads form 64 groups (128 for a top of more than 32): as
-// many values as groups' maxima reach the `top`th largest of these, so no token below it counts, and some 1.2 `top` values
-// reach it. The threads whose own maximum does read their values again (from the cache) and collect the keys in LDS,
-// where one wave sorts them. Rows that more keys pass than LDS holds (many equal ones), or that are not finite, take
-// another way: each wave keeps the 64 largest keys of what it reads sorted over its lanes.
+// row keeps no more for them than each thread's maximum, the batch it was in and the largest value of the others. The
+// threads form 64 groups (128 for a top of more than 32): as many values as groups' maxima reach the `top`th largest of
+// these, so no token below it counts, and some 1.2 `top` values reach it. The threads whose own maximum does read that
+// batch again (from the cache) and collect the keys in LDS, where one wave sorts them. Rows that more keys pass than LDS
+// holds (many equal ones), or that are not finite, take another way: each wave keeps the 64 largest keys of what it
+// reads sorted over its lanes.
 #include <algorithm>
 #include <cfloat>
 
@@ -36,6 +37,13 @@ template <int TYPE>
 struct Vec {  // the values of 16 bytes
   static constexpr int kValues = TYPE == FTX_LOGITS_FP32 ? 4 : 8;
   u32x4 w;
+  __device__ __forceinline__ float pick(int i) const {  // of a number that is not known when this is compiled
+    const int j = TYPE == FTX_LOGITS_FP32 ? i : i / 2;
+    Vec one;
+    one.w[0] = j & 2 ? j & 1 ? w[3] : w[2] : j & 1 ? w[1] : w[0];
+    if constexpr (TYPE != FTX_LOGITS_FP32) one.w[0] >>= 16 * (i % 2);
+    return one[0];
+  }
   __device__ __forceinline__ float operator[](int i) const {
     if constexpr (TYPE == FTX_LOGITS_FP32) return __uint_as_float(w[i]);
     if constexpr (TYPE == FTX_LOGITS_BF16) return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
@@ -114,13 +122,14 @@ __device__ __forceinline__ K sort_step(K key, int lane) {
   return key;
 }
 template <typename K>
-__device__ __forceinline__ K sorted(K key, int lane) {
+__device__ __forceinline__ K sorted(K key, int lane, int count = kWave) {  // the lanes from count on hold 0
   key = sort_step<2, 1>(key, lane);
   key = sort_step<4, 2>(key, lane);
   key = sort_step<8, 4>(key, lane);
   key = sort_step<16, 8>(key, lane);
+  if (count <= 16) return key;
   key = sort_step<32, 16>(key, lane);
-  return clean(key, lane);
+  return count <= 32 ? key : clean(key, lane);
 }
 // The 64 largest of two sorted lists.
 __device__ __forceinline__ Key merged(Key a, Key b, int lane) {
@@ -320,6 +329,8 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 8 : 4) void logprobs_kern
   if (TOP && threadIdx.x == 0) collected = 0;
 
   float top = -INFINITY, c = -kFar * kLog2e, s = 0.f, t = 0.f;  // y = x log2(e) + c
+  float second = -INFINITY;  // no batch but the one at `where` has a value above it
+  int where = first;
   const auto work = [&](Vec<TYPE> (&v)[kVecs], int u) {
     part.trim(v, u);
     float high = v[0][0], low = v[0][0];
@@ -329,7 +340,9 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 8 : 4) void logprobs_kern
       high = fmaxf(fmaxf(high, a), b);
       low = fminf(fminf(low, a), b);
     }
+    if (TOP) second = fmaxf(second, fminf(high, top));
     if (high > top) {
+      where = u;
       top = high;
       const float now = -__builtin_amdgcn_fmed3f(top, kFar, -kFar) * kLog2e, y = now - c, w = __builtin_amdgcn_exp2f(y);
       t = (t + fmaxf(y, -1000.f) * s) * w;
@@ -417,57 +430,73 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 8 : 4) void logprobs_kern
     mine = all_parts();
   }
 
+  // The wave that sorts and writes: with wave 0 in all of them, those of the workgroups that share a CU would be on one SIMD
+  // (0.4 us of 2048 rows).
+  int writer = static_cast<int>(blockIdx.x / 256 % kWaves);
   Key list = 0;
   if constexpr (TOP) {
-    uint32_t groups = sorted(group_max[lane], lane);
-    if (fine) {
-      const uint32_t others = __shfl(sorted(group_max[kWave + lane], lane), kWave - 1 - lane);
-      groups = clean(max(groups, others), lane);
+    if (wave == writer) {
+      uint32_t groups = sorted(group_max[lane], lane);
+      if (fine) {
+        const uint32_t others = __shfl(sorted(group_max[kWave + lane], lane), kWave - 1 - lane);
+        groups = clean(max(groups, others), lane);
+      }
+      if (lane == p.top - 1) group_max[0] = groups;
     }
-    const uint32_t least = __builtin_amdgcn_readlane(static_cast<int>(groups), p.top - 1);
+    __syncthreads();
+    const uint32_t least = uniform(group_max[0]);
     bool exact = mine.s == mine.s;  // else a NaN may be among the values, which no maximum shows
     if (exact) {
       const float bound = least == 0 ? -INFINITY : unordered(least);
-      // four of the threads at a time, a unit a lane
-      uint64_t those = __ballot(mine0 < part.end && top >= bound);
+      const auto collect = [&](const Vec<TYPE> &v, int u) {
+        uint32_t passed = 0;
+#pragma unroll
+        for (int e = 0; e < kValues; ++e) passed |= v[e] >= bound ? 1u << e : 0;
+        while (passed) {
+          const int e = __builtin_ctz(passed), at = u * kValues - part.lead + e;
+          passed &= passed - 1;
+          if (at < 0 || at >= part.vocab) continue;
+          const int slot = atomicAdd(&collected, 1);
+          if (slot < kKeys) lists[slot] = key_of(v.pick(e), at);
+        }
+      };
+      // A thread looks at the batch of its maximum again, and where another one of its reaches the bound too the wave at
+      // all that the thread had, a unit a lane. A unit takes a whole line of the cache with it: all units of the 24
+      // threads or so that have the 20 likeliest were most of the row's lines (2048 rows of 32000 bf16 33.0 us, 29.7
+      // now; 512 of 128000 fp32 60.8 and 43.9).
+      const bool passes = mine0 < part.end && top >= bound;
+      if (passes && second < bound) {
+        Vec<TYPE> v[kVecs];
+        const int u0 = where + static_cast<int>(threadIdx.x);
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) v[i].w = part.units[min(u0 + i * THREADS, part.end - 1)];
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i)
+          if (u0 + i * THREADS < part.end) collect(v[i], u0 + i * THREADS);
+      }
+      uint64_t those = __ballot(passes && !(second < bound));
       while (those) {
-        int whose[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          whose[i] = those ? __builtin_ctzll(those) : -1;
-          those &= those - 1;
-        }
-        const int thread = lane < 16 ? whose[0] : lane < 32 ? whose[1] : lane < 48 ? whose[2] : whose[3];
-        if (thread < 0) continue;
-        for (int u = first + wave * kWave + thread + lane % 16 * THREADS; u < part.end; u += 16 * THREADS) {
-          const Vec<TYPE> v = {part.units[u]};
-          uint32_t passed = 0;
-#pragma unroll
-          for (int e = 0; e < kValues; ++e) passed |= v[e] >= bound ? 1u << e : 0;
-          while (passed) {
-            const int e = __builtin_ctz(passed), at = u * kValues - part.lead + e;
-            passed &= passed - 1;
-            if (at < 0 || at >= part.vocab) continue;
-            const int slot = atomicAdd(&collected, 1);
-            if (slot < kKeys) lists[slot] = key_of(value_at<TYPE>(x, at), at);
-          }
-        }
+        const int thread = __builtin_ctzll(those);
+        those &= those - 1;
+        for (int u = first + wave * kWave + thread + lane * THREADS; u < part.end; u += kWave * THREADS)
+          collect({part.units[u]}, u);
       }
       __syncthreads();
       exact = collected <= kKeys;
     }
     if (exact) {
-      if (wave == 0)
+      if (wave == writer)
         for (int i = 0; i < collected; i += kWave) {
-          const Key fresh = sorted(i + lane < collected ? lists[i + lane] : 0, lane);
+          const Key fresh = sorted(i + lane < collected ? lists[i + lane] : 0, lane, uniform(collected) - i);
           list = i == 0 ? fresh : merged(list, fresh, lane);
         }
     } else {
       __syncthreads();
       list = largest_keys<TYPE, THREADS>(part, first, p.top, lists, wave, lane);
+      writer = 0;
     }
   }
-  if (wave > 0) return;
+  if (wave != writer) return;
   if (p.splits == 1) {
     write_row<TYPE>(p, row, x, mine, list, lane);
     return;
