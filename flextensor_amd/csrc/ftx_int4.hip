@@ -96,7 +96,9 @@ __global__ __launch_bounds__(512) void int4_rows_kernel(Int4Linear p) {
   const int64_t tile0 = static_cast<int64_t>(blockIdx.x) * p.tiles / p.items;
   const int count = static_cast<int>(static_cast<int64_t>(blockIdx.x + 1) * p.tiles / p.items - tile0);
   const int chunks = (count + NT - 1) / NT, steps = (p.units + kWaves - 1) / kWaves;
-  const auto chunk_at = [&](int i) { return static_cast<int>(static_cast<uint32_t>(i * count) / static_cast<uint32_t>(chunks)); };
+  const auto chunk_at = [&](int i) {  // the chunk's first tile of `count`, at most 60000
+    return static_cast<int>(static_cast<uint32_t>(i * count) / static_cast<uint32_t>(chunks));
+  };
   const uint16_t *xr = p.x + min(r, m - 1) * p.x_stride + 8 * q;
 
   struct Unit {
@@ -195,9 +197,9 @@ __global__ __launch_bounds__(512) void int4_rows_kernel(Int4Linear p) {
 // ---- tiles -----------------------------------------------------------------------------------------------------------
 //
 // Up to TM tokens x TN channels a workgroup, K in units of 128: the tokens are dealt evenly to the tiles, in 16s, and
-// products of 16s that a tile does not have are left out (777 rows in four tiles of 208). A unit's x goes straight from memory into one of STAGES stages
-// of LDS while another is multiplied, with one barrier a unit; row R's 16-byte chunk c lies at slot c ^ (R % 16), so the
-// 16 rows that a read touches lie in different banks. The codes go from memory into the registers of the wave that
+// products of 16s that a tile does not have are left out (777 rows in four tiles of 208). A unit's x goes straight from
+// memory into one of STAGES stages of LDS while another is multiplied, with one barrier a unit; row R's 16-byte chunk c
+// lies at slot c ^ (R % 16), so the 16 rows that a read touches lie in different banks. The codes go from memory into the registers of the wave that
 // multiplies by them, as the operands that they are, DEPTH units ahead: they take no LDS and no barrier. A wave makes the
 // weights of its channels for the next 32 inputs, (c - z) s in fp32 rounded to bf16, between the products of these ones.
 //

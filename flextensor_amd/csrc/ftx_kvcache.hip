@@ -557,7 +557,7 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
     each = tiles_each(a);
     share = share_at(a, group * each, each);
   }
-  while (!TREE || share.at < share.end) {
+  while (!TREE || share.at < share.end) {  // of a tree's pieces; the others end in the first round
   int split = 0, tile, kvh, blocks, first = 0, end;
   [[maybe_unused]] bool alone = true;  // the share holds all of the head's tiles
   int64_t b, tile_item;

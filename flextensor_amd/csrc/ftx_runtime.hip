@@ -1530,7 +1530,8 @@ int ftx_kv8_append_norm(const ftx_kv8_cache *cache, const void *q, const void *k
   if (rc != FTX_OK) return rc;
   if (positions < 0 || positions > (int64_t(1) << 40)) return ftx::fail(FTX_ERR_INVALID, "rotary positions");
   if (!q_weight != !k_weight) return ftx::fail(FTX_ERR_INVALID, "append takes norm weights for both q and k, or none");
-  if (q_weight && !(eps >= 0.f && eps < INFINITY)) return ftx::fail(FTX_ERR_INVALID, "append needs a finite eps, not negative");
+  if (q_weight && !(eps >= 0.f && eps < INFINITY))
+    return ftx::fail(FTX_ERR_INVALID, "append needs a finite eps, not negative");
   if (batch == 0 || t == 0) return FTX_OK;
   if (!strides) return ftx::fail(FTX_ERR_INVALID, "strides is null");
   const int d = cache->d, kv = cache->kv_heads;
@@ -1673,7 +1674,8 @@ int ftx_kv8_keep(const ftx_kv8_cache *cache, int64_t layers, const int32_t *path
   ftx::Kv8Keep p{};
   int rc = kv8_pages(cache, layers == 0 ? 0 : batch, n, cache ? cache->kv_heads : 0, &p.kv);
   if (rc != FTX_OK) return rc;
-  if (layers < 0 || layers > 65536 || n > 64) return ftx::fail(FTX_ERR_INVALID, "keep takes up to 65536 layers and 64 nodes");
+  if (layers < 0 || layers > 65536 || n > 64)
+    return ftx::fail(FTX_ERR_INVALID, "keep takes up to 65536 layers and 64 nodes");
   if (layers == 0 || batch == 0 || n == 0) return FTX_OK;
   if (layers > ftx::kMaxThreads / 256 / (batch * cache->kv_heads * 2))
     return ftx::fail(FTX_ERR_UNSUPPORTED, "keep: more workgroups than one launch holds");

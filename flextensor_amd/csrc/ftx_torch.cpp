@@ -1,4 +1,5 @@
-// Calls of the 8-bit cache, the 8- and 4-bit linears and the token log probabilities from torch tensors, without Python between the checks and the library.
+// Calls of the 8-bit cache, the 8- and 4-bit linears and the token log probabilities from torch tensors, without Python
+// between the checks and the library.
 //
 // A decode step's kernels take 5 to 8 us; checking their tensors attribute by attribute in Python and packing the
 // C call's arguments took 13 to 18. Each function here looks at its arguments, allocates the result and the workspace

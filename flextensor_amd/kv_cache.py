@@ -246,9 +246,10 @@ def tree_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, t
 
     ``starts[b]``: the first tokens of a sequence, which every row sees. The ``nodes`` tokens (None: t; at most 64) cached
     after them are the tree's nodes, and ``tree`` (int64 [batch, t]) says which of them a row sees: bit j of
-    ``tree[b, i]`` the token ``starts[b] + j`` (one tree may be expanded over the batch). A row's own node is one of its bits, its ancestors the others; rows may be
-    a part of the nodes (a level of the tree). Rows from ``new[b]`` on, and rows that see no token, are 0. ``max_tokens``
-    counts the nodes. A NaN that a sequence's nodes hold may reach rows that do not see it.
+    ``tree[b, i]`` the token ``starts[b] + j`` (one tree may be expanded over the batch). A row's own node is one of its
+    bits, its ancestors the others; rows may be a part of the nodes (a level of the tree). Rows from ``new[b]`` on, and
+    rows that see no token, are 0. ``max_tokens`` counts the nodes. A NaN that a sequence's nodes hold may reach rows that
+    do not see it. Many rows are shared out by the lengths of the whole batch, which may change the order of a sum.
     """
     device = _device(q)
     if device >= 0 and torch.autograd.forward_ad._current_level < 0:
@@ -280,8 +281,8 @@ def tree_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, t
     ws_bytes = int(got.value)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     nat.call("ftx_kv8_tree_attention", ctypes.byref(cache), q.data_ptr(), out.data_ptr(), tree.data_ptr(),
-             tree.stride(0) if b > 1 else t, nodes, b, t, h, _Strides6(*strides), d ** -0.5 if scale is None else scale, longest,
-             ws.data_ptr() if ws is not None else None, ws_bytes, hip._stream(device))
+             tree.stride(0) if b > 1 else t, nodes, b, t, h, _Strides6(*strides), d ** -0.5 if scale is None else scale,
+             longest, ws.data_ptr() if ws is not None else None, ws_bytes, hip._stream(device))
     return out
 
 
