@@ -258,6 +258,41 @@ __device__ __forceinline__ Share share_at(const Kv8Attention &a, uint32_t at, ui
   }
   return s;
 }
+// Or, where they fit, pieces of one head each, so that no workgroup starts twice: a head's keys in as few pieces of up to
+// `each` tiles as they take, `each` the least for which there is a workgroup for every piece. A second start takes as
+// long as some three tiles (the case above: 37.7 us with them). Returns whether it is so, with the workgroup's share and its head's `each`.
+constexpr uint32_t kSecondStart = 3;
+__device__ __forceinline__ bool whole_pieces(const Kv8Attention &a, uint32_t group, Share &s, uint32_t &each) {
+  if (a.batch > kWave) return false;
+  const int lane = threadIdx.x & (kWave - 1);
+  uint32_t tiles = 0, heads = 0;
+  if (lane < a.batch) {
+    const Span span = tree_span(a, lane);
+    tiles = key_tiles(tile_blocks<true>(a, span, 0));
+    heads = tiles > 0 ? a.kv.kv_heads * live_tiles(a, span) : 0;
+  }
+  const auto sum = [](uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(sums_before(v), kWave - 1));
+  };
+  const uint32_t even = max((sum(heads * tiles) + a.items - 1) / a.items, kLeastShare);
+  uint32_t parts = 0, e = even;
+  for (;; ++e) {
+    if (e > even + kSecondStart) return false;
+    parts = (tiles + e - 1) / e;
+    if (sum(heads * parts) <= a.items) break;
+  }
+  const uint32_t upto = sums_before(heads * parts);
+  const int b = uniform(__popcll(__ballot(upto <= group)));
+  s = {0, 0, 0, 0, b};
+  if (b >= kWave) return true;  // none left
+  const uint32_t of = __builtin_amdgcn_readlane(parts, b), held = __builtin_amdgcn_readlane(tiles, b);
+  const uint32_t inner = group - (__builtin_amdgcn_readlane(upto, b) - of * __builtin_amdgcn_readlane(heads, b));
+  const uint32_t head = uniform(inner / of), part = inner - head * of;
+  each = uniform((held + of - 1) / of);
+  s.at = head * held + part * each;
+  s.end = s.at + min(each, held - part * each);
+  return true;
+}
 __device__ __forceinline__ Piece piece_at(const Kv8Attention &a, const Share &s) {
   Piece p;
   p.span = tree_span(a, s.b);
@@ -531,8 +566,9 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
 // operands are written in that order.
 //
 // Trees: the sequences' lengths are known on the device alone, so a workgroup a CU reads them all and takes an equal
-// share of the batch's tiles. Where a share ends inside a head's tiles, its sums go to `part`, one place for the head it
-// begins and one for the head that it goes on with (kv8_join_shares_kernel); SPLIT does not matter.
+// share of the batch's tiles (8 ragged sequences of 25 nodes over up to 4096 tokens, 64 / 8 heads, int8: 31.6 us, and 51 in
+// chunks of the longest one's length). Where a share ends inside a head's tiles, its sums go to `part`, one place for the
+// head it begins and one for the head that it goes on with (kv8_join_shares_kernel); SPLIT does not matter.
 template <int D, bool FP8, bool SPLIT, bool TREE>
 __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Attention a) {
   constexpr int kThreads = kTileWaves * kWave;
@@ -554,8 +590,10 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
   [[maybe_unused]] uint32_t each = 0;
   [[maybe_unused]] Join join{};
   if constexpr (TREE) {
-    each = tiles_each(a);
-    share = share_at(a, group * each, each);
+    if (!whole_pieces(a, group, share, each)) {
+      each = tiles_each(a);
+      share = share_at(a, group * each, each);
+    }
   }
   while (!TREE || share.at < share.end) {  // of a tree's pieces; the others end in the first round
   int split = 0, tile, kvh, blocks, first = 0, end;
@@ -1548,11 +1586,14 @@ __global__ __launch_bounds__(256) void kv8_copy_kernel(Kv8Copy) {
 // 32 splits, 21.9 in 63, 36 in 4; 256 heads over 4096 keys 48.5 unsplit, 56 in two. 512 rows over 500 keys 10.9 in
 // tiles of 32 and 26.8 in tiles of 256, over 4000 31.4 and 38.0, over 30000 132 and 98; 128 heads of 512 rows over
 // 2000 keys 205 and 111, 32 heads 52.5 and 62. Up to 64 rows tiles of 32 were never slower (14.6 and 18.7 over 4000).
-// Trees in tiles of 256 rows are dealt to the CUs, without rounds but with two starts for many, in units again:
+// Trees in tiles of 256 rows are dealt to the CUs, without rounds; up to half as many heads as CUs start once, more of
+// them about twice. In units again:
 //   a block 10, with more than 128 rows 12 (two waves of a SIMD at work); a start 80; 32 rows of the other kernel 3
-// Measured, us, int8, in tiles of 32 and of 256: 80 rows of 64 heads over 4096 keys at most 39.5 and 32.1, of 128 heads
-// over 8000 145 and 121; 128 rows of 16 heads over 32000 82.3 and 76.7, of 64 over 1000 19.7 and 27.7, over 4096 48.4 and
-// 48.4; 150 of 12 over 20000 54.2 and 58.0; 512 of 8 over 4096 30.8 and 39.5; 96 of 256 over 1000 at most 34.0 and 56.0.
+// Sequences of a batch are rarely all of the longest one's length, and dealing takes the mean: a fifth less. Measured,
+// us, int8, in tiles of 32 and of 256: 80 rows of 64 heads over 4096 keys at most 38.9 and 28.2, of 128 heads over 8000
+// 147 and 118; 128 rows of 16 heads over 32000 82.3 and 73.1, of 64 over 1000 19.5 and 28.2, over 4096 48.2 and 45.1, of
+// 128 over 2000 at most 38.0 and 31.0; 512 of 8 over 4096 31.4 and 39.5; 96 of 256 over 1000 at most 34.2 and 58.5, 80 of
+// 512 over 2000 at most 68.3 and 109.
 void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, bool tree, int cus, int xcds) {
   p->xcds = std::max(1, xcds);
   p->rep = p->heads / p->kv.kv_heads;
@@ -1578,10 +1619,12 @@ void plan_kv8_attention(Kv8Attention *p, int64_t max_tokens, bool tree, int cus,
   } else {
     weigh(32, tree && p->rows > 64 ? 3 : 2, 30);
     if (p->rows > 64 && !tree) weigh(32 * kTileWaves, 10, 40);
-    if (p->rows > 64 && tree) {  // dealt: no rounds, but a start for each piece
+    if (p->rows > 64 && tree) {
       const int64_t items = heads * ((p->rows + 32 * kTileWaves - 1) / (32 * kTileWaves));
-      const int64_t cost = (items * blocks * (p->rows > 128 ? 12 : 10) + (items + cus) * 80) / cus + 30 +
-                           (items + cus) * std::min(p->rows, 32 * kTileWaves) / 900;
+      const bool whole = items <= cus / 2;
+      int64_t cost = (items * blocks * (p->rows > 128 ? 12 : 10) + (whole ? cus : items + cus) * 80) / cus + 30 +
+                     (items + cus) * std::min(p->rows, 32 * kTileWaves) / 900;
+      if (whole && p->batch > 1) cost = cost * 4 / 5;
       if (cost < best) p->tile_rows = 32 * kTileWaves;
     }
   }
