@@ -73,10 +73,10 @@ struct Scales {
   }
 };
 
-// ---- up to 16 rows -------------------------------------------------------------------------------------------------
+// ---- up to 32 rows -------------------------------------------------------------------------------------------------
 //
-// A workgroup a CU walks its share of the tiles of channels, up to NT at a time, over the whole of K; its eight waves take
-// units in turn, codes and x straight into registers as operands, three units in flight across the ends of the chunks, and
+// A workgroup a CU walks its share of the tiles of channels, up to NT at a time, over the whole of K, with RT times 16 rows;
+// its eight waves take units in turn, codes and x straight into registers as operands, three units in flight across the ends of the chunks, and
 // join their sums through LDS. Bound by the bytes of w: 28672 x 8192 (G 128) of four rows 28 us, 4.3 TB/s where plain
 // reads of as many bytes reach 6.2 (without the products 27); with G 64 and zeros 31 us for one row, 33 for 13; 4096 x 4096
 // of one row 5.5 us.
@@ -85,10 +85,10 @@ struct Scales {
 // leading one. What that adds comes out again for each group: with a column of ones the matrix cores sum the rows' x in
 // the layout of the products, and sum_g s (sum x (128 + c) - (128 + z) sum x) is the product with s and z in fp32. The
 // sums are 16 times the weights' own at most, four bits of the 24.
-template <int NT, int PARTS, bool ZERO>
+template <int NT, int RT, int PARTS, bool ZERO>
 __global__ __launch_bounds__(512) void int4_rows_kernel(Int4Linear p) {
   constexpr int kWaves = 8, kSteps = 4 / PARTS;  // products of 32 inputs in a group
-  __shared__ f32x4 part[2][kWaves][NT][kWave];
+  __shared__ f32x4 part[2][kWaves][NT][RT][kWave];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 15, q = lane >> 4;
@@ -99,22 +99,25 @@ __global__ __launch_bounds__(512) void int4_rows_kernel(Int4Linear p) {
   const auto chunk_at = [&](int i) {  // the chunk's first tile of `count`, at most 60000
     return static_cast<int>(static_cast<uint32_t>(i * count) / static_cast<uint32_t>(chunks));
   };
-  const uint16_t *xr = p.x + min(r, m - 1) * p.x_stride + 8 * q;
+  const uint16_t *xr[RT];
+#pragma unroll
+  for (int j = 0; j < RT; ++j) xr[j] = p.x + min(16 * j + r, m - 1) * p.x_stride + 8 * q;
 
   struct Unit {
-    u32x4 x[4], w[NT];
+    u32x4 x[RT][4], w[NT];
     Scales<PARTS> s[NT], z[ZERO ? NT : 1];
   };
   int load_chunk = 0, load_step = 0, load_first = 0, load_tiles = chunk_at(1);
   const auto load = [&](Unit &v) {  // the wave's next unit; past K, x is 0 and w the last one
     if (load_chunk >= chunks) return;
     const int u = load_step * kWaves + wave, held = min(u, p.units - 1);
-    const uint16_t *from = xr + held * kUnit;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v.x[i] = (u32x4){0u, 0u, 0u, 0u};
-      if (u * kUnit + 32 * i < p.k) v.x[i] = *reinterpret_cast<const u32x4 *>(from + 32 * i);
-    }
+    for (int j = 0; j < RT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v.x[j][i] = (u32x4){0u, 0u, 0u, 0u};
+        if (u * kUnit + 32 * i < p.k) v.x[j][i] = *reinterpret_cast<const u32x4 *>(xr[j] + held * kUnit + 32 * i);
+      }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       if (t >= load_tiles) continue;
@@ -130,49 +133,63 @@ __global__ __launch_bounds__(512) void int4_rows_kernel(Int4Linear p) {
       load_tiles = chunk_at(load_chunk + 1) - load_first;
     }
   };
-  f32x4 y[NT];
+  f32x4 y[NT][RT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) y[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int j = 0; j < RT; ++j) y[t][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
   const bf16x8 ones = __builtin_bit_cast(bf16x8, (u32x4){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
   int chunk = 0, step = 0, first = 0, tiles = chunk_at(1), side = 0;
   const auto work = [&](const Unit &v) {  // returns whether it was the last one
 #pragma unroll
     for (int g = 0; g < PARTS; ++g) {
-      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+      f32x4 sum[RT];
 #pragma unroll
-      for (int i = g * kSteps; i < (g + 1) * kSteps; ++i)
-        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v.x[i]), ones, sum, 0, 0, 0);
+      for (int j = 0; j < RT; ++j) {
+        sum[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = g * kSteps; i < (g + 1) * kSteps; ++i)
+          sum[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v.x[j][i]), ones, sum[j], 0, 0, 0);
+      }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         if (t >= tiles) continue;
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        f32x4 acc[RT];
+#pragma unroll
+        for (int j = 0; j < RT; ++j) acc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = g * kSteps; i < (g + 1) * kSteps; ++i) {
           u32x4 c;
 #pragma unroll
           for (int j = 0; j < 4; ++j) c[j] = (v.w[t][i] >> (4 * j) & 0x000f000fu) | 0x43004300u;
-          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v.x[i]), __builtin_bit_cast(bf16x8, c),
-                                                        acc, 0, 0, 0);
+#pragma unroll
+          for (int j = 0; j < RT; ++j)
+            acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v.x[j][i]),
+                                                             __builtin_bit_cast(bf16x8, c), acc[j], 0, 0, 0);
         }
         const float s = v.s[t][g], offset = ZERO ? -128.f - v.z[t][g] : -136.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[t][e] = fmaf(s, fmaf(offset, sum[e], acc[e]), y[t][e]);
+        for (int j = 0; j < RT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[t][j][e] = fmaf(s, fmaf(offset, sum[j][e], acc[j][e]), y[t][j][e]);
       }
     }
     if (++step < steps) return false;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      part[side][wave][t][lane] = y[t];
-      y[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int j = 0; j < RT; ++j) {
+        part[side][wave][t][j][lane] = y[t][j];
+        y[t][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      }
     ring_barrier();  // the other side's sums have been read by all
-    for (int i = threadIdx.x; i < 16 * 16 * tiles; i += 512) {
-      const int ch = i % 16, row = i / 16 % 16, t = i / 256;
+    for (int i = threadIdx.x; i < 16 * 16 * RT * tiles; i += 512) {
+      const int ch = i % 16, row = i / 16 % (16 * RT), t = i / (256 * RT);
       const int64_t at = (tile0 + first + t) * 16 + ch;
       if (row >= m || at >= p.n) continue;
       float all = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) all += part[side][w][t][ch + 16 * (row / 4)][row % 4];
+      for (int w = 0; w < kWaves; ++w) all += part[side][w][t][row / 16][ch + 16 * (row % 16 / 4)][row % 4];
       p.y[row * p.n + at] = static_cast<uint16_t>(pack_bf16(all, 0.f));
     }
     step = 0;
@@ -406,9 +423,9 @@ __global__ __launch_bounds__(256) void int4_join_kernel(Int4Linear p) {
     if (ch + e < p.n) p.y[t * p.n + ch + e] = static_cast<uint16_t>(pack_bf16(sum[e], 0.f));
 }
 
-template <int PARTS, bool ZERO, int NT>
+template <int PARTS, bool ZERO, int NT, int RT>
 void start_rows(const Int4Linear &p, hipStream_t stream) {
-  hipLaunchKernelGGL((int4_rows_kernel<NT, PARTS, ZERO>), dim3(p.items), dim3(512), 0, stream, p);
+  hipLaunchKernelGGL((int4_rows_kernel<NT, RT, PARTS, ZERO>), dim3(p.items), dim3(512), 0, stream, p);
 }
 
 template <int PARTS, bool ZERO, int TM, int TN, int WN, int STAGES, int DEPTH>
@@ -423,9 +440,13 @@ template <int PARTS, bool ZERO>
 void start(const Int4Linear &p, hipStream_t stream) {
   switch (p.tile_m) {
     case 16:
-      if (p.row_tiles == 1) start_rows<PARTS, ZERO, 1>(p, stream);
-      else if (p.row_tiles == 2) start_rows<PARTS, ZERO, 2>(p, stream);
-      else start_rows<PARTS, ZERO, 4>(p, stream);
+      if (p.row_tiles == 1) start_rows<PARTS, ZERO, 1, 1>(p, stream);
+      else if (p.row_tiles == 2) start_rows<PARTS, ZERO, 2, 1>(p, stream);
+      else start_rows<PARTS, ZERO, 4, 1>(p, stream);
+      break;
+    case 32:
+      if (p.row_tiles == 1) start_rows<PARTS, ZERO, 1, 2>(p, stream);
+      else start_rows<PARTS, ZERO, 2, 2>(p, stream);
       break;
     case 64: start_tiles<PARTS, ZERO, 64, 128, 4, 3, 4>(p, stream); break;
     default: start_tiles<PARTS, ZERO, 256, 256, 8, 2, 2>(p, stream); break;
@@ -440,6 +461,10 @@ void start(const Int4Linear &p, hipStream_t stream) {
 //                    a unit   a 16   start
 //   64 x 128             65      8     500
 //   256 x 256           120     15    1000
+// The kernel of few rows takes 17 to 32 where that is less: 4 us, x for each chunk of a CU's tiles at 29 KB a us; what is
+// above stands a fifth below what such calls take. Measured, us, in tiles of 64 and in that kernel: 4096 x 4096 of 17
+// rows 13.5 and 8.9, of 32 14.1 and 11.7; 32000 x 4096 of 25 rows 39.7 and 33.1; 8192 x 28672 61.8 and 52.7; 28672 x 8192
+// 56.5 and 61.6, of 32 rows 57.0 and 71.7; 1024 x 8192 of 25 14.3 and 16.8.
 // Measured, us: 8192 x 28672 of 777 rows 366 in tiles of 256 split in two, 585 unsplit and as much in tiles of 64; 28672 x
 // 8192 of 100 rows 98 and 94, of 200 119 and 167, of 512 217 and 302, of 64 rows 60 split in three and 74 unsplit; 4096 x
 // 4096 of 17 rows 13.1 split in eight, 36 unsplit.
@@ -450,13 +475,11 @@ void plan_int4_linear(Int4Linear *p, int cus, int xcds) {
   p->part_stride = (p->n + 3) / 4 * 4;
   p->splits = 1;
   p->part_bytes = 0;
-  if (p->m <= 16) {
-    p->tile_m = 16;
-    p->items = static_cast<uint32_t>(std::min<int64_t>(p->tiles, cus));
-    const int64_t each = p->items > 0 ? (p->tiles + p->items - 1) / p->items : 0;
-    p->row_tiles = each == 1 ? 1 : each == 2 ? 2 : 4;
-    return;
-  }
+  p->items = static_cast<uint32_t>(std::min<int64_t>(p->tiles, cus));
+  const int64_t tiles_each = p->items > 0 ? (p->tiles + p->items - 1) / p->items : 0;
+  p->row_tiles = tiles_each == 1 ? 1 : tiles_each == 2 || p->m > 16 ? 2 : 4;
+  p->tile_m = 16;
+  if (p->m <= 16) return;
   int64_t best = INT64_MAX, splits = 1;
   int tile_n = 128;
   const int64_t reading = p->n * p->k / 106000;
@@ -476,6 +499,14 @@ void plan_int4_linear(Int4Linear *p, int cus, int xcds) {
   };
   weigh(64, 128, 65, 8, 500);
   if (p->m > 64) weigh(256, 256, 120, 15, 1000);
+  if (p->m <= 32) {  // a workgroup reads all of x for each chunk of its tiles
+    const int64_t chunks = (tiles_each + p->row_tiles - 1) / p->row_tiles;
+    const int64_t cost = 400 + std::max(chunks * p->k * p->m * 2 / 290, p->n * p->k / 85000);
+    if (cost * 5 < best * 6) {
+      p->tile_m = 32;
+      return;
+    }
+  }
   p->m_tiles = static_cast<uint32_t>((p->m + p->tile_m - 1) / p->tile_m);
   p->tile_rows = static_cast<int>(((p->m + 15) / 16 + p->m_tiles - 1) / p->m_tiles * 16);
   p->n_tiles = static_cast<uint32_t>((p->n + tile_n - 1) / tile_n);

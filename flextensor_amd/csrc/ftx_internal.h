@@ -292,8 +292,8 @@ struct Int4Linear {
   int k, parts;           // parts: groups of a unit
   // planned
   int64_t tiles;          // of 16 channels
-  int units, tile_m, tile_rows, row_tiles, splits, split_units, band, xcds;  // tile_m 16: the kernel of up to 16 rows;
-                          // tile_rows: of x in a tile, up to tile_m
+  int units, tile_m, tile_rows, row_tiles, splits, split_units, band, xcds;  // tile_m 16 or 32: the kernel of few
+                          // rows; tile_rows: of x in a tile, up to tile_m
   uint32_t m_tiles, n_tiles, items;
   size_t part_bytes;
 };

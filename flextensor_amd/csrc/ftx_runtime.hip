@@ -1764,7 +1764,7 @@ int plan_int4(int64_t m, int64_t n, int64_t k, int group, ftx::Int4Linear *p) {
   const int64_t join = p->splits > 1 ? m * p->part_stride / 4 : 0;
   if (static_cast<int64_t>(p->items) + p->xcds > ftx::kMaxThreads / 512 || join > ftx::kMaxThreads - 256)
     return ftx::fail(FTX_ERR_UNSUPPORTED, "int4 linear: more workgroups than one launch holds");
-  if (p->tile_m == 16 && p->tiles > int64_t(60000) * p->items)  // a workgroup's tiles are told apart in 32 bits
+  if (p->tile_m <= 32 && p->tiles > int64_t(60000) * p->items)  // a workgroup's tiles are told apart in 32 bits
     return ftx::fail(FTX_ERR_UNSUPPORTED, "int4 linear: more channels than one launch holds");
   return FTX_OK;
 }
