@@ -159,6 +159,30 @@ __device__ __forceinline__ float row_sum(float v) {
   return half_sum(__uint_as_float(s[0]) + __uint_as_float(s[1]));
 }
 
+// v of lane ^ J in a row of 16 lanes, by moves within the vector registers.
+template <int J>
+__device__ __forceinline__ int row_xor(int v) {
+  if constexpr (J == 1) return __builtin_amdgcn_mov_dpp(v, 0xb1, 15, 15, true);  // quad_perm 1 0 3 2
+  if constexpr (J == 2) return __builtin_amdgcn_mov_dpp(v, 0x4e, 15, 15, true);  // quad_perm 2 3 0 1
+  if constexpr (J == 4)                                                          // eights mirrored, then quads
+    return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(v, 0x141, 15, 15, true), 0x1b, 15, 15, true);
+  return __builtin_amdgcn_mov_dpp(v, 0x128, 15, 15, true);  // row_ror 8
+}
+// All lanes' bits together, as the scalars that they are.
+__device__ __forceinline__ uint32_t wave_or(uint32_t v) {
+  v |= row_xor<1>(v);
+  v |= row_xor<2>(v);
+  v |= row_xor<4>(v);
+  v |= row_xor<8>(v);
+  const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = s[0] | s[1];
+  const auto t = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return __builtin_amdgcn_readfirstlane(t[0] | t[1]);
+}
+__device__ __forceinline__ uint64_t wave_or(uint64_t v) {
+  return static_cast<uint64_t>(wave_or(static_cast<uint32_t>(v >> 32))) << 32 | wave_or(static_cast<uint32_t>(v));
+}
+
 // A call over a tree of drafted tokens: `count` rows that see the `start` first tokens and, of the `nodes` after them,
 // the ones in their set.
 __device__ __forceinline__ Span tree_span(const Kv8Attention &a, int64_t b) {
@@ -177,16 +201,30 @@ __device__ __forceinline__ int length_of(const Kv8Attention &a, Span s) {
   if constexpr (TREE) return min(s.start + a.nodes, a.kv.width * a.kv.page_blocks * kKvBlock);
   return s.start + s.count;
 }
+__device__ __forceinline__ uint64_t held_nodes(uint64_t set, int held) {
+  return held >= 64 ? set : set & ((1ull << max(held, 0)) - 1);
+}
 // The nodes that a row sees.
 __device__ __forceinline__ uint64_t node_set(const Kv8Attention &a, int64_t b, int token, int held) {
-  const uint64_t set = static_cast<uint64_t>(a.tree[b * a.tree_stride + token]);
-  return held >= 64 ? set : set & ((1ull << max(held, 0)) - 1);
+  return held_nodes(static_cast<uint64_t>(a.tree[b * a.tree_stride + token]), held);
 }
 // Of the 32 tokens from `at` on (counted from the nodes' first one), the ones that a row with this set sees.
 __device__ __forceinline__ uint32_t tokens_seen(uint64_t set, int at) {
   if (at >= 64) return 0;
   if (at >= 0) return static_cast<uint32_t>(set >> at);
   return at <= -32 ? ~0u : static_cast<uint32_t>(set << -at) | ((1u << -at) - 1);
+}
+
+// Nodes that no row sees may never have been written: a sequence adds fewer than the tree has, or its rows are some of
+// them. Codes there would meet probabilities of 0 in the products, and a NaN among them, or for a scale, every row. So
+// the keys and values end behind the last node that a row of the tile sees, and a block before it of which none sees a
+// token is a hole: the first one that holds nodes alone (64 nodes reach into one more).
+struct Reach {
+  int length, blocks, gap;
+};
+__device__ __forceinline__ Reach reach_of(uint64_t any, int start) {  // any: all that the tile's rows see
+  const int length = start + (any ? 64 - __builtin_clzll(any) : 0), first = (start + kKvBlock - 1) / kKvBlock;
+  return {length, (length + kKvBlock - 1) / kKvBlock, tokens_seen(any, first * kKvBlock - start) == 0 ? first : -1};
 }
 
 // The blocks that the rows of a tile see.
@@ -345,7 +383,7 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 15, g = lane >> 4;
   const int row0 = tile * (16 * RT);
-  const int length = length_of<TREE>(a, span);
+  int length = length_of<TREE>(a, span);
   const int last_token = (min(row0 + 16 * RT, a.rows) - 1) / a.rep;
   // every row sees keys below this
   const int whole = last_token >= span.count ? 0 : TREE ? span.start : span.start + row0 / a.rep + 1;
@@ -386,6 +424,7 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
     bool hole;
   };
   BlockList list;
+  [[maybe_unused]] Reach reach{};
   const uint32_t k_lane = g * (16 * kKvBlock) + (8 * (r >> 2) + (r & 3)) * 16, v_lane = r * kKvBlock + 8 * g;
   const auto load = [&](Block &x, int nth) {  // the wave's nth block; past the chunk's end its last one again
     const int at = nth % kWave;
@@ -423,6 +462,7 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
       }
     }
     const int key0 = block * kKvBlock;
+    if (TREE && (block >= reach.blocks || block == reach.gap)) x.hole = true;
     float scale = a.scale_log2 * x.k_scale;
     const bool zeros = no_scale(x.v_scale);
     if (x.hole || zeros || key0 + kKvBlock > whole) {
@@ -501,6 +541,10 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
   if (n > 0) {
     Block x, y;
     load(x, 0);
+    if constexpr (TREE) {  // while the first block is on its way
+      reach = reach_of(wave_or(sets[0] | sets[RT - 1]), span.start);
+      length = reach.length;
+    }
     for (int i = 0;;) {
       load(y, i + 1);
       work(x, first + wave + i * kWaves);
@@ -623,8 +667,6 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
     if (SPLIT && first >= blocks) return;
     end = !SPLIT || split == a.splits - 1 ? blocks : min(blocks, first + a.chunk);
   }
-  const int n_tiles = (end - first + kSub - 1) / kSub;
-
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 31, g = lane >> 5;
@@ -632,18 +674,48 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
   const int row = min(row0 + r, a.rows - 1);
   const int token = row / a.rep;
   const int head = kvh * a.rep + (row - token * a.rep);
-  const int length = length_of<TREE>(a, span);
+  int length = length_of<TREE>(a, span);
   const bool live = row0 + r < a.rows && token < span.count;
   const int seen = live ? span.start + token + 1 : 0;  // keys this lane's row sees
   const uint64_t set = TREE && live ? node_set(a, b, token, length - span.start) : 0;  // of a tree: the nodes
+  int64_t any[kTileWaves / 2] = {};  // of a tree: what the workgroup's rows see
+  if constexpr (TREE) {
+    const int token0 = tile * (32 * kTileWaves) / a.rep;
+    const int last_token = min((min((tile + 1) * (32 * kTileWaves), a.rows) - 1) / a.rep, span.count - 1);
+#pragma unroll
+    for (int i = 0; i < kTileWaves / 2; ++i)
+      if (token0 + i * kWave <= last_token)
+        any[i] = a.tree[b * a.tree_stride + min(token0 + i * kWave + lane, last_token)];
+  }
   const int last_row = min(row0 + 32, a.rows) - 1;
-  const int wave_end = row0 >= a.rows || row0 / a.rep >= span.count ? 0
-                       : TREE                                       ? length
-                                                                    : min(span.start + last_row / a.rep + 1, length);
   // Every row of the wave sees keys below this. A tree's rows that are left out see them too, and are cleared at the end:
   // masks for their sake took 0.4 us a tile.
   const bool all_live = row0 + 32 <= a.rows && last_row / a.rep < span.count;
   const int whole = TREE ? span.start : !all_live ? 0 : span.start + row0 / a.rep + 1;
+
+  // Queries: lane (r, g) holds elements 16 ks + 8 g .. + 7 of its row for every step ks.
+  bf16x8 qf[kQSteps];
+  {
+    const uint16_t *qp = a.q + b * a.q_stride[0] + token * a.q_stride[1] + head * a.q_stride[2] + 8 * g;
+#pragma unroll
+    for (int ks = 0; ks < kQSteps; ++ks)
+      qf[ks] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(qp + 16 * ks));
+  }
+  // The queries are in registers before the loop: where they may still be on their way as it is entered, every
+  // round waits for the codes that it has just asked for (2.0 us a tile).
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  asm volatile("" ::: "memory");
+  [[maybe_unused]] Reach reach{};
+  if constexpr (TREE) {
+    reach = reach_of(held_nodes(wave_or(static_cast<uint64_t>(any[0] | any[1] | any[2] | any[3])), length - span.start),
+                     span.start);
+    length = reach.length;
+  }
+  const int n_tiles = (end - first + kSub - 1) / kSub;
+  const int wave_end = row0 >= a.rows || row0 / a.rep >= span.count ? 0
+                       : TREE                                       ? length
+                                                                    : min(span.start + last_row / a.rep + 1, length);
 
   const auto side_of = [&](int i) {  // known when compiled where a unit of all waves is of one side
     return kSideUnits >= kThreads ? i * kThreads / kSideUnits : (i * kThreads + wave * kWave) / kSideUnits;
@@ -660,7 +732,13 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
   BlockList list;
   const auto load = [&](int t) {  // past the chunk's last block it again, masked
     const int at = t * kSub % kWave;
-    if (at == 0) list = block_list(a.kv, b, kvh, first + t * kSub, 1, end - 1);
+    if (at == 0) {
+      list = block_list(a.kv, b, kvh, first + t * kSub, 1, end - 1);
+      if constexpr (TREE) {
+        const int block = first + t * kSub + lane;
+        if (block >= reach.blocks || block == reach.gap) list.page = -1;
+      }
+    }
     Scales x;
     int page[kSub];
 #pragma unroll
@@ -710,19 +788,6 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Atte
     }
   };
 
-  // Queries: lane (r, g) holds elements 16 ks + 8 g .. + 7 of its row for every step ks.
-  bf16x8 qf[kQSteps];
-  {
-    const uint16_t *qp = a.q + b * a.q_stride[0] + token * a.q_stride[1] + head * a.q_stride[2] + 8 * g;
-#pragma unroll
-    for (int ks = 0; ks < kQSteps; ++ks)
-      qf[ks] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(qp + 16 * ks));
-  }
-  // The queries are in registers before the loop: where they may still be on their way as it is entered, every
-  // round waits for the codes that it has just asked for (2.0 us a tile).
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-  asm volatile("" ::: "memory");
   f32x16 o[kDTiles];
 #pragma unroll
   for (int d = 0; d < kDTiles; ++d)
@@ -1170,15 +1235,6 @@ struct Row {  // a thread's values, and the ones that they turn against
     }
   }
 };
-// v of lane ^ J in a row of 16 lanes, by moves within the vector registers.
-template <int J>
-__device__ __forceinline__ int row_xor(int v) {
-  if constexpr (J == 1) return __builtin_amdgcn_mov_dpp(v, 0xb1, 15, 15, true);  // quad_perm 1 0 3 2
-  if constexpr (J == 2) return __builtin_amdgcn_mov_dpp(v, 0x4e, 15, 15, true);  // quad_perm 2 3 0 1
-  if constexpr (J == 4)                                                          // eights mirrored, then quads
-    return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(v, 0x141, 15, 15, true), 0x1b, 15, 15, true);
-  return __builtin_amdgcn_mov_dpp(v, 0x128, 15, 15, true);  // row_ror 8
-}
 template <int J>
 __device__ __forceinline__ double row_xor(double v) {
   const uint64_t b = __builtin_bit_cast(uint64_t, v);

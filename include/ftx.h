@@ -515,6 +515,9 @@ int ftx_token_logprobs(const void *logits, int64_t row_stride, int type, const i
  * whose bit is set in the row's set tree[b][i] (int64, rows tree_stride apart, 0
  * for one tree of all sequences).
  * news: the rows that take part; the others, and rows that see no token, are 0.
+ * Nodes behind the last one that a row of the sequence sees may never have been
+ * written, nor a block of 32 tokens of which none sees one: both may hold
+ * anything. A NaN value in a block that is seen may reach rows that do not see it.
  * The rest as ftx_kv8_attention; max_tokens counts the nodes. workspace:
  * ftx_kv8_tree_attention_workspace bytes.
  *
