@@ -507,15 +507,19 @@ void plan_int4_linear(Int4Linear *p, int cus, int xcds) {
       return;
     }
   }
-  p->m_tiles = static_cast<uint32_t>((p->m + p->tile_m - 1) / p->tile_m);
+  const int64_t m_tiles = (p->m + p->tile_m - 1) / p->tile_m, n_tiles = (p->n + tile_n - 1) / tile_n;
+  if (m_tiles * n_tiles * splits > INT32_MAX) {  // too many for a launch, and for the numbers below: the caller refuses
+    p->items = UINT32_MAX;
+    return;
+  }
+  p->m_tiles = static_cast<uint32_t>(m_tiles);
   p->tile_rows = static_cast<int>(((p->m + 15) / 16 + p->m_tiles - 1) / p->m_tiles * 16);
-  p->n_tiles = static_cast<uint32_t>((p->n + tile_n - 1) / tile_n);
+  p->n_tiles = static_cast<uint32_t>(n_tiles);
   const uint32_t runs = (p->m_tiles + 11) / 12;
   p->band = static_cast<int>((p->m_tiles + runs - 1) / runs);
   p->split_units = static_cast<int>((p->units + splits - 1) / splits);
   p->splits = static_cast<int>((p->units + p->split_units - 1) / p->split_units);
-  const int64_t items = static_cast<int64_t>(p->m_tiles) * p->n_tiles * p->splits;
-  p->items = static_cast<uint32_t>(std::min<int64_t>(items, UINT32_MAX));  // too many for a launch: the caller refuses
+  p->items = p->m_tiles * p->n_tiles * static_cast<uint32_t>(p->splits);
   p->part_bytes = p->splits > 1 ? static_cast<size_t>(p->splits) * p->m * p->part_stride * 4 : 0;
 }
 
