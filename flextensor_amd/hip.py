@@ -948,7 +948,8 @@ def int4_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, zero
     """``x @ w.T`` of bf16 rows [m, k] and the 4-bit weights ``w = scale * (code - zero)`` of :func:`int4_pack`
     (``ftx_int4_linear``), ``n`` channels of them (None: all that the tiles hold).
 
-    Up to 16 rows take the weights as they are; for more rows they may be rounded to bf16, as a dequantised copy would be.
+    Up to 16 rows take the weights as they are, in fp32 sums of ``x`` times numbers up to 143 (weights of 0 leave up to
+    2^-24 of these, not nothing); for more rows they may be rounded to bf16, as a dequantised copy would be.
     ``k`` is a multiple of the group; rows may be strided. A row that holds an infinity or a NaN gives infinities or NaNs.
     No backward.
     """

@@ -436,7 +436,8 @@ int ftx_int8_linear(const void *x, int64_t x_stride, const void *w, const float 
  * their 32-bit word i inputs 32 i + 8 q + (0 .. 7), input 2 j at bit 4 j and 2 j + 1
  * at bit 16 + 4 j. scale and zero are bf16 [tile][unit][16][128 / G]; zero NULL is 8
  * for all. What lies past n and k is finite. Up to 16 rows use the weights as they
- * are; for more rows s (c - z) may be rounded to bf16. Sums are fp32: they stay finite
+ * are, in fp32 sums that lose up to 2^-24 (271 + |z|) s sum |x| of a group at each of
+ * its additions; for more rows s (c - z) may be rounded to bf16. Sums stay finite
  * while 256 sum |x| does, and a row that holds an infinity or a NaN has NaN or
  * infinite results. workspace: ftx_int4_linear_workspace bytes (0 unless K is split).
  * Pointers are 16-byte aligned. */
