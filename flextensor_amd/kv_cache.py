@@ -651,10 +651,13 @@ class PagedKVCache:
             self._lengths[s] += c
 
     def _check_step(self, step: KVStep) -> None:
-        moved = step.moves != self._moves
-        if step.cache is not self or any(
-                self._lengths.get(s) != was[0] or not moved and self._state(s, c) != was
-                for s, c, was in zip(step.sequences, step.counts, step.held)):
+        def changed(sequence: int, count: int, was: tuple[int, list[int]]) -> bool:
+            if self._lengths.get(sequence) != was[0]:
+                return True
+            now = self._state(sequence, count)
+            return now != was if step.moves == self._moves else len(now[1]) != len(was[1])  # moved: as many pages
+
+        if step.cache is not self or any(map(changed, step.sequences, step.counts, step.held)):
             raise ValueError("the step was committed before, or its sequences have changed since it began")
 
     def draft(self, sequences: list[int], parents: list[int]) -> KVTree:
