@@ -75,17 +75,17 @@ struct Scales {
 
 // ---- up to 32 rows -------------------------------------------------------------------------------------------------
 //
-// A workgroup a CU walks its share of the tiles of channels, up to NT at a time, over the whole of K, with RT times 16 rows;
-// its eight waves take units in turn, codes and x straight into registers as operands, three units in flight across the ends of the chunks, and
-// join their sums through LDS. Bound by the bytes of w: 28672 x 8192 (G 128) of four rows 28 us, 4.3 TB/s where plain
-// reads of as many bytes reach 6.2 (without the products 27); with G 64 and zeros 31 us for one row, 33 for 13; 4096 x 4096
-// of one row 5.5 us.
+// A workgroup a CU walks its share of the tiles of channels, up to NT at a time, over the whole of K, with RT times 16
+// rows; its eight waves take units in turn, codes and x straight into registers as operands, three units in flight across
+// the ends of the chunks, and join their sums through LDS. Bound by the bytes of w: 28672 x 8192 (G 128) of four rows
+// 28 us, 4.3 TB/s where plain reads of as many bytes reach 6.2 (without the products 27); with G 64 and zeros 31 us for
+// one row, 33 for 13; 4096 x 4096 of one row 5.5 us.
 //
 // A code becomes the bf16 number 128 + c by an AND and an OR of two codes at a time, exact in the seven bits below the
 // leading one. What that adds comes out again for each group: with a column of ones the matrix cores sum the rows' x in
 // the layout of the products, and sum_g s (sum x (128 + c) - (128 + z) sum x) is the product with s and z in fp32. Each
-// addition to either sum loses up to 2^-24 of it, together (271 + |z|) s sum |x| of the group, whatever the weights are:
-// ones of 0 leave that too (one input of 3000 among 127 of about 1: 0.03 s, 0.13 s at most). With 16 + c it would be a
+// addition to either sum loses up to 2^-24 of it, together (271 + |z|) s sum |x| of the group, whatever the weights
+// are: ones of 0 leave that too (one input of 3000 among 127 of about 1: 0.03 s, 0.13 s at most). With 16 + c it would be a
 // sixth, for a shift more of each word: 13 rows of 28672 x 8192 30.0 us where these take 29.5.
 template <int NT, int RT, int PARTS, bool ZERO>
 __global__ __launch_bounds__(512) void int4_rows_kernel(Int4Linear p) {
@@ -218,14 +218,15 @@ __global__ __launch_bounds__(512) void int4_rows_kernel(Int4Linear p) {
 // Up to TM tokens x TN channels a workgroup, K in units of 128: the tokens are dealt evenly to the tiles, in 16s, and
 // products of 16s that a tile does not have are left out (777 rows in four tiles of 208). A unit's x goes straight from
 // memory into one of STAGES stages of LDS while another is multiplied, with one barrier a unit; row R's 16-byte chunk c
-// lies at slot c ^ (R % 16), so the 16 rows that a read touches lie in different banks. The codes go from memory into the registers of the wave that
-// multiplies by them, as the operands that they are, DEPTH units ahead: they take no LDS and no barrier. A wave makes the
-// weights of its channels for the next 32 inputs, (c - z) s in fp32 rounded to bf16, between the products of these ones.
+// lies at slot c ^ (R % 16), so the 16 rows that a read touches lie in different banks. The codes go from memory into
+// the registers of the wave that multiplies by them, as the operands that they are, DEPTH units ahead: they take no LDS
+// and no barrier. A wave makes the weights of its channels for the next 32 inputs, (c - z) s in fp32 rounded to bf16,
+// between the products of these ones.
 //
 // Rounding the weights is what lets the matrix cores sum over groups: an error of 2^-8 of each at most, 0.0022 of the
-// result in relative norm where the output's own rounding is 0.0017. v_mfma_f32_16x16x32_bf16 takes the channels as rows
-// and the tokens as columns, so a lane ends with four neighbouring channels of a token; they reach y through LDS, in whole
-// lines.
+// result in relative norm where the output's own rounding is 0.0017. v_mfma_f32_16x16x32_bf16 takes the channels as
+// rows and the tokens as columns, so a lane ends with four neighbouring channels of a token; they reach y through LDS,
+// in whole lines.
 
 // Eight codes as weights, s c + b.
 __device__ __forceinline__ bf16x8 weights(uint32_t w, float s, float b) {

@@ -296,9 +296,10 @@ __device__ __forceinline__ Share share_at(const Kv8Attention &a, uint32_t at, ui
   }
   return s;
 }
-// Or, where they fit, pieces of one head each, so that no workgroup starts twice: a head's keys in as few pieces of up to
-// `each` tiles as they take, `each` the least for which there is a workgroup for every piece. A second start takes as
-// long as some three tiles (the case above: 37.7 us with them). Returns whether it is so, with the workgroup's share and its head's `each`.
+// Or, where they fit, pieces of one head each, so that no workgroup starts twice: a head's keys in as few pieces of up
+// to `each` tiles as they take, `each` the least for which there is a workgroup for every piece. A second start takes as
+// long as some three tiles (8 ragged sequences of 25 nodes over up to 4096 tokens: 37.7 us with second starts, 31.6
+// without). Returns whether it is so, with the workgroup's share and its head's `each`.
 constexpr uint32_t kSecondStart = 3;
 __device__ __forceinline__ bool whole_pieces(const Kv8Attention &a, uint32_t group, Share &s, uint32_t &each) {
   if (a.batch > kWave) return false;
@@ -610,8 +611,8 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_rows_kernel(Kv8Atte
 // operands are written in that order.
 //
 // Trees: the sequences' lengths are known on the device alone, so a workgroup a CU reads them all and takes an equal
-// share of the batch's tiles (8 ragged sequences of 25 nodes over up to 4096 tokens, 64 / 8 heads, int8: 31.6 us, and 51 in
-// chunks of the longest one's length). Where a share ends inside a head's tiles, its sums go to `part`, one place for the
+// share of the batch's tiles (8 ragged sequences of 25 nodes over up to 4096 tokens, 64 / 8 heads, int8: 32.4 us, and 51
+// in chunks of the longest one's length). Where a share ends inside a head's tiles, its sums go to `part`, one place for the
 // head it begins and one for the head that it goes on with (kv8_join_shares_kernel); SPLIT does not matter.
 template <int D, bool FP8, bool SPLIT, bool TREE>
 __global__ __launch_bounds__(kTileWaves * kWave, 2) void kv8_tile_kernel(Kv8Attention a) {

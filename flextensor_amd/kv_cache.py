@@ -250,7 +250,8 @@ def tree_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, t
     bits, its ancestors the others; rows may be a part of the nodes (a level of the tree). Rows from ``new[b]`` on, and
     rows that see no token, are 0. Nodes behind the last one that a row of the sequence sees, and blocks of 32 tokens of
     which none sees one, may hold anything: they need not have been written. A NaN that another node's value holds may
-    reach rows that do not see it. ``max_tokens`` counts the nodes. Many rows are shared out by the lengths of the whole batch, which may change the order of a sum.
+    reach rows that do not see it. ``max_tokens`` counts the nodes. Many rows are shared out by the lengths of the whole
+    batch, which may change the order of a sum.
     """
     device = _device(q)
     if device >= 0 and torch.autograd.forward_ad._current_level < 0:
