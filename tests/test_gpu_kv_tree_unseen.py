@@ -100,3 +100,26 @@ def test_a_block_of_nodes_that_no_row_sees_may_hold_anything(gpu, dtype, b, t, k
         unseen += [(n, block, 0, True) for block in range(first + 1, first + 4) if t == 1 or block != end // BLOCK]
         unseen.append((n, end // BLOCK, end % BLOCK, False))
     _compare(gpu, q, codes, scales, table, starts, sets, None, nodes, unseen)
+
+
+@pytest.mark.parametrize("dtype", FORMATS)
+@pytest.mark.parametrize("b,t,kv,rep,start", [(1, 3, 2, 4, 1040), (2, 8, 2, 4, 16), (8, 32, 8, 8, 4112)])
+def test_nodes_that_no_row_sees_within_a_block_change_nothing(gpu, dtype, b, t, kv, rep, start):
+    """The largest finite codes at such places, the block's scales being those of the nodes that are seen."""
+    d, page, nodes = 128, 32, 64
+    q, codes, scales, table = _case(gpu, b, t, kv * rep, kv, d, page, [start], nodes, dtype)
+    assert _dealt(gpu, b, t, kv * rep, kv, d, table.shape[1] * page) == (b == 8)
+    seen = list(range(0, 63, 3))  # every third node
+    sets = torch.tensor([[sum(1 << n for n in seen if n <= seen[i % 21]) for i in range(t)]])
+    sets[0, -1] = sum(1 << n for n in seen)
+    sets = sets.expand(b, t)
+    args = (table, _i32([start] * b, gpu), sets.to(gpu))
+    clean = kvc.tree_attention(q, codes, scales, *args, nodes=nodes)
+    want = _exact(q, codes, scales, table, [start] * b, sets, None, nodes)
+    assert (clean.double() - want).norm() <= TWO_ROUNDINGS * want.norm()
+    raw, largest = codes.view(torch.uint8), 0x7e if dtype is torch.float8_e4m3fn else 127
+    for token in (start + n for n in range(nodes) if n not in seen):
+        pages, cell = table[:, token // page].long(), token % BLOCK
+        raw[:, 0, :, 0].view(-1, kv, d // 16, BLOCK, 16)[pages, :, :, cell] = largest
+        raw[:, 1, :, 0].view(-1, kv, d, BLOCK)[pages, :, :, cell] = largest
+    assert torch.equal(kvc.tree_attention(q, codes, scales, *args, nodes=nodes), clean)
